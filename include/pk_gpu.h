@@ -416,6 +416,55 @@ int pk_gpu_encoder_set_numerics(pk_gpu_encoder *enc, int mode);
 int pk_gpu_encoder_get_numerics(pk_gpu_encoder *enc);
 void pk_gpu_encoder_destroy(pk_gpu_encoder *enc);
 
+/* ---- autoregressive decoder (device pointers, no synchronisation) ------
+ * The operators of one block's step of a decoder that reads the encoder's
+ * frames token by token: norm, projection of 8-bit rows, a paged key-value
+ * cache and the attention of one new token over it.  No counterpart in the
+ * reference (its decoder is an LSTM, decoder.c:1-132).  None of them allocates,
+ * waits or keeps anything between calls, so all may be captured in a HIP
+ * graph.  Pointers are of the library's device, whichever device is current.
+ * Results do not depend on timing: no atomics, fixed orders of summation. */
+
+/* Element types. */
+#define PK_GPU_F32  0
+#define PK_GPU_F16  1
+#define PK_GPU_BF16 2
+#define PK_GPU_I8   3
+#define PK_GPU_E4M3 4   /* 8-bit float, 4 exponent and 3 mantissa bits, +-448 at most */
+
+/* A paged key-value cache of one layer; the memory is the caller's.
+ *   k, v              [n_pages][heads][page_size][head_dim] of `dtype`: F16,
+ *                     BF16, I8 or E4M3
+ *   k_scale, v_scale  [n_pages][heads][page_size] floats, what a row's codes
+ *                     are multiplied with (I8 and E4M3; unused otherwise)
+ * head_dim 64, 128 or 256; page_size a power of two, at least 16; n_pages *
+ * page_size below 2^31 (the arrays may pass 4 GiB); arrays 16-byte aligned.
+ * Slot s is offset s % page_size of page s / page_size. */
+typedef struct {
+    void  *k, *v;
+    float *k_scale, *v_scale;
+    int    dtype, n_pages, page_size, heads, head_dim;
+} pk_gpu_kv_cache;
+
+/* Write n tokens' keys and values, rows of heads * head_dim elements of `dtype`
+ * (F32, F16 or BF16) ldk and ldv apart, into the cache's slots dslots[0..n).
+ * A slot below 0 or past the cache skips its row (padding).  Two rows of one
+ * call must not name the same slot (what that slot then holds is one row or a
+ * mixture; other slots are not touched).  16-bit caches take the rounded value.
+ * 8-bit caches take, per token and head, with a the row's largest magnitude
+ * and top = 127 (I8) or 448 (E4M3): scale = a / top, codes x * (top / a)
+ * rounded to nearest, ties to even, all in fp32 (scale a float lower where
+ * top * scale would overflow).  A row with a < 2^-100 is
+ * written as zeros (scale 0); a row that holds an infinity or a NaN reads back
+ * as NaN (scale NaN).  Rows 16-byte aligned. */
+int pk_gpu_kv_write_dev(const pk_gpu_kv_cache *cache, int dtype, const void *dk, int ldk,
+                        const void *dv, int ldv, const int *dslots, int n, void *stream);
+/* Read them back: row i of dk and dv receives slot dslots[i], code * scale in
+ * fp32, rounded once to `dtype`.  Rows whose slot is below 0 or past the cache
+ * are left as they were; a slot may be named any number of times. */
+int pk_gpu_kv_read_dev(const pk_gpu_kv_cache *cache, int dtype, const int *dslots, int n, void *dk,
+                       int ldk, void *dv, int ldv, void *stream);
+
 /* ---- tuning / introspection ------------------------------------------- */
 
 /* Number of kernel tile configurations, and a description of one:

@@ -16,6 +16,9 @@ int hip_error(hipError_t e, const char* what);
 // Initialise the library if needed and bind the calling thread to its
 // device; *thread_stream (if given) receives the thread's own stream.
 int bind(hipStream_t* thread_stream);
+// Initialise the library if needed; *device receives the index of its device.
+// Creates nothing and leaves the thread's current device to the caller.
+int enter(int* device);
 // Launch one weight GEMM (launch_gemm with the thread's forced config, which
 // implies exact chains), mapping launch errors to pk_gpu_status codes.
 int gemm(const GemmProblem& p, hipStream_t s, Tolerance tol = TOL_NONE);

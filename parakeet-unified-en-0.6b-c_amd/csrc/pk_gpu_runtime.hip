@@ -1169,6 +1169,14 @@ int bind(hipStream_t* thread_stream)
     return PK_GPU_OK;
 }
 
+int enter(int* device)
+{
+    std::lock_guard<std::mutex> lk(g_mu);
+    const int rc = init_locked(-1);
+    if (rc == PK_GPU_OK) *device = g_device;
+    return rc;
+}
+
 Tolerance tolerance_of(int numerics)
 {
     return numerics == PK_GPU_NUMERICS_DEFAULT ? TOL_SMALL_M

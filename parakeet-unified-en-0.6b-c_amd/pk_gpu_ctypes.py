@@ -89,12 +89,16 @@ _PROTOS = {
     "pk_gpu_encoder_pre_encode_dev": (_i, [_p, _p, _i, _p, _p]),
     "pk_gpu_encoder_run_mel": (_i, [_p, _p, _i, _i, _i, _p]),
     "pk_gpu_encoder_profile_read": (_i, [_p, _i, _p, _p, _p, _p]),
+    "pk_gpu_kv_write_dev": (_i, [_p, _i, _p, _i, _p, _i, _p, _i, _p]),
+    "pk_gpu_kv_read_dev": (_i, [_p, _i, _p, _i, _p, _i, _p, _i, _p]),
 }
 
-EPI_NONE, EPI_SWISH, EPI_HALF_RESIDUAL, EPI_RESIDUAL = 0, 1, 2, 3
+EPI_NONE, EPI_SWISH, EPI_HALF_RESIDUAL, EPI_RESIDUAL, EPI_RELU = 0, 1, 2, 3, 4
 NUMERICS_DEFAULT, NUMERICS_EXACT, NUMERICS_FAST = 0, 1, 2
 # PK_GPU_STAGE_*: pk_gpu_encoder_profile_read's stages
 STAGE_GEMM_I4, STAGE_GEMM_I8, STAGE_GEMM_F32, STAGE_ATTENTION, STAGE_LAYER_NORM, STAGE_CONV, STAGE_COPY = range(7)
+# PK_GPU_F32 ...: element types
+F32, F16, BF16, I8, E4M3 = range(5)
 NOALLOC_BYTES = 64 << 20          # PK_GPU_NOALLOC_BYTES
 SPLIT_WORKSPACE_BYTES = 32 << 20  # PK_GPU_SPLIT_WORKSPACE_BYTES
 
@@ -134,6 +138,13 @@ class PreEncodeWeights(ctypes.Structure):
     _fields_ = [("conv0_w", _p), ("conv0_b", _p), ("conv2_w", _p), ("conv2_b", _p),
                 ("conv3_w", _p), ("conv3_b", _p), ("conv5_w", _p), ("conv5_b", _p),
                 ("conv6_w", _p), ("conv6_b", _p), ("out_w", Weight), ("out_b", _p)]
+
+
+class KvCache(ctypes.Structure):
+    """pk_gpu_kv_cache (include/pk_gpu.h): a paged key-value cache, device pointers."""
+    _fields_ = [("k", _p), ("v", _p), ("k_scale", _p), ("v_scale", _p), ("dtype", _i),
+                ("n_pages", _i), ("page_size", _i), ("heads", _i), ("head_dim", _i)]
+
 
 STATUS = {0: "OK", -1: "EINVAL", -2: "ENOTSUP", -3: "ENOMEM", -4: "EHIP", -5: "ENODEV", -6: "EBUSY"}
 

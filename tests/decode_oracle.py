@@ -1,0 +1,127 @@
+"""Plain 64-bit (numpy) forms of the decoder operators, and the small helpers
+their tests share.  Nothing here calls the library's kernels."""
+import ctypes
+
+import numpy as np
+
+from pkgpu import pk
+
+FLOATS = {"f32": pk.F32, "f16": pk.F16, "bf16": pk.BF16}
+KINDS = dict(FLOATS, int8=pk.I8, e4m3=pk.E4M3)
+TOP = {"int8": 127.0, "e4m3": 448.0}
+# half a step of a type, relative to the value: what one rounding is off by at most
+HALF = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8, "e4m3": 2.0 ** -4}
+TINY = 2.0 ** -100
+
+
+def torch_type(name):
+    import torch
+    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16,
+            "int8": torch.int8, "e4m3": torch.float8_e4m3fn}[name]
+
+
+def rounded(x, name):
+    """float32 array rounded to a type and back (the CPU's conversions)."""
+    import torch
+    return torch.from_numpy(np.ascontiguousarray(x, np.float32)).to(torch_type(name)).float().numpy()
+
+
+def values(t):
+    """A torch tensor of any of the types as float64 numpy."""
+    return t.detach().cpu().float().double().numpy()
+
+
+def codes(x, kind):
+    """The documented fp32 formula: codes (as the values they are) and scales of the last axis's rows."""
+    x = np.asarray(x, np.float32)
+    top = np.float32(TOP[kind])
+    a = np.abs(x).max(-1)
+    bad = ~np.isfinite(x).all(-1)
+    none = (a < np.float32(TINY)) | bad
+    with np.errstate(all="ignore"):
+        inv = np.where(none, np.float32(0), top / a).astype(np.float32)
+        scale = np.where(none, np.float32(0), a / top).astype(np.float32)
+        scale = np.minimum(scale, np.float32(float.fromhex("0x1.020406p+121")))   # 127 times it is finite
+        y = np.where(none[..., None], np.float32(0), x * inv[..., None]).astype(np.float32)
+    scale = np.where(bad, np.float32(np.nan), scale)
+    return (np.rint(y) if kind == "int8" else rounded(y, "e4m3")), scale
+
+
+def code_bound(x, kind):
+    """How far code * scale may be from x (64 bits): half a step of the code, at
+    the row's unit u = max|x| / top, plus the three fp32 roundings of inv, x * inv
+    and scale, each at most 2^-24 of a value of at most max|x| (3.01: with their
+    products)."""
+    x = np.asarray(x, np.float64)
+    a = np.abs(x).max(-1, keepdims=True)
+    u = a / TOP[kind]
+    if kind == "int8":
+        half = 0.5 * u * np.ones_like(x)
+    else:  # 3 bits behind the leading one; the smallest exponent is -6
+        m = np.maximum(np.abs(x) / np.where(u == 0, 1, u), 2.0 ** -6)
+        # the quotient may round up over a power of two: its step then is the larger one
+        half = 0.5 * u * 2.0 ** (np.floor(np.log2(m * (1 + 2.0 ** -22))) - 3)
+    return half + 3.01 * 2.0 ** -24 * a
+
+
+class Cache:
+    """A cache on the device (torch tensors) with guard elements on both sides of each array."""
+
+    GUARD = 64
+
+    def __init__(self, kind, pages, heads, page, dim, seed=0, filled=True):
+        import torch
+        self.kind, self.pages, self.heads, self.page, self.dim = kind, pages, heads, page, dim
+        rng = np.random.default_rng(seed)
+        self.arrays = {}
+        shape = (pages, heads, page, dim)
+        for name in ("k", "v"):
+            if not filled:
+                x = np.zeros(shape, np.float32)
+            elif kind == "int8":
+                x = rng.integers(-127, 128, shape).astype(np.float32)
+            elif kind == "e4m3":
+                x = np.clip(rng.normal(0, 120, shape), -448, 448)
+            else:
+                x = rng.normal(0, 1, shape)
+            self._put(name, torch.from_numpy(np.asarray(x, np.float32)).to(torch_type(kind)))
+            if kind in TOP:
+                sc = rng.uniform(0.5, 2.0, shape[:3]) / TOP[kind] if filled else np.zeros(shape[:3])
+                self._put(name + "_scale", torch.from_numpy(np.asarray(sc, np.float32)))
+
+    def _put(self, name, t):
+        import torch
+        flat = t.contiguous().view(torch.uint8).reshape(-1)
+        guard = torch.full((self.GUARD,), 0x5A, dtype=torch.uint8)
+        whole = torch.cat([guard, flat, guard]).to("cuda:0")
+        self.arrays[name] = (whole, t.shape, t.dtype)
+
+    def part(self, name):
+        whole, shape, dtype = self.arrays[name]
+        return whole[self.GUARD:-self.GUARD].view(dtype).view(shape)
+
+    def guards_whole(self):
+        return all(bool((w[:self.GUARD] == 0x5A).all() and (w[-self.GUARD:] == 0x5A).all())
+                   for w, _, _ in self.arrays.values())
+
+    def struct(self):
+        p = {n: self.part(n).data_ptr() for n in self.arrays}
+        return pk.KvCache(p["k"], p["v"], p.get("k_scale"), p.get("v_scale"), KINDS[self.kind],
+                          self.pages, self.page, self.heads, self.dim)
+
+    def rows(self, name):
+        """float64 [slots][heads][dim], what the cache's rows stand for."""
+        x = values(self.part(name)).transpose(0, 2, 1, 3).reshape(-1, self.heads, self.dim)
+        if self.kind in TOP:
+            sc = values(self.part(name + "_scale")).transpose(0, 2, 1).reshape(-1, self.heads, 1)
+            x = x * sc
+        return x
+
+
+def ref(struct):
+    return ctypes.byref(struct)
+
+
+def stream():
+    import torch
+    return torch.cuda.current_stream().cuda_stream
