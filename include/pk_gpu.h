@@ -465,6 +465,36 @@ int pk_gpu_kv_write_dev(const pk_gpu_kv_cache *cache, int dtype, const void *dk,
 int pk_gpu_kv_read_dev(const pk_gpu_kv_cache *cache, int dtype, const int *dslots, int n, void *dk,
                        int ldk, void *dv, int ldv, void *stream);
 
+/* Attention of one new token per sequence over the cache.  Sequence b's token
+ * t (0 <= t < dlens[b]) is at offset t % page_size of page
+ * dpages[b * ld_pages + t / page_size]; the new token is the last one (write
+ * it first), and every one of the `heads` query heads, a multiple of the
+ * cache's, attends over the key-value head it shares with heads / cache->heads
+ * - 1 neighbours: softmax of scale * q . k_t over the tokens it sees, times v.
+ *   q, out    [B] rows of heads * head_dim elements of `dtype`, ldq and ldo apart:
+ *             any of F32, F16, BF16 over I8 and E4M3 caches, F16 over F16,
+ *             BF16 or F32 over BF16; 16-byte aligned rows
+ *   window    > 0: only the last `window` tokens; 0: all
+ *   max_len   at most 2^30; no sequence is longer (a larger dlens[b] counts as max_len, one
+ *             below 0 as 0); page table rows hold max_len tokens.  Work is split
+ *             by it, so a close bound is the fast one.
+ *   lse       NULL, or [B][heads] floats: log of the sum of the exponentials,
+ *             what another part of a split softmax is joined with
+ * Page entries outside [0, n_pages) are absent: their tokens take no part, and
+ * entries from dlens[b] on are not read.  Tokens that take no part may hold
+ * anything, NaN included.  A sequence without tokens gives zeros (lse -inf).
+ * Scores, sums and the softmax are fp32; its weights enter the second product
+ * with 8, 16 or 24 bits for BF16, F16 and F32 output (11 over F16 caches).
+ * dws: a 16-byte aligned workspace of at least pk_gpu_paged_attention_ws_floats
+ * floats for the same sizes (0: none is needed), free again when the call's
+ * work is done; calls that may overlap on the device must not share it. */
+size_t pk_gpu_paged_attention_ws_floats(const pk_gpu_kv_cache *cache, int B, int heads, int max_len,
+                                        int window);
+int pk_gpu_paged_attention_dev(const pk_gpu_kv_cache *cache, int dtype, const void *dq, int ldq,
+                               int heads, const int *dpages, int ld_pages, const int *dlens, int B,
+                               int max_len, float scale, int window, void *dout, int ldo,
+                               float *dlse, float *dws, size_t ws_floats, void *stream);
+
 /* ---- tuning / introspection ------------------------------------------- */
 
 /* Number of kernel tile configurations, and a description of one:

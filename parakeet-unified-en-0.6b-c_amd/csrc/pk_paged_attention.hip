@@ -1,0 +1,236 @@
+// pk_paged_attention.hip - host side of the attention over a paged cache, and
+// the kernel that joins a sequence's chunks.
+#include "pk_paged_attention.h"
+
+namespace pkgpu {
+namespace decode {
+namespace {
+
+constexpr int kMaxSplits = 256;     // the join's threads: one a chunk
+
+struct JoinArgs {
+    const float *part, *ml;
+    const int* lens;
+    char* out;
+    size_t ldo;
+    float* lse;
+    int heads, splits, chunk, max_len, window;
+};
+
+// One workgroup joins the chunks of one head: out = sum_c 2^(m_c - m) o_c /
+// sum_c 2^(m_c - m) l_c.  DIM / 4 lanes cover the head, the other lanes take
+// every PARTS-th chunk; sums run in a fixed order.
+template <int T, int DIM>
+__global__ void __launch_bounds__(256) paged_join(JoinArgs a)
+{
+    constexpr int LANES = DIM / 4, PARTS = 256 / LANES;
+    __shared__ float red[2][4];
+    __shared__ float wgt[kMaxSplits];
+    __shared__ f32x4 sum[PARTS][LANES];
+    const int b = blockIdx.x / (uint32_t)a.heads, head = blockIdx.x % (uint32_t)a.heads;
+    const int chunks = span_of(a.lens[b], a.max_len, a.window, a.chunk).chunks;
+    if (chunks <= 1) return;                        // written by the first launch
+    const size_t row = (size_t)b * a.heads + head;
+    const int i = threadIdx.x, lane = i & 63, wave = i >> 6;
+    const float* ml = a.ml + row * a.splits * 2;
+    float m = -FLT_MAX, l = 0.0f;
+    if (i < chunks) { m = ml[2 * i]; l = ml[2 * i + 1]; }
+    float mx = m;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
+    if (lane == 0) red[0][wave] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    const float w = i < chunks ? __builtin_amdgcn_exp2f(m - mx) : 0.0f;
+    wgt[i] = w;
+    float lt = __fmul_rn(l, w);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) lt = __fadd_rn(lt, __shfl_xor(lt, d));
+    if (lane == 0) red[1][wave] = lt;
+    __syncthreads();
+    lt = __fadd_rn(__fadd_rn(red[1][0], red[1][1]), __fadd_rn(red[1][2], red[1][3]));
+    const int part = i / LANES, d4 = i % LANES;
+    f32x4 o = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    const float* src = a.part + row * a.splits * DIM + 4 * d4;
+#pragma unroll 4
+    for (int c = part; c < chunks; c += PARTS) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(src + (size_t)c * DIM);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = __fmaf_rn(v[r], wgt[c], o[r]);
+    }
+    sum[part][d4] = o;
+    __syncthreads();
+    if (part) return;
+#pragma unroll
+    for (int p = 1; p < PARTS; ++p)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = __fadd_rn(o[r], sum[p][d4][r]);
+    const float inv = lt == 0.0f ? 0.0f : __fdiv_rn(1.0f, lt);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] = lt == 0.0f ? 0.0f : __fmul_rn(o[r], inv);
+    char* p = a.out + (size_t)b * a.ldo + ((size_t)head * DIM + 4 * d4) * size_of(T);
+    if constexpr (T == F32) *reinterpret_cast<f32x4*>(p) = o;
+    else
+        *reinterpret_cast<u32x2*>(p) = T == F16 ? (u32x2){pack_f16(o[0], o[1]), pack_f16(o[2], o[3])}
+                                                : (u32x2){pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3])};
+    if (d4 == 0 && a.lse)
+        a.lse[row] = lt == 0.0f ? -__builtin_inff()
+                                : __fmul_rn(__fadd_rn(mx, __builtin_amdgcn_logf(lt)), 0.69314718055994531f);
+}
+
+template <int T>
+hipError_t launch_join(int dim, const JoinArgs& a, uint32_t rows, hipStream_t s)
+{
+    return dim == 64    ? launch(paged_join<T, 64>, dim3(rows), dim3(256), 0, s, a)
+           : dim == 128 ? launch(paged_join<T, 128>, dim3(rows), dim3(256), 0, s, a)
+                        : launch(paged_join<T, 256>, dim3(rows), dim3(256), 0, s, a);
+}
+
+struct Plan { int chunk, splits; };
+
+// Tokens per workgroup.  A round of its waves is kPagedWaves tiles of 32
+// tokens; chunks are whole rounds.  Few (sequence, head) pairs: as many chunks
+// as fill the chip; many: chunks short enough that ragged sequences even out.
+Plan plan(long long pairs, int max_len, int window)
+{
+    const int round = 32 * kPagedWaves;
+    long long span = window > 0 && window < max_len ? (long long)window + 31 : max_len;
+    if (span < 1) span = 1;
+    const long long rounds = (span + round - 1) / round;
+    long long splits = (2048 + pairs - 1) / pairs;
+    if (splits > rounds) splits = rounds;
+    if (splits > kMaxSplits) splits = kMaxSplits;
+    if (splits < 1) splits = 1;
+    const long long chunk = (rounds + splits - 1) / splits * round;
+    return {(int)chunk, (int)((span + chunk - 1) / chunk)};
+}
+
+// 16 query heads of a key-value head a workgroup.
+int head_tiles(int group) { return (group + 15) / 16; }
+
+int check_attention(const pk_gpu_kv_cache* c, int B, int heads, int max_len, int window)
+{
+    const char* who = "paged attention";
+    const int rc = check_cache(c, who);
+    if (rc) return rc;
+    if (B < 0 || max_len < 0 || window < 0)
+        return rt::error(PK_GPU_EINVAL, "%s: B = %d, max_len = %d, window = %d", who, B, max_len, window);
+    if (max_len > 1 << 30)      // token indices of a round ahead stay below 2^31
+        return rt::error(PK_GPU_EINVAL, "%s: max_len = %d is above 2^30", who, max_len);
+    if (heads < 1 || heads % c->heads)
+        return rt::error(PK_GPU_EINVAL, "%s: %d query heads over %d key-value heads", who, heads, c->heads);
+    const Plan p = plan((long long)(B ? B : 1) * c->heads * head_tiles(heads / c->heads), max_len, window);
+    if ((long long)B * c->heads * head_tiles(heads / c->heads) * p.splits > 0x7fffffff ||
+        (long long)B * heads > 0x7fffffff)
+        return rt::error(PK_GPU_EINVAL, "%s: %d sequences of %d heads exceed the grid", who, B, heads);
+    return PK_GPU_OK;
+}
+
+size_t ws_floats_of(const pk_gpu_kv_cache* c, int B, int heads, const Plan& p)
+{
+    return p.splits <= 1 ? 0 : (size_t)B * heads * p.splits * (c->head_dim + 2);
+}
+
+}  // namespace
+}  // namespace decode
+}  // namespace pkgpu
+
+extern "C" {
+
+using namespace pkgpu::decode;
+
+size_t pk_gpu_paged_attention_ws_floats(const pk_gpu_kv_cache* cache, int B, int heads, int max_len, int window)
+{
+    if (check_attention(cache, B, heads, max_len, window) != PK_GPU_OK || B == 0) return 0;
+    return ws_floats_of(cache, B, heads,
+                        plan((long long)B * cache->heads * head_tiles(heads / cache->heads), max_len, window));
+}
+
+int pk_gpu_paged_attention_dev(const pk_gpu_kv_cache* cache, int dtype, const void* dq, int ldq, int heads,
+                               const int* dpages, int ld_pages, const int* dlens, int B, int max_len,
+                               float scale, int window, void* dout, int ldo, float* dlse, float* dws,
+                               size_t ws_floats, void* stream)
+{
+    namespace rt = pkgpu::rt;
+    const char* who = "paged attention";
+    int rc = check_attention(cache, B, heads, max_len, window);
+    if (rc) return rc;
+    if (!is_float(dtype))
+        return rt::error(PK_GPU_EINVAL, "%s: queries of type %d (F32, F16 or BF16)", who, dtype);
+    if ((cache->dtype == F16 && dtype != F16) || (cache->dtype == BF16 && dtype == F16))
+        return rt::error(PK_GPU_ENOTSUP, "%s: queries of type %d over a cache of type %d (F16 caches take F16, "
+                         "BF16 caches BF16 or F32)", who, dtype, cache->dtype);
+    const long long wide = (long long)heads * cache->head_dim;
+    if (ldq < wide || ldo < wide)
+        return rt::error(PK_GPU_EINVAL, "%s: rows of %lld elements, ldq = %d, ldo = %d", who, wide, ldq, ldo);
+    if (ld_pages < 0 || ((long long)ld_pages << __builtin_ctz(cache->page_size)) < max_len)
+        return rt::error(PK_GPU_EINVAL, "%s: %d pages a sequence do not hold max_len = %d tokens", who, ld_pages,
+                         max_len);
+    if (B && (!dq || !dout || !dlens || (max_len && !dpages)))
+        return rt::error(PK_GPU_EINVAL, "%s: NULL operand", who);
+    const size_t es = size_of(dtype);
+    if (!aligned16(dq) || !aligned16(dout) || (size_t)ldq * es % 16 || (size_t)ldo * es % 16)
+        return rt::error(PK_GPU_EINVAL, "%s: query and output rows must be 16-byte aligned", who);
+    const long long pairs = (long long)B * cache->heads * head_tiles(heads / cache->heads);
+    const Plan p = plan(pairs ? pairs : 1, max_len, window);
+    const size_t need = ws_floats_of(cache, B, heads, p);
+    if (need && (!dws || ws_floats < need || !aligned16(dws)))
+        return rt::error(PK_GPU_EINVAL, "%s: needs a 16-byte aligned workspace of %zu floats "
+                         "(pk_gpu_paged_attention_ws_floats)", who, need);
+    OnDevice on;
+    if (on.rc) return on.rc;
+    if (!B) return PK_GPU_OK;
+    PagedArgs a{};
+    a.k = static_cast<const char*>(cache->k);
+    a.v = static_cast<const char*>(cache->v);
+    a.k_scale = cache->k_scale;
+    a.v_scale = cache->v_scale;
+    a.q = static_cast<const char*>(dq);
+    a.ldq = (size_t)ldq * es;
+    a.pages = dpages;
+    a.ld_pages = ld_pages;
+    a.lens = dlens;
+    a.out = static_cast<char*>(dout);
+    a.ldo = (size_t)ldo * es;
+    a.lse = dlse;
+    a.part = dws;
+    a.ml = dws ? dws + (size_t)B * heads * p.splits * cache->head_dim : nullptr;
+    a.scale2 = scale * 1.4426950408889634f;
+    a.max_len = max_len;
+    a.window = window;
+    a.kv_heads = cache->heads;
+    a.group = heads / cache->heads;
+    a.head_tiles = head_tiles(a.group);
+    a.n_pages = cache->n_pages;
+    a.page_shift = __builtin_ctz(cache->page_size);
+    a.chunk = p.chunk;
+    a.splits = p.splits;
+    const dim3 grid((uint32_t)(pairs * p.splits));
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const int dim = cache->head_dim;
+    hipError_t e = cache->dtype == F16    ? launch_paged_f16(dtype, dim, a, grid, s)
+                   : cache->dtype == BF16 ? launch_paged_bf16(dtype, dim, a, grid, s)
+                   : cache->dtype == I8   ? launch_paged_i8(dtype, dim, a, grid, s)
+                                          : launch_paged_e4m3(dtype, dim, a, grid, s);
+    if (e == hipSuccess && p.splits > 1) {
+        JoinArgs j{};
+        j.part = a.part;
+        j.ml = a.ml;
+        j.lens = dlens;
+        j.out = a.out;
+        j.ldo = a.ldo;
+        j.lse = dlse;
+        j.heads = heads;
+        j.splits = p.splits;
+        j.chunk = p.chunk;
+        j.max_len = max_len;
+        j.window = window;
+        const uint32_t rows = (uint32_t)((long long)B * heads);
+        e = dtype == F32   ? launch_join<F32>(dim, j, rows, s)
+            : dtype == F16 ? launch_join<F16>(dim, j, rows, s)
+                           : launch_join<BF16>(dim, j, rows, s);
+    }
+    return e == hipSuccess ? PK_GPU_OK : rt::hip_error(e, who);
+}
+
+}  // extern "C"

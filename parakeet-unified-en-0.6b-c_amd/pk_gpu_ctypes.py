@@ -91,6 +91,8 @@ _PROTOS = {
     "pk_gpu_encoder_profile_read": (_i, [_p, _i, _p, _p, _p, _p]),
     "pk_gpu_kv_write_dev": (_i, [_p, _i, _p, _i, _p, _i, _p, _i, _p]),
     "pk_gpu_kv_read_dev": (_i, [_p, _i, _p, _i, _p, _i, _p, _i, _p]),
+    "pk_gpu_paged_attention_ws_floats": (_sz, [_p, _i, _i, _i, _i]),
+    "pk_gpu_paged_attention_dev": (_i, [_p, _i, _p, _i, _i, _p, _i, _p, _i, _i, _f, _i, _p, _i, _p, _p, _sz, _p]),
 }
 
 EPI_NONE, EPI_SWISH, EPI_HALF_RESIDUAL, EPI_RESIDUAL, EPI_RELU = 0, 1, 2, 3, 4

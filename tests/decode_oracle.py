@@ -118,6 +118,54 @@ class Cache:
         return x
 
 
+def attention(cache, q, table, lens, max_len, scale, window):
+    """Outputs and log-sums [B][heads][dim], [B][heads] in 64 bits, and per output the sums
+    that its tolerance is made of: a = sum p |v|, s = the largest |score| and x = the
+    largest scale * k_scale * sum |q| |k| of its head."""
+    B, heads, dim = q.shape
+    k, v = cache.rows("k"), cache.rows("v")
+    group = heads // cache.heads
+    out, lse = np.zeros(q.shape), np.full((B, heads), -np.inf)
+    a, s_top, x_top = np.zeros(q.shape), np.zeros((B, heads)), np.zeros((B, heads))
+    for b in range(B):
+        n = min(max(int(lens[b]), 0), max_len)
+        t = np.arange(max(0, n - window) if window else 0, n)
+        page = table[b][t // cache.page] if n else t
+        t = t[(page >= 0) & (page < cache.pages)]
+        if not len(t):
+            continue
+        at = table[b][t // cache.page].astype(np.int64) * cache.page + t % cache.page
+        for h in range(heads):
+            kk, vv = k[at, h // group], v[at, h // group]
+            s = scale * (kk @ q[b, h])
+            m = s.max()
+            p = np.exp(s - m)
+            l = p.sum()
+            out[b, h], lse[b, h] = (p @ vv) / l, m + np.log(l)
+            a[b, h] = (p @ np.abs(vv)) / l
+            s_top[b, h] = np.abs(s).max()
+            x_top[b, h] = abs(scale) * (np.abs(kk) @ np.abs(q[b, h])).max()
+    return out, lse, a, s_top, x_top
+
+
+def attention_bound(want, a, s_top, x_top, n, dim, kind, rows):
+    """What the kernel's roundings add up to at most (first order, worst case), per output.
+
+    Score: dim products and their sum in fp32, one rounding (2^-23, the matrix
+    instructions may cut) each, then two products and the subtraction of m:
+    d = (dim + 8) 2^-23 x + 6 2^-24 s, in the exponent.  It enters a weight and the sum of the
+    weights: 2 d.  exp2: 2 units in the last place, twice.  The weight's rounding
+    for the second product: half a step of what the output's type gets (8, 16 or 24 bits; 11 for
+    F16 caches, and 2^-32 of the maximum below their normal range).  Sums: n / 16 + 64 additions for l,
+    n / 4 + 64 for o, half of the roundings' worst case each 2^-23.  The division and the output's rounding."""
+    half_p = 2.0 ** -11 if kind == "f16" else {"bf16": 2.0 ** -8, "f16": 2.0 ** -16, "f32": 2.0 ** -24}[rows]
+    d = (dim + 8) * 2.0 ** -23 * x_top + 6 * 2.0 ** -24 * s_top
+    rel = 2 * d + 4 * 2.0 ** -23 + half_p + (n / 16 + 64 + n / 4 + 64) * 2.0 ** -23
+    small = n * 2.0 ** -32 if kind == "f16" else 0.0
+    vmax = 8.0 if kind == "f16" else 0.0
+    return rel[..., None] * a * 1.01 + small * vmax + HALF[rows] * np.abs(want) * 1.01 + 2.0 ** -24 * (rows == "f16")
+
+
 def ref(struct):
     return ctypes.byref(struct)
 

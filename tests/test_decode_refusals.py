@@ -23,6 +23,13 @@ def refused(fn, *args, code=-1, text=None):
     assert msg and (text is None or text in msg), msg
 
 
+def attention(code=-1, text=None, **kw):
+    d = dict(c=None, dtype=pk.F32, q=P, ldq=512, heads=4, pages=P, ld_pages=8, lens=P, B=3, max_len=128, scale=1.0,
+             window=0, out=P, ldo=512, lse=None, ws=P, floats=1 << 30)
+    d.update(kw)
+    refused("pk_gpu_paged_attention_dev", *d.values(), None, code=code, text=text)
+
+
 BAD_CACHES = [
     (dict(k=None), -1, "NULL"), (dict(v=None), -1, "NULL"), (dict(k_scale=None), -1, "NULL"),
     (dict(v_scale=None), -1, "NULL"), (dict(k=P + 8), -1, "aligned"), (dict(v_scale=P + 4), -1, "aligned"),
@@ -38,6 +45,8 @@ def test_bad_caches(bad, code, text):
     c = ctypes.byref(cache(**bad))
     refused("pk_gpu_kv_write_dev", c, pk.F32, P, 1 << 30, P, 1 << 30, P, 1, None, code=code, text=text)
     refused("pk_gpu_kv_read_dev", c, pk.F32, P, 1, P, 1 << 30, P, 1 << 30, None, code=code, text=text)
+    attention(c=c, ldq=1 << 30, ldo=1 << 30, heads=1 << 25 if bad.get("heads") else 2, code=code, text=text)
+    assert pk.load().pk_gpu_paged_attention_ws_floats(c, 1, 2, 1000, 0) == 0
 
 
 def test_16_bit_caches_need_no_scales():
@@ -62,3 +71,35 @@ def test_bad_rows(dtype, k, ldk, v, ldv, slots, n, text):
 def test_null_cache():
     refused("pk_gpu_kv_write_dev", None, pk.F32, P, 256, P, 256, P, 1, None, text="NULL cache")
     refused("pk_gpu_kv_read_dev", None, pk.F32, P, 1, P, 256, P, 256, None, text="NULL cache")
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(dtype=pk.I8), -1, "type"), (dict(dtype=7), -1, "type"), (dict(heads=0), -1, "heads"),
+    (dict(heads=3), -1, "heads"), (dict(heads=-2), -1, "heads"), (dict(B=-1), -1, "B ="),
+    (dict(max_len=-1), -1, "max_len"), (dict(max_len=(1 << 30) + 1), -1, "max_len"), (dict(window=-1), -1, "window"),
+    (dict(ldq=511), -1, "ldq"), (dict(ldo=511), -1, "ldo"), (dict(ld_pages=7), -1, "pages"),
+    (dict(ld_pages=-1), -1, "pages"), (dict(q=None), -1, "NULL"), (dict(out=None), -1, "NULL"),
+    (dict(lens=None), -1, "NULL"), (dict(pages=None), -1, "NULL"), (dict(q=P + 8), -1, "aligned"),
+    (dict(out=P + 4), -1, "aligned"), (dict(ldq=513), -1, "aligned"), (dict(ldo=514), -1, "aligned"),
+    (dict(B=1 << 30), -1, "grid"),
+])
+def test_bad_attention(kw, code, text):
+    attention(c=ctypes.byref(cache()), code=code, text=text, **kw)
+
+
+@pytest.mark.parametrize("held,dtype", [(pk.F16, pk.F32), (pk.F16, pk.BF16), (pk.BF16, pk.F16)])
+def test_queries_a_16_bit_cache_does_not_take(held, dtype):
+    attention(c=ctypes.byref(cache(dtype=held)), dtype=dtype, code=-2, text="queries")
+
+
+def test_attention_workspace():
+    c = ctypes.byref(cache())
+    lib = pk.load()
+    need = lib.pk_gpu_paged_attention_ws_floats(c, 3, 4, 1000, 0)
+    assert need > 0 and need % (3 * 4 * 130) == 0
+    for ws, floats in ((None, need), (P, need - 1), (P + 4, need)):
+        attention(c=c, max_len=1000, ld_pages=63, ws=ws, floats=floats, text="workspace")
+    assert lib.pk_gpu_paged_attention_ws_floats(c, 3, 4, 32, 0) == 0         # one chunk
+    assert lib.pk_gpu_paged_attention_ws_floats(c, 0, 4, 1000, 0) == 0
+    assert lib.pk_gpu_paged_attention_ws_floats(c, 3, 3, 1000, 0) == 0       # refused sizes
+    assert lib.pk_gpu_paged_attention_ws_floats(c, 3, 4, 1000, 64) <= need   # a window needs no more
