@@ -495,6 +495,45 @@ int pk_gpu_paged_attention_dev(const pk_gpu_kv_cache *cache, int dtype, const vo
                                int max_len, float scale, int window, void *dout, int ldo,
                                float *dlse, float *dws, size_t ws_floats, void *stream);
 
+/* Root-mean-square norm of `rows` rows of D elements, any D >= 1, with the
+ * residual's addition:
+ *   h   = x + res in fp32, rounded to `dtype`  (res NULL: h = x)
+ *   y   = h * r * gamma,  r = 1 / sqrt(mean(h^2) + eps) in fp64, rounded once
+ *   out = y rounded to out_dtype (F32, F16, BF16), or its codes (I8) with one
+ *         scale a row in dscales, by pk_gpu_kv_write_dev's formula
+ * x, res, sum are of `dtype` (F32, F16 or BF16); sum receives h unless NULL;
+ * gamma NULL counts as ones; dscales is used for I8 only.  Leading dimensions in
+ * elements; what lies between rows is not touched.  sum may be x or res in
+ * place; so may out where its elements are as wide; other overlaps are the
+ * caller's error.  Any alignment of whole elements; rows that are 16-byte aligned
+ * with D a multiple of 8 are the fast ones. */
+int pk_gpu_rms_norm_dev(int dtype, const void *dx, int ldx, const void *dres, int ldr, void *dsum,
+                        int lds, const float *dgamma, float eps, int out_dtype, void *dout, int ldo,
+                        float *dscales, int rows, int D, void *stream);
+
+/* int8 weights for pk_gpu_gemm_w8a8_dev: the panel of dB [K][ldb] (as the
+ * int8 GEMMs take it) in the order the kernels read, made once into the
+ * caller's memory dpanel of pk_gpu_w8_panel_bytes(K, N) bytes (0: refused
+ * sizes), 16-byte aligned.  1 <= K <= 131071 (sums stay within int32), N <=
+ * 2^30. */
+size_t pk_gpu_w8_panel_bytes(int K, int N);
+int pk_gpu_w8_panel_dev(int K, int N, const int8_t *dB, int ldb, void *dpanel, void *stream);
+/* C = epilogue(A * B) for int8 rows with a scale each (pk_gpu_rms_norm_dev's I8
+ * output) and an int8 weight's panel of the same K and N:
+ *   v = fp32(sum_k A[i][k] B[k][j]) * (A_scales[i] * s_j) + bias[j],
+ *   s_j = B_scales[j], or B_scale where B_scales is NULL; bias may be NULL
+ * The sum is exact; then one fp32 rounding per operation, the epilogue, and one to
+ * C's `dtype` (F32, F16 or BF16).  Epilogues are PK_GPU_EPI_*, with the
+ * residual in dres (of C's type; in place where dres is dC with ldr = ldc):
+ *   SWISH v / (1 + e^-v); RELU; RESIDUAL res + v; HALF_RESIDUAL res + 0.5 v
+ * A's rows are 16-byte aligned and take lda bytes each, a multiple of 16, the
+ * last one too (what lies past K may be anything).  C and the residual may have any
+ * leading dimension and alignment of whole elements. */
+int pk_gpu_gemm_w8a8_dev(int M, int N, int K, const int8_t *dA, int lda, const float *dA_scales,
+                         const void *dpanel, float B_scale, const float *dB_scales,
+                         const float *dbias, int epilogue, const void *dres, int ldr, int dtype,
+                         void *dC, int ldc, void *stream);
+
 /* ---- tuning / introspection ------------------------------------------- */
 
 /* Number of kernel tile configurations, and a description of one:

@@ -1,0 +1,306 @@
+// pk_rms_norm.hip - root-mean-square norm with the residual's addition and an
+// output in 8 bits with row scales (pk_gpu_rms_norm_dev).
+//
+//   h = T(x + res)                         stored if asked for
+//   r = fl32(1 / sqrt(mean(h^2) + eps))    squares, mean, root in fp64
+//   y = fl(fl(h r) gamma)                  fp32
+//   out = y rounded to its type, or codes and a scale (pk_decode.h)
+//
+// The norm is of the stored sum, so that what a later layer reads and what was
+// normalised here are the same numbers.  h^2 is exact in fp64 and the sum's
+// error is below 2^-43 for any row, so r does not depend on the order of the
+// additions but once in 2^18 rows or so: codes are reproducible across launch
+// shapes.  The fp64 work is two instructions an element.
+//
+// A row stays in registers between its statistics and its output: TPR threads
+// (a wave, or a workgroup of four) hold CH pieces of W consecutive elements
+// each.  Rows that are not 16-byte aligned (odd D) take W = 1.  Longer rows are
+// read again for each pass.  Bound by the rows' bytes.
+#include "pk_decode.h"
+
+namespace pkgpu {
+namespace decode {
+namespace {
+
+struct NormArgs {
+    const char *x, *res;
+    char* sum;
+    const float* gamma;
+    char* out;
+    float* scales;
+    size_t ldx, ldr, lds, ldo;      // bytes
+    double eps;
+    int rows, D;
+};
+
+constexpr int kNormThreads = 256;
+
+__device__ inline double wave_sum(double v)
+{
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v = v + __shfl_xor(v, d);
+    return v;
+}
+__device__ inline uint32_t wave_max(uint32_t v)
+{
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+        const uint32_t o = __shfl_xor(v, d);
+        v = o > v ? o : v;
+    }
+    return v;
+}
+
+__device__ inline float norm_factor(double sum, int D, double eps)
+{
+    return (float)(1.0 / __dsqrt_rn(sum / (double)D + eps));
+}
+
+template <int T, int W>
+__device__ inline void load_piece(const char* p, size_t i, float* v)
+{
+    if constexpr (W == 8) load8<T>(p + i * size_of(T), v);
+    else v[0] = load1<T>(p, i);
+}
+template <int T, int W>
+__device__ inline void store_piece(char* p, size_t i, const float* v)
+{
+    if constexpr (W == 8) store8<T>(p + i * size_of(T), v);
+    else if constexpr (T == I8) reinterpret_cast<signed char*>(p)[i] = (signed char)(int)__builtin_rintf(v[0]);
+    else store1<T>(p, i, v[0]);
+}
+
+// h of W elements, stored where the caller wants it
+template <int T, int W>
+__device__ inline void load_sum(const NormArgs& a, size_t row, size_t i, float* h)
+{
+    load_piece<T, W>(a.x + row * a.ldx, i, h);
+    if (a.res) {
+        float v[W];
+        load_piece<T, W>(a.res + row * a.ldr, i, v);
+#pragma unroll
+        for (int j = 0; j < W; ++j) h[j] = as_type<T>(__fadd_rn(h[j], v[j]));
+    }
+}
+
+template <int T, int OUT, int TPR, int CH, int W>
+__global__ void __launch_bounds__(kNormThreads) rms_norm(NormArgs a)
+{
+    constexpr int RPB = kNormThreads / TPR;              // rows a workgroup has at a time
+    __shared__ double red_sum[2][4];
+    __shared__ uint32_t red_max[2][4];
+    const int t = threadIdx.x % TPR, wave = threadIdx.x / 64;
+    float gm[CH][W];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int i = (c * TPR + t) * W;
+#pragma unroll
+        for (int j = 0; j < W; ++j) gm[c][j] = a.gamma && i < a.D ? a.gamma[i + j] : 1.0f;
+    }
+    int turn = 0;
+    for (long long r0 = (long long)blockIdx.x * RPB; r0 < a.rows; r0 += (long long)gridDim.x * RPB, turn ^= 1) {
+        const long long row = r0 + threadIdx.x / TPR;
+        const bool live = TPR == kNormThreads || row < a.rows;
+        float h[CH][W];
+        double sum = 0.0;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int i = (c * TPR + t) * W;
+#pragma unroll
+            for (int j = 0; j < W; ++j) h[c][j] = 0.0f;
+            if (live && i < a.D) load_sum<T, W>(a, row, i, h[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int i = (c * TPR + t) * W;
+            if (a.sum && live && i < a.D) store_piece<T, W>(a.sum + row * a.lds, i, h[c]);
+#pragma unroll
+            for (int j = 0; j < W; ++j) sum = __fma_rn((double)h[c][j], (double)h[c][j], sum);
+        }
+        sum = wave_sum(sum);
+        if constexpr (TPR > 64) {
+            if (threadIdx.x % 64 == 0) red_sum[turn][wave] = sum;
+            __syncthreads();
+            sum = (red_sum[turn][0] + red_sum[turn][1]) + (red_sum[turn][2] + red_sum[turn][3]);
+        }
+        const float r = norm_factor(sum, a.D, a.eps);
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                h[c][j] = __fmul_rn(__fmul_rn(h[c][j], r), gm[c][j]);
+                if constexpr (OUT == I8) {
+                    const uint32_t b = __float_as_uint(h[c][j]) & 0x7fffffffu;
+                    if ((c * TPR + t) * W < a.D) top = b > top ? b : top;
+                }
+            }
+        if constexpr (OUT == I8) {
+            top = wave_max(top);
+            if constexpr (TPR > 64) {
+                if (threadIdx.x % 64 == 0) red_max[turn][wave] = top;
+                __syncthreads();
+#pragma unroll
+                for (int w = 0; w < 4; ++w) top = red_max[turn][w] > top ? red_max[turn][w] : top;
+            }
+            const RowCode code = row_code(top, top_of(I8));
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int j = 0; j < W; ++j) h[c][j] = coded(h[c][j], code);
+            if (live && t == 0) a.scales[row] = code.scale;
+        }
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int i = (c * TPR + t) * W;
+            if (live && i < a.D) store_piece<OUT, W>(a.out + row * a.ldo, i, h[c]);
+        }
+    }
+}
+
+// Rows longer than the registers hold, any alignment: each pass reads the row
+// again (from the stored sum, if there is one; each thread its own elements).
+template <int T, int OUT>
+__global__ void __launch_bounds__(1024) rms_norm_long(NormArgs a)
+{
+    __shared__ double red_sum[16];
+    __shared__ uint32_t red_max[16];
+    const int wave = threadIdx.x / 64;
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        double sum = 0.0;
+        for (int i = threadIdx.x; i < a.D; i += 1024) {
+            float h;
+            load_sum<T, 1>(a, row, i, &h);
+            if (a.sum) store1<T>(a.sum + row * a.lds, i, h);
+            sum = __fma_rn((double)h, (double)h, sum);
+        }
+        sum = wave_sum(sum);
+        __syncthreads();                                  // the last row's readers are done
+        if (threadIdx.x % 64 == 0) red_sum[wave] = sum;
+        __syncthreads();
+        sum = 0.0;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) sum = sum + red_sum[w];
+        const float r = norm_factor(sum, a.D, a.eps);
+        auto value = [&](int i) {
+            float h;
+            if (a.sum) h = load1<T>(a.sum + row * a.lds, i);
+            else load_sum<T, 1>(a, row, i, &h);
+            return __fmul_rn(__fmul_rn(h, r), a.gamma ? a.gamma[i] : 1.0f);
+        };
+        RowCode code{};
+        if constexpr (OUT == I8) {
+            uint32_t top = 0;
+            for (int i = threadIdx.x; i < a.D; i += 1024) {
+                const uint32_t b = __float_as_uint(value(i)) & 0x7fffffffu;
+                top = b > top ? b : top;
+            }
+            top = wave_max(top);
+            if (threadIdx.x % 64 == 0) red_max[wave] = top;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < 16; ++w) top = red_max[w] > top ? red_max[w] : top;
+            code = row_code(top, top_of(I8));
+            if (threadIdx.x == 0) a.scales[row] = code.scale;
+        }
+        for (int i = threadIdx.x; i < a.D; i += 1024) {
+            float y = value(i);
+            if constexpr (OUT == I8) y = coded(y, code);
+            store_piece<OUT, 1>(a.out + row * a.ldo, i, &y);
+        }
+    }
+}
+
+// A wave a row while its pieces fit 4 (8 elements each, 1024 single ones) a
+// lane, else a workgroup.
+template <int T, int OUT>
+hipError_t launch_norm(const NormArgs& a, bool wide, hipStream_t s)
+{
+    const auto grid = [&](int rows_each) {
+        const long long n = ((long long)a.rows + rows_each - 1) / rows_each;
+        return dim3((uint32_t)(n < 4096 ? n : 4096));
+    };
+    const dim3 block(kNormThreads);
+    if (wide) {
+        const int pieces = a.D / 8;
+        if (pieces <= 64) return launch(rms_norm<T, OUT, 64, 1, 8>, grid(4), block, 0, s, a);
+        if (pieces <= 128) return launch(rms_norm<T, OUT, 64, 2, 8>, grid(4), block, 0, s, a);
+        if (pieces <= 256) return launch(rms_norm<T, OUT, 64, 4, 8>, grid(4), block, 0, s, a);
+        if (pieces <= 512) return launch(rms_norm<T, OUT, 256, 2, 8>, grid(1), block, 0, s, a);
+        if (pieces <= 1024) return launch(rms_norm<T, OUT, 256, 4, 8>, grid(1), block, 0, s, a);
+    } else {
+        if (a.D <= 512) return launch(rms_norm<T, OUT, 64, 8, 1>, grid(4), block, 0, s, a);
+        if (a.D <= 1024) return launch(rms_norm<T, OUT, 64, 16, 1>, grid(4), block, 0, s, a);
+        if (a.D <= 4096) return launch(rms_norm<T, OUT, 256, 16, 1>, grid(1), block, 0, s, a);
+    }
+    return launch(rms_norm_long<T, OUT>, grid(1), dim3(1024), 0, s, a);
+}
+
+template <int T>
+hipError_t launch_out(int out, const NormArgs& a, bool wide, hipStream_t s)
+{
+    return out == I8    ? launch_norm<T, I8>(a, wide, s)
+           : out == F32 ? launch_norm<T, F32>(a, wide, s)
+           : out == F16 ? launch_norm<T, F16>(a, wide, s)
+                        : launch_norm<T, BF16>(a, wide, s);
+}
+
+}  // namespace
+}  // namespace decode
+}  // namespace pkgpu
+
+extern "C" int pk_gpu_rms_norm_dev(int dtype, const void* dx, int ldx, const void* dres, int ldr, void* dsum,
+                                   int lds, const float* dgamma, float eps, int out_dtype, void* dout, int ldo,
+                                   float* dscales, int rows, int D, void* stream)
+{
+    using namespace pkgpu::decode;
+    namespace rt = pkgpu::rt;
+    const char* who = "rms norm";
+    if (!is_float(dtype)) return rt::error(PK_GPU_EINVAL, "%s: rows of type %d (F32, F16 or BF16)", who, dtype);
+    if (!is_float(out_dtype) && out_dtype != I8)
+        return rt::error(PK_GPU_EINVAL, "%s: output of type %d (F32, F16, BF16 or I8)", who, out_dtype);
+    if (rows < 0 || D < 1) return rt::error(PK_GPU_EINVAL, "%s: rows = %d, D = %d", who, rows, D);
+    if (!(eps >= 0.0f)) return rt::error(PK_GPU_EINVAL, "%s: eps = %g", who, (double)eps);
+    if (ldx < D || ldo < D || (dres && ldr < D) || (dsum && lds < D))
+        return rt::error(PK_GPU_EINVAL, "%s: a leading dimension of %d, %d, %d, %d is below D = %d", who, ldx, ldr,
+                         lds, ldo, D);
+    if (rows && (!dx || !dout || (out_dtype == I8 && !dscales)))
+        return rt::error(PK_GPU_EINVAL, "%s: NULL operand", who);
+    const int es = size_of(dtype), os = size_of(out_dtype);
+    const auto off = [](const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; };
+    if (off(dx, es) || off(dres, es) || off(dsum, es) || off(dout, os) || off(dgamma, 4) || off(dscales, 4))
+        return rt::error(PK_GPU_EINVAL, "%s: an operand is not aligned to its elements", who);
+    // one thread reads and writes an element in place; other overlaps would race
+    if (rows && ((dout == dx && (os != es || ldo != ldx)) || (dout == dres && dres && (os != es || ldo != ldr)) ||
+        (dsum && ((dsum == dx && lds != ldx) || (dsum == dres && lds != ldr) || dsum == dout))))
+        return rt::error(PK_GPU_EINVAL, "%s: out or sum in place needs the input's type and leading dimension, and "
+                         "sum may not be out", who);
+    OnDevice on;
+    if (on.rc) return on.rc;
+    if (!rows) return PK_GPU_OK;
+    NormArgs a{};
+    a.x = static_cast<const char*>(dx);
+    a.res = static_cast<const char*>(dres);
+    a.sum = static_cast<char*>(dsum);
+    a.gamma = dgamma;
+    a.out = static_cast<char*>(dout);
+    a.scales = dscales;
+    a.ldx = (size_t)ldx * es;
+    a.ldr = (size_t)ldr * es;
+    a.lds = (size_t)lds * es;
+    a.ldo = (size_t)ldo * os;
+    a.eps = (double)eps;
+    a.rows = rows;
+    a.D = D;
+    // 8 elements at a time: whole pieces, all of them aligned (codes: 8 bytes)
+    const auto fits = [](const void* p, size_t ld, size_t bytes) {
+        return reinterpret_cast<uintptr_t>(p) % bytes == 0 && ld % bytes == 0;
+    };
+    const bool wide = D % 8 == 0 && fits(dx, a.ldx, 16) && (!dres || fits(dres, a.ldr, 16)) &&
+                      (!dsum || fits(dsum, a.lds, 16)) && fits(dout, a.ldo, out_dtype == I8 ? 8 : 16);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const hipError_t e = dtype == F32   ? launch_out<F32>(out_dtype, a, wide, s)
+                         : dtype == F16 ? launch_out<F16>(out_dtype, a, wide, s)
+                                        : launch_out<BF16>(out_dtype, a, wide, s);
+    return e == hipSuccess ? PK_GPU_OK : rt::hip_error(e, who);
+}

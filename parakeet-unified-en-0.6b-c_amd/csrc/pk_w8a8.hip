@@ -1,0 +1,394 @@
+// pk_w8a8.hip - int8 rows times int8 weights with bias, activation and residual
+// in the epilogue (pk_gpu_gemm_w8a8_dev), for rows that pk_gpu_rms_norm_dev
+// wrote with one scale each.
+//
+//   acc_ij = sum_k a_ik b_kj                     int32, exact (K <= 131071)
+//   v      = fl(fl32(acc) * fl(sa_i sb_j)) (+ bias_j)
+//   C_ij   = epilogue(v), rounded once to C's type
+//
+// v_mfma_i32_16x16x64_i8 with the weights as its first operand: a lane then
+// holds 4 consecutive columns of one row of C.  Both operands want 16
+// consecutive k of one row (column) per lane.  Activations are stored that way;
+// weights [K][N] are not, so a panel holds them re-laid out once, in the order
+// lanes read them: [N / 16][K / 64][lane][16 bytes], zero past N and K (K to a
+// multiple of 128).  A lane's 16 bytes of lane l, block (nb, kb): column
+// 16 nb + l % 16, k from 64 kb + 16 (l / 16).
+//
+// Tiled kernel: a workgroup's tile of A and of the panel goes through LDS in
+// that same fragment order, 128 of K at a time, two stages; every LDS access
+// is 16 bytes a lane at consecutive addresses.  The next stage's global loads
+// are in registers while this stage is multiplied.
+// Few-row kernel (M <= 64): nothing is shared between waves but the sums, so
+// there is no staging: a workgroup takes 16 columns and its waves take every
+// 8th block of K, A straight from the caches, and the waves' int32 sums are
+// added in LDS.  Bound by the weights' bytes and latency.
+#include "pk_decode.h"
+
+namespace pkgpu {
+namespace decode {
+namespace {
+
+struct W8Args {
+    const int8_t* A;
+    const float* sa;
+    const char* panel;
+    const float* sb;                // per column, or null: sb1
+    const float* bias;
+    const char* res;
+    char* C;
+    size_t lda, ldr, ldc;           // bytes
+    float sb1;
+    int M, N, K, kb;                // kb: blocks of 64 of K in the panel
+    int epi;
+    int vec;                        // C and the residual take 4 columns at a time
+    int mt, nt;                     // tiles
+};
+
+__global__ void __launch_bounds__(256) w8_panel(const int8_t* B, int ldb, int K, int N, int kb, u32x4* panel,
+                                                long long blocks)
+{
+    const long long blk = (long long)blockIdx.x * 4 + threadIdx.x / 64;
+    if (blk >= blocks) return;
+    const int lane = threadIdx.x & 63;
+    const long long nb = blk / kb;
+    const long long n = nb * 16 + (lane & 15);
+    const int k0 = (int)(blk - nb * kb) * 64 + 16 * (lane >> 4);
+    u32x4 w = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        uint32_t v = 0;
+        if (n < N && k0 + i < K) v = (uint8_t)B[(size_t)(k0 + i) * ldb + n];
+        w[i / 4] |= v << (8 * (i % 4));
+    }
+    panel[blk * 64 + lane] = w;
+}
+
+__device__ inline i32x4 mfma_i8(u32x4 b, u32x4 a, i32x4 c)
+{
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, b), __builtin_bit_cast(i32x4, a), c,
+                                                 0, 0, 0);
+}
+
+// v / (1 + e^-v), e^-v = 2^t (1 + ln2 t') with t + t' = -v log2(e) to 48 bits:
+// within 3 2^-23 of its value.  (The fp32 GEMMs' Swish follows the reference's
+// polynomial, whose e^-v is off by up to 2.4e-6.)  Below v = -88.73
+// e^-v overflows and the result is -0, off by at most 2^-121.
+__device__ inline float swish(float v)
+{
+    const float x = fminf(fmaxf(-v, -100.0f), 100.0f);
+    const float t = __fmul_rn(x, 0x1.715476p+0f);
+    const float lo = __fmaf_rn(x, 0x1.4ae0cp-26f, __fmaf_rn(x, 0x1.715476p+0f, -t));
+    const float e = __builtin_amdgcn_exp2f(t);
+    return __fdiv_rn(v, __fadd_rn(1.0f, __fmul_rn(e, __fmaf_rn(lo, 0x1.62e43p-1f, 1.0f))));
+}
+
+__device__ inline float finish(float v, float res, int epi)
+{
+    switch (epi) {
+    case PK_GPU_EPI_SWISH: return swish(v);
+    case PK_GPU_EPI_HALF_RESIDUAL: return __fadd_rn(res, __fmul_rn(0.5f, v));
+    case PK_GPU_EPI_RESIDUAL: return __fadd_rn(res, v);
+    case PK_GPU_EPI_RELU: return v > 0.0f ? v : 0.0f;
+    default: return v;
+    }
+}
+
+// 4 sums of row i, columns j .. j + 3, to C
+template <int T>
+__device__ inline void store_c(const W8Args& a, int i, int j, i32x4 acc)
+{
+    if (i >= a.M || j >= a.N) return;
+    const float sa = a.sa[i];
+    const bool residual = a.epi == PK_GPU_EPI_RESIDUAL || a.epi == PK_GPU_EPI_HALF_RESIDUAL;
+    const char* r = a.res + (size_t)i * a.ldr;
+    char* c = a.C + (size_t)i * a.ldc;
+    float v[4], old[4] = {};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int col = j + e < a.N ? j + e : a.N - 1;
+        v[e] = __fmul_rn((float)acc[e], __fmul_rn(sa, a.sb ? a.sb[col] : a.sb1));
+        if (a.bias) v[e] = __fadd_rn(v[e], a.bias[col]);
+    }
+    if (a.vec && j + 4 <= a.N) {
+        if (residual) {
+            if constexpr (T == F32) {
+                const f32x4 o = *reinterpret_cast<const f32x4*>(r + (size_t)j * 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) old[e] = o[e];
+            } else {
+                const u32x2 o = *reinterpret_cast<const u32x2*>(r + (size_t)j * 2);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t w = o[e];       // a bit cast of o[e] itself takes o[0]'s bits
+                    const f16x2 h = __builtin_bit_cast(f16x2, w);
+                    old[2 * e] = T == F16 ? (float)h[0] : bf16_lo(w);
+                    old[2 * e + 1] = T == F16 ? (float)h[1] : bf16_hi(w);
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = finish(v[e], old[e], a.epi);
+        if constexpr (T == F32)
+            *reinterpret_cast<f32x4*>(c + (size_t)j * 4) = (f32x4){v[0], v[1], v[2], v[3]};
+        else
+            *reinterpret_cast<u32x2*>(c + (size_t)j * 2) =
+                T == F16 ? (u32x2){pack_f16(v[0], v[1]), pack_f16(v[2], v[3])}
+                         : (u32x2){pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (j + e < a.N) {
+            if (residual) old[e] = load1<T>(r, j + e);
+            store1<T>(c, j + e, finish(v[e], old[e], a.epi));
+        }
+}
+
+// WM x WN waves of MB x NB blocks of 16 x 16.
+template <int T, int WM, int WN, int MB, int NB>
+__global__ void __launch_bounds__(64 * WM * WN) w8_tiled(W8Args a)
+{
+    constexpr int NW = WM * WN, AB = WM * MB, BB = WN * NB;    // blocks of a tile
+    constexpr int PIECES = 2 * (AB + BB);                      // 1 KB pieces of a stage (128 of K)
+    static_assert(PIECES % NW == 0);
+    constexpr int P = PIECES / NW;                             // pieces a wave loads
+    __shared__ u32x4 lds[2][PIECES][64];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave % WM, wn = wave / WM;
+    const int mt = blockIdx.x % (uint32_t)a.mt, nt = blockIdx.x / (uint32_t)a.mt;
+    const int steps = a.kb / 2;
+
+    // piece q < 2 AB: block q / 2 of A, half q % 2 of the stage; then the panel's
+    const char* src[P];
+    int klim[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const int q = wave * P + i;
+        if (q < 2 * AB) {
+            int m = (mt * AB + q / 2) * 16 + (lane & 15);
+            m = m < a.M ? m : a.M - 1;
+            klim[i] = 64 * (q % 2) + 16 * (lane >> 4);
+            src[i] = reinterpret_cast<const char*>(a.A) + (size_t)m * a.lda;
+        } else {
+            const int nblocks = (a.N + 15) / 16;
+            int nb = nt * BB + (q - 2 * AB) / 2;
+            nb = nb < nblocks ? nb : nblocks - 1;
+            klim[i] = -1;
+            src[i] = a.panel + (((size_t)nb * a.kb + q % 2) * 64 + lane) * 16;
+        }
+    }
+    u32x4 stage[P];
+    auto load = [&](int step) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int q = wave * P + i;
+            if (q < 2 * AB) {
+                // past K the panel is zero: any of the row's bytes will do
+                const int k = klim[i] + 128 * step;
+                stage[i] = *reinterpret_cast<const u32x4*>(src[i] + (k < a.K ? k : 0));
+            } else {
+                stage[i] = *reinterpret_cast<const u32x4*>(src[i] + (size_t)step * 2048);
+            }
+        }
+    };
+    i32x4 acc[MB][NB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[i][j] = (i32x4){0, 0, 0, 0};
+
+    load(0);
+#pragma unroll
+    for (int i = 0; i < P; ++i) lds[0][wave * P + i][lane] = stage[i];
+    __syncthreads();
+    for (int step = 0; step < steps; ++step) {
+        const int cur = step & 1;
+        const bool more = step + 1 < steps;
+        if (more) load(step + 1);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            u32x4 fa[MB], fb[NB];
+#pragma unroll
+            for (int i = 0; i < MB; ++i) fa[i] = lds[cur][2 * (wm * MB + i) + h][lane];
+#pragma unroll
+            for (int j = 0; j < NB; ++j) fb[j] = lds[cur][2 * (AB + wn * NB + j) + h][lane];
+#pragma unroll
+            for (int i = 0; i < MB; ++i)
+#pragma unroll
+                for (int j = 0; j < NB; ++j) acc[i][j] = mfma_i8(fb[j], fa[i], acc[i][j]);
+        }
+        if (more) {
+#pragma unroll
+            for (int i = 0; i < P; ++i) lds[cur ^ 1][wave * P + i][lane] = stage[i];
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+            store_c<T>(a, (mt * AB + wm * MB + i) * 16 + (lane & 15),
+                       (nt * BB + wn * NB + j) * 16 + 4 * (lane >> 4), acc[i][j]);
+}
+
+constexpr int kFewWaves = 8;
+
+// MB blocks of 16 rows, 16 columns a workgroup.
+template <int T, int MB>
+__global__ void __launch_bounds__(64 * kFewWaves) w8_few(W8Args a)
+{
+    __shared__ i32x4 sums[kFewWaves][MB][64];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int nb = blockIdx.x;
+    const char* rows[MB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+        const int m = 16 * i + (lane & 15);
+        rows[i] = reinterpret_cast<const char*>(a.A) + (size_t)(m < a.M ? m : a.M - 1) * a.lda;
+    }
+    const char* w = a.panel + ((size_t)nb * a.kb * 64 + lane) * 16;
+    i32x4 acc[MB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i) acc[i] = (i32x4){0, 0, 0, 0};
+#pragma unroll 4
+    for (int kb = wave; kb < a.kb; kb += kFewWaves) {
+        const u32x4 fb = *reinterpret_cast<const u32x4*>(w + (size_t)kb * 1024);
+        const int k = 64 * kb + 16 * (lane >> 4);
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+            const u32x4 fa = *reinterpret_cast<const u32x4*>(rows[i] + (k < a.K ? k : 0));
+            acc[i] = mfma_i8(fb, fa, acc[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MB; ++i) sums[wave][i][lane] = acc[i];
+    __syncthreads();
+    if (wave >= MB) return;
+    i32x4 sum = sums[0][wave][lane];
+#pragma unroll
+    for (int v = 1; v < kFewWaves; ++v) sum += sums[v][wave][lane];
+    store_c<T>(a, 16 * wave + (lane & 15), 16 * nb + 4 * (lane >> 4), sum);
+}
+
+template <int T, int WM, int WN, int MB, int NB>
+hipError_t launch_tiled(W8Args a, hipStream_t s)
+{
+    constexpr int BM = 16 * WM * MB, BN = 16 * WN * NB;
+    a.mt = (a.M + BM - 1) / BM;
+    a.nt = (a.N + BN - 1) / BN;
+    const long long tiles = (long long)a.mt * a.nt;
+    if (tiles > 0x7fffffff) return hipErrorInvalidValue;
+    return launch(w8_tiled<T, WM, WN, MB, NB>, dim3((uint32_t)tiles), dim3(64 * WM * WN), 0, s, a);
+}
+
+long long tiles_of(const W8Args& a, int bm, int bn)
+{
+    return (long long)((a.M + bm - 1) / bm) * ((a.N + bn - 1) / bn);
+}
+
+template <int T>
+hipError_t launch_w8(const W8Args& a, hipStream_t s)
+{
+    if (a.M <= 64) {
+        const dim3 grid((a.N + 15) / 16), block(64 * kFewWaves);
+        switch ((a.M + 15) / 16) {
+        case 1: return launch(w8_few<T, 1>, grid, block, 0, s, a);
+        case 2: return launch(w8_few<T, 2>, grid, block, 0, s, a);
+        case 3: return launch(w8_few<T, 3>, grid, block, 0, s, a);
+        default: return launch(w8_few<T, 4>, grid, block, 0, s, a);
+        }
+    }
+    // the largest tile of which there are enough for the 256 CUs
+    if (tiles_of(a, 256, 256) >= 200) return launch_tiled<T, 2, 4, 8, 4>(a, s);
+    if (tiles_of(a, 128, 128) >= 200) return launch_tiled<T, 2, 2, 4, 4>(a, s);
+    return launch_tiled<T, 2, 2, 2, 2>(a, s);
+}
+
+}  // namespace
+}  // namespace decode
+}  // namespace pkgpu
+
+extern "C" {
+
+using namespace pkgpu::decode;
+
+size_t pk_gpu_w8_panel_bytes(int K, int N)
+{
+    if (K < 1 || N < 1 || K > 131071 || N > 1 << 30) return 0;
+    return (size_t)((N + 15ll) / 16) * ((K + 127ll) / 128) * 2048;
+}
+
+int pk_gpu_w8_panel_dev(int K, int N, const int8_t* dB, int ldb, void* dpanel, void* stream)
+{
+    namespace rt = pkgpu::rt;
+    const char* who = "w8 panel";
+    if (K < 1 || N < 1 || K > 131071 || N > 1 << 30)
+        return rt::error(PK_GPU_EINVAL, "%s: K = %d (1..131071), N = %d (1..2^30)", who, K, N);
+    if (ldb < N) return rt::error(PK_GPU_EINVAL, "%s: ldb = %d < N = %d", who, ldb, N);
+    if (!dB || !dpanel) return rt::error(PK_GPU_EINVAL, "%s: NULL operand", who);
+    if (!aligned16(dpanel)) return rt::error(PK_GPU_EINVAL, "%s: the panel must be 16-byte aligned", who);
+    const int kb = (K + 127) / 128 * 2;
+    const long long blocks = (N + 15ll) / 16 * kb;
+    if ((blocks + 3) / 4 > 0x7fffffff) return rt::error(PK_GPU_EINVAL, "%s: %d x %d exceeds the grid", who, K, N);
+    OnDevice on;
+    if (on.rc) return on.rc;
+    w8_panel<<<dim3((uint32_t)((blocks + 3) / 4)), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
+        dB, ldb, K, N, kb, static_cast<u32x4*>(dpanel), blocks);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? PK_GPU_OK : rt::hip_error(e, who);
+}
+
+int pk_gpu_gemm_w8a8_dev(int M, int N, int K, const int8_t* dA, int lda, const float* dA_scales,
+                         const void* dpanel, float B_scale, const float* dB_scales, const float* dbias,
+                         int epilogue, const void* dres, int ldr, int dtype, void* dC, int ldc, void* stream)
+{
+    namespace rt = pkgpu::rt;
+    const char* who = "w8a8 gemm";
+    if (M < 0 || N < 0 || M > 1 << 30 || N > 1 << 30 || K < 1 || K > 131071)
+        return rt::error(PK_GPU_EINVAL, "%s: M = %d, N = %d (0..2^30), K = %d (1..131071)", who, M, N, K);
+    if (!is_float(dtype)) return rt::error(PK_GPU_EINVAL, "%s: output of type %d (F32, F16 or BF16)", who, dtype);
+    if (epilogue < PK_GPU_EPI_NONE || epilogue > PK_GPU_EPI_RELU)
+        return rt::error(PK_GPU_EINVAL, "%s: epilogue %d is not one of PK_GPU_EPI_*", who, epilogue);
+    if (lda < K || lda % 16) return rt::error(PK_GPU_EINVAL, "%s: lda = %d (a multiple of 16, at least K = %d)", who, lda, K);
+    const bool residual = epilogue == PK_GPU_EPI_RESIDUAL || epilogue == PK_GPU_EPI_HALF_RESIDUAL;
+    if (ldc < N || (residual && ldr < N))
+        return rt::error(PK_GPU_EINVAL, "%s: ldc = %d, ldr = %d below N = %d", who, ldc, ldr, N);
+    if (M && N && (!dA || !dA_scales || !dpanel || !dC || (residual && !dres)))
+        return rt::error(PK_GPU_EINVAL, "%s: NULL operand", who);
+    if (!aligned16(dA) || !aligned16(dpanel))
+        return rt::error(PK_GPU_EINVAL, "%s: A and the panel must be 16-byte aligned", who);
+    const int es = size_of(dtype);
+    const auto off = [](const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; };
+    if (off(dC, es) || (residual && off(dres, es)) || off(dA_scales, 4) || off(dB_scales, 4) || off(dbias, 4))
+        return rt::error(PK_GPU_EINVAL, "%s: an operand is not aligned to its elements", who);
+    if (residual && dres == dC && ldr != ldc)
+        return rt::error(PK_GPU_EINVAL, "%s: a residual in place needs C's leading dimension", who);
+    OnDevice on;
+    if (on.rc) return on.rc;
+    if (!M || !N) return PK_GPU_OK;
+    W8Args a{};
+    a.A = dA;
+    a.lda = lda;
+    a.sa = dA_scales;
+    a.panel = static_cast<const char*>(dpanel);
+    a.sb = dB_scales;
+    a.sb1 = B_scale;
+    a.bias = dbias;
+    a.res = residual ? static_cast<const char*>(dres) : nullptr;
+    a.ldr = residual ? (size_t)ldr * es : 0;
+    a.C = static_cast<char*>(dC);
+    a.ldc = (size_t)ldc * es;
+    a.M = M; a.N = N; a.K = K;
+    a.kb = (K + 127) / 128 * 2;
+    a.epi = epilogue;
+    const size_t run = 4 * es;
+    a.vec = !off(dC, run) && a.ldc % run == 0 && (!residual || (!off(dres, run) && a.ldr % run == 0));
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const hipError_t e = dtype == F32 ? launch_w8<F32>(a, s) : dtype == F16 ? launch_w8<F16>(a, s) : launch_w8<BF16>(a, s);
+    if (e == hipErrorInvalidValue) return rt::error(PK_GPU_EINVAL, "%s: %d x %d exceeds the grid", who, M, N);
+    return e == hipSuccess ? PK_GPU_OK : rt::hip_error(e, who);
+}
+
+}  // extern "C"

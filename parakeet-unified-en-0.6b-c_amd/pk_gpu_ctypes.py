@@ -91,6 +91,10 @@ _PROTOS = {
     "pk_gpu_encoder_profile_read": (_i, [_p, _i, _p, _p, _p, _p]),
     "pk_gpu_kv_write_dev": (_i, [_p, _i, _p, _i, _p, _i, _p, _i, _p]),
     "pk_gpu_kv_read_dev": (_i, [_p, _i, _p, _i, _p, _i, _p, _i, _p]),
+    "pk_gpu_rms_norm_dev": (_i, [_i, _p, _i, _p, _i, _p, _i, _p, _f, _i, _p, _i, _p, _i, _i, _p]),
+    "pk_gpu_w8_panel_bytes": (_sz, [_i, _i]),
+    "pk_gpu_w8_panel_dev": (_i, [_i, _i, _p, _i, _p, _p]),
+    "pk_gpu_gemm_w8a8_dev": (_i, [_i, _i, _i, _p, _i, _p, _p, _f, _p, _p, _i, _p, _i, _i, _p, _i, _p]),
     "pk_gpu_paged_attention_ws_floats": (_sz, [_p, _i, _i, _i, _i]),
     "pk_gpu_paged_attention_dev": (_i, [_p, _i, _p, _i, _i, _p, _i, _p, _i, _i, _f, _i, _p, _i, _p, _p, _sz, _p]),
 }

@@ -103,3 +103,57 @@ def test_attention_workspace():
     assert lib.pk_gpu_paged_attention_ws_floats(c, 0, 4, 1000, 0) == 0
     assert lib.pk_gpu_paged_attention_ws_floats(c, 3, 3, 1000, 0) == 0       # refused sizes
     assert lib.pk_gpu_paged_attention_ws_floats(c, 3, 4, 1000, 64) <= need   # a window needs no more
+
+
+def norm(code=-1, text=None, **kw):
+    d = dict(dtype=pk.F32, x=P, ldx=64, res=P + 4096, ldr=64, sum=P + 8192, lds=64, gamma=P, eps=1e-5, out_dtype=pk.I8,
+             out=P + 12288, ldo=64, scales=P, rows=2, D=64)
+    d.update(kw)
+    refused("pk_gpu_rms_norm_dev", *d.values(), None, code=code, text=text)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(dtype=pk.I8), "type"), (dict(dtype=-1), "type"), (dict(out_dtype=pk.E4M3), "type"),
+    (dict(out_dtype=12), "type"), (dict(rows=-1), "rows"), (dict(D=0), "D ="), (dict(eps=-1.0), "eps"),
+    (dict(eps=float("nan")), "eps"), (dict(ldx=63), "leading"), (dict(ldr=63), "leading"), (dict(lds=63), "leading"),
+    (dict(ldo=63), "leading"), (dict(x=None), "NULL"), (dict(out=None), "NULL"), (dict(scales=None), "NULL"),
+    (dict(x=P + 2), "aligned"), (dict(res=P + 1), "aligned"), (dict(sum=P + 3), "aligned"),
+    (dict(out=P + 2, out_dtype=pk.F32), "aligned"), (dict(gamma=P + 2), "aligned"), (dict(scales=P + 1), "aligned"),
+    (dict(out=P), "in place"), (dict(out=P, out_dtype=pk.F32, ldo=72), "in place"),
+    (dict(out=P + 4096, out_dtype=pk.F16), "in place"), (dict(sum=P, lds=65), "in place"),
+    (dict(sum=P + 4096, lds=72), "in place"), (dict(sum=P + 12288), "in place"),
+])
+def test_bad_norms(kw, text):
+    norm(text=text, **kw)
+
+
+def gemm(code=-1, text=None, **kw):
+    d = dict(M=4, N=32, K=64, A=P, lda=64, sa=P, panel=P, B_scale=1.0, sb=P, bias=P, epi=pk.EPI_RESIDUAL, res=P, ldr=32,
+             dtype=pk.BF16, C=P, ldc=32)
+    d.update(kw)
+    refused("pk_gpu_gemm_w8a8_dev", *d.values(), None, code=code, text=text)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(M=-1), "M ="), (dict(N=-1), "N ="), (dict(N=(1 << 30) + 1, ldc=(1 << 30) + 1), "N ="), (dict(K=0), "K ="),
+    (dict(K=131072, lda=131072), "K ="), (dict(dtype=pk.I8), "type"), (dict(epi=5), "epilogue"),
+    (dict(epi=-1), "epilogue"), (dict(lda=72), "lda"), (dict(lda=48), "lda"), (dict(ldc=31), "ldc"),
+    (dict(ldr=31), "ldr"), (dict(A=None), "NULL"), (dict(sa=None), "NULL"), (dict(panel=None), "NULL"),
+    (dict(C=None), "NULL"), (dict(res=None), "NULL"), (dict(A=P + 8), "aligned"), (dict(panel=P + 8), "aligned"),
+    (dict(C=P + 1), "aligned"), (dict(res=P + 1), "aligned"), (dict(sa=P + 2), "aligned"), (dict(sb=P + 2), "aligned"),
+    (dict(bias=P + 1), "aligned"), (dict(ldr=40), "in place"),
+])
+def test_bad_products(kw, text):
+    gemm(text=text, **kw)
+
+
+def test_bad_panels():
+    lib = pk.load()
+    assert lib.pk_gpu_w8_panel_bytes(1, 1) == 2048 and lib.pk_gpu_w8_panel_bytes(129, 17) == 2 * 2 * 2048
+    for K, N in ((0, 1), (1, 0), (-1, 5), (131072, 1), (1, (1 << 30) + 1)):
+        assert lib.pk_gpu_w8_panel_bytes(K, N) == 0
+        refused("pk_gpu_w8_panel_dev", K, N, P, max(N, 1), P, None)
+    refused("pk_gpu_w8_panel_dev", 16, 16, P, 15, P, None, text="ldb")
+    refused("pk_gpu_w8_panel_dev", 16, 16, None, 16, P, None, text="NULL")
+    refused("pk_gpu_w8_panel_dev", 16, 16, P, 16, None, None, text="NULL")
+    refused("pk_gpu_w8_panel_dev", 16, 16, P, 16, P + 8, None, text="aligned")
