@@ -481,10 +481,10 @@ int pk_gpu_kv_read_dev(const pk_gpu_kv_cache *cache, int dtype, const int *dslot
  *   lse       NULL, or [B][heads] floats: log of the sum of the exponentials,
  *             what another part of a split softmax is joined with
  * Page entries outside [0, n_pages) are absent: their tokens take no part, and
- * entries from dlens[b] on are not read.  Tokens that take no part may hold
+ * entries from dlens[b] on have no effect.  Tokens that take no part may hold
  * anything, NaN included.  A sequence without tokens gives zeros (lse -inf).
  * Scores, sums and the softmax are fp32; its weights enter the second product
- * with 8, 16 or 24 bits for BF16, F16 and F32 output (11 over F16 caches).
+ * with 16 bits for BF16 and F16 output, 24 for F32 (11 over F16 caches).
  * dws: a 16-byte aligned workspace of at least pk_gpu_paged_attention_ws_floats
  * floats for the same sizes (0: none is needed), free again when the call's
  * work is done; calls that may overlap on the device must not share it. */

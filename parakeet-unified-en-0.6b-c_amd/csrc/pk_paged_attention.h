@@ -27,11 +27,17 @@
 // Arithmetic: int8 and e4m3 codes are exact in bf16, and so are the caches'
 // 16-bit elements in their own type.  Queries enter as sums of bf16 terms (1
 // for bf16, 2 for f16, 3 for f32: all bits), so scores have fp32 accuracy.
-// p v_scale enters the second product in as many bf16 terms as the output's
-// type can show (1, 2, 3): a term's rounding is half a step (2^-8, 2^-16,
-// 2^-24) of each p.  An F16 cache takes f16 queries and p in f16, raised by
-// 2^7 so that a p down to 2^-21 of the running maximum keeps its 11 bits.
+// p v_scale enters the second product in 2 bf16 terms for 16-bit outputs (16
+// bits of it; one term would add as much error as the output's own rounding,
+// and the matrix instructions have the time) and 3 for f32 (24).  An F16 cache
+// takes f16 queries and p in f16, raised by 2^7 so that a p down to 2^-21 of
+// the running maximum keeps its 11 bits.
 // Maxima, sums and outputs are fp32 throughout.
+//
+// Bytes of K and V are the bound, and registers hold what is in flight: 8 waves
+// a workgroup, one or two workgroups a CU, each wave with a tile's keys and
+// values (8 KB of int8 at 128) on the way.  96 sequences of 3000 tokens, 8 heads of 128:
+// 111 us in int8 (5.5 TB/s), 205 us in bf16 (5.75 TB/s).
 //
 // The running maximum m only moves when a score passes it by more than 8
 // (powers of two, where p and its sums lose nothing), so most tiles need no
@@ -45,6 +51,7 @@
 #include "pk_decode.h"
 
 #include <cfloat>
+#include <type_traits>
 
 namespace pkgpu {
 namespace decode {
@@ -63,10 +70,11 @@ struct PagedArgs {
     float* part;                 // [B][heads][splits][dim], then
     float* ml;                   // [B][heads][splits][2]
     float scale2;                // scale * log2(e)
-    int max_len, window;
+    int B, max_len, window;
     int kv_heads, group, head_tiles;
     int n_pages, page_shift;
     int chunk, splits;
+    int longest_first;
 };
 
 // Tokens a sequence's new token sees, from `first` on; chunks start at `base`.
@@ -81,11 +89,42 @@ __device__ __host__ inline Span span_of(int len, int max_len, int window, int ch
     return s;
 }
 
-constexpr int kPagedWaves = 4;
+// Waves of a workgroup, all of one chunk.  8 keep one CU's share of the memory
+// busy by themselves, so that 128 or more pairs need not be split at all; the
+// kernel with most registers (16-bit keys and values of 256, queries in 3
+// terms) runs one wave a SIMD.
+constexpr int waves_of(int cache, int t, int dim) { return cache == BF16 && t == F32 && dim == 256 ? 4 : 8; }
+
+// The sequence with nth sequences before it in order of falling length (ties
+// by index), counted by every workgroup for itself: lens of the launch's up to
+// kSortedMax sequences in LDS, a thread a sequence.
+constexpr int kSortedMax = 256;
+__device__ inline int nth_longest(const PagedArgs& a, int nth, int* lens, int wave)
+{
+    const int i = threadIdx.x;
+    const int quads = (a.B + 3) / 4;
+    int mine = i < a.B ? a.lens[i] : -1;
+    mine = mine < 0 ? (i < a.B ? 0 : -1) : mine > a.max_len ? a.max_len : mine;
+    if (i < 4 * quads) lens[i] = mine;
+    __syncthreads();
+    int rank = 0;
+    if (64 * wave < a.B) {
+        for (int q = 0; q < quads; ++q) {
+            const i32x4 l = reinterpret_cast<const i32x4*>(lens)[q];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) rank += l[j] > mine || (l[j] == mine && 4 * q + j < i);
+        }
+        if (i < a.B && rank == nth) lens[kSortedMax] = i;
+    }
+    __syncthreads();
+    const int b = __builtin_amdgcn_readfirstlane(lens[kSortedMax]);
+    __syncthreads();                           // the array is free again
+    return b;
+}
 
 // Terms of the query and of p: see above.
 constexpr int q_terms(int cache, int t) { return cache == F16 || t == BF16 ? 1 : t == F16 ? 2 : 3; }
-constexpr int p_terms(int cache, int t) { return q_terms(cache, t); }
+constexpr int p_terms(int cache, int t) { return cache == F16 ? 1 : t == F32 ? 3 : 2; }
 
 template <int CACHE>
 __device__ inline f32x4 mfma(u32x4 a, u32x4 b, f32x4 c)
@@ -131,9 +170,10 @@ __device__ inline void split_pair(float x, float y, uint32_t* t)
     }
 }
 
-template <int CACHE, int T, int DIM, int NW>
-__global__ void __launch_bounds__(64 * NW) paged_attention(PagedArgs a)
+template <int CACHE, int T, int DIM>
+__global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, T, DIM) / 4) paged_attention(PagedArgs a)
 {
+    constexpr int NW = waves_of(CACHE, T, DIM);
     constexpr int S = size_of(CACHE);
     constexpr bool CODED = CACHE == I8 || CACHE == E4M3;
     constexpr int KL = DIM * S / 64;           // 16-byte pieces of a key a lane holds
@@ -144,22 +184,41 @@ __global__ void __launch_bounds__(64 * NW) paged_attention(PagedArgs a)
     constexpr int QT = q_terms(CACHE, T), PT = p_terms(CACHE, T);
     constexpr float BIAS = CACHE == F16 ? 7.0f : 0.0f;
 
+    union Shared {
+        int lens[kSortedMax + 4];
+        u32x4 q[STEPS][QT][64];
+        f32x4 buf[NW - 1][E][64];
+    };
+    __shared__ Shared sh;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
 
-    uint32_t x = blockIdx.x;
-    const int split = x % (uint32_t)a.splits;
-    x /= (uint32_t)a.splits;
+    // Workgroups go round the 8 L2s.  Chunks slowest, and the pairs of a chunk
+    // rotated by its index, so that neither a chunk index (the last ones of ragged
+    // sequences are mostly empty) nor a long sequence stays on one of them.
+    const uint32_t pairs = (uint32_t)a.B * a.kv_heads * a.head_tiles;
+    const int split = blockIdx.x / pairs;
+    uint32_t x = (blockIdx.x + split) % pairs;
     const int htile = x % (uint32_t)a.head_tiles;
     x /= (uint32_t)a.head_tiles;
     const int kvh = x % (uint32_t)a.kv_heads;
-    const int b = x / (uint32_t)a.kv_heads;
+    int b = x / (uint32_t)a.kv_heads;
+    if (a.longest_first) b = nth_longest(a, b, sh.lens, wave);
 
-    const Span sp = span_of(a.lens[b], a.max_len, a.window, a.chunk);
-    if (split > 0 && split >= sp.chunks) return;
-    const int begin = sp.base + split * a.chunk;
-    const int end = sp.chunks ? min(sp.len, begin + a.chunk) : begin;
+    const int* const pages = a.pages + (size_t)b * a.ld_pages;
+    const int page_mask = (1 << a.page_shift) - 1;
+    const int len = a.lens[b];
+    // entries of the first two tiles, before the length is here (no window: the
+    // chunk's tokens do not depend on it; table rows hold max_len tokens)
+    int early[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const long long tt = (long long)split * a.chunk + 32 * (wave + i * NW) + 16 * u;
+            early[i][u] = a.window == 0 && tt < a.max_len ? pages[tt >> a.page_shift] : -1;
+        }
 
     const int in_group = htile * 16 + n;
     const bool head_ok = in_group < a.group;
@@ -167,36 +226,36 @@ __global__ void __launch_bounds__(64 * NW) paged_attention(PagedArgs a)
     const int head = kvh * a.group + in_group;
 
     // queries: step c takes elements el(c, i) = i + 8 g + 32 c of a 16-bit cache's
-    // rows, i + 16 g + 8 (c % 2) + 64 (c / 2) of an 8-bit one's
-    u32x4 q[QT][STEPS];
+    // rows, i + 16 g + 8 (c % 2) + 64 (c / 2) of an 8-bit one's; every wave reads
+    // the same ones, in the order they are multiplied, from LDS
+    constexpr int QS = (STEPS + NW - 1) / NW;  // steps a wave stages
+    float qv[QS][8] = {};
 #pragma unroll
-    for (int c = 0; c < STEPS; ++c) {
+    for (int i = 0; i < QS; ++i) {
+        const int c = wave + i * NW;
         const int el = S == 2 ? 32 * c + 8 * g : 64 * (c / 2) + 16 * g + 8 * (c % 2);
-        float v[8] = {};
-        if (head_ok) load8<T>(a.q + (size_t)b * a.ldq + ((size_t)head * DIM + el) * size_of(T), v);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t t[QT];
-            split_pair<CACHE, QT>(v[2 * i], v[2 * i + 1], t);
-#pragma unroll
-            for (int j = 0; j < QT; ++j) q[j][c][i] = t[j];
-        }
+        if (c < STEPS && head_ok)
+            load8<T>(a.q + (size_t)b * a.ldq + ((size_t)head * DIM + el) * size_of(T), qv[i]);
     }
 
-    const int* const pages = a.pages + (size_t)b * a.ld_pages;
-    const int page_mask = (1 << a.page_shift) - 1;
+    const Span sp = span_of(len, a.max_len, a.window, a.chunk);
+    if (split > 0 && split >= sp.chunks) return;
+    const int begin = sp.base + split * a.chunk;
+    const int end = sp.chunks ? min(sp.len, begin + a.chunk) : begin;
 
     // the two 16-token halves of the tile at token t: first cache row, presence
     struct Halves { size_t row[2]; bool ok[2]; };
+    auto half = [&](Halves& h, int u, int tt, int id) {
+        id = __builtin_amdgcn_readfirstlane(tt < end ? id : -1);     // the wave's: rows' addresses stay scalar
+        h.ok[u] = (uint32_t)id < (uint32_t)a.n_pages;
+        h.row[u] = (((size_t)(h.ok[u] ? id : 0) * a.kv_heads + kvh) << a.page_shift) + (tt & page_mask);
+    };
     auto halves = [&](int t) {
         Halves h;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int tt = t + 16 * u;
-            int id = -1;
-            if (tt < end) id = pages[tt >> a.page_shift];
-            h.ok[u] = (uint32_t)id < (uint32_t)a.n_pages;
-            h.row[u] = (((size_t)(h.ok[u] ? id : 0) * a.kv_heads + kvh) << a.page_shift) + (tt & page_mask);
+            half(h, u, tt, tt < end ? pages[tt >> a.page_shift] : -1);
         }
         return h;
     };
@@ -204,36 +263,43 @@ __global__ void __launch_bounds__(64 * NW) paged_attention(PagedArgs a)
     u32x4 kr[2][KL];
     uint32_t vr[2][4][VW];
     f32x4 ks[2], vs[2];
+    // scalar base + this lane's offset + a constant
+    const uint32_t k_off = n * (DIM * S) + 16 * g;
+    const uint32_t v_off = 4 * g * (DIM * S) + n * (VB > 16 ? 16 : VB);
+    const uint32_t s_off = 16 * g;
     auto load_k = [&](const Halves& h) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const char* p = a.k + (h.row[u] + n) * (DIM * S) + 16 * g;
+            const char* base = a.k + h.row[u] * (DIM * S);
 #pragma unroll
-            for (int j = 0; j < KL; ++j) kr[u][j] = *reinterpret_cast<const u32x4*>(p + 64 * j);
-            if constexpr (CODED) ks[u] = *reinterpret_cast<const f32x4*>(a.k_scale + h.row[u] + 4 * g);
+            for (int j = 0; j < KL; ++j) kr[u][j] = *reinterpret_cast<const u32x4*>(base + k_off + 64 * j);
+            if constexpr (CODED)
+                ks[u] = *reinterpret_cast<const f32x4*>(reinterpret_cast<const char*>(a.k_scale + h.row[u]) + s_off);
         }
     };
     auto load_v = [&](const Halves& h) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
+            const char* base = a.v + h.row[u] * (DIM * S);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const char* p = a.v + (h.row[u] + 4 * g + i) * (DIM * S);
+                const char* p = base + v_off + i * (DIM * S);
                 if constexpr (VB == 4) {
-                    vr[u][i][0] = *reinterpret_cast<const uint32_t*>(p + 4 * n);
+                    vr[u][i][0] = *reinterpret_cast<const uint32_t*>(p);
                 } else if constexpr (VB == 8) {
-                    const u32x2 w = *reinterpret_cast<const u32x2*>(p + 8 * n);
+                    const u32x2 w = *reinterpret_cast<const u32x2*>(p);
                     vr[u][i][0] = w[0]; vr[u][i][1] = w[1];
                 } else {
 #pragma unroll
                     for (int j = 0; j < VB / 16; ++j) {
-                        const u32x4 w = *reinterpret_cast<const u32x4*>(p + 16 * n + 256 * j);
+                        const u32x4 w = *reinterpret_cast<const u32x4*>(p + 256 * j);
 #pragma unroll
                         for (int d = 0; d < 4; ++d) vr[u][i][4 * j + d] = w[d];
                     }
                 }
             }
-            if constexpr (CODED) vs[u] = *reinterpret_cast<const f32x4*>(a.v_scale + h.row[u] + 4 * g);
+            if constexpr (CODED)
+                vs[u] = *reinterpret_cast<const f32x4*>(reinterpret_cast<const char*>(a.v_scale + h.row[u]) + s_off);
         }
     };
 
@@ -245,23 +311,52 @@ __global__ void __launch_bounds__(64 * NW) paged_attention(PagedArgs a)
     int t = begin + 32 * wave;
     Halves cur{}, next{};
     if (t < end) {
-        cur = halves(t);
+        if (a.window == 0) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                half(cur, u, t + 16 * u, early[0][u]);
+                half(next, u, t + 32 * NW + 16 * u, early[1][u]);
+            }
+        } else {
+            cur = halves(t);
+            next = halves(t + 32 * NW);
+        }
         load_k(cur);
         load_v(cur);
-        next = halves(t + 32 * NW);
     }
-    while (t < end) {
-        const int tn = t + 32 * NW;
-        const bool more = tn < end;
-        const Halves after = halves(tn + 32 * NW);
+#pragma unroll
+    for (int i = 0; i < QS; ++i) {
+        const int c = wave + i * NW;
+        if (c >= STEPS) break;
+        u32x4 f[QT];
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            uint32_t w[QT];
+            split_pair<CACHE, QT>(qv[i][2 * d], qv[i][2 * d + 1], w);
+#pragma unroll
+            for (int j = 0; j < QT; ++j) f[j][d] = w[j];
+        }
+#pragma unroll
+        for (int j = 0; j < QT; ++j) sh.q[c][j][lane] = f[j];
+    }
+    __syncthreads();
+    // One tile.  The last one of a wave is a copy of its own without loads: loads
+    // on a condition would have every wait for this tile's values wait for the
+    // next one's keys too.
+    auto tile = [&](auto last) {
+        constexpr bool MORE = !decltype(last)::value;
+        Halves after{};
+        if constexpr (MORE) after = halves(t + 64 * NW);
 
         // scores
-        f32x4 s[2];
+        f32x4 s[2] = {(f32x4){0.0f, 0.0f, 0.0f, 0.0f}, (f32x4){0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            s[u] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        for (int c = 0; c < STEPS; ++c) {
+            u32x4 qf[QT];
 #pragma unroll
-            for (int c = 0; c < STEPS; ++c) {
+            for (int j = 0; j < QT; ++j) qf[j] = sh.q[c][j][lane];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
                 u32x4 f;
                 if constexpr (CODED) {
                     const u32x2 lo = codes_bf16<CACHE>(kr[u][c / 2][2 * (c % 2)]);
@@ -271,13 +366,15 @@ __global__ void __launch_bounds__(64 * NW) paged_attention(PagedArgs a)
                     f = kr[u][c];
                 }
 #pragma unroll
-                for (int j = QT - 1; j >= 0; --j) s[u] = mfma<CACHE>(f, q[j][c], s[u]);
+                for (int j = QT - 1; j >= 0; --j) s[u] = mfma<CACHE>(f, qf[j], s[u]);
             }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 s[u][r] = __fmul_rn(s[u][r], CODED ? __fmul_rn(ks[u][r], a.scale2) : a.scale2);
-        }
-        if (more) load_k(next);
+        if constexpr (MORE) load_k(next);
 
         const bool whole = t >= sp.first && t + 32 <= end && cur.ok[0] && cur.ok[1];
         if (!whole) {
@@ -373,19 +470,22 @@ __global__ void __launch_bounds__(64 * NW) paged_attention(PagedArgs a)
                 }
             }
         }
-        if (more) load_v(next);
+        if constexpr (MORE) load_v(next);
         cur = next;
         next = after;
-        t = tn;
+        t += 32 * NW;
+    };
+    if (t < end) {
+        while (t + 32 * NW < end) tile(std::false_type{});
+        tile(std::true_type{});
     }
 
     // join the waves: the same registers of the same lanes, in wave order
     l = __fadd_rn(l, __shfl_xor(l, 16));
     l = __fadd_rn(l, __shfl_xor(l, 32));
     __shared__ float ml[NW][2][16];
-    __shared__ f32x4 buf[NW - 1][E][64];
     if (g == 0) { ml[wave][0][n] = m; ml[wave][1][n] = l; }
-    __syncthreads();
+    __syncthreads();                           // and nobody reads queries any more
     float mx = ml[0][0][n];
 #pragma unroll
     for (int w = 1; w < NW; ++w) mx = fmaxf(mx, ml[w][0][n]);
@@ -394,7 +494,7 @@ __global__ void __launch_bounds__(64 * NW) paged_attention(PagedArgs a)
     for (int e = 0; e < E; ++e) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) acc[e][r] = __fmul_rn(acc[e][r], f);
-        if (wave > 0) buf[wave - 1][e][lane] = acc[e];
+        if (wave > 0) sh.buf[wave - 1][e][lane] = acc[e];
     }
     __syncthreads();
     if (wave > 0) return;
@@ -402,11 +502,11 @@ __global__ void __launch_bounds__(64 * NW) paged_attention(PagedArgs a)
 #pragma unroll
     for (int w = 0; w < NW; ++w)
         lt = __fadd_rn(lt, __fmul_rn(ml[w][1][n], __builtin_amdgcn_exp2f(ml[w][0][n] - mx)));
-#pragma unroll
+#pragma unroll 1                   // the loop above, not this one, sets the registers
     for (int w = 0; w < NW - 1; ++w)
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const f32x4 o = buf[w][e][lane];
+            const f32x4 o = sh.buf[w][e][lane];
 #pragma unroll
             for (int r = 0; r < 4; ++r) acc[e][r] = __fadd_rn(acc[e][r], o[r]);
         }
@@ -467,11 +567,10 @@ hipError_t launch_paged_e4m3(int t, int dim, const PagedArgs& a, dim3 grid, hipS
 template <int CACHE, int T>
 hipError_t launch_paged(int dim, const PagedArgs& a, dim3 grid, hipStream_t s)
 {
-    constexpr int NW = kPagedWaves;
-    const dim3 block(64 * NW);
-    return dim == 64    ? launch(paged_attention<CACHE, T, 64, NW>, grid, block, 0, s, a)
-           : dim == 128 ? launch(paged_attention<CACHE, T, 128, NW>, grid, block, 0, s, a)
-                        : launch(paged_attention<CACHE, T, 256, NW>, grid, block, 0, s, a);
+    const dim3 block(64 * waves_of(CACHE, T, dim));
+    return dim == 64    ? launch(paged_attention<CACHE, T, 64>, grid, block, 0, s, a)
+           : dim == 128 ? launch(paged_attention<CACHE, T, 128>, grid, block, 0, s, a)
+                        : launch(paged_attention<CACHE, T, 256>, grid, block, 0, s, a);
 }
 
 }  // namespace decode

@@ -19,22 +19,32 @@ struct JoinArgs {
 
 // One workgroup joins the chunks of one head: out = sum_c 2^(m_c - m) o_c /
 // sum_c 2^(m_c - m) l_c.  DIM / 4 lanes cover the head, the other lanes take
-// every PARTS-th chunk; sums run in a fixed order.
+// every PARTS-th chunk; sums run in a fixed order.  All that it reads first,
+// the length, the chunks' (m, l) and EARLY chunks' outputs of a thread, is asked
+// for at once: the workspace holds them whether the sequence has them or not.
 template <int T, int DIM>
 __global__ void __launch_bounds__(256) paged_join(JoinArgs a)
 {
-    constexpr int LANES = DIM / 4, PARTS = 256 / LANES;
+    constexpr int LANES = DIM / 4, PARTS = 256 / LANES, EARLY = 4;
     __shared__ float red[2][4];
     __shared__ float wgt[kMaxSplits];
     __shared__ f32x4 sum[PARTS][LANES];
     const int b = blockIdx.x / (uint32_t)a.heads, head = blockIdx.x % (uint32_t)a.heads;
-    const int chunks = span_of(a.lens[b], a.max_len, a.window, a.chunk).chunks;
-    if (chunks <= 1) return;                        // written by the first launch
     const size_t row = (size_t)b * a.heads + head;
     const int i = threadIdx.x, lane = i & 63, wave = i >> 6;
+    const int part = i / LANES, d4 = i % LANES;
+    const int len = a.lens[b];
     const float* ml = a.ml + row * a.splits * 2;
     float m = -FLT_MAX, l = 0.0f;
-    if (i < chunks) { m = ml[2 * i]; l = ml[2 * i + 1]; }
+    if (i < a.splits) { m = ml[2 * i]; l = ml[2 * i + 1]; }
+    const float* src = a.part + row * a.splits * DIM + 4 * d4;
+    f32x4 v[EARLY];
+#pragma unroll
+    for (int e = 0; e < EARLY; ++e)
+        if (part + e * PARTS < a.splits) v[e] = *reinterpret_cast<const f32x4*>(src + (size_t)(part + e * PARTS) * DIM);
+    const int chunks = span_of(len, a.max_len, a.window, a.chunk).chunks;
+    if (chunks <= 1) return;                        // written by the first launch
+    if (i >= chunks) { m = -FLT_MAX; l = 0.0f; }
     float mx = m;
 #pragma unroll
     for (int d = 32; d; d >>= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
@@ -49,14 +59,19 @@ __global__ void __launch_bounds__(256) paged_join(JoinArgs a)
     if (lane == 0) red[1][wave] = lt;
     __syncthreads();
     lt = __fadd_rn(__fadd_rn(red[1][0], red[1][1]), __fadd_rn(red[1][2], red[1][3]));
-    const int part = i / LANES, d4 = i % LANES;
     f32x4 o = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-    const float* src = a.part + row * a.splits * DIM + 4 * d4;
-#pragma unroll 4
-    for (int c = part; c < chunks; c += PARTS) {
-        const f32x4 v = *reinterpret_cast<const f32x4*>(src + (size_t)c * DIM);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[r] = __fmaf_rn(v[r], wgt[c], o[r]);
+    for (int e = 0; e < EARLY; ++e) {
+        const int c = part + e * PARTS;
+        if (c < chunks)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = __fmaf_rn(v[e][r], wgt[c], o[r]);
+    }
+#pragma unroll 4
+    for (int c = part + EARLY * PARTS; c < chunks; c += PARTS) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(src + (size_t)c * DIM);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = __fmaf_rn(x[r], wgt[c], o[r]);
     }
     sum[part][d4] = o;
     __syncthreads();
@@ -86,27 +101,41 @@ hipError_t launch_join(int dim, const JoinArgs& a, uint32_t rows, hipStream_t s)
                         : launch(paged_join<T, 256>, dim3(rows), dim3(256), 0, s, a);
 }
 
+// 16 query heads of a key-value head a workgroup.
+int head_tiles(int group) { return (group + 15) / 16; }
+
 struct Plan { int chunk, splits; };
 
-// Tokens per workgroup.  A round of its waves is kPagedWaves tiles of 32
-// tokens; chunks are whole rounds.  Few (sequence, head) pairs: as many chunks
-// as fill the chip; many: chunks short enough that ragged sequences even out.
-Plan plan(long long pairs, int max_len, int window)
+// Chunks of a sequence, in rounds of 256 tokens (8 waves' tiles).  Up to 3
+// rounds one workgroup takes the whole: a round costs about 2 us, the second
+// launch that joins chunks 4 to 5 us.  Longer ones are cut until there is a
+// workgroup for each of the 256 CUs, and up to two where chunks keep 384 KB of
+// cache.  Measured (us; one chunk, 256, 512 workgroups):
+//   1 sequence of 100003 tokens, 8 heads of 128 in bf16     1059, 76, 78
+//   4 ragged ones up to 30000, 2 heads of 256 in bf16        615, 36, 29
+//   8 ragged ones up to 4000, 8 heads of 128 in int8           34, 16, 19.5
+//   32 ragged ones up to 2000, the same (256 unsplit)           22, 22, 27
+//   160 windows of 1024 over a head of 256 (160 unsplit)       21, 21, 30
+Plan plan(const pk_gpu_kv_cache* c, int B, int heads, int max_len, int window)
 {
-    const int round = 32 * kPagedWaves;
+    const long long pairs = (long long)(B > 0 ? B : 1) * c->heads * head_tiles(heads / c->heads);
+    const int round = 256;
     long long span = window > 0 && window < max_len ? (long long)window + 31 : max_len;
     if (span < 1) span = 1;
     const long long rounds = (span + round - 1) / round;
-    long long splits = (2048 + pairs - 1) / pairs;
+    const long long bytes = span * 2 * c->head_dim * size_of(c->dtype);
+    long long splits = 1;
+    if (rounds > 3) {
+        const long long fill = 256 / pairs, two = 512 / pairs, large = bytes / (384 << 10);
+        splits = two < large ? two : large;
+        if (splits < fill) splits = fill;
+    }
     if (splits > rounds) splits = rounds;
     if (splits > kMaxSplits) splits = kMaxSplits;
     if (splits < 1) splits = 1;
     const long long chunk = (rounds + splits - 1) / splits * round;
     return {(int)chunk, (int)((span + chunk - 1) / chunk)};
 }
-
-// 16 query heads of a key-value head a workgroup.
-int head_tiles(int group) { return (group + 15) / 16; }
 
 int check_attention(const pk_gpu_kv_cache* c, int B, int heads, int max_len, int window)
 {
@@ -119,7 +148,7 @@ int check_attention(const pk_gpu_kv_cache* c, int B, int heads, int max_len, int
         return rt::error(PK_GPU_EINVAL, "%s: max_len = %d is above 2^30", who, max_len);
     if (heads < 1 || heads % c->heads)
         return rt::error(PK_GPU_EINVAL, "%s: %d query heads over %d key-value heads", who, heads, c->heads);
-    const Plan p = plan((long long)(B ? B : 1) * c->heads * head_tiles(heads / c->heads), max_len, window);
+    const Plan p = plan(c, B, heads, max_len, window);
     if ((long long)B * c->heads * head_tiles(heads / c->heads) * p.splits > 0x7fffffff ||
         (long long)B * heads > 0x7fffffff)
         return rt::error(PK_GPU_EINVAL, "%s: %d sequences of %d heads exceed the grid", who, B, heads);
@@ -142,8 +171,7 @@ using namespace pkgpu::decode;
 size_t pk_gpu_paged_attention_ws_floats(const pk_gpu_kv_cache* cache, int B, int heads, int max_len, int window)
 {
     if (check_attention(cache, B, heads, max_len, window) != PK_GPU_OK || B == 0) return 0;
-    return ws_floats_of(cache, B, heads,
-                        plan((long long)B * cache->heads * head_tiles(heads / cache->heads), max_len, window));
+    return ws_floats_of(cache, B, heads, plan(cache, B, heads, max_len, window));
 }
 
 int pk_gpu_paged_attention_dev(const pk_gpu_kv_cache* cache, int dtype, const void* dq, int ldq, int heads,
@@ -172,7 +200,7 @@ int pk_gpu_paged_attention_dev(const pk_gpu_kv_cache* cache, int dtype, const vo
     if (!aligned16(dq) || !aligned16(dout) || (size_t)ldq * es % 16 || (size_t)ldo * es % 16)
         return rt::error(PK_GPU_EINVAL, "%s: query and output rows must be 16-byte aligned", who);
     const long long pairs = (long long)B * cache->heads * head_tiles(heads / cache->heads);
-    const Plan p = plan(pairs ? pairs : 1, max_len, window);
+    const Plan p = plan(cache, B, heads, max_len, window);
     const size_t need = ws_floats_of(cache, B, heads, p);
     if (need && (!dws || ws_floats < need || !aligned16(dws)))
         return rt::error(PK_GPU_EINVAL, "%s: needs a 16-byte aligned workspace of %zu floats "
@@ -196,6 +224,7 @@ int pk_gpu_paged_attention_dev(const pk_gpu_kv_cache* cache, int dtype, const vo
     a.part = dws;
     a.ml = dws ? dws + (size_t)B * heads * p.splits * cache->head_dim : nullptr;
     a.scale2 = scale * 1.4426950408889634f;
+    a.B = B;
     a.max_len = max_len;
     a.window = window;
     a.kv_heads = cache->heads;
@@ -205,6 +234,12 @@ int pk_gpu_paged_attention_dev(const pk_gpu_kv_cache* cache, int dtype, const vo
     a.page_shift = __builtin_ctz(cache->page_size);
     a.chunk = p.chunk;
     a.splits = p.splits;
+    // Where there are more workgroups than the 512 that run at a time, the longest
+    // sequences go first: 96 ragged sequences of up to 6000 tokens and 8 heads 122
+    // us against 139 in order, the same number of equal ones 114 against 111; of
+    // short sequences the counting costs more (256 of up to 1000: 87 against 67).
+    a.longest_first = B > 1 && B <= kSortedMax && pairs * p.splits > 512 && max_len / 16 >= B &&
+                      (window == 0 || window / 16 >= B);
     const dim3 grid((uint32_t)(pairs * p.splits));
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int dim = cache->head_dim;

@@ -155,10 +155,10 @@ def attention_bound(want, a, s_top, x_top, n, dim, kind, rows):
     instructions may cut) each, then two products and the subtraction of m:
     d = (dim + 8) 2^-23 x + 6 2^-24 s, in the exponent.  It enters a weight and the sum of the
     weights: 2 d.  exp2: 2 units in the last place, twice.  The weight's rounding
-    for the second product: half a step of what the output's type gets (8, 16 or 24 bits; 11 for
+    for the second product: half a step of what the output's type gets (16 or 24 bits; 11 for
     F16 caches, and 2^-32 of the maximum below their normal range).  Sums: n / 16 + 64 additions for l,
     n / 4 + 64 for o, half of the roundings' worst case each 2^-23.  The division and the output's rounding."""
-    half_p = 2.0 ** -11 if kind == "f16" else {"bf16": 2.0 ** -8, "f16": 2.0 ** -16, "f32": 2.0 ** -24}[rows]
+    half_p = 2.0 ** -11 if kind == "f16" else {"bf16": 2.0 ** -16, "f16": 2.0 ** -16, "f32": 2.0 ** -24}[rows]
     d = (dim + 8) * 2.0 ** -23 * x_top + 6 * 2.0 ** -24 * s_top
     rel = 2 * d + 4 * 2.0 ** -23 + half_p + (n / 16 + 64 + n / 4 + 64) * 2.0 ** -23
     small = n * 2.0 ** -32 if kind == "f16" else 0.0

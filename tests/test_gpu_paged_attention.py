@@ -73,7 +73,7 @@ class Call:
             ltol = d + (n / 16 + 72) * 2.0 ** -23 + 4 * 2.0 ** -24 * np.where(np.isfinite(lse), np.abs(lse), 0)
             none = np.isneginf(lse)
             assert np.array_equal(np.isneginf(got), none)
-            assert np.all(np.abs(got - lse)[~none] <= ltol[~none])
+            assert np.all(np.abs(got[~none] - lse[~none]) <= ltol[~none])
 
 
 def queries(rng, B, heads, dim, rows):
@@ -122,6 +122,21 @@ def test_many_sequences_one_launch():
     table = tables(rng, cache, B, (most + page - 1) // page)
     q = queries(rng, B, kv, dim, "bf16")
     Call(cache, q, "bf16", table, lens, most, 0.125, 0, lse=False).check(q, table, lens)
+
+
+@pytest.mark.parametrize("window", [0, 1130])
+def test_longest_first(window):
+    """More workgroups than run at a time: sequences in order of length, many of them equal,
+    lengths out of range among them."""
+    rng = np.random.default_rng(19)
+    B, kv, dim, page, most = 67, 8, 64, 16, 1200
+    cache = do.Cache("e4m3", 500, kv, page, dim, seed=2)
+    lens = rng.integers(0, most + 1, B)
+    lens[10:30] = 640
+    lens[3], lens[5], lens[66] = -4, 1 << 30, most
+    table = tables(rng, cache, B, (most + page - 1) // page)
+    q = queries(rng, B, kv, dim, "f16")
+    Call(cache, q, "f16", table, lens, most, 0.125, window).check(q, table, np.clip(lens, 0, most))
 
 
 def test_more_pairs_than_chunks():
