@@ -526,7 +526,7 @@ int pk_gpu_w8_panel_dev(int K, int N, const int8_t *dB, int ldb, void *dpanel, v
  * C's `dtype` (F32, F16 or BF16).  Epilogues are PK_GPU_EPI_*, with the
  * residual in dres (of C's type; in place where dres is dC with ldr = ldc):
  *   SWISH v / (1 + e^-v); RELU; RESIDUAL res + v; HALF_RESIDUAL res + 0.5 v
- * A's rows are 16-byte aligned and take lda bytes each, a multiple of 16, the
+ * A's rows are 16-byte aligned and take lda bytes each, a multiple of 16 up to 2^27, the
  * last one too (what lies past K may be anything).  C and the residual may have any
  * leading dimension and alignment of whole elements. */
 int pk_gpu_gemm_w8a8_dev(int M, int N, int K, const int8_t *dA, int lda, const float *dA_scales,

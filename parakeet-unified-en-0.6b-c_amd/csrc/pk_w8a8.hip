@@ -82,35 +82,61 @@ __device__ inline float swish(float v)
     return __fdiv_rn(v, __fadd_rn(1.0f, __fmul_rn(e, __fmaf_rn(lo, 0x1.62e43p-1f, 1.0f))));
 }
 
-__device__ inline float finish(float v, float res, int epi)
+template <int EPI>
+__device__ inline float finish(float v, float res)
 {
-    switch (epi) {
-    case PK_GPU_EPI_SWISH: return swish(v);
-    case PK_GPU_EPI_HALF_RESIDUAL: return __fadd_rn(res, __fmul_rn(0.5f, v));
-    case PK_GPU_EPI_RESIDUAL: return __fadd_rn(res, v);
-    case PK_GPU_EPI_RELU: return v > 0.0f ? v : 0.0f;
-    default: return v;
-    }
+    if constexpr (EPI == PK_GPU_EPI_SWISH) return swish(v);
+    else if constexpr (EPI == PK_GPU_EPI_HALF_RESIDUAL) return __fadd_rn(res, __fmul_rn(0.5f, v));
+    else if constexpr (EPI == PK_GPU_EPI_RESIDUAL) return __fadd_rn(res, v);
+    else if constexpr (EPI == PK_GPU_EPI_RELU) return v > 0.0f ? v : 0.0f;
+    else return v;
 }
 
-// 4 sums of row i, columns j .. j + 3, to C
-template <int T>
-__device__ inline void store_c(const W8Args& a, int i, int j, i32x4 acc)
+// What the 4 columns from j on are multiplied with and biased by.
+struct Columns { float s[4], b[4]; };
+__device__ inline Columns columns_of(const W8Args& a, int j)
+{
+    Columns c;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { c.s[e] = a.sb1; c.b[e] = 0.0f; }
+    if (a.vec && j + 4 <= a.N) {
+        if (a.sb) {
+            const f32x4 s = *reinterpret_cast<const f32x4*>(a.sb + j);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c.s[e] = s[e];
+        }
+        if (a.bias) {
+            const f32x4 b = *reinterpret_cast<const f32x4*>(a.bias + j);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c.b[e] = b[e];
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (j + e < a.N) {
+                if (a.sb) c.s[e] = a.sb[j + e];
+                if (a.bias) c.b[e] = a.bias[j + e];
+            }
+    }
+    return c;
+}
+
+// 4 sums of row i (scale sa), columns j .. j + 3, to C
+template <int T, int EPI>
+__device__ inline void store_c(const W8Args& a, int i, float sa, int j, const Columns& col, i32x4 acc)
 {
     if (i >= a.M || j >= a.N) return;
-    const float sa = a.sa[i];
-    const bool residual = a.epi == PK_GPU_EPI_RESIDUAL || a.epi == PK_GPU_EPI_HALF_RESIDUAL;
+    constexpr bool residual = EPI == PK_GPU_EPI_RESIDUAL || EPI == PK_GPU_EPI_HALF_RESIDUAL;
     const char* r = a.res + (size_t)i * a.ldr;
     char* c = a.C + (size_t)i * a.ldc;
     float v[4], old[4] = {};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const int col = j + e < a.N ? j + e : a.N - 1;
-        v[e] = __fmul_rn((float)acc[e], __fmul_rn(sa, a.sb ? a.sb[col] : a.sb1));
-        if (a.bias) v[e] = __fadd_rn(v[e], a.bias[col]);
+        v[e] = __fmul_rn((float)acc[e], __fmul_rn(sa, col.s[e]));
+        if (a.bias) v[e] = __fadd_rn(v[e], col.b[e]);
     }
     if (a.vec && j + 4 <= a.N) {
-        if (residual) {
+        if constexpr (residual) {
             if constexpr (T == F32) {
                 const f32x4 o = *reinterpret_cast<const f32x4*>(r + (size_t)j * 4);
 #pragma unroll
@@ -127,7 +153,7 @@ __device__ inline void store_c(const W8Args& a, int i, int j, i32x4 acc)
             }
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = finish(v[e], old[e], a.epi);
+        for (int e = 0; e < 4; ++e) v[e] = finish<EPI>(v[e], old[e]);
         if constexpr (T == F32)
             *reinterpret_cast<f32x4*>(c + (size_t)j * 4) = (f32x4){v[0], v[1], v[2], v[3]};
         else
@@ -139,58 +165,85 @@ __device__ inline void store_c(const W8Args& a, int i, int j, i32x4 acc)
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (j + e < a.N) {
-            if (residual) old[e] = load1<T>(r, j + e);
-            store1<T>(c, j + e, finish(v[e], old[e], a.epi));
+            if constexpr (residual) old[e] = load1<T>(r, j + e);
+            store1<T>(c, j + e, finish<EPI>(v[e], old[e]));
         }
 }
 
+// 16 bytes a lane from base + off to LDS at lds + 16 * lane, past the registers.
+// The caller counts and waits (wait_loads): the compiler does not see it.
+__device__ inline void load_to_lds(uint32_t lds, const char* base, uint32_t off)
+{
+    __asm__ volatile("s_mov_b32 m0, %0\n\t"
+                     "s_nop 0\n\t"
+                     "global_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
+}
+template <int LEFT>
+__device__ inline void wait_loads()
+{
+    __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory");
+}
+
 // WM x WN waves of MB x NB blocks of 16 x 16.
-template <int T, int WM, int WN, int MB, int NB>
-__global__ void __launch_bounds__(64 * WM * WN) w8_tiled(W8Args a)
+template <int T, int EPI, int WM, int WN, int MB, int NB>
+__global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) w8_tiled(W8Args a)
 {
     constexpr int NW = WM * WN, AB = WM * MB, BB = WN * NB;    // blocks of a tile
-    constexpr int PIECES = 2 * (AB + BB);                      // 1 KB pieces of a stage (128 of K)
+    constexpr int PIECES = AB + BB;                            // 1 KB pieces of a stage (64 of K)
+    constexpr int STAGES = 4;
     static_assert(PIECES % NW == 0);
     constexpr int P = PIECES / NW;                             // pieces a wave loads
-    __shared__ u32x4 lds[2][PIECES][64];
+    __shared__ u32x4 lds[STAGES][PIECES][64];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave % WM, wn = wave / WM;
-    const int mt = blockIdx.x % (uint32_t)a.mt, nt = blockIdx.x / (uint32_t)a.mt;
-    const int steps = a.kb / 2;
 
-    // piece q < 2 AB: block q / 2 of A, half q % 2 of the stage; then the panel's
-    const char* src[P];
-    int klim[P];
+    // Consecutive workgroups go round the 8 L2s: each L2 gets a run of the tiles
+    // in an order that goes down 8 of them before it moves right, so that the
+    // tiles it has at a time share rows and columns.
+    const uint32_t tiles = (uint32_t)a.mt * a.nt, per = tiles / 8, rest = tiles % 8;
+    const uint32_t l2 = blockIdx.x % 8, at = blockIdx.x / 8;
+    const uint32_t id = l2 * per + (l2 < rest ? l2 : rest) + at;
+    const uint32_t band = id / (8u * a.nt), first = band * 8, rows = min(8u, a.mt - first);
+    const int mt = first + (id - band * 8 * a.nt) % rows, nt = (id - band * 8 * a.nt) / rows;
+
+    // piece q < AB: block q of A's rows; then the panel's
+    const char* base[P];
+    uint32_t off[P];
+    const uint32_t klast = (uint32_t)(a.K - 1) / 16 * 16, k0 = 16 * (lane >> 4);
 #pragma unroll
     for (int i = 0; i < P; ++i) {
         const int q = wave * P + i;
-        if (q < 2 * AB) {
-            int m = (mt * AB + q / 2) * 16 + (lane & 15);
-            m = m < a.M ? m : a.M - 1;
-            klim[i] = 64 * (q % 2) + 16 * (lane >> 4);
-            src[i] = reinterpret_cast<const char*>(a.A) + (size_t)m * a.lda;
+        if (q < AB) {
+            int m0 = (mt * AB + q) * 16;
+            m0 = m0 < a.M ? m0 : a.M - 1;
+            const int m = m0 + (lane & 15) < a.M ? lane & 15 : a.M - 1 - m0;
+            base[i] = reinterpret_cast<const char*>(a.A) + (size_t)m0 * a.lda;
+            off[i] = (uint32_t)m * (uint32_t)a.lda;
         } else {
             const int nblocks = (a.N + 15) / 16;
-            int nb = nt * BB + (q - 2 * AB) / 2;
+            int nb = nt * BB + q - AB;
             nb = nb < nblocks ? nb : nblocks - 1;
-            klim[i] = -1;
-            src[i] = a.panel + (((size_t)nb * a.kb + q % 2) * 64 + lane) * 16;
+            base[i] = a.panel + (size_t)nb * a.kb * 1024;
+            off[i] = 16 * lane;
         }
     }
-    u32x4 stage[P];
-    auto load = [&](int step) {
+    const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) char*)(char*)&lds[0][0][0];
+    auto load = [&](int s) {
+        const uint32_t k = 64 * s + k0;
+        const uint32_t ka = k < klast ? k : klast;     // past K the panel is zero: any of the row's bytes will do
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             const int q = wave * P + i;
-            if (q < 2 * AB) {
-                // past K the panel is zero: any of the row's bytes will do
-                const int k = klim[i] + 128 * step;
-                stage[i] = *reinterpret_cast<const u32x4*>(src[i] + (k < a.K ? k : 0));
-            } else {
-                stage[i] = *reinterpret_cast<const u32x4*>(src[i] + (size_t)step * 2048);
-            }
+            load_to_lds(lds0 + ((s % STAGES) * PIECES + q) * 1024, base[i], q < AB ? off[i] + ka : off[i] + 1024 * s);
         }
+    };
+    struct Frags { u32x4 a[MB], b[NB]; };
+    auto read = [&](int s, Frags& f) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) f.b[j] = lds[s % STAGES][AB + wn * NB + j][lane];
+#pragma unroll
+        for (int i = 0; i < MB; ++i) f.a[i] = lds[s % STAGES][wm * MB + i][lane];
     };
     i32x4 acc[MB][NB];
 #pragma unroll
@@ -198,44 +251,54 @@ __global__ void __launch_bounds__(64 * WM * WN) w8_tiled(W8Args a)
 #pragma unroll
         for (int j = 0; j < NB; ++j) acc[i][j] = (i32x4){0, 0, 0, 0};
 
+    const int steps = a.kb;                            // even, at least 2
+    // Step s multiplies what the last step read, while it reads stage s + 1 and
+    // stage s + 3 is on its way into the buffer that step s - 1 was read from: its
+    // readers have multiplied, so read, before this step's barrier.
+    auto step = [&](int s, const Frags& now, Frags& next) {
+        if (s + 2 < steps) wait_loads<P>();
+        else wait_loads<0>();
+        __builtin_amdgcn_s_barrier();
+        if (s + 3 < steps) load(s + 3);
+        if (s + 1 < steps) read(s + 1, next);
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) acc[i][j] = mfma_i8(now.b[j], now.a[i], acc[i][j]);
+    };
+    Frags f0, f1;
     load(0);
-#pragma unroll
-    for (int i = 0; i < P; ++i) lds[0][wave * P + i][lane] = stage[i];
-    __syncthreads();
-    for (int step = 0; step < steps; ++step) {
-        const int cur = step & 1;
-        const bool more = step + 1 < steps;
-        if (more) load(step + 1);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            u32x4 fa[MB], fb[NB];
-#pragma unroll
-            for (int i = 0; i < MB; ++i) fa[i] = lds[cur][2 * (wm * MB + i) + h][lane];
-#pragma unroll
-            for (int j = 0; j < NB; ++j) fb[j] = lds[cur][2 * (AB + wn * NB + j) + h][lane];
-#pragma unroll
-            for (int i = 0; i < MB; ++i)
-#pragma unroll
-                for (int j = 0; j < NB; ++j) acc[i][j] = mfma_i8(fb[j], fa[i], acc[i][j]);
-        }
-        if (more) {
-#pragma unroll
-            for (int i = 0; i < P; ++i) lds[cur ^ 1][wave * P + i][lane] = stage[i];
-        }
-        __syncthreads();
+    load(1);
+    if (steps > 2) {
+        load(2);
+        wait_loads<2 * P>();
+    } else {
+        wait_loads<P>();
     }
+    __builtin_amdgcn_s_barrier();
+    read(0, f0);
+    for (int s = 0; s < steps; s += 2) {
+        step(s, f0, f1);
+        step(s + 1, f1, f0);
+    }
+
+    Columns col[NB];
 #pragma unroll
-    for (int i = 0; i < MB; ++i)
+    for (int j = 0; j < NB; ++j) col[j] = columns_of(a, (nt * BB + wn * NB + j) * 16 + 4 * (lane >> 4));
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+        const int row = (mt * AB + wm * MB + i) * 16 + (lane & 15);
+        const float sa = a.sa[row < a.M ? row : a.M - 1];
 #pragma unroll
         for (int j = 0; j < NB; ++j)
-            store_c<T>(a, (mt * AB + wm * MB + i) * 16 + (lane & 15),
-                       (nt * BB + wn * NB + j) * 16 + 4 * (lane >> 4), acc[i][j]);
+            store_c<T, EPI>(a, row, sa, (nt * BB + wn * NB + j) * 16 + 4 * (lane >> 4), col[j], acc[i][j]);
+    }
 }
 
 constexpr int kFewWaves = 8;
 
 // MB blocks of 16 rows, 16 columns a workgroup.
-template <int T, int MB>
+template <int T, int EPI, int MB>
 __global__ void __launch_bounds__(64 * kFewWaves) w8_few(W8Args a)
 {
     __shared__ i32x4 sums[kFewWaves][MB][64];
@@ -269,10 +332,11 @@ __global__ void __launch_bounds__(64 * kFewWaves) w8_few(W8Args a)
     i32x4 sum = sums[0][wave][lane];
 #pragma unroll
     for (int v = 1; v < kFewWaves; ++v) sum += sums[v][wave][lane];
-    store_c<T>(a, 16 * wave + (lane & 15), 16 * nb + 4 * (lane >> 4), sum);
+    const int row = 16 * wave + (lane & 15), j = 16 * nb + 4 * (lane >> 4);
+    store_c<T, EPI>(a, row, a.sa[row < a.M ? row : a.M - 1], j, columns_of(a, j), sum);
 }
 
-template <int T, int WM, int WN, int MB, int NB>
+template <int T, int EPI, int WM, int WN, int MB, int NB>
 hipError_t launch_tiled(W8Args a, hipStream_t s)
 {
     constexpr int BM = 16 * WM * MB, BN = 16 * WN * NB;
@@ -280,7 +344,7 @@ hipError_t launch_tiled(W8Args a, hipStream_t s)
     a.nt = (a.N + BN - 1) / BN;
     const long long tiles = (long long)a.mt * a.nt;
     if (tiles > 0x7fffffff) return hipErrorInvalidValue;
-    return launch(w8_tiled<T, WM, WN, MB, NB>, dim3((uint32_t)tiles), dim3(64 * WM * WN), 0, s, a);
+    return launch(w8_tiled<T, EPI, WM, WN, MB, NB>, dim3((uint32_t)tiles), dim3(64 * WM * WN), 0, s, a);
 }
 
 long long tiles_of(const W8Args& a, int bm, int bn)
@@ -288,22 +352,34 @@ long long tiles_of(const W8Args& a, int bm, int bn)
     return (long long)((a.M + bm - 1) / bm) * ((a.N + bn - 1) / bn);
 }
 
-template <int T>
+template <int T, int EPI>
 hipError_t launch_w8(const W8Args& a, hipStream_t s)
 {
     if (a.M <= 64) {
         const dim3 grid((a.N + 15) / 16), block(64 * kFewWaves);
         switch ((a.M + 15) / 16) {
-        case 1: return launch(w8_few<T, 1>, grid, block, 0, s, a);
-        case 2: return launch(w8_few<T, 2>, grid, block, 0, s, a);
-        case 3: return launch(w8_few<T, 3>, grid, block, 0, s, a);
-        default: return launch(w8_few<T, 4>, grid, block, 0, s, a);
+        case 1: return launch(w8_few<T, EPI, 1>, grid, block, 0, s, a);
+        case 2: return launch(w8_few<T, EPI, 2>, grid, block, 0, s, a);
+        case 3: return launch(w8_few<T, EPI, 3>, grid, block, 0, s, a);
+        default: return launch(w8_few<T, EPI, 4>, grid, block, 0, s, a);
         }
     }
     // the largest tile of which there are enough for the 256 CUs
-    if (tiles_of(a, 256, 256) >= 200) return launch_tiled<T, 2, 4, 8, 4>(a, s);
-    if (tiles_of(a, 128, 128) >= 200) return launch_tiled<T, 2, 2, 4, 4>(a, s);
-    return launch_tiled<T, 2, 2, 2, 2>(a, s);
+    if (tiles_of(a, 256, 256) >= 200) return launch_tiled<T, EPI, 2, 4, 8, 4>(a, s);
+    if (tiles_of(a, 128, 128) >= 200) return launch_tiled<T, EPI, 2, 2, 4, 4>(a, s);
+    return launch_tiled<T, EPI, 2, 2, 2, 2>(a, s);
+}
+
+template <int T>
+hipError_t launch_epi(const W8Args& a, hipStream_t s)
+{
+    switch (a.epi) {
+    case PK_GPU_EPI_SWISH: return launch_w8<T, PK_GPU_EPI_SWISH>(a, s);
+    case PK_GPU_EPI_HALF_RESIDUAL: return launch_w8<T, PK_GPU_EPI_HALF_RESIDUAL>(a, s);
+    case PK_GPU_EPI_RESIDUAL: return launch_w8<T, PK_GPU_EPI_RESIDUAL>(a, s);
+    case PK_GPU_EPI_RELU: return launch_w8<T, PK_GPU_EPI_RELU>(a, s);
+    default: return launch_w8<T, PK_GPU_EPI_NONE>(a, s);
+    }
 }
 
 }  // namespace
@@ -351,7 +427,8 @@ int pk_gpu_gemm_w8a8_dev(int M, int N, int K, const int8_t* dA, int lda, const f
     if (!is_float(dtype)) return rt::error(PK_GPU_EINVAL, "%s: output of type %d (F32, F16 or BF16)", who, dtype);
     if (epilogue < PK_GPU_EPI_NONE || epilogue > PK_GPU_EPI_RELU)
         return rt::error(PK_GPU_EINVAL, "%s: epilogue %d is not one of PK_GPU_EPI_*", who, epilogue);
-    if (lda < K || lda % 16) return rt::error(PK_GPU_EINVAL, "%s: lda = %d (a multiple of 16, at least K = %d)", who, lda, K);
+    if (lda < K || lda % 16 || lda > 1 << 27)          // 16 rows within 32 bits
+        return rt::error(PK_GPU_EINVAL, "%s: lda = %d (a multiple of 16 from K = %d to 2^27)", who, lda, K);
     const bool residual = epilogue == PK_GPU_EPI_RESIDUAL || epilogue == PK_GPU_EPI_HALF_RESIDUAL;
     if (ldc < N || (residual && ldr < N))
         return rt::error(PK_GPU_EINVAL, "%s: ldc = %d, ldr = %d below N = %d", who, ldc, ldr, N);
@@ -384,9 +461,9 @@ int pk_gpu_gemm_w8a8_dev(int M, int N, int K, const int8_t* dA, int lda, const f
     a.kb = (K + 127) / 128 * 2;
     a.epi = epilogue;
     const size_t run = 4 * es;
-    a.vec = !off(dC, run) && a.ldc % run == 0 && (!residual || (!off(dres, run) && a.ldr % run == 0));
+    a.vec = !off(dB_scales, 16) && !off(dbias, 16) && !off(dC, run) && a.ldc % run == 0 && (!residual || (!off(dres, run) && a.ldr % run == 0));
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const hipError_t e = dtype == F32 ? launch_w8<F32>(a, s) : dtype == F16 ? launch_w8<F16>(a, s) : launch_w8<BF16>(a, s);
+    const hipError_t e = dtype == F32 ? launch_epi<F32>(a, s) : dtype == F16 ? launch_epi<F16>(a, s) : launch_epi<BF16>(a, s);
     if (e == hipErrorInvalidValue) return rt::error(PK_GPU_EINVAL, "%s: %d x %d exceeds the grid", who, M, N);
     return e == hipSuccess ? PK_GPU_OK : rt::hip_error(e, who);
 }
