@@ -24,6 +24,8 @@
 // added in LDS.  Bound by the weights' bytes and latency.
 #include "pk_decode.h"
 
+#include <type_traits>
+
 namespace pkgpu {
 namespace decode {
 namespace {
@@ -69,23 +71,33 @@ __device__ inline i32x4 mfma_i8(u32x4 b, u32x4 a, i32x4 c)
                                                  0, 0, 0);
 }
 
-// v / (1 + e^-v), e^-v = 2^t (1 + ln2 t') with t + t' = -v log2(e) to 48 bits:
-// within 3 2^-23 of its value.  (The fp32 GEMMs' Swish follows the reference's
-// polynomial, whose e^-v is off by up to 2.4e-6.)  Below v = -88.73
-// e^-v overflows and the result is -0, off by at most 2^-121.
+// v / (1 + e^-v) as v times the hardware's reciprocal (within 2^-23), e^-v =
+// 2^t with t = -v log2(e).  For f32 outputs e^-v takes the product's rounding
+// t' in, 2^t (1 + ln2 t'), and the whole is within 2^-21 of its value; for
+// 16-bit ones t is off by up to 2^-24 |t|, so the value by 2^-21 + 2^-24 |v|.
+// (The fp32 GEMMs' Swish follows the reference's polynomial, whose e^-v is off
+// by up to 2.4e-6.)  Below v = -87.3 e^-v's reciprocal leaves the normal range and
+// the result is -0, off by at most 2^-119.  The IEEE division took 12 of this
+// epilogue's 35 instructions an element.
+template <int T>
 __device__ inline float swish(float v)
 {
-    const float x = fminf(fmaxf(-v, -100.0f), 100.0f);
-    const float t = __fmul_rn(x, 0x1.715476p+0f);
-    const float lo = __fmaf_rn(x, 0x1.4ae0cp-26f, __fmaf_rn(x, 0x1.715476p+0f, -t));
-    const float e = __builtin_amdgcn_exp2f(t);
-    return __fdiv_rn(v, __fadd_rn(1.0f, __fmul_rn(e, __fmaf_rn(lo, 0x1.62e43p-1f, 1.0f))));
+    float e;
+    if constexpr (T == F32) {
+        const float x = fminf(fmaxf(-v, -100.0f), 100.0f);
+        const float t = __fmul_rn(x, 0x1.715476p+0f);
+        const float lo = __fmaf_rn(x, 0x1.4ae0cp-26f, __fmaf_rn(x, 0x1.715476p+0f, -t));
+        e = __fmul_rn(__builtin_amdgcn_exp2f(t), __fmaf_rn(lo, 0x1.62e43p-1f, 1.0f));
+    } else {
+        e = __builtin_amdgcn_exp2f(__fmul_rn(v, -0x1.715476p+0f));
+    }
+    return __fmul_rn(v, __builtin_amdgcn_rcpf(__fadd_rn(1.0f, e)));
 }
 
-template <int EPI>
+template <int T, int EPI>
 __device__ inline float finish(float v, float res)
 {
-    if constexpr (EPI == PK_GPU_EPI_SWISH) return swish(v);
+    if constexpr (EPI == PK_GPU_EPI_SWISH) return swish<T>(v);
     else if constexpr (EPI == PK_GPU_EPI_HALF_RESIDUAL) return __fadd_rn(res, __fmul_rn(0.5f, v));
     else if constexpr (EPI == PK_GPU_EPI_RESIDUAL) return __fadd_rn(res, v);
     else if constexpr (EPI == PK_GPU_EPI_RELU) return v > 0.0f ? v : 0.0f;
@@ -153,7 +165,7 @@ __device__ inline void store_c(const W8Args& a, int i, float sa, int j, const Co
             }
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = finish<EPI>(v[e], old[e]);
+        for (int e = 0; e < 4; ++e) v[e] = finish<T, EPI>(v[e], old[e]);
         if constexpr (T == F32)
             *reinterpret_cast<f32x4*>(c + (size_t)j * 4) = (f32x4){v[0], v[1], v[2], v[3]};
         else
@@ -166,7 +178,7 @@ __device__ inline void store_c(const W8Args& a, int i, float sa, int j, const Co
     for (int e = 0; e < 4; ++e)
         if (j + e < a.N) {
             if constexpr (residual) old[e] = load1<T>(r, j + e);
-            store1<T>(c, j + e, finish<EPI>(v[e], old[e]));
+            store1<T>(c, j + e, finish<T, EPI>(v[e], old[e]));
         }
 }
 
@@ -178,10 +190,11 @@ __device__ inline void load_to_lds(uint32_t lds, const char* base, uint32_t off)
                      "s_nop 0\n\t"
                      "global_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
+// Until LEFT of them are outstanding, and no LDS read is.
 template <int LEFT>
 __device__ inline void wait_loads()
 {
-    __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory");
+    __asm__ volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LEFT) : "memory");
 }
 
 // WM x WN waves of MB x NB blocks of 16 x 16.
@@ -253,34 +266,50 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) w8_tiled(W8Args a)
 
     const int steps = a.kb;                            // even, at least 2
     // Step s multiplies what the last step read, while it reads stage s + 1 and
-    // stage s + 3 is on its way into the buffer that step s - 1 was read from: its
-    // readers have multiplied, so read, before this step's barrier.
-    auto step = [&](int s, const Frags& now, Frags& next) {
-        if (s + 2 < steps) wait_loads<P>();
-        else wait_loads<0>();
+    // stage s + STAGES is on its way into the buffer that stage s was read from:
+    // all waves' reads of it are back before this step's barrier.  The last steps
+    // are copies without loads and reads: on a condition, the wait for this step's
+    // operands would be one for the next one's too.
+    auto step = [&](int s, const Frags& now, Frags& next, auto loads, auto left, auto reads) {
+        wait_loads<decltype(left)::value * P>();
         __builtin_amdgcn_s_barrier();
-        if (s + 3 < steps) load(s + 3);
-        if (s + 1 < steps) read(s + 1, next);
+        if constexpr (decltype(loads)::value) load(s + STAGES);
+        if constexpr (decltype(reads)::value) read(s + 1, next);
 #pragma unroll
         for (int i = 0; i < MB; ++i)
 #pragma unroll
             for (int j = 0; j < NB; ++j) acc[i][j] = mfma_i8(now.b[j], now.a[i], acc[i][j]);
     };
+    const std::true_type yes;
+    const std::false_type no;
+    const std::integral_constant<int, 0> c0;           // stages that may still be on their way
+    const std::integral_constant<int, 1> c1;
+    const std::integral_constant<int, 2> c2;
+    static_assert(STAGES == 4);
     Frags f0, f1;
     load(0);
     load(1);
     if (steps > 2) {
         load(2);
-        wait_loads<2 * P>();
+        load(3);
+        wait_loads<3 * P>();
     } else {
         wait_loads<P>();
     }
     __builtin_amdgcn_s_barrier();
     read(0, f0);
-    for (int s = 0; s < steps; s += 2) {
-        step(s, f0, f1);
-        step(s + 1, f1, f0);
+    int s = 0;
+    for (; s + 4 < steps; s += 2) {
+        step(s, f0, f1, yes, c2, yes);
+        step(s + 1, f1, f0, yes, c2, yes);
     }
+    if (steps > 2) {
+        step(s, f0, f1, no, c2, yes);
+        step(s + 1, f1, f0, no, c1, yes);
+        s += 2;
+    }
+    step(s, f0, f1, no, c0, yes);
+    step(s + 1, f1, f0, no, c0, no);
 
     Columns col[NB];
 #pragma unroll
