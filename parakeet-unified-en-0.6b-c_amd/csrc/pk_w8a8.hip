@@ -14,10 +14,12 @@
 // multiple of 128).  A lane's 16 bytes of lane l, block (nb, kb): column
 // 16 nb + l % 16, k from 64 kb + 16 (l / 16).
 //
-// Tiled kernel: a workgroup's tile of A and of the panel goes through LDS in
-// that same fragment order, 128 of K at a time, two stages; every LDS access
-// is 16 bytes a lane at consecutive addresses.  The next stage's global loads
-// are in registers while this stage is multiplied.
+// Tiled kernel: a workgroup's tile of A and of the panel goes from memory to LDS
+// past the registers, 128 of K at a time in 2 or 4 stages; half a stage is read
+// into registers while the half before it is multiplied, with one barrier a
+// stage.  Bound by the matrix cores at full size (8192 x 8192 x 8192: 2.1
+// PFLOP/s, where the library's int8 product reaches 2.07 on the same card), by
+// what the caches bring to a CU below.
 // Few-row kernel (M <= 64): nothing is shared between waves but the sums, so
 // there is no staging: a workgroup takes 16 columns and its waves take every
 // 8th block of K, A straight from the caches, and the waves' int32 sums are
@@ -197,13 +199,18 @@ __device__ inline void wait_loads()
     __asm__ volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LEFT) : "memory");
 }
 
-// WM x WN waves of MB x NB blocks of 16 x 16.
-template <int T, int EPI, int WM, int WN, int MB, int NB>
+// WM x WN waves of MB x NB blocks of 16 x 16; STAGES of 128 of K in LDS.
+//
+// A stage's block of 16 rows of A is 2 pieces of 8 rows x 128 bytes, so that
+// every load takes whole cache lines; slot c of row r holds the row's 16-byte
+// chunk c ^ (r % 8), so that the 8 rows a quarter wave reads of one chunk are in
+// different banks.  A stage's block of 16 columns is 2 pieces of the panel, for
+// its two halves of K.
+template <int T, int EPI, int WM, int WN, int MB, int NB, int STAGES>
 __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) w8_tiled(W8Args a)
 {
     constexpr int NW = WM * WN, AB = WM * MB, BB = WN * NB;    // blocks of a tile
-    constexpr int PIECES = AB + BB;                            // 1 KB pieces of a stage (64 of K)
-    constexpr int STAGES = 4;
+    constexpr int PIECES = 2 * (AB + BB);                      // 1 KB pieces of a stage
     static_assert(PIECES % NW == 0);
     constexpr int P = PIECES / NW;                             // pieces a wave loads
     __shared__ u32x4 lds[STAGES][PIECES][64];
@@ -220,107 +227,104 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) w8_tiled(W8Args a)
     const uint32_t band = id / (8u * a.nt), first = band * 8, rows = min(8u, a.mt - first);
     const int mt = first + (id - band * 8 * a.nt) % rows, nt = (id - band * 8 * a.nt) / rows;
 
-    // piece q < AB: block q of A's rows; then the panel's
+    // piece q < 2 AB: rows 8 q on of the tile's; then the panel's
     const char* base[P];
     uint32_t off[P];
-    const uint32_t klast = (uint32_t)(a.K - 1) / 16 * 16, k0 = 16 * (lane >> 4);
+    const uint32_t klast = (uint32_t)(a.K - 1) / 16 * 16;
+    const uint32_t k0 = 16 * ((lane & 7) ^ (lane >> 3));
 #pragma unroll
     for (int i = 0; i < P; ++i) {
         const int q = wave * P + i;
-        if (q < AB) {
-            int m0 = (mt * AB + q) * 16;
+        if (q < 2 * AB) {
+            int m0 = mt * AB * 16 + 8 * q;
             m0 = m0 < a.M ? m0 : a.M - 1;
-            const int m = m0 + (lane & 15) < a.M ? lane & 15 : a.M - 1 - m0;
+            const int m = m0 + (lane >> 3) < a.M ? lane >> 3 : a.M - 1 - m0;
             base[i] = reinterpret_cast<const char*>(a.A) + (size_t)m0 * a.lda;
             off[i] = (uint32_t)m * (uint32_t)a.lda;
         } else {
             const int nblocks = (a.N + 15) / 16;
-            int nb = nt * BB + q - AB;
+            int nb = nt * BB + (q - 2 * AB) / 2;
             nb = nb < nblocks ? nb : nblocks - 1;
-            base[i] = a.panel + (size_t)nb * a.kb * 1024;
+            base[i] = a.panel + ((size_t)nb * a.kb + q % 2) * 1024;
             off[i] = 16 * lane;
         }
     }
     const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) char*)(char*)&lds[0][0][0];
     auto load = [&](int s) {
-        const uint32_t k = 64 * s + k0;
+        const uint32_t k = 128 * s + k0;
         const uint32_t ka = k < klast ? k : klast;     // past K the panel is zero: any of the row's bytes will do
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             const int q = wave * P + i;
-            load_to_lds(lds0 + ((s % STAGES) * PIECES + q) * 1024, base[i], q < AB ? off[i] + ka : off[i] + 1024 * s);
+            load_to_lds(lds0 + ((s % STAGES) * PIECES + q) * 1024, base[i], q < 2 * AB ? off[i] + ka : off[i] + 2048 * s);
         }
     };
     struct Frags { u32x4 a[MB], b[NB]; };
-    auto read = [&](int s, Frags& f) {
+    const int row = lane & 15;
+    auto read = [&](int s, int half, Frags& f) {
+        const int slot = row * 8 + ((4 * half + (lane >> 4)) ^ (row & 7));
 #pragma unroll
-        for (int j = 0; j < NB; ++j) f.b[j] = lds[s % STAGES][AB + wn * NB + j][lane];
+        for (int j = 0; j < NB; ++j) f.b[j] = lds[s % STAGES][2 * (AB + wn * NB + j) + half][lane];
 #pragma unroll
-        for (int i = 0; i < MB; ++i) f.a[i] = lds[s % STAGES][wm * MB + i][lane];
+        for (int i = 0; i < MB; ++i) f.a[i] = lds[s % STAGES][2 * (wm * MB + i)][slot];
     };
     i32x4 acc[MB][NB];
 #pragma unroll
     for (int i = 0; i < MB; ++i)
 #pragma unroll
         for (int j = 0; j < NB; ++j) acc[i][j] = (i32x4){0, 0, 0, 0};
-
-    const int steps = a.kb;                            // even, at least 2
-    // Step s multiplies what the last step read, while it reads stage s + 1 and
-    // stage s + STAGES is on its way into the buffer that stage s was read from:
-    // all waves' reads of it are back before this step's barrier.  The last steps
-    // are copies without loads and reads: on a condition, the wait for this step's
-    // operands would be one for the next one's too.
-    auto step = [&](int s, const Frags& now, Frags& next, auto loads, auto left, auto reads) {
-        wait_loads<decltype(left)::value * P>();
-        __builtin_amdgcn_s_barrier();
-        if constexpr (decltype(loads)::value) load(s + STAGES);
-        if constexpr (decltype(reads)::value) read(s + 1, next);
+    auto multiply = [&](const Frags& f) {
 #pragma unroll
         for (int i = 0; i < MB; ++i)
 #pragma unroll
-            for (int j = 0; j < NB; ++j) acc[i][j] = mfma_i8(now.b[j], now.a[i], acc[i][j]);
+            for (int j = 0; j < NB; ++j) acc[i][j] = mfma_i8(f.b[j], f.a[i], acc[i][j]);
     };
-    const std::true_type yes;
-    const std::false_type no;
-    const std::integral_constant<int, 0> c0;           // stages that may still be on their way
-    const std::integral_constant<int, 1> c1;
-    const std::integral_constant<int, 2> c2;
-    static_assert(STAGES == 4);
+
+    const int steps = a.kb / 2;
+    // Each half of a step is read while the half before it is multiplied.  At the
+    // second half of step s all waves' reads of stage s are back before the
+    // barrier, so stage s + STAGES may overwrite it behind it.  The last steps are
+    // copies without loads: on a condition, the wait for one half's operands
+    // would be one for the next half's too.
+    auto step = [&](int s, Frags& f0, Frags& f1, auto loads, auto left) {
+        read(s, 1, f1);
+        multiply(f0);
+        wait_loads<decltype(left)::value * P>();
+        __builtin_amdgcn_s_barrier();
+        if constexpr (decltype(loads)::value) load(s + STAGES);
+        read(s + 1, 0, f0);
+        multiply(f1);
+    };
+    const std::integral_constant<int, 0> all;          // stages that may still be on their way
+    const std::integral_constant<int, STAGES - 2> ahead;
     Frags f0, f1;
-    load(0);
-    load(1);
-    if (steps > 2) {
-        load(2);
-        load(3);
-        wait_loads<3 * P>();
+    if (steps >= STAGES) {
+#pragma unroll
+        for (int i = 0; i < STAGES; ++i) load(i);
+        wait_loads<(STAGES - 1) * P>();
     } else {
-        wait_loads<P>();
+        for (int i = 0; i < steps; ++i) load(i);
+        wait_loads<0>();
     }
     __builtin_amdgcn_s_barrier();
-    read(0, f0);
+    read(0, 0, f0);
     int s = 0;
-    for (; s + 4 < steps; s += 2) {
-        step(s, f0, f1, yes, c2, yes);
-        step(s + 1, f1, f0, yes, c2, yes);
-    }
-    if (steps > 2) {
-        step(s, f0, f1, no, c2, yes);
-        step(s + 1, f1, f0, no, c1, yes);
-        s += 2;
-    }
-    step(s, f0, f1, no, c0, yes);
-    step(s + 1, f1, f0, no, c0, no);
+    for (; s + STAGES < steps; ++s) step(s, f0, f1, std::true_type{}, ahead);
+    for (; s + 1 < steps; ++s) step(s, f0, f1, std::false_type{}, all);
+    read(s, 1, f1);
+    multiply(f0);
+    multiply(f1);
 
     Columns col[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j) col[j] = columns_of(a, (nt * BB + wn * NB + j) * 16 + 4 * (lane >> 4));
 #pragma unroll
     for (int i = 0; i < MB; ++i) {
-        const int row = (mt * AB + wm * MB + i) * 16 + (lane & 15);
-        const float sa = a.sa[row < a.M ? row : a.M - 1];
+        const int m = (mt * AB + wm * MB + i) * 16 + row;
+        const float sa = a.sa[m < a.M ? m : a.M - 1];
 #pragma unroll
         for (int j = 0; j < NB; ++j)
-            store_c<T, EPI>(a, row, sa, (nt * BB + wn * NB + j) * 16 + 4 * (lane >> 4), col[j], acc[i][j]);
+            store_c<T, EPI>(a, m, sa, (nt * BB + wn * NB + j) * 16 + 4 * (lane >> 4), col[j], acc[i][j]);
     }
 }
 
@@ -365,7 +369,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) w8_few(W8Args a)
     store_c<T, EPI>(a, row, a.sa[row < a.M ? row : a.M - 1], j, columns_of(a, j), sum);
 }
 
-template <int T, int EPI, int WM, int WN, int MB, int NB>
+template <int T, int EPI, int WM, int WN, int MB, int NB, int STAGES>
 hipError_t launch_tiled(W8Args a, hipStream_t s)
 {
     constexpr int BM = 16 * WM * MB, BN = 16 * WN * NB;
@@ -373,7 +377,7 @@ hipError_t launch_tiled(W8Args a, hipStream_t s)
     a.nt = (a.N + BN - 1) / BN;
     const long long tiles = (long long)a.mt * a.nt;
     if (tiles > 0x7fffffff) return hipErrorInvalidValue;
-    return launch(w8_tiled<T, EPI, WM, WN, MB, NB>, dim3((uint32_t)tiles), dim3(64 * WM * WN), 0, s, a);
+    return launch(w8_tiled<T, EPI, WM, WN, MB, NB, STAGES>, dim3((uint32_t)tiles), dim3(64 * WM * WN), 0, s, a);
 }
 
 long long tiles_of(const W8Args& a, int bm, int bn)
@@ -393,10 +397,21 @@ hipError_t launch_w8(const W8Args& a, hipStream_t s)
         default: return launch(w8_few<T, EPI, 4>, grid, block, 0, s, a);
         }
     }
-    // the largest tile of which there are enough for the 256 CUs
-    if (tiles_of(a, 256, 256) >= 200) return launch_tiled<T, EPI, 2, 4, 8, 4>(a, s);
-    if (tiles_of(a, 128, 128) >= 200) return launch_tiled<T, EPI, 2, 2, 4, 4>(a, s);
-    return launch_tiled<T, EPI, 2, 2, 2, 2>(a, s);
+    // The largest tile of which there are enough for the 256 CUs; 128 x 128 with
+    // two workgroups a CU (2 stages each) where there are more tiles than CUs, with
+    // 4 stages where there are not.  Measured (us; 256 x 256, 128 x 128 in 2 and in
+    // 4 stages, 64 x 64), bf16 output:
+    //   8192 x 4096 x 8192   276, 306, 348, 477
+    //   4001 x 4096 x 1024    30, 30.5, 37, 47
+    //   2000 x 4096 x 1024    26, 17.6, 20.4, 25
+    //   4001 x 1024 x 4096    63, 29, 26.7, 36
+    //    512 x 4096 x 4096    61, 27, 23.7, 18.8
+    //    128 x 4096 x 1024    23, 9.2, 9.3, 5.9
+    if (tiles_of(a, 256, 256) >= 200) return launch_tiled<T, EPI, 2, 4, 8, 4, 2>(a, s);
+    const long long mid = tiles_of(a, 128, 128);
+    if (mid > 256) return launch_tiled<T, EPI, 2, 4, 4, 2, 2>(a, s);
+    if (mid >= 200) return launch_tiled<T, EPI, 2, 4, 4, 2, 4>(a, s);
+    return launch_tiled<T, EPI, 2, 4, 2, 1, 4>(a, s);
 }
 
 template <int T>

@@ -62,6 +62,9 @@ CASES = [
     (300, 260, 129, "bf16", "relu", 0, 0, True, True), (1111, 1023, 777, "bf16", "residual", 0, 1, True, True),
     (2000, 2304, 256, "f32", "swish", 0, 0, True, True), (4001, 4096, 384, "bf16", "swish", 0, 0, True, True),
     (3500, 4100, 1024, "f16", "half", 0, 0, True, True),
+    (3200, 1024, 1100, "f32", "relu", 0, 0, True, True), (3200, 1024, 100, "bf16", "none", 0, 0, True, True),
+    (2000, 2500, 650, "bf16", "half", 16, 0, True, True), (4001, 4001, 130, "f16", "none", 0, 0, True, True),
+    (70, 65, 513, "f32", "none", 0, 0, True, True), (200, 500, 2049, "f32", "swish", 0, 0, True, True),
 ]
 
 
