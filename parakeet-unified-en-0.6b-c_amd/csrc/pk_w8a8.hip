@@ -20,10 +20,11 @@
 // stage.  Bound by the matrix cores at full size (8192 x 8192 x 8192: 2.1
 // PFLOP/s, where the library's int8 product reaches 2.07 on the same card), by
 // what the caches bring to a CU below.
-// Few-row kernel (M <= 64): nothing is shared between waves but the sums, so
-// there is no staging: a workgroup takes 16 columns and its waves take every
-// 8th block of K, A straight from the caches, and the waves' int32 sums are
-// added in LDS.  Bound by the weights' bytes and latency.
+// Few-row kernel: nothing is shared between waves but the sums, so there is no
+// staging: a workgroup takes 16 columns and its 16 waves every 16th block of K,
+// A straight from the caches, and the waves' int32 sums are added in LDS.  Bound
+// by the launch and one load's latency (33 x 4096 x 1024: 4.8 us), for longer
+// rows by what the caches bring to a CU (1 x 4096 x 4096: 5.9 us, 2.9 TB/s).
 #include "pk_decode.h"
 
 #include <type_traits>
@@ -328,20 +329,20 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) w8_tiled(W8Args a)
     }
 }
 
-constexpr int kFewWaves = 8;
+constexpr int kFewWaves = 16;
 
-// MB blocks of 16 rows, 16 columns a workgroup.
+// MB blocks of 16 rows from block MB * blockIdx.y on, 16 columns.
 template <int T, int EPI, int MB>
 __global__ void __launch_bounds__(64 * kFewWaves) w8_few(W8Args a)
 {
     __shared__ i32x4 sums[kFewWaves][MB][64];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int nb = blockIdx.x;
+    const int nb = blockIdx.x, m0 = 16 * MB * blockIdx.y;
     const char* rows[MB];
 #pragma unroll
     for (int i = 0; i < MB; ++i) {
-        const int m = 16 * i + (lane & 15);
+        const int m = m0 + 16 * i + (lane & 15);
         rows[i] = reinterpret_cast<const char*>(a.A) + (size_t)(m < a.M ? m : a.M - 1) * a.lda;
     }
     const char* w = a.panel + ((size_t)nb * a.kb * 64 + lane) * 16;
@@ -365,7 +366,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) w8_few(W8Args a)
     i32x4 sum = sums[0][wave][lane];
 #pragma unroll
     for (int v = 1; v < kFewWaves; ++v) sum += sums[v][wave][lane];
-    const int row = 16 * wave + (lane & 15), j = 16 * nb + 4 * (lane >> 4);
+    const int row = m0 + 16 * wave + (lane & 15), j = 16 * nb + 4 * (lane >> 4);
     store_c<T, EPI>(a, row, a.sa[row < a.M ? row : a.M - 1], j, columns_of(a, j), sum);
 }
 
@@ -388,14 +389,22 @@ long long tiles_of(const W8Args& a, int bm, int bn)
 template <int T, int EPI>
 hipError_t launch_w8(const W8Args& a, hipStream_t s)
 {
-    if (a.M <= 64) {
-        const dim3 grid((a.N + 15) / 16), block(64 * kFewWaves);
-        switch ((a.M + 15) / 16) {
-        case 1: return launch(w8_few<T, EPI, 1>, grid, block, 0, s, a);
-        case 2: return launch(w8_few<T, EPI, 2>, grid, block, 0, s, a);
-        case 3: return launch(w8_few<T, EPI, 3>, grid, block, 0, s, a);
-        default: return launch(w8_few<T, EPI, 4>, grid, block, 0, s, a);
-        }
+    // Few rows, or too few 64 x 64 tiles to be worth staging (us; this kernel,
+    // 64 x 64 tiles): 33 x 4096 x 4096 9.8, 11.2; 64 x 4096 x 4096 12.5, 11.5; 64 x
+    // 1024 x 4096 5.8, 10.1; 128 x 1024 x 4096 8.0, 10.0; 256 x 1024 x 4096 12.3, 11.4;
+    // 17 x 16384 x 4096 17.8, 14.7.
+    const long long small = tiles_of(a, 64, 64);
+    if (a.M <= 16 || small < 48 || (small < 128 && a.M <= 48)) {
+        // as many blocks of rows a workgroup as leave 256 workgroups (33 x 1024 x
+        // 4096: 5.6 us in 64 x 3 workgroups, 8.0 in 64)
+        const int cols = (a.N + 15) / 16, blocks = (a.M + 15) / 16;
+        int mb = blocks < 4 ? blocks : 4;
+        while (mb > 1 && (long long)cols * ((blocks + mb - 1) / mb) < 256) --mb;
+        const dim3 grid(cols, (blocks + mb - 1) / mb), block(64 * kFewWaves);
+        return mb == 1   ? launch(w8_few<T, EPI, 1>, grid, block, 0, s, a)
+               : mb == 2 ? launch(w8_few<T, EPI, 2>, grid, block, 0, s, a)
+               : mb == 3 ? launch(w8_few<T, EPI, 3>, grid, block, 0, s, a)
+                         : launch(w8_few<T, EPI, 4>, grid, block, 0, s, a);
     }
     // The largest tile of which there are enough for the 256 CUs; 128 x 128 with
     // two workgroups a CU (2 stages each) where there are more tiles than CUs, with

@@ -64,6 +64,8 @@ CASES = [
     (3500, 4100, 1024, "f16", "half", 0, 0, True, True),
     (3200, 1024, 1100, "f32", "relu", 0, 0, True, True), (3200, 1024, 100, "bf16", "none", 0, 0, True, True),
     (2000, 2500, 650, "bf16", "half", 16, 0, True, True), (4001, 4001, 130, "f16", "none", 0, 0, True, True),
+    (130, 300, 700, "f32", "residual", 0, 1, True, True), (250, 100, 64, "bf16", "swish", 0, 0, True, True),
+    (40, 2100, 333, "f16", "relu", 0, 0, True, True), (50, 4200, 260, "f32", "half", 0, 0, True, True),
     (70, 65, 513, "f32", "none", 0, 0, True, True), (200, 500, 2049, "f32", "swish", 0, 0, True, True),
 ]
 
