@@ -27,7 +27,10 @@ struct RowsArgs {
     int page_shift, page_size, n_slots;
 };
 
-constexpr int kThreads = 256;
+// Threads of a workgroup: a launch of many rows takes 1024 (20011 tokens of 8
+// heads of 128 from int8 to bf16: 25.6 us against 27.5 of 256), one of few 256, on
+// more CUs.
+constexpr int kMostThreads = 1024;
 
 // Index of the cache row that row r = token * heads + head names, or -1.
 __device__ inline long long cache_row(const RowsArgs& a, uint32_t token, uint32_t head)
@@ -75,10 +78,10 @@ __device__ inline void write_part(void* cache, float* scales, long long row, int
 }
 
 template <int CACHE, int ROWS, int DIM>
-__global__ void __launch_bounds__(kThreads) kv_write(RowsArgs a)
+__global__ void __launch_bounds__(kMostThreads) kv_write(RowsArgs a)
 {
     constexpr int LANES = DIM / 8;
-    const uint32_t r = blockIdx.x * (uint32_t)(kThreads / LANES) + threadIdx.x / LANES;
+    const uint32_t r = blockIdx.x * (blockDim.x / LANES) + threadIdx.x / LANES;
     const int part = threadIdx.x % LANES;
     if (r >= a.rows) return;                       // whole lane groups leave together
     const uint32_t token = r / a.heads, head = r - token * a.heads;
@@ -93,10 +96,10 @@ __global__ void __launch_bounds__(kThreads) kv_write(RowsArgs a)
 }
 
 template <int CACHE, int ROWS, int DIM>
-__global__ void __launch_bounds__(kThreads) kv_read(RowsArgs a)
+__global__ void __launch_bounds__(kMostThreads) kv_read(RowsArgs a)
 {
     constexpr int LANES = DIM / 8;
-    const uint32_t r = blockIdx.x * (uint32_t)(kThreads / LANES) + threadIdx.x / LANES;
+    const uint32_t r = blockIdx.x * (blockDim.x / LANES) + threadIdx.x / LANES;
     const int part = threadIdx.x % LANES;
     if (r >= a.rows) return;
     const uint32_t token = r / a.heads, head = r - token * a.heads;
@@ -122,8 +125,9 @@ __global__ void __launch_bounds__(kThreads) kv_read(RowsArgs a)
 template <int CACHE, int ROWS>
 hipError_t launch_dim(bool write, int dim, const RowsArgs& a, hipStream_t s)
 {
-    const uint32_t per = kThreads / (dim / 8);
-    const dim3 grid((a.rows + per - 1) / per), block(kThreads);
+    const uint32_t lanes = dim / 8, threads = a.rows / 1024 * lanes >= 256 ? kMostThreads : 256;
+    const uint32_t per = threads / lanes;
+    const dim3 grid((uint32_t)(((uint64_t)a.rows + per - 1) / per)), block(threads);
 #define PK_ROWS_DIM(D) launch(write ? kv_write<CACHE, ROWS, D> : kv_read<CACHE, ROWS, D>, grid, block, 0, s, a)
     return dim == 64 ? PK_ROWS_DIM(64) : dim == 128 ? PK_ROWS_DIM(128) : PK_ROWS_DIM(256);
 #undef PK_ROWS_DIM
