@@ -197,7 +197,8 @@ inline hipError_t launch(void (*fn)(Args), dim3 grid, dim3 block, size_t lds, hi
 }
 
 inline bool is_float(int t) { return t == F32 || t == F16 || t == BF16; }
-inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+inline bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+inline bool aligned16(const void* p) { return aligned(p, 16); }
 // PK_GPU_OK, or the error of a cache description
 int check_cache(const pk_gpu_kv_cache* c, const char* who);
 

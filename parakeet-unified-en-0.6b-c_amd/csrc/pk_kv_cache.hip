@@ -158,6 +158,7 @@ int kv_call(bool write, const pk_gpu_kv_cache* c, int dtype, const void* dk, int
     const int es = size_of(dtype);
     if (!aligned16(dk) || !aligned16(dv) || (size_t)ldk * es % 16 || (size_t)ldv * es % 16)
         return rt::error(PK_GPU_EINVAL, "%s: rows must be 16-byte aligned", who);
+    if (!aligned(dslots, 4)) return rt::error(PK_GPU_EINVAL, "%s: slots are not aligned to an int", who);
     OnDevice on;
     if (on.rc) return on.rc;
     if (!n) return PK_GPU_OK;

@@ -199,6 +199,8 @@ int pk_gpu_paged_attention_dev(const pk_gpu_kv_cache* cache, int dtype, const vo
     const size_t es = size_of(dtype);
     if (!aligned16(dq) || !aligned16(dout) || (size_t)ldq * es % 16 || (size_t)ldo * es % 16)
         return rt::error(PK_GPU_EINVAL, "%s: query and output rows must be 16-byte aligned", who);
+    if (!aligned(dpages, 4) || !aligned(dlens, 4) || !aligned(dlse, 4))
+        return rt::error(PK_GPU_EINVAL, "%s: pages, lengths or lse are not aligned to their elements", who);
     const long long pairs = (long long)B * cache->heads * head_tiles(heads / cache->heads);
     const Plan p = plan(cache, B, heads, max_len, window);
     const size_t need = ws_floats_of(cache, B, heads, p);

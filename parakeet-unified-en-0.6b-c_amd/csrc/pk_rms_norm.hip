@@ -13,9 +13,10 @@
 // shapes.  The fp64 work is two instructions an element.
 //
 // A row stays in registers between its statistics and its output: TPR threads
-// (a wave, or a workgroup of four) hold CH pieces of W consecutive elements
-// each.  Rows that are not 16-byte aligned (odd D) take W = 1.  Longer rows are
-// read again for each pass.  Bound by the rows' bytes.
+// (a wave, or a workgroup of 4 or 16) hold CH pieces of W consecutive elements
+// each.  Rows that are not 16-byte aligned (odd D) take W = 1.  Longer rows
+// (above 16384, or 4096 single elements) are read again for each pass.  Bound by
+// the rows' bytes.
 #include "pk_decode.h"
 
 namespace pkgpu {
@@ -106,12 +107,15 @@ __device__ inline void load_sum(const NormArgs& a, size_t row, size_t i, float* 
     }
 }
 
+constexpr int norm_threads(int tpr) { return tpr > kNormThreads ? tpr : kNormThreads; }
+
 template <int T, int OUT, int TPR, int CH, int W>
-__global__ void __launch_bounds__(kNormThreads) rms_norm(NormArgs a)
+__global__ void __launch_bounds__(norm_threads(TPR)) rms_norm(NormArgs a)
 {
-    constexpr int RPB = kNormThreads / TPR;              // rows a workgroup has at a time
-    __shared__ double red_sum[2][4];
-    __shared__ uint32_t red_max[2][4];
+    constexpr int RPB = norm_threads(TPR) / TPR;         // rows a workgroup has at a time
+    constexpr int WAVES = norm_threads(TPR) / 64;
+    __shared__ double red_sum[2][WAVES];
+    __shared__ uint32_t red_max[2][WAVES];
     const int t = threadIdx.x % TPR, wave = threadIdx.x / 64;
     float gm[CH][W];
 #pragma unroll
@@ -167,7 +171,9 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm(NormArgs a)
         if constexpr (TPR > 64) {
             if (threadIdx.x % 64 == 0) red_sum[turn][wave] = sum;
             __syncthreads();
-            sum = (red_sum[turn][0] + red_sum[turn][1]) + (red_sum[turn][2] + red_sum[turn][3]);
+            sum = red_sum[turn][0];
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w) sum = sum + red_sum[turn][w];
         }
         const float r = norm_factor(sum, a.D, a.eps);
         uint32_t top = 0;
@@ -187,7 +193,7 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm(NormArgs a)
                 if (threadIdx.x % 64 == 0) red_max[turn][wave] = top;
                 __syncthreads();
 #pragma unroll
-                for (int w = 0; w < 4; ++w) top = red_max[turn][w] > top ? red_max[turn][w] : top;
+                for (int w = 0; w < WAVES; ++w) top = red_max[turn][w] > top ? red_max[turn][w] : top;
             }
             const RowCode code = row_code(top, top_of(I8));
 #pragma unroll
@@ -257,8 +263,8 @@ __global__ void __launch_bounds__(1024) rms_norm_long(NormArgs a)
     }
 }
 
-// A wave a row while its pieces fit 4 (8 elements each, 1024 single ones) a
-// lane, else a workgroup.
+// A wave a row while its pieces fit 4 a lane (8 elements each; 16 single ones),
+// else a workgroup.
 template <int T, int OUT>
 hipError_t launch_norm(const NormArgs& a, bool wide, hipStream_t s)
 {
@@ -279,6 +285,7 @@ hipError_t launch_norm(const NormArgs& a, bool wide, hipStream_t s)
         if (pieces <= 256) return launch(rms_norm<T, OUT, 64, 4, 8>, grid(4), block, 0, s, a);
         if (pieces <= 512) return launch(rms_norm<T, OUT, 256, 2, 8>, grid(1), block, 0, s, a);
         if (pieces <= 1024) return launch(rms_norm<T, OUT, 256, 4, 8>, grid(1), block, 0, s, a);
+        if (pieces <= 2048) return launch(rms_norm<T, OUT, 1024, 2, 8>, grid(1), dim3(1024), 0, s, a);
     } else {
         if (a.D <= 512) return launch(rms_norm<T, OUT, 64, 8, 1>, grid(4), block, 0, s, a);
         if (a.D <= 1024) return launch(rms_norm<T, OUT, 64, 16, 1>, grid(4), block, 0, s, a);
@@ -318,7 +325,7 @@ extern "C" int pk_gpu_rms_norm_dev(int dtype, const void* dx, int ldx, const voi
     if (rows && (!dx || !dout || (out_dtype == I8 && !dscales)))
         return rt::error(PK_GPU_EINVAL, "%s: NULL operand", who);
     const int es = size_of(dtype), os = size_of(out_dtype);
-    const auto off = [](const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; };
+    const auto off = [](const void* p, size_t bytes) { return !aligned(p, bytes); };
     if (off(dx, es) || off(dres, es) || off(dsum, es) || off(dout, os) || off(dgamma, 4) || off(dscales, 4))
         return rt::error(PK_GPU_EINVAL, "%s: an operand is not aligned to its elements", who);
     // one thread reads and writes an element in place; other overlaps would race
@@ -345,7 +352,7 @@ extern "C" int pk_gpu_rms_norm_dev(int dtype, const void* dx, int ldx, const voi
     a.D = D;
     // 8 elements at a time: whole pieces, all of them aligned (codes: 8 bytes)
     const auto fits = [](const void* p, size_t ld, size_t bytes) {
-        return reinterpret_cast<uintptr_t>(p) % bytes == 0 && ld % bytes == 0;
+        return aligned(p, bytes) && ld % bytes == 0;
     };
     const bool wide = D % 8 == 0 && fits(dx, a.ldx, 16) && (!dres || fits(dres, a.ldr, 16)) &&
                       (!dsum || fits(dsum, a.lds, 16)) && fits(dout, a.ldo, out_dtype == I8 ? 8 : 16);

@@ -49,11 +49,18 @@ struct W8Args {
     int mt, nt;                     // tiles
 };
 
-__global__ void __launch_bounds__(256) w8_panel(const int8_t* B, int ldb, int K, int N, int kb, u32x4* panel,
-                                                long long blocks)
+struct PanelArgs {
+    const int8_t* B;
+    u32x4* panel;
+    long long blocks;
+    int ldb, K, N, kb;
+};
+
+__global__ void __launch_bounds__(256) w8_panel(PanelArgs p)
 {
+    const int kb = p.kb, K = p.K, N = p.N;
     const long long blk = (long long)blockIdx.x * 4 + threadIdx.x / 64;
-    if (blk >= blocks) return;
+    if (blk >= p.blocks) return;
     const int lane = threadIdx.x & 63;
     const long long nb = blk / kb;
     const long long n = nb * 16 + (lane & 15);
@@ -62,10 +69,10 @@ __global__ void __launch_bounds__(256) w8_panel(const int8_t* B, int ldb, int K,
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         uint32_t v = 0;
-        if (n < N && k0 + i < K) v = (uint8_t)B[(size_t)(k0 + i) * ldb + n];
+        if (n < N && k0 + i < K) v = (uint8_t)p.B[(size_t)(k0 + i) * p.ldb + n];
         w[i / 4] |= v << (8 * (i % 4));
     }
-    panel[blk * 64 + lane] = w;
+    p.panel[blk * 64 + lane] = w;
 }
 
 __device__ inline i32x4 mfma_i8(u32x4 b, u32x4 a, i32x4 c)
@@ -463,9 +470,9 @@ int pk_gpu_w8_panel_dev(int K, int N, const int8_t* dB, int ldb, void* dpanel, v
     if ((blocks + 3) / 4 > 0x7fffffff) return rt::error(PK_GPU_EINVAL, "%s: %d x %d exceeds the grid", who, K, N);
     OnDevice on;
     if (on.rc) return on.rc;
-    w8_panel<<<dim3((uint32_t)((blocks + 3) / 4)), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
-        dB, ldb, K, N, kb, static_cast<u32x4*>(dpanel), blocks);
-    const hipError_t e = hipGetLastError();
+    const PanelArgs p{dB, static_cast<u32x4*>(dpanel), blocks, ldb, K, N, kb};
+    const hipError_t e = launch(w8_panel, dim3((uint32_t)((blocks + 3) / 4)), dim3(256), 0,
+                                static_cast<hipStream_t>(stream), p);
     return e == hipSuccess ? PK_GPU_OK : rt::hip_error(e, who);
 }
 
@@ -490,7 +497,7 @@ int pk_gpu_gemm_w8a8_dev(int M, int N, int K, const int8_t* dA, int lda, const f
     if (!aligned16(dA) || !aligned16(dpanel))
         return rt::error(PK_GPU_EINVAL, "%s: A and the panel must be 16-byte aligned", who);
     const int es = size_of(dtype);
-    const auto off = [](const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; };
+    const auto off = [](const void* p, size_t bytes) { return !aligned(p, bytes); };
     if (off(dC, es) || (residual && off(dres, es)) || off(dA_scales, 4) || off(dB_scales, 4) || off(dbias, 4))
         return rt::error(PK_GPU_EINVAL, "%s: an operand is not aligned to its elements", who);
     if (residual && dres == dC && ldr != ldc)

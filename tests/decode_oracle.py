@@ -53,6 +53,8 @@ def code_bound(x, kind):
     and scale, each at most 2^-24 of a value of at most max|x| (3.01: with their
     products)."""
     x = np.asarray(x, np.float64)
+    if kind not in TOP:                     # a 16-bit cache: one rounding
+        return HALF[kind] * np.abs(x)
     a = np.abs(x).max(-1, keepdims=True)
     u = a / TOP[kind]
     if kind == "int8":

@@ -60,7 +60,7 @@ def test_16_bit_caches_need_no_scales():
     (pk.F32, P, 256, P, 256, P, -1, "n ="), (pk.F32, None, 256, P, 256, P, 1, "NULL"),
     (pk.F32, P, 256, None, 256, P, 1, "NULL"), (pk.F32, P, 256, P, 256, None, 1, "NULL"),
     (pk.F32, P + 4, 256, P, 256, P, 1, "aligned"), (pk.BF16, P, 256, P, 260, P, 1, "aligned"),
-    (pk.F32, P, 256, P, 256, P, 1 << 30, "2^31"),
+    (pk.F32, P, 256, P, 256, P, 1 << 30, "2^31"), (pk.F32, P, 256, P, 256, P + 2, 1, "aligned"),
 ])
 def test_bad_rows(dtype, k, ldk, v, ldv, slots, n, text):
     c = ctypes.byref(cache())
@@ -81,7 +81,8 @@ def test_null_cache():
     (dict(ld_pages=-1), -1, "pages"), (dict(q=None), -1, "NULL"), (dict(out=None), -1, "NULL"),
     (dict(lens=None), -1, "NULL"), (dict(pages=None), -1, "NULL"), (dict(q=P + 8), -1, "aligned"),
     (dict(out=P + 4), -1, "aligned"), (dict(ldq=513), -1, "aligned"), (dict(ldo=514), -1, "aligned"),
-    (dict(B=1 << 30), -1, "grid"),
+    (dict(B=1 << 30), -1, "grid"), (dict(pages=P + 1), -1, "aligned"), (dict(lens=P + 2), -1, "aligned"),
+    (dict(lse=P + 3), -1, "aligned"),
 ])
 def test_bad_attention(kw, code, text):
     attention(c=ctypes.byref(cache()), code=code, text=text, **kw)
@@ -137,7 +138,8 @@ def gemm(code=-1, text=None, **kw):
 @pytest.mark.parametrize("kw,text", [
     (dict(M=-1), "M ="), (dict(N=-1), "N ="), (dict(N=(1 << 30) + 1, ldc=(1 << 30) + 1), "N ="), (dict(K=0), "K ="),
     (dict(K=131072, lda=131072), "K ="), (dict(dtype=pk.I8), "type"), (dict(epi=5), "epilogue"),
-    (dict(epi=-1), "epilogue"), (dict(lda=72), "lda"), (dict(lda=48), "lda"), (dict(ldc=31), "ldc"),
+    (dict(epi=-1), "epilogue"), (dict(lda=72), "lda"), (dict(lda=48), "lda"),
+    (dict(lda=(1 << 27) + 16), "lda"), (dict(M=(1 << 30) + 1), "M ="), (dict(ldc=31), "ldc"),
     (dict(ldr=31), "ldr"), (dict(A=None), "NULL"), (dict(sa=None), "NULL"), (dict(panel=None), "NULL"),
     (dict(C=None), "NULL"), (dict(res=None), "NULL"), (dict(A=P + 8), "aligned"), (dict(panel=P + 8), "aligned"),
     (dict(C=P + 1), "aligned"), (dict(res=P + 1), "aligned"), (dict(sa=P + 2), "aligned"), (dict(sb=P + 2), "aligned"),

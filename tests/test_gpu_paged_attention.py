@@ -278,6 +278,47 @@ def test_a_step_writes_then_attends():
             Call(cache, q, "f32", table, lens, steps, 0.125, 0).check(q, table, lens)
 
 
+def test_a_cache_past_4_gib():
+    """The last pages of 4.5 GiB of keys and of values: element offsets beyond 32 bits."""
+    import torch
+    heads, dim, page, n = 8, 256, 256, 300
+    pages = (9 << 29) // (heads * dim * page)
+    k = torch.zeros((pages * heads * page * dim,), dtype=torch.int8, device="cuda:0")
+    v = torch.zeros_like(k)
+    ks, vs = (torch.zeros((pages * heads * page,), device="cuda:0") for _ in range(2))
+    c = pk.KvCache(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), pk.I8, pages, page, heads, dim)
+    table = torch.tensor([[pages - 1, pages - 2]], dtype=torch.int32, device="cuda:0")
+    slots = (table[0].repeat_interleave(page) * page + torch.arange(page, device="cuda:0").repeat(2))[:n].int()
+    wide = heads * dim
+    x, y = (torch.randn((n, wide), device="cuda:0") for _ in range(2))
+    pk.call("pk_gpu_kv_write_dev", do.ref(c), pk.F32, x.data_ptr(), wide, y.data_ptr(), wide, slots.data_ptr(), n,
+            do.stream())
+    rk, rv = torch.empty_like(x), torch.empty_like(y)
+    pk.call("pk_gpu_kv_read_dev", do.ref(c), pk.F32, slots.data_ptr(), n, rk.data_ptr(), wide, rv.data_ptr(), wide,
+            do.stream())
+    q = torch.randn((1, wide), device="cuda:0")
+    out = torch.zeros_like(q)
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda:0")
+    floats = pk.load().pk_gpu_paged_attention_ws_floats(do.ref(c), 1, heads, n, 0)
+    ws = torch.empty((floats + 4,), device="cuda:0")
+    pk.call("pk_gpu_paged_attention_dev", do.ref(c), pk.F32, q.data_ptr(), wide, heads, table.data_ptr(), 2,
+            lens.data_ptr(), 1, n, 0.0625, 0, out.data_ptr(), wide, None, ws.data_ptr(), floats, do.stream())
+    torch.cuda.synchronize()
+
+    class Rows:          # what the cache's rows stand for, by token
+        pass
+    r = Rows()
+    r.heads, r.page, r.pages, r.dim, r.kind = heads, 1, n, dim, "int8"
+    back = {"k": do.values(rk).reshape(n, heads, dim), "v": do.values(rv).reshape(n, heads, dim)}
+    r.rows = back.__getitem__
+    qh = do.values(q).reshape(1, heads, dim)
+    want, _, a, s, xx = do.attention(r, qh, np.arange(n)[None], [n], n, 0.0625, 0)
+    err = np.abs(do.values(out).reshape(1, heads, dim) - want)
+    # the rows read back are rounded once more than the kernel's codes * scale
+    assert np.all(err <= do.attention_bound(want, a, s, xx, n, dim, "int8", "f32") +
+                  2.0 ** -23 * (1 + 2 * xx[..., None]) * a)
+
+
 def test_no_sequences():
     cache = do.Cache("int8", 2, 1, 16, 64)
     pk.call("pk_gpu_paged_attention_dev", do.ref(cache.struct()), pk.F32, None, 64, 1, None, 2, None, 0, 32, 1.0, 0,

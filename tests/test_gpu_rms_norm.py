@@ -50,6 +50,7 @@ CASES = [
     (2, 4095, "bf16", "int8", True, True, True, 1, 0), (5, 4096, "f16", "f16", True, False, True, 0, 0),
     (3, 4097, "f32", "int8", True, True, True, 0, 0), (2, 4097, "f32", "int8", True, False, True, 0, 0),
     (2, 8192, "f32", "int8", False, False, False, 0, 0), (2, 8200, "bf16", "bf16", True, True, True, 0, 0),
+    (3, 16384, "f32", "int8", True, True, True, 0, 0), (2, 16392, "bf16", "f32", True, False, True, 0, 0),
     (1, 50001, "f16", "int8", True, False, True, 0, 0), (9000, 24, "bf16", "int8", True, True, True, 0, 0),
     (5001, 2304, "bf16", "bf16", True, True, True, 0, 0),
 ]
