@@ -90,10 +90,11 @@ __device__ __host__ inline Span span_of(int len, int max_len, int window, int ch
 }
 
 // Waves of a workgroup, all of one chunk.  8 keep one CU's share of the memory
-// busy by themselves, so that 128 or more pairs need not be split at all; the
-// kernel with most registers (16-bit keys and values of 256, queries in 3
-// terms) runs one wave a SIMD.
-constexpr int waves_of(int cache, int t, int dim) { return cache == BF16 && t == F32 && dim == 256 ? 4 : 8; }
+// busy by themselves, so that 128 or more pairs need not be split at all.  The
+// kernels with most registers (heads of 256, queries in 3 terms) run one wave a
+// SIMD: 64 sequences of 2000 tokens, 2 heads of 256 in int8, f32 queries 34.8 us;
+// 8 waves, which spill, 44.
+constexpr int waves_of(int cache, int t, int dim) { return t == F32 && dim == 256 ? 4 : 8; }
 
 // The sequence with nth sequences before it in order of falling length (ties
 // by index), counted by every workgroup for itself: lens of the launch's up to
@@ -109,6 +110,7 @@ __device__ inline int nth_longest(const PagedArgs& a, int nth, int* lens, int wa
     __syncthreads();
     int rank = 0;
     if (64 * wave < a.B) {
+#pragma unroll 1
         for (int q = 0; q < quads; ++q) {
             const i32x4 l = reinterpret_cast<const i32x4*>(lens)[q];
 #pragma unroll
