@@ -158,6 +158,44 @@ __device__ inline RowCode row_code(uint32_t amax_bits, float top)
 // x * inv, 0 where the row has no codes (x may be NaN or infinite there)
 __device__ inline float coded(float x, RowCode c) { return c.inv == 0.0f ? 0.0f : __fmul_rn(x, c.inv); }
 
+// x of the lane's partner among 2, 4, 8 or 16 lanes (STEP 1, 2, 4, 8) where the
+// lanes of each half group hold the same value already: mirrors of the group, so
+// a few cycles in the vector unit instead of a trip through LDS.
+template <int STEP>
+__device__ inline uint32_t mirrored(uint32_t x)
+{
+    constexpr int CTRL = STEP == 1 ? 0xB1 : STEP == 2 ? 0x4E : STEP == 4 ? 0x141 : 0x140;
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xF, 0xF, true);
+}
+template <int STEP>
+__device__ inline uint32_t partner(uint32_t x)
+{
+    if constexpr (STEP < 16) return mirrored<STEP>(x);
+    else return __shfl_xor(x, STEP);
+}
+// The largest over aligned groups of LANES lanes.
+template <int LANES, int STEP = 1>
+__device__ inline uint32_t max_over(uint32_t x)
+{
+    if constexpr (STEP < LANES) {
+        const uint32_t o = partner<STEP>(x);
+        return max_over<LANES, 2 * STEP>(o > x ? o : x);
+    } else {
+        return x;
+    }
+}
+// The sum over the wave, the same on every lane (a + b = b + a).
+template <int STEP = 1>
+__device__ inline double sum_over_wave(double x)
+{
+    if constexpr (STEP < 64) {
+        const uint32_t lo = partner<STEP>((uint32_t)__double2loint(x)), hi = partner<STEP>((uint32_t)__double2hiint(x));
+        return sum_over_wave<2 * STEP>(x + __hiloint2double((int)hi, (int)lo));
+    } else {
+        return x;
+    }
+}
+
 // ---- host ------------------------------------------------------------------
 
 // One entry point's time on the library's device: initialises the library if

@@ -41,17 +41,6 @@ __device__ inline long long cache_row(const RowsArgs& a, uint32_t token, uint32_
     return ((long long)page * a.heads + head) * a.page_size + off;
 }
 
-template <int DIM>
-__device__ inline uint32_t group_max(uint32_t m)
-{
-#pragma unroll
-    for (int d = 1; d < DIM / 8; d *= 2) {
-        const uint32_t o = __shfl_xor(m, d);
-        m = o > m ? o : m;
-    }
-    return m;
-}
-
 __device__ inline uint32_t max_bits(const float* x)
 {
     uint32_t m = 0;
@@ -68,7 +57,7 @@ template <int CACHE, int DIM>
 __device__ inline void write_part(void* cache, float* scales, long long row, int part, float* x)
 {
     if constexpr (CACHE == I8 || CACHE == E4M3) {
-        const RowCode c = row_code(group_max<DIM>(max_bits(x)), top_of(CACHE));
+        const RowCode c = row_code(max_over<DIM / 8>(max_bits(x)), top_of(CACHE));
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = coded(x[i], c);
         if (row >= 0 && part == 0) scales[row] = c.scale;

@@ -36,22 +36,6 @@ struct NormArgs {
 
 constexpr int kNormThreads = 256;
 
-__device__ inline double wave_sum(double v)
-{
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v = v + __shfl_xor(v, d);
-    return v;
-}
-__device__ inline uint32_t wave_max(uint32_t v)
-{
-#pragma unroll
-    for (int d = 32; d; d >>= 1) {
-        const uint32_t o = __shfl_xor(v, d);
-        v = o > v ? o : v;
-    }
-    return v;
-}
-
 __device__ inline float norm_factor(double sum, int D, double eps)
 {
     return (float)(1.0 / __dsqrt_rn(sum / (double)D + eps));
@@ -117,13 +101,6 @@ __global__ void __launch_bounds__(norm_threads(TPR)) rms_norm(NormArgs a)
     __shared__ double red_sum[2][WAVES];
     __shared__ uint32_t red_max[2][WAVES];
     const int t = threadIdx.x % TPR, wave = threadIdx.x / 64;
-    float gm[CH][W];
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        const int i = (c * TPR + t) * W;
-#pragma unroll
-        for (int j = 0; j < W; ++j) gm[c][j] = a.gamma && i < a.D ? a.gamma[i + j] : 1.0f;
-    }
     // the next row's pieces are on their way while this one is summed
     Piece<T, W> nx[CH], nr[CH];
     auto ask = [&](long long row) {
@@ -138,6 +115,14 @@ __global__ void __launch_bounds__(norm_threads(TPR)) rms_norm(NormArgs a)
     };
     const long long stride = (long long)gridDim.x * RPB;
     ask((long long)blockIdx.x * RPB + threadIdx.x / TPR);
+    float gm[CH][W];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int i = (c * TPR + t) * W;
+#pragma unroll
+        for (int j = 0; j < W; ++j) gm[c][j] = 1.0f;
+        if (a.gamma && i < a.D) load_piece<F32, W>(reinterpret_cast<const char*>(a.gamma), i, gm[c]);
+    }
     int turn = 0;
     for (long long r0 = (long long)blockIdx.x * RPB; r0 < a.rows; r0 += stride, turn ^= 1) {
         const long long row = r0 + threadIdx.x / TPR;
@@ -167,7 +152,7 @@ __global__ void __launch_bounds__(norm_threads(TPR)) rms_norm(NormArgs a)
 #pragma unroll
             for (int j = 0; j < W; ++j) sum = __fma_rn((double)h[c][j], (double)h[c][j], sum);
         }
-        sum = wave_sum(sum);
+        sum = sum_over_wave(sum);
         if constexpr (TPR > 64) {
             if (threadIdx.x % 64 == 0) red_sum[turn][wave] = sum;
             __syncthreads();
@@ -188,7 +173,7 @@ __global__ void __launch_bounds__(norm_threads(TPR)) rms_norm(NormArgs a)
                 }
             }
         if constexpr (OUT == I8) {
-            top = wave_max(top);
+            top = max_over<64>(top);
             if constexpr (TPR > 64) {
                 if (threadIdx.x % 64 == 0) red_max[turn][wave] = top;
                 __syncthreads();
@@ -226,7 +211,7 @@ __global__ void __launch_bounds__(1024) rms_norm_long(NormArgs a)
             if (a.sum) store1<T>(a.sum + row * a.lds, i, h);
             sum = __fma_rn((double)h, (double)h, sum);
         }
-        sum = wave_sum(sum);
+        sum = sum_over_wave(sum);
         __syncthreads();                                  // the last row's readers are done
         if (threadIdx.x % 64 == 0) red_sum[wave] = sum;
         __syncthreads();
@@ -247,7 +232,7 @@ __global__ void __launch_bounds__(1024) rms_norm_long(NormArgs a)
                 const uint32_t b = __float_as_uint(value(i)) & 0x7fffffffu;
                 top = b > top ? b : top;
             }
-            top = wave_max(top);
+            top = max_over<64>(top);
             if (threadIdx.x % 64 == 0) red_max[wave] = top;
             __syncthreads();
 #pragma unroll
@@ -269,7 +254,7 @@ template <int T, int OUT>
 hipError_t launch_norm(const NormArgs& a, bool wide, hipStream_t s)
 {
     // 1024 workgroups of wide rows, each with the next row on its way (8192 rows of
-    // 4096 in bf16 with residual and sum: 52 us, 5.1 TB/s; 2048 workgroups 57, 512 59,
+    // 4096 in bf16 with residual and sum: 50.5 us, 5.3 TB/s; 2048 workgroups 57, 512 59,
     // 4096 without the next row 62); rows of single elements want more in flight
     // (8192 of 2047 in bf16: 4096 workgroups 46 us, one a row 52).
     const auto grid = [&](int rows_each) {
@@ -354,7 +339,7 @@ extern "C" int pk_gpu_rms_norm_dev(int dtype, const void* dx, int ldx, const voi
     const auto fits = [](const void* p, size_t ld, size_t bytes) {
         return aligned(p, bytes) && ld % bytes == 0;
     };
-    const bool wide = D % 8 == 0 && fits(dx, a.ldx, 16) && (!dres || fits(dres, a.ldr, 16)) &&
+    const bool wide = D % 8 == 0 && aligned16(dgamma) && fits(dx, a.ldx, 16) && (!dres || fits(dres, a.ldr, 16)) &&
                       (!dsum || fits(dsum, a.lds, 16)) && fits(dout, a.ldo, out_dtype == I8 ? 8 : 16);
     hipStream_t s = static_cast<hipStream_t>(stream);
     const hipError_t e = dtype == F32   ? launch_out<F32>(out_dtype, a, wide, s)
