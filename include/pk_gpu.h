@@ -505,8 +505,7 @@ int pk_gpu_paged_attention_dev(const pk_gpu_kv_cache *cache, int dtype, const vo
  * gamma NULL counts as ones; dscales is used for I8 only.  Leading dimensions in
  * elements; what lies between rows is not touched.  sum may be x or res in
  * place; so may out where its elements are as wide; other overlaps are the
- * caller's error.  Any alignment of whole elements; rows that are 16-byte aligned
- * with D a multiple of 8 are the fast ones. */
+ * caller's error.  Any alignment of whole elements. */
 int pk_gpu_rms_norm_dev(int dtype, const void *dx, int ldx, const void *dres, int ldr, void *dsum,
                         int lds, const float *dgamma, float eps, int out_dtype, void *dout, int ldo,
                         float *dscales, int rows, int D, void *stream);

@@ -36,6 +36,13 @@ using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
 using f32x2 = __attribute__((ext_vector_type(2))) float;
 
+// The same vectors at an address that is only aligned to their elements: the
+// compiler keeps them one access (global memory takes any alignment on this
+// target), which may touch one cache line more.
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+
 // element types as template parameters
 constexpr int F32 = PK_GPU_F32, F16 = PK_GPU_F16, BF16 = PK_GPU_BF16, I8 = PK_GPU_I8, E4M3 = PK_GPU_E4M3;
 constexpr int size_of(int t) { return t == F32 ? 4 : t == F16 || t == BF16 ? 2 : 1; }

@@ -13,10 +13,13 @@
 // shapes.  The fp64 work is two instructions an element.
 //
 // A row stays in registers between its statistics and its output: TPR threads
-// (a wave, or a workgroup of 4 or 16) hold CH pieces of W consecutive elements
-// each.  Rows that are not 16-byte aligned (odd D) take W = 1.  Longer rows
-// (above 16384, or 4096 single elements) are read again for each pass.  Bound by
-// the rows' bytes.
+// (a wave, or a workgroup of 4 or 16) hold CH pieces of 8 consecutive elements
+// each.  Pieces are read and written whole whatever their alignment (rows of odd
+// D begin anywhere): 8192 rows of 2047 in bf16 31 us, 46 by single elements.
+// Rows above 16384 are read again for each pass.  Sums and
+// maxima over a wave go by mirrors of lane groups in the vector unit (33 rows of
+// 1024: 3.1 us; 4.7 through LDS).  Bound by the rows' bytes, for few rows by the
+// launch and one load's latency.
 #include "pk_decode.h"
 
 namespace pkgpu {
@@ -41,75 +44,88 @@ __device__ inline float norm_factor(double sum, int D, double eps)
     return (float)(1.0 / __dsqrt_rn(sum / (double)D + eps));
 }
 
-template <int T, int W>
-__device__ inline void load_piece(const char* p, size_t i, float* v)
-{
-    if constexpr (W == 8) load8<T>(p + i * size_of(T), v);
-    else v[0] = load1<T>(p, i);
-}
-template <int T, int W>
-__device__ inline void store_piece(char* p, size_t i, const float* v)
-{
-    if constexpr (W == 8) store8<T>(p + i * size_of(T), v);
-    else if constexpr (T == I8) reinterpret_cast<signed char*>(p)[i] = (signed char)(int)__builtin_rintf(v[0]);
-    else store1<T>(p, i, v[0]);
-}
-
-// W elements as they lie in memory
-template <int T, int W>
+// 8 elements of a row, from element i on, as they lie in memory; at the `edge`,
+// a constant of the unrolled loops, the row's last piece may have n < 8 of them.
+// (Loads on a condition make every wait longer, so there is a kernel without
+// them for D % 8 == 0.)  Rows are aligned to their elements only.
+template <int T>
 struct Piece {
-    static constexpr int WORDS = W == 8 ? size_of(T) / 2 : 1;
+    static constexpr int WORDS = size_of(T) / 2;
     u32x4 w[WORDS];
-    __device__ void load(const char* p, size_t i)
+    __device__ inline __attribute__((always_inline)) void load(const char* p, int i, int n, bool edge)
     {
-        if constexpr (W == 8) {
+        p += (size_t)i * size_of(T);
+        if (!edge || n >= 8) {
 #pragma unroll
-            for (int k = 0; k < WORDS; ++k) w[k] = reinterpret_cast<const u32x4*>(p + i * size_of(T))[k];
-        } else if constexpr (T == F32) {
-            w[0][0] = reinterpret_cast<const uint32_t*>(p)[i];
+            for (int k = 0; k < WORDS; ++k) w[k] = reinterpret_cast<const u32x4_any*>(p)[k];
         } else {
-            w[0][0] = reinterpret_cast<const uint16_t*>(p)[i];
+            uint32_t e[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                e[j] = j >= n ? 0u : T == F32 ? reinterpret_cast<const uint32_t*>(p)[j]
+                                              : reinterpret_cast<const uint16_t*>(p)[j];
+#pragma unroll
+            for (int j = 0; j < 4 * WORDS; ++j) w[j / 4][j % 4] = T == F32 ? e[j] : e[2 * (j % 4)] | e[2 * (j % 4) + 1] << 16;
         }
     }
-    __device__ void values(float* x) const
-    {
-        if constexpr (W == 8) load8<T>(w, x);
-        else load_piece<T, 1>(reinterpret_cast<const char*>(w), 0, x);
-    }
+    __device__ void values(float* x) const { load8<T>(w, x); }
 };
 
-// h of W elements, stored where the caller wants it
-template <int T, int W>
-__device__ inline void load_sum(const NormArgs& a, size_t row, size_t i, float* h)
+template <int T>
+__device__ inline __attribute__((always_inline)) void store_piece(char* p, int i, int n, const float* x, bool edge)
 {
-    load_piece<T, W>(a.x + row * a.ldx, i, h);
-    if (a.res) {
-        float v[W];
-        load_piece<T, W>(a.res + row * a.ldr, i, v);
+    p += (size_t)i * size_of(T);
+    if (!edge || n >= 8) {
+        u32x4 w[T == F32 ? 2 : 1];
+        store8<T>(w, x);
+        if constexpr (T == I8) {
+            *reinterpret_cast<u32x2_any*>(p) = (u32x2){w[0][0], w[0][1]};
+        } else {
 #pragma unroll
-        for (int j = 0; j < W; ++j) h[j] = as_type<T>(__fadd_rn(h[j], v[j]));
+            for (int k = 0; k < (T == F32 ? 2 : 1); ++k) reinterpret_cast<u32x4_any*>(p)[k] = w[k];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 7; ++j)
+            if (j < n) {
+                if constexpr (T == I8) reinterpret_cast<signed char*>(p)[j] = (signed char)(int)__builtin_rintf(x[j]);
+                else store1<T>(p, j, x[j]);
+            }
     }
+}
+
+// one element of h, for the rows that are read again
+template <int T>
+__device__ inline float sum_at(const NormArgs& a, size_t row, int i)
+{
+    float h = load1<T>(a.x + row * a.ldx, i);
+    if (a.res) h = as_type<T>(__fadd_rn(h, load1<T>(a.res + row * a.ldr, i)));
+    return h;
 }
 
 constexpr int norm_threads(int tpr) { return tpr > kNormThreads ? tpr : kNormThreads; }
 
-template <int T, int OUT, int TPR, int CH, int W>
+template <int T, int OUT, int TPR, int CH, bool EDGE>
 __global__ void __launch_bounds__(norm_threads(TPR)) rms_norm(NormArgs a)
 {
     constexpr int RPB = norm_threads(TPR) / TPR;         // rows a workgroup has at a time
     constexpr int WAVES = norm_threads(TPR) / 64;
     __shared__ double red_sum[2][WAVES];
     __shared__ uint32_t red_max[2][WAVES];
+    constexpr int W = 8;
+    // only rows of more than CH / 2 * TPR pieces come here (launch_norm), so the first
+    // CH / 2 of a thread's are whole ones
+    const auto at_edge = [](int c) { return EDGE && (CH == 1 || c >= CH / 2); };
     const int t = threadIdx.x % TPR, wave = threadIdx.x / 64;
     // the next row's pieces are on their way while this one is summed
-    Piece<T, W> nx[CH], nr[CH];
+    Piece<T> nx[CH], nr[CH];
     auto ask = [&](long long row) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int i = (c * TPR + t) * W;
             if (row < a.rows && i < a.D) {
-                nx[c].load(a.x + row * a.ldx, i);
-                if (a.res) nr[c].load(a.res + row * a.ldr, i);
+                nx[c].load(a.x + row * a.ldx, i, a.D - i, at_edge(c));
+                if (a.res) nr[c].load(a.res + row * a.ldr, i, a.D - i, at_edge(c));
             }
         }
     };
@@ -121,7 +137,11 @@ __global__ void __launch_bounds__(norm_threads(TPR)) rms_norm(NormArgs a)
         const int i = (c * TPR + t) * W;
 #pragma unroll
         for (int j = 0; j < W; ++j) gm[c][j] = 1.0f;
-        if (a.gamma && i < a.D) load_piece<F32, W>(reinterpret_cast<const char*>(a.gamma), i, gm[c]);
+        if (a.gamma && i < a.D) {
+            Piece<F32> g;
+            g.load(reinterpret_cast<const char*>(a.gamma), i, a.D - i, at_edge(c));
+            g.values(gm[c]);
+        }
     }
     int turn = 0;
     for (long long r0 = (long long)blockIdx.x * RPB; r0 < a.rows; r0 += stride, turn ^= 1) {
@@ -148,7 +168,7 @@ __global__ void __launch_bounds__(norm_threads(TPR)) rms_norm(NormArgs a)
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int i = (c * TPR + t) * W;
-            if (a.sum && live && i < a.D) store_piece<T, W>(a.sum + row * a.lds, i, h[c]);
+            if (a.sum && live && i < a.D) store_piece<T>(a.sum + row * a.lds, i, a.D - i, h[c], at_edge(c));
 #pragma unroll
             for (int j = 0; j < W; ++j) sum = __fma_rn((double)h[c][j], (double)h[c][j], sum);
         }
@@ -190,7 +210,7 @@ __global__ void __launch_bounds__(norm_threads(TPR)) rms_norm(NormArgs a)
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int i = (c * TPR + t) * W;
-            if (live && i < a.D) store_piece<OUT, W>(a.out + row * a.ldo, i, h[c]);
+            if (live && i < a.D) store_piece<OUT>(a.out + row * a.ldo, i, a.D - i, h[c], at_edge(c));
         }
     }
 }
@@ -206,8 +226,7 @@ __global__ void __launch_bounds__(1024) rms_norm_long(NormArgs a)
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         double sum = 0.0;
         for (int i = threadIdx.x; i < a.D; i += 1024) {
-            float h;
-            load_sum<T, 1>(a, row, i, &h);
+            const float h = sum_at<T>(a, row, i);
             if (a.sum) store1<T>(a.sum + row * a.lds, i, h);
             sum = __fma_rn((double)h, (double)h, sum);
         }
@@ -220,9 +239,7 @@ __global__ void __launch_bounds__(1024) rms_norm_long(NormArgs a)
         for (int w = 0; w < 16; ++w) sum = sum + red_sum[w];
         const float r = norm_factor(sum, a.D, a.eps);
         auto value = [&](int i) {
-            float h;
-            if (a.sum) h = load1<T>(a.sum + row * a.lds, i);
-            else load_sum<T, 1>(a, row, i, &h);
+            const float h = a.sum ? load1<T>(a.sum + row * a.lds, i) : sum_at<T>(a, row, i);
             return __fmul_rn(__fmul_rn(h, r), a.gamma ? a.gamma[i] : 1.0f);
         };
         RowCode code{};
@@ -243,49 +260,45 @@ __global__ void __launch_bounds__(1024) rms_norm_long(NormArgs a)
         for (int i = threadIdx.x; i < a.D; i += 1024) {
             float y = value(i);
             if constexpr (OUT == I8) y = coded(y, code);
-            store_piece<OUT, 1>(a.out + row * a.ldo, i, &y);
+            store_piece<OUT>(a.out + row * a.ldo, i, 1, &y, true);
         }
     }
 }
 
-// A wave a row while its pieces fit 4 a lane (8 elements each; 16 single ones),
-// else a workgroup.
-template <int T, int OUT>
-hipError_t launch_norm(const NormArgs& a, bool wide, hipStream_t s)
+// A wave a row while its pieces fit 4 a lane, else a workgroup.  1024 workgroups,
+// each with the next row on its way (8192 rows of 4096 in bf16 with residual and
+// sum: 50.5 us, 5.3 TB/s; 2048 workgroups 57, 512 59, 4096 without the next row 62).
+template <int T, int OUT, bool EDGE>
+hipError_t launch_norm(const NormArgs& a, hipStream_t s)
 {
-    // 1024 workgroups of wide rows, each with the next row on its way (8192 rows of
-    // 4096 in bf16 with residual and sum: 50.5 us, 5.3 TB/s; 2048 workgroups 57, 512 59,
-    // 4096 without the next row 62); rows of single elements want more in flight
-    // (8192 of 2047 in bf16: 4096 workgroups 46 us, one a row 52).
     const auto grid = [&](int rows_each) {
         const long long n = ((long long)a.rows + rows_each - 1) / rows_each;
-        const long long most = wide ? 1024 : 4096;
-        return dim3((uint32_t)(n < most ? n : most));
+        return dim3((uint32_t)(n < 1024 ? n : 1024));
     };
     const dim3 block(kNormThreads);
-    if (wide) {
-        const int pieces = a.D / 8;
-        if (pieces <= 64) return launch(rms_norm<T, OUT, 64, 1, 8>, grid(4), block, 0, s, a);
-        if (pieces <= 128) return launch(rms_norm<T, OUT, 64, 2, 8>, grid(4), block, 0, s, a);
-        if (pieces <= 256) return launch(rms_norm<T, OUT, 64, 4, 8>, grid(4), block, 0, s, a);
-        if (pieces <= 512) return launch(rms_norm<T, OUT, 256, 2, 8>, grid(1), block, 0, s, a);
-        if (pieces <= 1024) return launch(rms_norm<T, OUT, 256, 4, 8>, grid(1), block, 0, s, a);
-        if (pieces <= 2048) return launch(rms_norm<T, OUT, 1024, 2, 8>, grid(1), dim3(1024), 0, s, a);
-    } else {
-        if (a.D <= 512) return launch(rms_norm<T, OUT, 64, 8, 1>, grid(4), block, 0, s, a);
-        if (a.D <= 1024) return launch(rms_norm<T, OUT, 64, 16, 1>, grid(4), block, 0, s, a);
-        if (a.D <= 4096) return launch(rms_norm<T, OUT, 256, 16, 1>, grid(1), block, 0, s, a);
-    }
+    const int pieces = a.D / 8 + (a.D % 8 != 0);
+    if (pieces <= 64) return launch(rms_norm<T, OUT, 64, 1, EDGE>, grid(4), block, 0, s, a);
+    if (pieces <= 128) return launch(rms_norm<T, OUT, 64, 2, EDGE>, grid(4), block, 0, s, a);
+    if (pieces <= 256) return launch(rms_norm<T, OUT, 64, 4, EDGE>, grid(4), block, 0, s, a);
+    if (pieces <= 512) return launch(rms_norm<T, OUT, 256, 2, EDGE>, grid(1), block, 0, s, a);
+    if (pieces <= 1024) return launch(rms_norm<T, OUT, 256, 4, EDGE>, grid(1), block, 0, s, a);
+    if (pieces <= 2048) return launch(rms_norm<T, OUT, 1024, 2, EDGE>, grid(1), dim3(1024), 0, s, a);
     return launch(rms_norm_long<T, OUT>, grid(1), dim3(1024), 0, s, a);
 }
 
-template <int T>
-hipError_t launch_out(int out, const NormArgs& a, bool wide, hipStream_t s)
+template <int T, int OUT>
+hipError_t launch_edge(const NormArgs& a, hipStream_t s)
 {
-    return out == I8    ? launch_norm<T, I8>(a, wide, s)
-           : out == F32 ? launch_norm<T, F32>(a, wide, s)
-           : out == F16 ? launch_norm<T, F16>(a, wide, s)
-                        : launch_norm<T, BF16>(a, wide, s);
+    return a.D % 8 ? launch_norm<T, OUT, true>(a, s) : launch_norm<T, OUT, false>(a, s);
+}
+
+template <int T>
+hipError_t launch_out(int out, const NormArgs& a, hipStream_t s)
+{
+    return out == I8    ? launch_edge<T, I8>(a, s)
+           : out == F32 ? launch_edge<T, F32>(a, s)
+           : out == F16 ? launch_edge<T, F16>(a, s)
+                        : launch_edge<T, BF16>(a, s);
 }
 
 }  // namespace
@@ -335,15 +348,9 @@ extern "C" int pk_gpu_rms_norm_dev(int dtype, const void* dx, int ldx, const voi
     a.eps = (double)eps;
     a.rows = rows;
     a.D = D;
-    // 8 elements at a time: whole pieces, all of them aligned (codes: 8 bytes)
-    const auto fits = [](const void* p, size_t ld, size_t bytes) {
-        return aligned(p, bytes) && ld % bytes == 0;
-    };
-    const bool wide = D % 8 == 0 && aligned16(dgamma) && fits(dx, a.ldx, 16) && (!dres || fits(dres, a.ldr, 16)) &&
-                      (!dsum || fits(dsum, a.lds, 16)) && fits(dout, a.ldo, out_dtype == I8 ? 8 : 16);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const hipError_t e = dtype == F32   ? launch_out<F32>(out_dtype, a, wide, s)
-                         : dtype == F16 ? launch_out<F16>(out_dtype, a, wide, s)
-                                        : launch_out<BF16>(out_dtype, a, wide, s);
+    const hipError_t e = dtype == F32   ? launch_out<F32>(out_dtype, a, s)
+                         : dtype == F16 ? launch_out<F16>(out_dtype, a, s)
+                                        : launch_out<BF16>(out_dtype, a, s);
     return e == hipSuccess ? PK_GPU_OK : rt::hip_error(e, who);
 }

@@ -45,7 +45,6 @@ struct W8Args {
     float sb1;
     int M, N, K, kb;                // kb: blocks of 64 of K in the panel
     int epi;
-    int vec;                        // C and the residual take 4 columns at a time
     int mt, nt;                     // tiles
 };
 
@@ -121,14 +120,14 @@ __device__ inline Columns columns_of(const W8Args& a, int j)
     Columns c;
 #pragma unroll
     for (int e = 0; e < 4; ++e) { c.s[e] = a.sb1; c.b[e] = 0.0f; }
-    if (a.vec && j + 4 <= a.N) {
+    if (j + 4 <= a.N) {
         if (a.sb) {
-            const f32x4 s = *reinterpret_cast<const f32x4*>(a.sb + j);
+            const f32x4 s = *reinterpret_cast<const f32x4_any*>(a.sb + j);
 #pragma unroll
             for (int e = 0; e < 4; ++e) c.s[e] = s[e];
         }
         if (a.bias) {
-            const f32x4 b = *reinterpret_cast<const f32x4*>(a.bias + j);
+            const f32x4 b = *reinterpret_cast<const f32x4_any*>(a.bias + j);
 #pragma unroll
             for (int e = 0; e < 4; ++e) c.b[e] = b[e];
         }
@@ -157,14 +156,14 @@ __device__ inline void store_c(const W8Args& a, int i, float sa, int j, const Co
         v[e] = __fmul_rn((float)acc[e], __fmul_rn(sa, col.s[e]));
         if (a.bias) v[e] = __fadd_rn(v[e], col.b[e]);
     }
-    if (a.vec && j + 4 <= a.N) {
+    if (j + 4 <= a.N) {                // whole accesses at any alignment
         if constexpr (residual) {
             if constexpr (T == F32) {
-                const f32x4 o = *reinterpret_cast<const f32x4*>(r + (size_t)j * 4);
+                const f32x4 o = *reinterpret_cast<const f32x4_any*>(r + (size_t)j * 4);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) old[e] = o[e];
             } else {
-                const u32x2 o = *reinterpret_cast<const u32x2*>(r + (size_t)j * 2);
+                const u32x2 o = *reinterpret_cast<const u32x2_any*>(r + (size_t)j * 2);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const uint32_t w = o[e];       // a bit cast of o[e] itself takes o[0]'s bits
@@ -177,9 +176,9 @@ __device__ inline void store_c(const W8Args& a, int i, float sa, int j, const Co
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = finish<T, EPI>(v[e], old[e]);
         if constexpr (T == F32)
-            *reinterpret_cast<f32x4*>(c + (size_t)j * 4) = (f32x4){v[0], v[1], v[2], v[3]};
+            *reinterpret_cast<f32x4_any*>(c + (size_t)j * 4) = (f32x4){v[0], v[1], v[2], v[3]};
         else
-            *reinterpret_cast<u32x2*>(c + (size_t)j * 2) =
+            *reinterpret_cast<u32x2_any*>(c + (size_t)j * 2) =
                 T == F16 ? (u32x2){pack_f16(v[0], v[1]), pack_f16(v[2], v[3])}
                          : (u32x2){pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
         return;
@@ -520,8 +519,6 @@ int pk_gpu_gemm_w8a8_dev(int M, int N, int K, const int8_t* dA, int lda, const f
     a.M = M; a.N = N; a.K = K;
     a.kb = (K + 127) / 128 * 2;
     a.epi = epilogue;
-    const size_t run = 4 * es;
-    a.vec = !off(dB_scales, 16) && !off(dbias, 16) && !off(dC, run) && a.ldc % run == 0 && (!residual || (!off(dres, run) && a.ldr % run == 0));
     hipStream_t s = static_cast<hipStream_t>(stream);
     const hipError_t e = dtype == F32 ? launch_epi<F32>(a, s) : dtype == F16 ? launch_epi<F16>(a, s) : launch_epi<BF16>(a, s);
     if (e == hipErrorInvalidValue) return rt::error(PK_GPU_EINVAL, "%s: %d x %d exceeds the grid", who, M, N);
