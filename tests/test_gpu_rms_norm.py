@@ -51,6 +51,11 @@ CASES = [
     (3, 4097, "f32", "int8", True, True, True, 0, 0), (2, 4097, "f32", "int8", True, False, True, 0, 0),
     (2, 8192, "f32", "int8", False, False, False, 0, 0), (2, 8200, "bf16", "bf16", True, True, True, 0, 0),
     (3, 16384, "f32", "int8", True, True, True, 0, 0), (2, 16392, "bf16", "f32", True, False, True, 0, 0),
+    # the borders of each number of pieces a thread holds, not whole pieces
+    (5, 7, "f16", "int8", True, True, True, 0, 0), (6, 1025, "bf16", "int8", True, True, True, 0, 3),
+    (5, 2047, "f32", "bf16", True, True, True, 1, 1), (3, 2049, "f16", "int8", True, True, True, 0, 0),
+    (3, 8191, "bf16", "f32", True, True, True, 0, 1), (3, 8193, "bf16", "int8", True, True, True, 2, 0),
+    (2, 16383, "f32", "int8", True, True, True, 0, 0), (2050, 1030, "f16", "int8", True, True, True, 0, 0),
     (1, 50001, "f16", "int8", True, False, True, 0, 0), (9000, 24, "bf16", "int8", True, True, True, 0, 0),
     (5001, 2304, "bf16", "bf16", True, True, True, 0, 0),
 ]
