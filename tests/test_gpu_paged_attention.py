@@ -259,6 +259,44 @@ def test_two_graphs_and_a_second_stream():
             assert np.array_equal(do.values(c.out)[:B, :c.wide].reshape(w.shape), w)
 
 
+def test_two_graphs_take_turns_with_one_workspace():
+    """Two captured calls that share a workspace, replayed one after the other on one stream in
+    changing order, with eager calls in between that share it too."""
+    import torch
+    rng = np.random.default_rng(15)
+    B, kv, group, dim, page = 2, 2, 4, 64, 16
+    calls, graphs = [], []
+    s = torch.cuda.Stream()
+    for i, most in enumerate((1500, 4000)):
+        per = (most + page - 1) // page
+        cache = do.Cache("e4m3", B * per, kv, page, dim, seed=30 + i)
+        table = tables(rng, cache, B, per)
+        q = queries(rng, B, kv * group, dim, "f32")
+        calls.append(Call(cache, q, "f32", table, [most, 777], most, 0.125, 0))
+    floats = max(c.floats for c in calls)
+    shared = torch.full((floats + 64,), float("nan"), device="cuda:0")
+    want = [c.run() for c in calls]
+    for c in calls:
+        c.ws = shared
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=s):
+            c.enqueue(s.cuda_stream)
+        graphs.append(g)
+    for order in ((0, 1), (1, 0), (1, 1, 0)):
+        for c in calls:
+            c.out[:B].zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            for i in order:
+                graphs[i].replay()
+                calls[1 - i].enqueue(s.cuda_stream)
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        for c, w in zip(calls, want):
+            assert np.array_equal(do.values(c.out)[:B, :c.wide].reshape(w.shape), w)
+
+
 def test_a_step_writes_then_attends():
     """The operators as a decoder uses them: 40 steps of write + attend from an empty int8 cache."""
     import torch
