@@ -5,7 +5,7 @@ import ctypes
 
 import pytest
 
-from pkgpu import pk
+from pkgpu import gpu_available, pk
 
 P = 1 << 20             # an aligned address no call may read
 
@@ -159,3 +159,16 @@ def test_bad_panels():
     refused("pk_gpu_w8_panel_dev", 16, 16, None, 16, P, None, text="NULL")
     refused("pk_gpu_w8_panel_dev", 16, 16, P, 16, None, None, text="NULL")
     refused("pk_gpu_w8_panel_dev", 16, 16, P, 16, P + 8, None, text="aligned")
+
+
+@pytest.mark.skipif(gpu_available(), reason="checks the no-device error path")
+def test_no_device_is_an_error_for_every_operator():
+    """Good arguments without a device: PK_GPU_ENODEV, with rows and without any."""
+    c = ctypes.byref(cache())
+    for n in (1, 0):
+        refused("pk_gpu_kv_write_dev", c, pk.F32, P, 256, P, 256, P, n, None, code=-5)
+        refused("pk_gpu_kv_read_dev", c, pk.F32, P, n, P, 256, P, 256, None, code=-5)
+        attention(c=c, B=n, code=-5)
+        norm(rows=n, code=-5)
+        gemm(M=n, code=-5)
+    refused("pk_gpu_w8_panel_dev", 16, 16, P, 16, P, None, code=-5)
