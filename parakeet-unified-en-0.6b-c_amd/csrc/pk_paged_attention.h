@@ -24,9 +24,10 @@
 // comes from rows by byte permutes in registers: a lane loads the same
 // head_dim / 16 elements of its 8 tokens and transposes them 4 x 4.
 //
-// Arithmetic: int8 and e4m3 codes are exact in bf16, and so are the caches'
-// 16-bit elements in their own type.  Queries enter as sums of bf16 terms (1
-// for bf16, 2 for f16, 3 for f32: all bits), so scores have fp32 accuracy.
+// Arithmetic: int8 and e4m3 codes are exact in bf16 and f16, and so are the
+// caches' 16-bit elements in their own type.  Queries enter with all their bits:
+// f16 and bf16 ones in their own type, f32 ones as a sum of 3 bf16 terms.  So
+// scores have fp32 accuracy.
 // p v_scale enters the second product in 2 bf16 terms for 16-bit outputs (16
 // bits of it; one term would add as much error as the output's own rounding,
 // and the matrix instructions have the time) and 3 for f32 (24).  An F16 cache
@@ -125,13 +126,16 @@ __device__ inline int nth_longest(const PagedArgs& a, int nth, int* lens, int wa
 }
 
 // Terms of the query and of p: see above.
-constexpr int q_terms(int cache, int t) { return cache == F16 || t == BF16 ? 1 : t == F16 ? 2 : 3; }
+// Whether the scores are formed in f16: its own caches, and f16 queries over
+// codes, which f16 holds exactly too.
+constexpr bool keys_f16(int cache, int t) { return cache == F16 || t == F16; }
+constexpr int q_terms(int cache, int t) { return t == F32 ? 3 : 1; }
 constexpr int p_terms(int cache, int t) { return cache == F16 ? 1 : t == F32 ? 3 : 2; }
 
-template <int CACHE>
+template <bool IN_F16>
 __device__ inline f32x4 mfma(u32x4 a, u32x4 b, f32x4 c)
 {
-    if constexpr (CACHE == F16)
+    if constexpr (IN_F16)
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
                                                       __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     else
@@ -139,16 +143,24 @@ __device__ inline f32x4 mfma(u32x4 a, u32x4 b, f32x4 c)
                                                        __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// 4 codes to 4 bf16, exactly.
-template <int CACHE>
-__device__ inline u32x2 codes_bf16(uint32_t w)
+// 4 codes to 4 bf16 or f16, exactly.
+template <int CACHE, bool IN_F16>
+__device__ inline u32x2 codes_16(uint32_t w)
 {
     if constexpr (CACHE == I8) {
         const uint32_t a = __float_as_uint((float)(int)(signed char)w);
         const uint32_t b = __float_as_uint((float)(int)(signed char)(w >> 8));
         const uint32_t c = __float_as_uint((float)(int)(signed char)(w >> 16));
         const uint32_t d = __float_as_uint((float)(int)(signed char)(w >> 24));
-        return (u32x2){__builtin_amdgcn_perm(b, a, 0x07060302u), __builtin_amdgcn_perm(d, c, 0x07060302u)};
+        if constexpr (IN_F16)
+            return (u32x2){__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__uint_as_float(a), __uint_as_float(b))),
+                           __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__uint_as_float(c), __uint_as_float(d)))};
+        else
+            return (u32x2){__builtin_amdgcn_perm(b, a, 0x07060302u), __builtin_amdgcn_perm(d, c, 0x07060302u)};
+    } else if constexpr (IN_F16) {
+        const f16x2 l = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false);
+        const f16x2 h = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true);
+        return (u32x2){__builtin_bit_cast(uint32_t, l), __builtin_bit_cast(uint32_t, h)};
     } else {
         const bf16x2 l = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false);
         const bf16x2 h = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true);
@@ -157,10 +169,11 @@ __device__ inline u32x2 codes_bf16(uint32_t w)
 }
 
 // x as TERMS terms of the matrix type, the first the largest.
-template <int CACHE, int TERMS>
+template <bool IN_F16, int TERMS>
 __device__ inline void split_pair(float x, float y, uint32_t* t)
 {
-    if constexpr (CACHE == F16) {
+    if constexpr (IN_F16) {
+        static_assert(TERMS == 1);
         t[0] = pack_f16(x, y);
     } else {
 #pragma unroll
@@ -185,6 +198,7 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
     constexpr int E = DIM / 16;                // elements of those, accumulators
     constexpr int QT = q_terms(CACHE, T), PT = p_terms(CACHE, T);
     constexpr float BIAS = CACHE == F16 ? 7.0f : 0.0f;
+    constexpr bool KF = keys_f16(CACHE, T), VF = CACHE == F16;  // types of the two products
 
     union Shared {
         int lens[kSortedMax + 4];
@@ -334,7 +348,7 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
             uint32_t w[QT];
-            split_pair<CACHE, QT>(qv[i][2 * d], qv[i][2 * d + 1], w);
+            split_pair<KF, QT>(qv[i][2 * d], qv[i][2 * d + 1], w);
 #pragma unroll
             for (int j = 0; j < QT; ++j) f[j][d] = w[j];
         }
@@ -361,14 +375,14 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
             for (int u = 0; u < 2; ++u) {
                 u32x4 f;
                 if constexpr (CODED) {
-                    const u32x2 lo = codes_bf16<CACHE>(kr[u][c / 2][2 * (c % 2)]);
-                    const u32x2 hi = codes_bf16<CACHE>(kr[u][c / 2][2 * (c % 2) + 1]);
+                    const u32x2 lo = codes_16<CACHE, KF>(kr[u][c / 2][2 * (c % 2)]);
+                    const u32x2 hi = codes_16<CACHE, KF>(kr[u][c / 2][2 * (c % 2) + 1]);
                     f = (u32x4){lo[0], lo[1], hi[0], hi[1]};
                 } else {
                     f = kr[u][c];
                 }
 #pragma unroll
-                for (int j = QT - 1; j >= 0; --j) s[u] = mfma<CACHE>(f, qf[j], s[u]);
+                for (int j = QT - 1; j >= 0; --j) s[u] = mfma<KF>(f, qf[j], s[u]);
             }
         }
 #pragma unroll
@@ -424,7 +438,7 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 uint32_t pt[PT];
-                split_pair<CACHE, PT>(w[2 * h], w[2 * h + 1], pt);
+                split_pair<VF, PT>(w[2 * h], w[2 * h + 1], pt);
 #pragma unroll
                 for (int j = 0; j < PT; ++j) p[j][2 * u + h] = pt[j];
             }
@@ -449,10 +463,10 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const u32x2 lo = codes_bf16<CACHE>(y[0][i]), hi = codes_bf16<CACHE>(y[1][i]);
+                    const u32x2 lo = codes_16<CACHE, VF>(y[0][i]), hi = codes_16<CACHE, VF>(y[1][i]);
                     const u32x4 f = (u32x4){lo[0], lo[1], hi[0], hi[1]};
 #pragma unroll
-                    for (int j = PT - 1; j >= 0; --j) acc[4 * w + i] = mfma<CACHE>(f, p[j], acc[4 * w + i]);
+                    for (int j = PT - 1; j >= 0; --j) acc[4 * w + i] = mfma<VF>(f, p[j], acc[4 * w + i]);
                 }
             }
         } else {
@@ -468,7 +482,7 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
                         f[2 * u + 1] = __builtin_amdgcn_perm(vr[u][3][w], vr[u][2][w], sel);
                     }
 #pragma unroll
-                    for (int j = PT - 1; j >= 0; --j) acc[2 * w + i] = mfma<CACHE>(f, p[j], acc[2 * w + i]);
+                    for (int j = PT - 1; j >= 0; --j) acc[2 * w + i] = mfma<VF>(f, p[j], acc[2 * w + i]);
                 }
             }
         }
