@@ -44,6 +44,14 @@
 // (powers of two, where p and its sums lose nothing), so most tiles need no
 // exchange between lanes at all.
 //
+// Values of the largest magnitudes: sums of up to 2^8 p v over 2^30 tokens can
+// pass the largest float where their mean does not.  A wave whose sums have
+// passed 2^100 (or have become NaN) takes its tiles once more with m raised by
+// 40: p stays below 2^-32, all its sums below 2^126, and the 8 waves' and 256 chunks'
+// sums below that still (their tokens are 2^30 together).  Exponents of p then hold up
+// to 48 + what they held, 2^-19 off.  Every other wave's sums are below 2^100, so what
+// they join to is finite.  F16 values are below 2^16 and cannot get there.
+//
 // A tile's keys and values stay in registers and are loaded one tile ahead: the
 // next keys once this tile's scores are formed, the next values once they
 // are added.  Bound by the cache's bytes.
@@ -358,8 +366,8 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
     __syncthreads();
     // One tile.  The last one of a wave is a copy of its own without loads: loads
     // on a condition would have every wait for this tile's values wait for the
-    // next one's keys too.
-    auto tile = [&](auto last) {
+    // next one's keys too.  So is one with m raised.
+    auto tile = [&](auto last, auto raised) {
         constexpr bool MORE = !decltype(last)::value;
         Halves after{};
         if constexpr (MORE) after = halves(t + 64 * NW);
@@ -412,6 +420,7 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
 
         float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                           fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        if constexpr (decltype(raised)::value) top = __fadd_rn(top, 40.0f);
         if (__any(top > m + 8.0f)) {
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
@@ -492,8 +501,29 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
         t += 32 * NW;
     };
     if (t < end) {
-        while (t + 32 * NW < end) tile(std::false_type{});
-        tile(std::true_type{});
+        while (t + 32 * NW < end) tile(std::false_type{}, std::false_type{});
+        tile(std::true_type{}, std::false_type{});
+        if constexpr (!VF) {
+            float size[4] = {};
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) size[r] = __fadd_rn(size[r], fabsf(acc[e][r]));
+            const float sum = __fadd_rn(__fadd_rn(size[0], size[1]), __fadd_rn(size[2], size[3]));
+            if (__any(!(sum < 0x1p100f))) {
+                m = -FLT_MAX;
+                l = 0.0f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+                for (t = begin + 32 * wave; t < end;) {
+                    cur = halves(t);
+                    load_k(cur);
+                    load_v(cur);
+                    tile(std::true_type{}, std::true_type{});
+                }
+            }
+        }
     }
 
     // join the waves: the same registers of the same lanes, in wave order
