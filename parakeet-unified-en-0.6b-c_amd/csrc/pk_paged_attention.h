@@ -26,7 +26,8 @@
 //
 // Arithmetic: int8 and e4m3 codes are exact in bf16 and f16, and so are the
 // caches' 16-bit elements in their own type.  Queries enter with all their bits:
-// f16 and bf16 ones in their own type, f32 ones as a sum of 3 bf16 terms.  So
+// f16 and bf16 ones in their own type, f32 ones as a sum of 3 bf16 terms (8 bits
+// each, cut off: rounded, a query near the largest float would become infinite).  So
 // scores have fp32 accuracy.
 // p v_scale enters the second product in 2 bf16 terms for 16-bit outputs (16
 // bits of it; one term would add as much error as the output's own rounding,
@@ -176,6 +177,16 @@ __device__ inline u32x2 codes_16(uint32_t w)
     }
 }
 
+// x as the sum of 3 bf16 terms, exactly: 8 bits of it each.
+__device__ inline void cut_pair(float x, float y, uint32_t* t)
+{
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        t[i] = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+        x = __fsub_rn(x, bf16_lo(t[i]));
+        y = __fsub_rn(y, bf16_hi(t[i]));
+    }
+}
 // x as TERMS terms of the matrix type, the first the largest.
 template <bool IN_F16, int TERMS>
 __device__ inline void split_pair(float x, float y, uint32_t* t)
@@ -356,7 +367,8 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
             uint32_t w[QT];
-            split_pair<KF, QT>(qv[i][2 * d], qv[i][2 * d + 1], w);
+            if constexpr (QT == 3) cut_pair(qv[i][2 * d], qv[i][2 * d + 1], w);
+            else split_pair<KF, QT>(qv[i][2 * d], qv[i][2 * d + 1], w);
 #pragma unroll
             for (int j = 0; j < QT; ++j) f[j][d] = w[j];
         }

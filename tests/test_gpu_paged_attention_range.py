@@ -81,3 +81,15 @@ def test_values_that_grow_along_a_sequence():
     got = c.run()
     want, _, a, s, x = do.attention(cache, q, table, [n], n, 1.0, 0)
     assert np.all(np.abs(got - want) <= do.attention_bound(want, a, s, x, n, dim, "bf16", "f32") + 2.0 ** -18 * a)
+
+
+def test_f32_queries_near_the_largest_float():
+    """Queries that bf16 would round to infinity, over a bf16 cache with keys small enough for scores of 1 or so."""
+    rng = np.random.default_rng(4)
+    page, n, dim = 16, 100, 64
+    cache = do.Cache("bf16", 7, 2, page, dim, seed=1)
+    k = cache.part("k")
+    k.copy_((k.float() * 2.0 ** -60).to(k.dtype))
+    table = np.arange(7, dtype=np.int32)[None]
+    q = rng.choice([-1.0, 1.0], (1, 4, dim)) * np.float32(3.4e38).astype(np.float64)
+    Call(cache, q, "f32", table, [n], n, 2.0 ** -71, 0).check(q, table, [n])
