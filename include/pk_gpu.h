@@ -486,7 +486,7 @@ int pk_gpu_kv_read_dev(const pk_gpu_kv_cache *cache, int dtype, const int *dslot
  * Over I8 and E4M3 caches |q| stays below 2^110: its products with codes are
  * summed before the row's scale enters.
  * Scores, sums and the softmax are fp32; its weights enter the second product
- * with 16 bits for BF16 and F16 output, 24 for F32 (11 over F16 caches).
+ * with 16 bits for BF16 and F16 output (22 over F16 caches), 24 for F32.
  * dws: a 16-byte aligned workspace of at least pk_gpu_paged_attention_ws_floats
  * floats for the same sizes (0: none is needed), free again when the call's
  * work is done; calls that may overlap on the device must not share it. */

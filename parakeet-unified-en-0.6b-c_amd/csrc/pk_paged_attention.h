@@ -32,8 +32,8 @@
 // p v_scale enters the second product in 2 bf16 terms for 16-bit outputs (16
 // bits of it; one term would add as much error as the output's own rounding,
 // and the matrix instructions have the time) and 3 for f32 (24).  An F16 cache
-// takes f16 queries and p in f16, raised by 2^7 so that a p down to 2^-21 of
-// the running maximum keeps its 11 bits.
+// takes f16 queries and p in 2 f16 terms (22 bits), raised by 2^7 so that a p down to
+// 2^-10 of the running maximum keeps all of them and one down to 2^-21 its first 11.
 // Maxima, sums and outputs are fp32 throughout.
 //
 // Bytes of K and V are the bound, and registers hold what is in flight: 8 waves
@@ -139,7 +139,7 @@ __device__ inline int nth_longest(const PagedArgs& a, int nth, int* lens, int wa
 // codes, which f16 holds exactly too.
 constexpr bool keys_f16(int cache, int t) { return cache == F16 || t == F16; }
 constexpr int q_terms(int cache, int t) { return t == F32 ? 3 : 1; }
-constexpr int p_terms(int cache, int t) { return cache == F16 ? 1 : t == F32 ? 3 : 2; }
+constexpr int p_terms(int t) { return t == F32 ? 3 : 2; }
 
 template <bool IN_F16>
 __device__ inline f32x4 mfma(u32x4 a, u32x4 b, f32x4 c)
@@ -191,16 +191,13 @@ __device__ inline void cut_pair(float x, float y, uint32_t* t)
 template <bool IN_F16, int TERMS>
 __device__ inline void split_pair(float x, float y, uint32_t* t)
 {
-    if constexpr (IN_F16) {
-        static_assert(TERMS == 1);
-        t[0] = pack_f16(x, y);
-    } else {
 #pragma unroll
-        for (int i = 0; i < TERMS; ++i) {
-            t[i] = pack_bf16(x, y);
-            x = __fsub_rn(x, bf16_lo(t[i]));
-            y = __fsub_rn(y, bf16_hi(t[i]));
-        }
+    for (int i = 0; i < TERMS; ++i) {
+        t[i] = IN_F16 ? pack_f16(x, y) : pack_bf16(x, y);
+        if (i + 1 == TERMS) break;
+        const f16x2 h = __builtin_bit_cast(f16x2, t[i]);
+        x = __fsub_rn(x, IN_F16 ? (float)h[0] : bf16_lo(t[i]));
+        y = __fsub_rn(y, IN_F16 ? (float)h[1] : bf16_hi(t[i]));
     }
 }
 
@@ -215,7 +212,7 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
     constexpr int VB = DIM * S / 16;           // bytes of a value a lane holds
     constexpr int VW = VB / 4;
     constexpr int E = DIM / 16;                // elements of those, accumulators
-    constexpr int QT = q_terms(CACHE, T), PT = p_terms(CACHE, T);
+    constexpr int QT = q_terms(CACHE, T), PT = p_terms(T);
     constexpr float BIAS = CACHE == F16 ? 7.0f : 0.0f;
     constexpr bool KF = keys_f16(CACHE, T), VF = CACHE == F16;  // types of the two products
 

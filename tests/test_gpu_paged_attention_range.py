@@ -1,4 +1,5 @@
-"""GPU: paged attention at the ends of its types' ranges against the plain 64-bit form."""
+"""GPU: paged attention at the ends of its types' ranges, and the bits that its
+softmax weights keep, against the plain 64-bit form."""
 import math
 
 import numpy as np
@@ -93,3 +94,25 @@ def test_f32_queries_near_the_largest_float():
     table = np.arange(7, dtype=np.int32)[None]
     q = rng.choice([-1.0, 1.0], (1, 4, dim)) * np.float32(3.4e38).astype(np.float64)
     Call(cache, q, "f32", table, [n], n, 2.0 ** -71, 0).check(q, table, [n])
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_weights_over_f16_caches_keep_22_bits(dim):
+    """Two f16 terms of a weight: half a step of the second relative to the weight is 2^-22, where a second
+    term is below f16's normal range 2^-25, which is 2^-32 of the maximum's weight, 2^7.  Few tokens with flat
+    scores and values that cancel: the outputs, and the other roundings, are small beside a weight's 2^-12."""
+    rng = np.random.default_rng(dim)
+    page, kv, group, lens = 16, 2, 3, [2, 3, 4, 6, 9, 33]
+    B, per = len(lens), 3
+    cache = do.Cache("f16", B * per, kv, page, dim, seed=3)
+    v = cache.part("v")
+    v[:, :, 1::2] = -v[:, :, 0::2]
+    table = np.arange(B * per, dtype=np.int32).reshape(B, per)
+    q = queries(rng, B, kv * group, dim, "f16")
+    got = Call(cache, q, "f16", table, lens, 48, 0.25 / dim, 0).run()
+    want, _, a, s, x = do.attention(cache, q, table, lens, 48, 0.25 / dim, 0)
+    for b, n in enumerate(lens):
+        tol = (do.attention_bound(want[b], a[b], s[b], x[b], n, dim, "f16", "f16")
+               - (2.0 ** -11 - 2.0 ** -22) * 1.01 * a[b])
+        err = np.abs(got[b] - want[b])
+        assert np.all(err <= tol), (n, float((err / tol).max()), int((err > tol).sum()))
