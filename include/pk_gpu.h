@@ -488,8 +488,10 @@ int pk_gpu_kv_read_dev(const pk_gpu_kv_cache *cache, int dtype, const int *dslot
  * Scores, sums and the softmax are fp32; its weights enter the second product
  * with 16 bits for BF16 and F16 output (22 over F16 caches), 24 for F32.
  * dws: a 16-byte aligned workspace of at least pk_gpu_paged_attention_ws_floats
- * floats for the same sizes (0: none is needed), free again when the call's
- * work is done; calls that may overlap on the device must not share it. */
+ * floats (0: none is needed), free again when the call's work is done; calls that
+ * may overlap on the device must not share it.  What is enough for B, max_len
+ * and window is enough for fewer sequences, a smaller max_len and a narrower
+ * window (0 being the widest). */
 size_t pk_gpu_paged_attention_ws_floats(const pk_gpu_kv_cache *cache, int B, int heads, int max_len,
                                         int window);
 int pk_gpu_paged_attention_dev(const pk_gpu_kv_cache *cache, int dtype, const void *dq, int ldq,

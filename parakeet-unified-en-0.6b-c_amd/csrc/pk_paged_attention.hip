@@ -106,7 +106,17 @@ int head_tiles(int group) { return (group + 15) / 16; }
 
 struct Plan { int chunk, splits; };
 
-// Chunks of a sequence, in rounds of 256 tokens (8 waves' tiles).  Up to 3
+// Tokens that the longest sequence's chunks cover: a window's begin up to 31 before it.
+long long span_at_most(int max_len, int window)
+{
+    const long long seen = window > 0 ? (long long)window + 31 : max_len;
+    const long long span = seen < max_len ? seen : max_len;
+    return span < 1 ? 1 : span;
+}
+
+constexpr int kRound = 256;         // 8 waves' tiles
+
+// Chunks that a sequence is cut into, before they are made whole rounds.  Up to 3
 // rounds one workgroup takes the whole: a round costs about 2 us, the second
 // launch that joins chunks 4 to 5 us.  Longer ones are cut until there is a
 // workgroup for each of the 256 CUs, and up to two where chunks keep 384 KB of
@@ -116,24 +126,28 @@ struct Plan { int chunk, splits; };
 //   8 ragged ones up to 4000, 8 heads of 128 in int8           34, 16, 19.5
 //   32 ragged ones up to 2000, the same (256 unsplit)           22, 22, 27
 //   160 windows of 1024 over a head of 256 (160 unsplit)       21, 21, 30
+long long cuts(const pk_gpu_kv_cache* c, long long pairs, long long span)
+{
+    const long long rounds = (span + kRound - 1) / kRound;
+    if (rounds <= 3) return 1;
+    const long long fill = 256 / pairs, two = 512 / pairs, large = span * 2 * c->head_dim * size_of(c->dtype) / (384 << 10);
+    long long n = two < large ? two : large;
+    if (n < fill) n = fill;
+    if (n > rounds) n = rounds;
+    if (n > kMaxSplits) n = kMaxSplits;
+    return n < 1 ? 1 : n;
+}
+
+long long pairs_of(const pk_gpu_kv_cache* c, int B, int heads)
+{
+    return (long long)B * c->heads * head_tiles(heads / c->heads);
+}
+
 Plan plan(const pk_gpu_kv_cache* c, int B, int heads, int max_len, int window)
 {
-    const long long pairs = (long long)(B > 0 ? B : 1) * c->heads * head_tiles(heads / c->heads);
-    const int round = 256;
-    long long span = window > 0 && window < max_len ? (long long)window + 31 : max_len;
-    if (span < 1) span = 1;
-    const long long rounds = (span + round - 1) / round;
-    const long long bytes = span * 2 * c->head_dim * size_of(c->dtype);
-    long long splits = 1;
-    if (rounds > 3) {
-        const long long fill = 256 / pairs, two = 512 / pairs, large = bytes / (384 << 10);
-        splits = two < large ? two : large;
-        if (splits < fill) splits = fill;
-    }
-    if (splits > rounds) splits = rounds;
-    if (splits > kMaxSplits) splits = kMaxSplits;
-    if (splits < 1) splits = 1;
-    const long long chunk = (rounds + splits - 1) / splits * round;
+    const long long span = span_at_most(max_len, window), rounds = (span + kRound - 1) / kRound;
+    const long long n = cuts(c, pairs_of(c, B > 0 ? B : 1, heads), span);
+    const long long chunk = (rounds + n - 1) / n * kRound;
     return {(int)chunk, (int)((span + chunk - 1) / chunk)};
 }
 
@@ -149,7 +163,7 @@ int check_attention(const pk_gpu_kv_cache* c, int B, int heads, int max_len, int
     if (heads < 1 || heads % c->heads)
         return rt::error(PK_GPU_EINVAL, "%s: %d query heads over %d key-value heads", who, heads, c->heads);
     const Plan p = plan(c, B, heads, max_len, window);
-    if ((long long)B * c->heads * head_tiles(heads / c->heads) * p.splits > 0x7fffffff ||
+    if (pairs_of(c, B, heads) * p.splits > 0x7fffffff ||
         (long long)B * heads > 0x7fffffff)
         return rt::error(PK_GPU_EINVAL, "%s: %d sequences of %d heads exceed the grid", who, B, heads);
     return PK_GPU_OK;
@@ -158,6 +172,20 @@ int check_attention(const pk_gpu_kv_cache* c, int B, int heads, int max_len, int
 size_t ws_floats_of(const pk_gpu_kv_cache* c, int B, int heads, const Plan& p)
 {
     return p.splits <= 1 ? 0 : (size_t)B * heads * p.splits * (c->head_dim + 2);
+}
+
+// What any call with up to B sequences, up to max_len tokens and a window up to this
+// one takes: cuts() does not fall as the span grows, and chunks are never more.
+// Above 256 pairs there are none.
+size_t ws_floats_up_to(const pk_gpu_kv_cache* c, int B, int heads, int max_len, int window)
+{
+    const long long span = span_at_most(max_len, window);
+    size_t most = 0;
+    for (int b = 1; b <= B && pairs_of(c, b, heads) <= 256; ++b) {
+        const size_t n = cuts(c, pairs_of(c, b, heads), span);
+        if (n > 1 && b * n > most) most = b * n;
+    }
+    return most * heads * (c->head_dim + 2);
 }
 
 }  // namespace
@@ -171,7 +199,7 @@ using namespace pkgpu::decode;
 size_t pk_gpu_paged_attention_ws_floats(const pk_gpu_kv_cache* cache, int B, int heads, int max_len, int window)
 {
     if (check_attention(cache, B, heads, max_len, window) != PK_GPU_OK || B == 0) return 0;
-    return ws_floats_of(cache, B, heads, plan(cache, B, heads, max_len, window));
+    return ws_floats_up_to(cache, B, heads, max_len, window);
 }
 
 int pk_gpu_paged_attention_dev(const pk_gpu_kv_cache* cache, int dtype, const void* dq, int ldq, int heads,
@@ -201,7 +229,7 @@ int pk_gpu_paged_attention_dev(const pk_gpu_kv_cache* cache, int dtype, const vo
         return rt::error(PK_GPU_EINVAL, "%s: query and output rows must be 16-byte aligned", who);
     if (!aligned(dpages, 4) || !aligned(dlens, 4) || !aligned(dlse, 4))
         return rt::error(PK_GPU_EINVAL, "%s: pages, lengths or lse are not aligned to their elements", who);
-    const long long pairs = (long long)B * cache->heads * head_tiles(heads / cache->heads);
+    const long long pairs = pairs_of(cache, B, heads);
     const Plan p = plan(cache, B, heads, max_len, window);
     const size_t need = ws_floats_of(cache, B, heads, p);
     if (need && (!dws || ws_floats < need || !aligned16(dws)))
