@@ -423,6 +423,9 @@ void pk_gpu_encoder_destroy(pk_gpu_encoder *enc);
  * reference (its decoder is an LSTM, decoder.c:1-132).  None of them allocates,
  * waits or keeps anything between calls, so all may be captured in a HIP
  * graph.  Pointers are of the library's device, whichever device is current.
+ * Sizes whose launch would pass 2^32 threads are refused: cache calls of 2^35
+ * elements, attention of 2^23 workgroups (sequences x key-value heads x 16 query heads x
+ * chunks), panels of 64 GiB, products of 2^23 tiles (2^26 columns at up to 16 rows).
  * Results do not depend on timing: no atomics, fixed orders of summation. */
 
 /* Element types. */

@@ -241,6 +241,12 @@ inline hipError_t launch(void (*fn)(Args), dim3 grid, dim3 block, size_t lds, hi
     return hipLaunchKernel(reinterpret_cast<const void*>(fn), grid, block, p, lds, s);
 }
 
+// Whether a launch of so many workgroups is one that HIP takes: below 2^32 threads.
+inline bool launchable(long long workgroups, int threads)
+{
+    return workgroups <= 0x7fffffff && workgroups * threads < 1ll << 32;
+}
+
 inline bool is_float(int t) { return t == F32 || t == F16 || t == BF16; }
 inline bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 inline bool aligned16(const void* p) { return aligned(p, 16); }

@@ -111,12 +111,19 @@ __global__ void __launch_bounds__(kMostThreads) kv_read(RowsArgs a)
     store8<ROWS>(a.rv + (token * a.ldv + at) * size_of(ROWS), v);
 }
 
+struct Launch { int threads; long long workgroups; };
+Launch launch_of(long long rows, int dim)
+{
+    const int lanes = dim / 8, threads = rows / 1024 * lanes >= 256 ? kMostThreads : 256;
+    const int per = threads / lanes;
+    return {threads, (rows + per - 1) / per};
+}
+
 template <int CACHE, int ROWS>
 hipError_t launch_dim(bool write, int dim, const RowsArgs& a, hipStream_t s)
 {
-    const uint32_t lanes = dim / 8, threads = a.rows / 1024 * lanes >= 256 ? kMostThreads : 256;
-    const uint32_t per = threads / lanes;
-    const dim3 grid((uint32_t)(((uint64_t)a.rows + per - 1) / per)), block(threads);
+    const Launch l = launch_of(a.rows, dim);
+    const dim3 grid((uint32_t)l.workgroups), block(l.threads);
 #define PK_ROWS_DIM(D) launch(write ? kv_write<CACHE, ROWS, D> : kv_read<CACHE, ROWS, D>, grid, block, 0, s, a)
     return dim == 64 ? PK_ROWS_DIM(64) : dim == 128 ? PK_ROWS_DIM(128) : PK_ROWS_DIM(256);
 #undef PK_ROWS_DIM
@@ -143,6 +150,9 @@ int kv_call(bool write, const pk_gpu_kv_cache* c, int dtype, const void* dk, int
         return rt::error(PK_GPU_EINVAL, "%s: rows of %lld elements, ldk = %d, ldv = %d", who, wide, ldk, ldv);
     if ((long long)n * c->heads > 0x7fffffff)
         return rt::error(PK_GPU_EINVAL, "%s: %d tokens of %d heads exceed 2^31 rows", who, n, c->heads);
+    const Launch l = launch_of((long long)n * c->heads, c->head_dim);
+    if (!launchable(l.workgroups, l.threads))
+        return rt::error(PK_GPU_EINVAL, "%s: %d tokens of %d heads of %d exceed the grid", who, n, c->heads, c->head_dim);
     if (n && (!dk || !dv || !dslots)) return rt::error(PK_GPU_EINVAL, "%s: NULL operand", who);
     const int es = size_of(dtype);
     if (!aligned16(dk) || !aligned16(dv) || (size_t)ldk * es % 16 || (size_t)ldv * es % 16)

@@ -163,8 +163,8 @@ int check_attention(const pk_gpu_kv_cache* c, int B, int heads, int max_len, int
     if (heads < 1 || heads % c->heads)
         return rt::error(PK_GPU_EINVAL, "%s: %d query heads over %d key-value heads", who, heads, c->heads);
     const Plan p = plan(c, B, heads, max_len, window);
-    if (pairs_of(c, B, heads) * p.splits > 0x7fffffff ||
-        (long long)B * heads > 0x7fffffff)
+    // 8 waves a workgroup at most; the join has 256 threads a head, of up to 16 * 256 heads
+    if (!launchable(pairs_of(c, B, heads) * p.splits, 512) || (long long)B * heads > 0x7fffffff)
         return rt::error(PK_GPU_EINVAL, "%s: %d sequences of %d heads exceed the grid", who, B, heads);
     return PK_GPU_OK;
 }

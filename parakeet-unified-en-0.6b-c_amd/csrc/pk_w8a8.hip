@@ -55,6 +55,9 @@ struct PanelArgs {
     int ldb, K, N, kb;
 };
 
+int blocks_of_k(int K) { return (K + 127) / 128 * 2; }
+long long panel_blocks(int K, int N) { return (N + 15ll) / 16 * blocks_of_k(K); }
+
 __global__ void __launch_bounds__(256) w8_panel(PanelArgs p)
 {
     const int kb = p.kb, K = p.K, N = p.N;
@@ -376,41 +379,32 @@ __global__ void __launch_bounds__(64 * kFewWaves) w8_few(W8Args a)
     store_c<T, EPI>(a, row, a.sa[row < a.M ? row : a.M - 1], j, columns_of(a, j), sum);
 }
 
-template <int T, int EPI, int WM, int WN, int MB, int NB, int STAGES>
-hipError_t launch_tiled(W8Args a, hipStream_t s)
+// The kernel that a product goes to, and its launch.
+enum Kernel { FEW, TILE_64, TILE_128_DEEP, TILE_128, TILE_256 };
+struct Choice { Kernel kernel; int bm, bn; long long workgroups; int threads; };
+
+long long tiles_of(int M, int N, int bm, int bn)
 {
-    constexpr int BM = 16 * WM * MB, BN = 16 * WN * NB;
-    a.mt = (a.M + BM - 1) / BM;
-    a.nt = (a.N + BN - 1) / BN;
-    const long long tiles = (long long)a.mt * a.nt;
-    if (tiles > 0x7fffffff) return hipErrorInvalidValue;
-    return launch(w8_tiled<T, EPI, WM, WN, MB, NB, STAGES>, dim3((uint32_t)tiles), dim3(64 * WM * WN), 0, s, a);
+    return ((long long)M + bm - 1) / bm * (((long long)N + bn - 1) / bn);
 }
 
-long long tiles_of(const W8Args& a, int bm, int bn)
+Choice choose(int M, int N)
 {
-    return (long long)((a.M + bm - 1) / bm) * ((a.N + bn - 1) / bn);
-}
-
-template <int T, int EPI>
-hipError_t launch_w8(const W8Args& a, hipStream_t s)
-{
+    const auto of = [&](Kernel k, int bm, int bn, int threads) {
+        return Choice{k, bm, bn, tiles_of(M, N, bm, bn), threads};
+    };
     // Few rows, or too few 64 x 64 tiles to be worth staging (us; this kernel,
     // 64 x 64 tiles): 33 x 4096 x 4096 9.8, 11.2; 64 x 4096 x 4096 12.5, 11.5; 64 x
     // 1024 x 4096 5.8, 10.1; 128 x 1024 x 4096 8.0, 10.0; 256 x 1024 x 4096 12.3, 11.4;
     // 17 x 16384 x 4096 17.8, 14.7.
-    const long long small = tiles_of(a, 64, 64);
-    if (a.M <= 16 || small < 48 || (small < 128 && a.M <= 48)) {
+    const long long small = tiles_of(M, N, 64, 64);
+    if (M <= 16 || small < 48 || (small < 128 && M <= 48)) {
         // as many blocks of rows a workgroup as leave 256 workgroups (33 x 1024 x
         // 4096: 5.6 us in 64 x 3 workgroups, 8.0 in 64)
-        const int cols = (a.N + 15) / 16, blocks = (a.M + 15) / 16;
+        const int blocks = (M + 15) / 16;
         int mb = blocks < 4 ? blocks : 4;
-        while (mb > 1 && (long long)cols * ((blocks + mb - 1) / mb) < 256) --mb;
-        const dim3 grid(cols, (blocks + mb - 1) / mb), block(64 * kFewWaves);
-        return mb == 1   ? launch(w8_few<T, EPI, 1>, grid, block, 0, s, a)
-               : mb == 2 ? launch(w8_few<T, EPI, 2>, grid, block, 0, s, a)
-               : mb == 3 ? launch(w8_few<T, EPI, 3>, grid, block, 0, s, a)
-                         : launch(w8_few<T, EPI, 4>, grid, block, 0, s, a);
+        while (mb > 1 && tiles_of(M, N, 16 * mb, 16) < 256) --mb;
+        return of(FEW, 16 * mb, 16, 64 * kFewWaves);
     }
     // The largest tile of which there are enough for the 256 CUs; 128 x 128 with
     // two workgroups a CU (2 stages each) where there are more tiles than CUs, with
@@ -422,22 +416,48 @@ hipError_t launch_w8(const W8Args& a, hipStream_t s)
     //   4001 x 1024 x 4096    63, 29, 26.7, 36
     //    512 x 4096 x 4096    61, 27, 23.7, 18.8
     //    128 x 4096 x 1024    23, 9.2, 9.3, 5.9
-    if (tiles_of(a, 256, 256) >= 200) return launch_tiled<T, EPI, 2, 4, 8, 4, 2>(a, s);
-    const long long mid = tiles_of(a, 128, 128);
-    if (mid > 256) return launch_tiled<T, EPI, 2, 4, 4, 2, 2>(a, s);
-    if (mid >= 200) return launch_tiled<T, EPI, 2, 4, 4, 2, 4>(a, s);
-    return launch_tiled<T, EPI, 2, 4, 2, 1, 4>(a, s);
+    if (tiles_of(M, N, 256, 256) >= 200) return of(TILE_256, 256, 256, 512);
+    const long long mid = tiles_of(M, N, 128, 128);
+    if (mid > 256) return of(TILE_128, 128, 128, 512);
+    if (mid >= 200) return of(TILE_128_DEEP, 128, 128, 512);
+    return of(TILE_64, 64, 64, 512);
+}
+
+template <int T, int EPI, int WM, int WN, int MB, int NB, int STAGES>
+hipError_t launch_tiled(W8Args a, const Choice& c, hipStream_t s)
+{
+    static_assert(WM * WN == 8);
+    a.mt = (a.M + c.bm - 1) / c.bm;
+    a.nt = (a.N + c.bn - 1) / c.bn;
+    return launch(w8_tiled<T, EPI, WM, WN, MB, NB, STAGES>, dim3((uint32_t)c.workgroups), dim3(c.threads), 0, s, a);
+}
+
+template <int T, int EPI>
+hipError_t launch_w8(const W8Args& a, const Choice& c, hipStream_t s)
+{
+    switch (c.kernel) {
+    case TILE_256: return launch_tiled<T, EPI, 2, 4, 8, 4, 2>(a, c, s);
+    case TILE_128: return launch_tiled<T, EPI, 2, 4, 4, 2, 2>(a, c, s);
+    case TILE_128_DEEP: return launch_tiled<T, EPI, 2, 4, 4, 2, 4>(a, c, s);
+    case TILE_64: return launch_tiled<T, EPI, 2, 4, 2, 1, 4>(a, c, s);
+    case FEW: break;
+    }
+    const dim3 grid((a.N + 15) / 16, (a.M + c.bm - 1) / c.bm), block(c.threads);
+    return c.bm == 16   ? launch(w8_few<T, EPI, 1>, grid, block, 0, s, a)
+           : c.bm == 32 ? launch(w8_few<T, EPI, 2>, grid, block, 0, s, a)
+           : c.bm == 48 ? launch(w8_few<T, EPI, 3>, grid, block, 0, s, a)
+                        : launch(w8_few<T, EPI, 4>, grid, block, 0, s, a);
 }
 
 template <int T>
-hipError_t launch_epi(const W8Args& a, hipStream_t s)
+hipError_t launch_epi(const W8Args& a, const Choice& c, hipStream_t s)
 {
     switch (a.epi) {
-    case PK_GPU_EPI_SWISH: return launch_w8<T, PK_GPU_EPI_SWISH>(a, s);
-    case PK_GPU_EPI_HALF_RESIDUAL: return launch_w8<T, PK_GPU_EPI_HALF_RESIDUAL>(a, s);
-    case PK_GPU_EPI_RESIDUAL: return launch_w8<T, PK_GPU_EPI_RESIDUAL>(a, s);
-    case PK_GPU_EPI_RELU: return launch_w8<T, PK_GPU_EPI_RELU>(a, s);
-    default: return launch_w8<T, PK_GPU_EPI_NONE>(a, s);
+    case PK_GPU_EPI_SWISH: return launch_w8<T, PK_GPU_EPI_SWISH>(a, c, s);
+    case PK_GPU_EPI_HALF_RESIDUAL: return launch_w8<T, PK_GPU_EPI_HALF_RESIDUAL>(a, c, s);
+    case PK_GPU_EPI_RESIDUAL: return launch_w8<T, PK_GPU_EPI_RESIDUAL>(a, c, s);
+    case PK_GPU_EPI_RELU: return launch_w8<T, PK_GPU_EPI_RELU>(a, c, s);
+    default: return launch_w8<T, PK_GPU_EPI_NONE>(a, c, s);
     }
 }
 
@@ -452,7 +472,8 @@ using namespace pkgpu::decode;
 size_t pk_gpu_w8_panel_bytes(int K, int N)
 {
     if (K < 1 || N < 1 || K > 131071 || N > 1 << 30) return 0;
-    return (size_t)((N + 15ll) / 16) * ((K + 127ll) / 128) * 2048;
+    const long long blocks = panel_blocks(K, N);
+    return launchable((blocks + 3) / 4, 256) ? (size_t)blocks * 1024 : 0;
 }
 
 int pk_gpu_w8_panel_dev(int K, int N, const int8_t* dB, int ldb, void* dpanel, void* stream)
@@ -464,12 +485,11 @@ int pk_gpu_w8_panel_dev(int K, int N, const int8_t* dB, int ldb, void* dpanel, v
     if (ldb < N) return rt::error(PK_GPU_EINVAL, "%s: ldb = %d < N = %d", who, ldb, N);
     if (!dB || !dpanel) return rt::error(PK_GPU_EINVAL, "%s: NULL operand", who);
     if (!aligned16(dpanel)) return rt::error(PK_GPU_EINVAL, "%s: the panel must be 16-byte aligned", who);
-    const int kb = (K + 127) / 128 * 2;
-    const long long blocks = (N + 15ll) / 16 * kb;
-    if ((blocks + 3) / 4 > 0x7fffffff) return rt::error(PK_GPU_EINVAL, "%s: %d x %d exceeds the grid", who, K, N);
+    const long long blocks = panel_blocks(K, N);
+    if (!launchable((blocks + 3) / 4, 256)) return rt::error(PK_GPU_EINVAL, "%s: %d x %d exceeds the grid", who, K, N);
     OnDevice on;
     if (on.rc) return on.rc;
-    const PanelArgs p{dB, static_cast<u32x4*>(dpanel), blocks, ldb, K, N, kb};
+    const PanelArgs p{dB, static_cast<u32x4*>(dpanel), blocks, ldb, K, N, blocks_of_k(K)};
     const hipError_t e = launch(w8_panel, dim3((uint32_t)((blocks + 3) / 4)), dim3(256), 0,
                                 static_cast<hipStream_t>(stream), p);
     return e == hipSuccess ? PK_GPU_OK : rt::hip_error(e, who);
@@ -501,6 +521,8 @@ int pk_gpu_gemm_w8a8_dev(int M, int N, int K, const int8_t* dA, int lda, const f
         return rt::error(PK_GPU_EINVAL, "%s: an operand is not aligned to its elements", who);
     if (residual && dres == dC && ldr != ldc)
         return rt::error(PK_GPU_EINVAL, "%s: a residual in place needs C's leading dimension", who);
+    const Choice c = M && N ? choose(M, N) : Choice{};
+    if (!launchable(c.workgroups, c.threads)) return rt::error(PK_GPU_EINVAL, "%s: %d x %d exceeds the grid", who, M, N);
     OnDevice on;
     if (on.rc) return on.rc;
     if (!M || !N) return PK_GPU_OK;
@@ -517,11 +539,12 @@ int pk_gpu_gemm_w8a8_dev(int M, int N, int K, const int8_t* dA, int lda, const f
     a.C = static_cast<char*>(dC);
     a.ldc = (size_t)ldc * es;
     a.M = M; a.N = N; a.K = K;
-    a.kb = (K + 127) / 128 * 2;
+    a.kb = blocks_of_k(K);
     a.epi = epilogue;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const hipError_t e = dtype == F32 ? launch_epi<F32>(a, s) : dtype == F16 ? launch_epi<F16>(a, s) : launch_epi<BF16>(a, s);
-    if (e == hipErrorInvalidValue) return rt::error(PK_GPU_EINVAL, "%s: %d x %d exceeds the grid", who, M, N);
+    const hipError_t e = dtype == F32   ? launch_epi<F32>(a, c, s)
+                         : dtype == F16 ? launch_epi<F16>(a, c, s)
+                                        : launch_epi<BF16>(a, c, s);
     return e == hipSuccess ? PK_GPU_OK : rt::hip_error(e, who);
 }
 

@@ -9,7 +9,7 @@ import re
 import pytest
 
 from pkgpu import gpu_available, pk
-from test_decode_refusals import P, cache
+from test_decode_refusals import P, attention, cache, gemm, refused
 
 # calls that are not refused end without a device, and only so
 pytestmark = pytest.mark.skipif(gpu_available(), reason="makes calls with addresses that nothing may read")
@@ -57,3 +57,43 @@ def test_a_closer_length_takes_the_bounds_workspace():
     bound = query(c, 1, 32, 1 << 20, 0)
     for n in (8192, 8193, 8448, 12000, 65536):
         assert 0 < needed(c, 1, 32, n, 0) <= bound
+
+
+# Launches take below 2^32 threads: the sizes on both sides of that.
+
+@pytest.mark.parametrize("heads,dim,n,code", [
+    (1, 256, 1 << 27, -1), (1, 256, (1 << 27) - 32, -5), (8, 128, 1 << 25, -1), (8, 128, (1 << 25) - 8, -5),
+    (1, 64, 1 << 29, -1), (1, 64, (1 << 29) - 128, -5), (3, 64, 178956971, -1),
+])
+def test_cache_rows(heads, dim, n, code):
+    c = ctypes.byref(cache(heads=heads, head_dim=dim))
+    wide = heads * dim
+    text = "grid" if code == -1 else None
+    refused("pk_gpu_kv_write_dev", c, pk.F32, P, wide, P, wide, P, n, None, code=code, text=text)
+    refused("pk_gpu_kv_read_dev", c, pk.BF16, P, n, P, wide, P, wide, None, code=code, text=text)
+
+
+@pytest.mark.parametrize("kv,group,B,code", [(1, 16, 1 << 23, -1), (1, 16, (1 << 23) - 1, -5), (8, 1, 1 << 20, -1),
+                                             (1, 40, 2796203, -1), (1, 40, 2796202, -5)])
+def test_sequences(kv, group, B, code):
+    c = cache(heads=kv)
+    wide = kv * group * 128
+    attention(c=ctypes.byref(c), heads=kv * group, ldq=wide, ldo=wide, B=B, code=code,
+              text="grid" if code == -1 else None)
+    if code == -1:
+        assert query(c, B, kv * group, 1000, 0) == 0
+
+
+@pytest.mark.parametrize("K,N,code", [(128, 1 << 29, -1), (128, (1 << 29) - 32, -5), (1, 1 << 30, -1),
+                                      (131071, 1 << 20, -1), (131071, (1 << 19) - 16, -5)])
+def test_panels(K, N, code):
+    assert (pk.load().pk_gpu_w8_panel_bytes(K, N) == 0) == (code == -1)
+    refused("pk_gpu_w8_panel_dev", K, N, P, N, P, None, code=code, text="grid" if code == -1 else None)
+
+
+@pytest.mark.parametrize("M,N,code", [
+    (1, 1 << 26, -1), (16, (1 << 26) - 15, -1), (1, (1 << 26) - 16, -5), (17, 1 << 26, -5), (1 << 30, 1, -5),
+    (1 << 20, 1 << 19, -1), ((1 << 20) - 256, 1 << 19, -5), (1 << 30, 1 << 30, -1), (0, 1 << 30, -5),
+])
+def test_products(M, N, code):
+    gemm(M=M, N=N, ldr=N, ldc=N, code=code, text="grid" if code == -1 else None)
