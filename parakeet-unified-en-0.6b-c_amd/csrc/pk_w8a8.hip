@@ -400,9 +400,10 @@ Choice choose(int M, int N)
     const long long small = tiles_of(M, N, 64, 64);
     if (M <= 16 || small < 48 || (small < 128 && M <= 48)) {
         // as many blocks of rows a workgroup as leave 256 workgroups (33 x 1024 x
-        // 4096: 5.6 us in 64 x 3 workgroups, 8.0 in 64)
+        // 4096: 5.6 us in 64 x 3 workgroups, 8.0 in 64).  4 never do: fewer than 48
+        // tiles of 64 x 64 are at most 4 * 47 of 64 x 16, and M <= 48 has 3.
         const int blocks = (M + 15) / 16;
-        int mb = blocks < 4 ? blocks : 4;
+        int mb = blocks < 3 ? blocks : 3;
         while (mb > 1 && tiles_of(M, N, 16 * mb, 16) < 256) --mb;
         return of(FEW, 16 * mb, 16, 64 * kFewWaves);
     }
@@ -445,8 +446,7 @@ hipError_t launch_w8(const W8Args& a, const Choice& c, hipStream_t s)
     const dim3 grid((a.N + 15) / 16, (a.M + c.bm - 1) / c.bm), block(c.threads);
     return c.bm == 16   ? launch(w8_few<T, EPI, 1>, grid, block, 0, s, a)
            : c.bm == 32 ? launch(w8_few<T, EPI, 2>, grid, block, 0, s, a)
-           : c.bm == 48 ? launch(w8_few<T, EPI, 3>, grid, block, 0, s, a)
-                        : launch(w8_few<T, EPI, 4>, grid, block, 0, s, a);
+                        : launch(w8_few<T, EPI, 3>, grid, block, 0, s, a);
 }
 
 template <int T>
