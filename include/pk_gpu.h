@@ -485,7 +485,8 @@ int pk_gpu_kv_read_dev(const pk_gpu_kv_cache *cache, int dtype, const int *dslot
  *             what another part of a split softmax is joined with
  * Page entries outside [0, n_pages) are absent: their tokens take no part, and
  * entries from dlens[b] on have no effect.  Tokens that take no part may hold
- * anything, NaN included.  A sequence without tokens gives zeros (lse -inf).
+ * anything, NaN included; an infinite value that does is passed on as it is.  A
+ * sequence without tokens gives zeros (lse -inf).
  * Over I8 and E4M3 caches |q| stays below 2^110: its products with codes are
  * summed before the row's scale enters.
  * Scores, sums and the softmax are fp32; its weights enter the second product

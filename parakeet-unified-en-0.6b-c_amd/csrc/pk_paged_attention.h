@@ -46,12 +46,14 @@
 // exchange between lanes at all.
 //
 // Values of the largest magnitudes: sums of up to 2^8 p v over 2^30 tokens can
-// pass the largest float where their mean does not.  A wave whose sums have
-// passed 2^100 (or have become NaN) takes its tiles once more with m raised by
-// 40: p stays below 2^-32, all its sums below 2^126, and the 8 waves' and 256 chunks'
-// sums below that still (their tokens are 2^30 together).  Exponents of p then hold up
-// to 48 + what they held, 2^-19 off.  Every other wave's sums are below 2^100, so what
-// they join to is finite.  F16 values are below 2^16 and cannot get there.
+// pass the largest float where their mean does not; and where v or k is infinite,
+// a second term of p or q that is 0 or negative makes NaN of it.  A wave whose sums have passed
+// 2^100 or become NaN takes its tiles once more, with infinities and NaN left out of all
+// products but the first term's, and with m raised by 40: p stays below 2^-32, all its
+// sums below 2^126, and the 8 waves' and 256 chunks' sums below that still (their tokens
+// are 2^30 together).  Exponents of p then hold up to 48 + what they held, 2^-19 off.
+// Every other wave's sums are below 2^100, so what they join to is finite.  Sums of F16
+// values stay below 2^61: there m is not raised.
 //
 // A tile's keys and values stay in registers and are loaded one tile ahead: the
 // next keys once this tile's scores are formed, the next values once they
@@ -177,6 +179,16 @@ __device__ inline u32x2 codes_16(uint32_t w)
     }
 }
 
+// 8 elements with infinities and NaN as zeros.
+template <bool IN_F16>
+__device__ inline u32x4 finite_of(u32x4 f)
+{
+    constexpr uint32_t EXP = IN_F16 ? 0x7c00u : 0x7f80u;
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+        f[d] &= ((f[d] & EXP) != EXP ? 0xffffu : 0u) | ((f[d] >> 16 & EXP) != EXP ? 0xffff0000u : 0u);
+    return f;
+}
 // x as the sum of 3 bf16 terms, exactly: 8 bits of it each.
 __device__ inline void cut_pair(float x, float y, uint32_t* t)
 {
@@ -375,9 +387,9 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
     __syncthreads();
     // One tile.  The last one of a wave is a copy of its own without loads: loads
     // on a condition would have every wait for this tile's values wait for the
-    // next one's keys too.  So is one with m raised.
-    auto tile = [&](auto last, auto raised) {
-        constexpr bool MORE = !decltype(last)::value;
+    // next one's keys too.  So are tiles that are taken once more.
+    auto tile = [&](auto last, auto again) {
+        constexpr bool MORE = !decltype(last)::value, AGAIN = decltype(again)::value;
         Halves after{};
         if constexpr (MORE) after = halves(t + 64 * NW);
 
@@ -399,7 +411,8 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
                     f = kr[u][c];
                 }
 #pragma unroll
-                for (int j = QT - 1; j >= 0; --j) s[u] = mfma<KF>(f, qf[j], s[u]);
+                for (int j = QT - 1; j >= 0; --j)
+                    s[u] = mfma<KF>(AGAIN && !CODED && j > 0 ? finite_of<KF>(f) : f, qf[j], s[u]);
             }
         }
 #pragma unroll
@@ -429,7 +442,7 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
 
         float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                           fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-        if constexpr (decltype(raised)::value) top = __fadd_rn(top, 40.0f);
+        if constexpr (AGAIN && !VF) top = __fadd_rn(top, 40.0f);
         if (__any(top > m + 8.0f)) {
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
@@ -500,7 +513,8 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
                         f[2 * u + 1] = __builtin_amdgcn_perm(vr[u][3][w], vr[u][2][w], sel);
                     }
 #pragma unroll
-                    for (int j = PT - 1; j >= 0; --j) acc[2 * w + i] = mfma<VF>(f, p[j], acc[2 * w + i]);
+                    for (int j = PT - 1; j >= 0; --j)
+                        acc[2 * w + i] = mfma<VF>(AGAIN && j > 0 ? finite_of<VF>(f) : f, p[j], acc[2 * w + i]);
                 }
             }
         }
@@ -512,25 +526,23 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
     if (t < end) {
         while (t + 32 * NW < end) tile(std::false_type{}, std::false_type{});
         tile(std::true_type{}, std::false_type{});
-        if constexpr (!VF) {
-            float size[4] = {};
+        float size[4] = {};
 #pragma unroll
-            for (int e = 0; e < E; ++e)
+        for (int e = 0; e < E; ++e)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) size[r] = __fadd_rn(size[r], fabsf(acc[e][r]));
-            const float sum = __fadd_rn(__fadd_rn(size[0], size[1]), __fadd_rn(size[2], size[3]));
-            if (__any(!(sum < 0x1p100f))) {
-                m = -FLT_MAX;
-                l = 0.0f;
+            for (int r = 0; r < 4; ++r) size[r] = __fadd_rn(size[r], fabsf(acc[e][r]));
+        const float sum = __fadd_rn(__fadd_rn(size[0], size[1]), __fadd_rn(size[2], size[3]));
+        if (__any(!(sum < 0x1p100f))) {
+            m = -FLT_MAX;
+            l = 0.0f;
 #pragma unroll
-                for (int e = 0; e < E; ++e) acc[e] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+            for (int e = 0; e < E; ++e) acc[e] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
-                for (t = begin + 32 * wave; t < end;) {
-                    cur = halves(t);
-                    load_k(cur);
-                    load_v(cur);
-                    tile(std::true_type{}, std::true_type{});
-                }
+            for (t = begin + 32 * wave; t < end;) {
+                cur = halves(t);
+                load_k(cur);
+                load_v(cur);
+                tile(std::true_type{}, std::true_type{});
             }
         }
     }

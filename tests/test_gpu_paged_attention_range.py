@@ -116,3 +116,47 @@ def test_weights_over_f16_caches_keep_22_bits(dim):
                - (2.0 ** -11 - 2.0 ** -22) * 1.01 * a[b])
         err = np.abs(got[b] - want[b])
         assert np.all(err <= tol), (n, float((err / tol).max()), int((err > tol).sum()))
+
+
+@pytest.mark.parametrize("kind,rows,dim,n", [("f16", "f16", 128, 100), ("f16", "f16", 256, 1500), ("bf16", "bf16", 64, 700),
+                                             ("bf16", "bf16", 256, 60), ("bf16", "f32", 128, 100), ("bf16", "f32", 64, 3000)])
+def test_infinite_values_that_are_seen(kind, rows, dim, n):
+    """A mean over an infinite value is that infinity, over both infinities or a NaN it is NaN, and the other
+    elements of the head are what they are without it (weights 2^-18 off, as for the largest values)."""
+    rng = np.random.default_rng(dim)
+    page, kv, group = 16, 2, 3
+    per = (n + page - 1) // page
+    cache = do.Cache(kind, per, kv, page, dim, seed=4)
+    table = np.arange(per, dtype=np.int32)[None]
+    q = queries(rng, 1, kv * group, dim, rows)
+    c = Call(cache, q, rows, table, [n], n, 0.05, 0)
+    v = cache.part("v")
+    v[0, 1, 3, [2, 7, 11, 40]] = 0.0
+    v[per - 1, 1, 1, [2, 7, 11, 40]] = 0.0
+    want, _, a, s, x = do.attention(cache, q, table, [n], n, 0.05, 0)
+    tol = do.attention_bound(want, a, s, x, n, dim, kind, rows) + 2.0 ** -18 * a
+    v[0, 1, 3, 2], v[0, 1, 3, 7], v[0, 1, 3, 11], v[per - 1, 1, 1, 11] = (float(t) for t in ("inf", "-inf", "inf", "-inf"))
+    v[per - 1, 1, 1, 40] = float("nan")
+    got = c.run()
+    far = got[0, group:]
+    assert np.all(far[:, 2] == np.inf) and np.all(far[:, 7] == -np.inf) and np.isnan(far[:, [11, 40]]).all()
+    got[0, group:, [2, 7, 11, 40]] = want[0, group:, [2, 7, 11, 40]]
+    assert np.all(np.abs(got - want) <= tol), float((np.abs(got - want) / tol).max())
+
+
+@pytest.mark.parametrize("kind,rows", [("f16", "f16"), ("bf16", "bf16"), ("bf16", "f32")])
+def test_infinite_keys_that_are_seen(kind, rows):
+    """Where a key makes a score -inf its token has no weight, where +inf the outputs are NaN; with queries whose
+    second and third terms are zeros."""
+    rng = np.random.default_rng(6)
+    n, dim, page = 90, 64, 16
+    cache = do.Cache(kind, 6, 1, page, dim, seed=4)
+    table = np.arange(6, dtype=np.int32)[None]
+    q = queries(rng, 1, 3, dim, "bf16" if kind == "bf16" else "f16")
+    q[0, :, 5] = [1.0, 0.5, -2.0]
+    want, _, a, s, x = do.attention(cache, q, table, [n - 1], n, 0.05, 0)
+    cache.part("k")[(n - 1) // page, 0, (n - 1) % page, 5] = -float("inf")
+    got = Call(cache, q, rows, table, [n], n, 0.05, 0).run()
+    assert np.isnan(got[0, 2]).all()
+    tol = do.attention_bound(want, a, s, x, n, dim, kind, rows)
+    assert np.all(np.abs(got - want)[0, :2] <= tol[0, :2])
