@@ -417,12 +417,13 @@ int pk_gpu_encoder_get_numerics(pk_gpu_encoder *enc);
 void pk_gpu_encoder_destroy(pk_gpu_encoder *enc);
 
 /* ---- autoregressive decoder (device pointers, no synchronisation) ------
- * The operators of one block's step of a decoder that reads the encoder's
- * frames token by token: norm, projection of 8-bit rows, a paged key-value
- * cache and the attention of one new token over it.  No counterpart in the
- * reference (its decoder is an LSTM, decoder.c:1-132).  None of them allocates,
- * waits or keeps anything between calls, so all may be captured in a HIP
- * graph.  Pointers are of the library's device, whichever device is current.
+ * Operators for a caller's own attention decoder beside the encoder, as one
+ * block's step needs them: norm, projection of 8-bit rows, a paged key-value
+ * cache and the attention of one new token over it.  Nothing else in this
+ * library calls them: the reference's decoder is an LSTM (decoder.c:1-132).
+ * None of them allocates, waits or keeps anything between calls, so all may be
+ * captured in a HIP graph.  Pointers are of the library's device, whichever
+ * device is current.
  * Sizes whose launch would pass 2^32 threads are refused: cache calls of 2^35
  * elements, attention of 2^23 workgroups (sequences x key-value heads x 16 query heads x
  * chunks), panels of 64 GiB, products of 2^23 tiles (2^26 columns at up to 16 rows).

@@ -36,7 +36,9 @@
 // 2^-10 of the running maximum keeps all of them and one down to 2^-21 its first 11.
 // Maxima, sums and outputs are fp32 throughout.
 //
-// Bytes of K and V are the bound, and registers hold what is in flight: 8 waves
+// Bytes of K and V are the bound (once for each 16 query heads of a key-value head: the
+// workgroups of further 16s fetch them again; 32 sequences of 3000 tokens over 1 head of
+// 128 in bf16 21.8 us with 16 query heads, 23.5 with 32, 37.3 with 64), and registers hold what is in flight: 8 waves
 // a workgroup, one or two workgroups a CU, each wave with a tile's keys and
 // values (8 KB of int8 at 128) on the way.  96 sequences of 3000 tokens, 8 heads of 128:
 // 111 us in int8 (5.5 TB/s), 205 us in bf16 (5.75 TB/s).
@@ -102,7 +104,7 @@ __device__ __host__ inline Span span_of(int len, int max_len, int window, int ch
 }
 
 // Waves of a workgroup, all of one chunk.  8 keep one CU's share of the memory
-// busy by themselves, so that 128 or more pairs need not be split at all.  The
+// busy by themselves; which sequences are split all the same, cuts() says.  The
 // kernels with most registers (heads of 256, queries in 3 terms) run one wave a
 // SIMD: 64 sequences of 2000 tokens, 2 heads of 256 in int8, f32 queries 34.8 us;
 // 8 waves, which spill, 44.
