@@ -36,12 +36,13 @@
 // 2^-10 of the running maximum keeps all of them and one down to 2^-21 its first 11.
 // Maxima, sums and outputs are fp32 throughout.
 //
-// Bytes of K and V are the bound (once for each 16 query heads of a key-value head: the
-// workgroups of further 16s fetch them again; 32 sequences of 3000 tokens over 1 head of
-// 128 in bf16 21.8 us with 16 query heads, 23.5 with 32, 37.3 with 64), and registers hold what is in flight: 8 waves
-// a workgroup, one or two workgroups a CU, each wave with a tile's keys and
-// values (8 KB of int8 at 128) on the way.  96 sequences of 3000 tokens, 8 heads of 128:
-// 111 us in int8 (5.5 TB/s), 205 us in bf16 (5.75 TB/s).
+// Bytes of K and V are the bound, once for each 16 query heads of a key-value head:
+// the workgroups of further 16s fetch them again (32 sequences of 3000 tokens over 1
+// head of 128 in bf16 21.8 us with 16 query heads, 23.5 with 32, 37.3 with 64).
+// Registers hold what is in flight: 8 waves a workgroup, one or two workgroups a CU,
+// each wave with a tile's keys and values (8 KB of int8 at 128) on the way.  96
+// sequences of 3000 tokens, 8 heads of 128: 111 us in int8 (5.5 TB/s), 205 us in bf16
+// (5.75 TB/s).
 //
 // The running maximum m only moves when a score passes it by more than 8
 // (powers of two, where p and its sums lose nothing), so most tiles need no
@@ -49,13 +50,14 @@
 //
 // Values of the largest magnitudes: sums of up to 2^8 p v over 2^30 tokens can
 // pass the largest float where their mean does not; and where v or k is infinite,
-// a second term of p or q that is 0 or negative makes NaN of it.  A wave whose sums have passed
-// 2^100 or become NaN takes its tiles once more, with infinities and NaN left out of all
-// products but the first term's, and with m raised by 40: p stays below 2^-32, all its
-// sums below 2^126, and the 8 waves' and 256 chunks' sums below that still (their tokens
-// are 2^30 together).  Exponents of p then hold up to 48 + what they held, 2^-19 off.
-// Every other wave's sums are below 2^100, so what they join to is finite.  Sums of F16
-// values stay below 2^61: there m is not raised.
+// a second term of p or q that is 0 or of the other sign makes NaN of it.  A wave
+// whose sums have passed 2^100 or become NaN takes its tiles once more, with
+// infinities and NaN left out of all products but the first term's, and with m raised
+// by 40: p stays below 2^-32, all its sums below 2^126, and the 8 waves' and 256
+// chunks' sums below that still (their tokens are 2^30 together).  Exponents of p then
+// hold up to 48 + what they held, 2^-19 off.  Every other wave's sums are below 2^100,
+// so what they join to is finite.  Sums of F16 values stay below 2^61: there m is not
+// raised.
 //
 // A tile's keys and values stay in registers and are loaded one tile ahead: the
 // next keys once this tile's scores are formed, the next values once they
