@@ -435,12 +435,18 @@ void pk_gpu_encoder_destroy(pk_gpu_encoder *enc);
 #define PK_GPU_BF16 2
 #define PK_GPU_I8   3
 #define PK_GPU_E4M3 4   /* 8-bit float, 4 exponent and 3 mantissa bits, +-448 at most */
+#define PK_GPU_E2M1 5   /* 4-bit float, 2 exponent bits and 1 mantissa bit: 0, 0.5, 1, 1.5, 2, 3,
+                         * 4, 6 as codes 0..7, their negatives 8..15; two in a byte, the even
+                         * element in the low half.  Caches only */
 
 /* A paged key-value cache of one layer; the memory is the caller's.
  *   k, v              [n_pages][heads][page_size][head_dim] of `dtype`: F16,
- *                     BF16, I8 or E4M3
- *   k_scale, v_scale  [n_pages][heads][page_size] floats, what a row's codes
- *                     are multiplied with (I8 and E4M3; unused otherwise)
+ *                     BF16, I8, E4M3 or E2M1
+ *   k_scale, v_scale  I8 and E4M3: [n_pages][heads][page_size] floats, what a row's
+ *                     codes are multiplied with.  E2M1: bytes behind the same pointers,
+ *                     [n_pages][heads][page_size][head_dim / 32]: the codes of each 32
+ *                     elements are multiplied with 2^(byte - 127) (255: NaN).  Unused
+ *                     otherwise
  * head_dim 64, 128 or 256; page_size a power of two, at least 16; n_pages *
  * page_size below 2^31 (the arrays may pass 4 GiB); arrays 16-byte aligned.
  * Slot s is offset s % page_size of page s / page_size. */
@@ -460,7 +466,11 @@ typedef struct {
  * rounded to nearest, ties to even, all in fp32 (scale a float lower where
  * top * scale would overflow).  A row with a < 2^-100 is
  * written as zeros (scale 0); a row that holds an infinity or a NaN reads back
- * as NaN (scale NaN).  Rows 16-byte aligned. */
+ * as NaN (scale NaN).  4-bit caches take, per token, head and 32 elements, with a
+ * their largest magnitude: the smallest power of two u with a <= 7 u (2^125 at most,
+ * where codes end at 6 u), codes x / u rounded to nearest, ties to the even code, so
+ * nothing is off by more than half a step; a < 2^-100 gives zeros (byte 0), an infinity
+ * or a NaN a group that reads back as NaN (byte 255).  Rows 16-byte aligned. */
 int pk_gpu_kv_write_dev(const pk_gpu_kv_cache *cache, int dtype, const void *dk, int ldk,
                         const void *dv, int ldv, const int *dslots, int n, void *stream);
 /* Read them back: row i of dk and dv receives slot dslots[i], code * scale in
@@ -476,7 +486,7 @@ int pk_gpu_kv_read_dev(const pk_gpu_kv_cache *cache, int dtype, const int *dslot
  * cache's, attends over the key-value head it shares with heads / cache->heads
  * - 1 neighbours: softmax of scale * q . k_t over the tokens it sees, times v.
  *   q, out    [B] rows of heads * head_dim elements of `dtype`, ldq and ldo apart:
- *             any of F32, F16, BF16 over I8 and E4M3 caches, F16 over F16,
+ *             any of F32, F16, BF16 over I8, E4M3 and E2M1 caches, F16 over F16,
  *             BF16 or F32 over BF16; 16-byte aligned rows
  *   window    > 0: only the last `window` tokens; 0: all
  *   max_len   at most 2^30; no sequence is longer (a larger dlens[b] counts as max_len, one

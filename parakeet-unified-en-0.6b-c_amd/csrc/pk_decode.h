@@ -14,6 +14,15 @@
 // scale 0 and codes 0 (inv of smaller rows could overflow); a row that holds
 // an infinity or a NaN gets scale NaN and codes 0, so all of it reads back as
 // NaN rather than as finite values of a wrong size.
+//
+// 4-bit rows (e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) are cut into
+// groups of 32 elements; with a = max |x| of a group its unit u is the smallest
+// power of two with a <= 7 u, so that no element is off by more than half a step (7 u
+// goes to 6 u), and code = x / u rounded to nearest, ties to even: exact steps all
+// of them, done by the matrix cores' own conversion.  u is stored as one byte,
+// its exponent + 127, at most 2^125 (6 u stays finite); a < 2^-100 gives zeros with
+// byte 0, a group with an infinity or a NaN byte 255, which reads back as NaN.
+// code * u is exact in bf16.
 #pragma once
 
 #include "pk_gpu.h"
@@ -44,8 +53,13 @@ typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
 // element types as template parameters
-constexpr int F32 = PK_GPU_F32, F16 = PK_GPU_F16, BF16 = PK_GPU_BF16, I8 = PK_GPU_I8, E4M3 = PK_GPU_E4M3;
-constexpr int size_of(int t) { return t == F32 ? 4 : t == F16 || t == BF16 ? 2 : 1; }
+constexpr int F32 = PK_GPU_F32, F16 = PK_GPU_F16, BF16 = PK_GPU_BF16, I8 = PK_GPU_I8, E4M3 = PK_GPU_E4M3,
+              E2M1 = PK_GPU_E2M1;
+constexpr int size_of(int t) { return t == F32 ? 4 : t == F16 || t == BF16 ? 2 : 1; }     // not of E2M1
+constexpr int bytes_of(int t, int elements) { return t == E2M1 ? elements / 2 : elements * size_of(t); }
+constexpr int kGroup = 32;                 // elements of an e2m1 row that share a unit
+// whether a cache holds codes with an fp32 scale for each row
+constexpr bool row_scaled(int t) { return t == I8 || t == E4M3; }
 constexpr float top_of(int t) { return t == I8 ? 127.0f : 448.0f; }
 constexpr float kTinyRow = 0x1p-100f;
 // The largest scale s whose 127 s is finite: fl(a / 127) of an a within an ulp
@@ -161,6 +175,38 @@ __device__ inline RowCode row_code(uint32_t amax_bits, float top)
     const float a = __uint_as_float(amax_bits);
     if (a < kTinyRow) return {0.0f, 0.0f};
     return {fminf(__fdiv_rn(a, top), kTopScale), __fdiv_rn(top, a)};
+}
+// The unit of a group of 4-bit codes from the bits of its max |x|: its byte. A
+// unit's bits as a float are byte << 23 (the conversions take 0 for 2^-127 and
+// infinity for NaN).
+__device__ inline uint32_t group_byte(uint32_t amax_bits)
+{
+    if (amax_bits >= 0x7f800000u) return 255;
+    if (__uint_as_float(amax_bits) < kTinyRow) return 0;
+    const uint32_t e = (amax_bits >> 23) - 2 + ((amax_bits & 0x7fffffu) > 0x600000u);
+    return e < 252 ? e : 252;
+}
+// 8 elements of a group as codes; zeros where it has none.
+__device__ inline uint32_t codes_e2m1(const float* x, uint32_t byte)
+{
+    const bool none = byte == 0 || byte == 255;
+    const float unit = __uint_as_float(byte << 23);
+    uint32_t w = 0;
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = none ? 0.0f : x[i];
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[0], y[1], unit, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[2], y[3], unit, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[4], y[5], unit, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[6], y[7], unit, 3);
+}
+__device__ inline void values_e2m1(uint32_t w, uint32_t byte, float* x)
+{
+    const float unit = __uint_as_float(byte << 23);
+    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, unit, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, unit, 1);
+    const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, unit, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, unit, 3);
+    x[0] = a[0]; x[1] = a[1]; x[2] = b[0]; x[3] = b[1];
+    x[4] = c[0]; x[5] = c[1]; x[6] = d[0]; x[7] = d[1];
 }
 // x * inv, 0 where the row has no codes (x may be NaN or infinite there)
 __device__ inline float coded(float x, RowCode c) { return c.inv == 0.0f ? 0.0f : __fmul_rn(x, c.inv); }

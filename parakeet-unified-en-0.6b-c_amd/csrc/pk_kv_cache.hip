@@ -3,9 +3,9 @@
 //
 // A cache row is one token's key (or value) of one head: head_dim elements at
 // ((page * heads + head) * page_size + offset) * head_dim.  8-bit caches hold
-// codes with one fp32 scale a row (pk_decode.h gives the formula); the row's
-// largest magnitude is exact whatever the order it is found in, so codes and
-// scales do not depend on the launch.
+// codes with one fp32 scale a row, 4-bit ones with a byte for each 32 elements
+// (pk_decode.h gives the formulas); the largest magnitude of a row or group is exact
+// whatever the order it is found in, so codes and scales do not depend on the launch.
 //
 // Both kernels move 8 elements of K and of V a thread, head_dim / 8 lanes a
 // row, so that a wave's loads and stores are whole rows; the maximum is
@@ -56,14 +56,22 @@ __device__ inline uint32_t max_bits(const float* x)
 template <int CACHE, int DIM>
 __device__ inline void write_part(void* cache, float* scales, long long row, int part, float* x)
 {
-    if constexpr (CACHE == I8 || CACHE == E4M3) {
+    if constexpr (CACHE == E2M1) {
+        const uint32_t byte = group_byte(max_over<kGroup / 8>(max_bits(x)));
+        const uint32_t w = codes_e2m1(x, byte);
+        if (row < 0) return;
+        if (part % (kGroup / 8) == 0)
+            reinterpret_cast<uint8_t*>(scales)[(size_t)row * (DIM / kGroup) + part / (kGroup / 8)] = (uint8_t)byte;
+        reinterpret_cast<uint32_t*>(cache)[(size_t)row * (DIM / 8) + part] = w;
+        return;
+    } else if constexpr (row_scaled(CACHE)) {
         const RowCode c = row_code(max_over<DIM / 8>(max_bits(x)), top_of(CACHE));
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = coded(x[i], c);
         if (row >= 0 && part == 0) scales[row] = c.scale;
     }
-    if (row >= 0)
-        store8<CACHE>(static_cast<char*>(cache) + ((size_t)row * DIM + 8 * part) * size_of(CACHE), x);
+    if constexpr (CACHE != E2M1)
+        if (row >= 0) store8<CACHE>(static_cast<char*>(cache) + ((size_t)row * DIM + 8 * part) * size_of(CACHE), x);
 }
 
 template <int CACHE, int ROWS, int DIM>
@@ -94,11 +102,18 @@ __global__ void __launch_bounds__(kMostThreads) kv_read(RowsArgs a)
     const uint32_t token = r / a.heads, head = r - token * a.heads;
     const long long row = cache_row(a, token, head);
     if (row < 0) return;
-    const size_t from = ((size_t)row * DIM + 8 * part) * size_of(CACHE);
     float k[8], v[8];
-    load8<CACHE>(static_cast<const char*>(a.k) + from, k);
-    load8<CACHE>(static_cast<const char*>(a.v) + from, v);
-    if constexpr (CACHE == I8 || CACHE == E4M3) {
+    if constexpr (CACHE == E2M1) {
+        const size_t word = (size_t)row * (DIM / 8) + part;
+        const size_t group = (size_t)row * (DIM / kGroup) + part / (kGroup / 8);
+        values_e2m1(static_cast<const uint32_t*>(a.k)[word], reinterpret_cast<const uint8_t*>(a.k_scale)[group], k);
+        values_e2m1(static_cast<const uint32_t*>(a.v)[word], reinterpret_cast<const uint8_t*>(a.v_scale)[group], v);
+    } else {
+        const size_t from = ((size_t)row * DIM + 8 * part) * size_of(CACHE);
+        load8<CACHE>(static_cast<const char*>(a.k) + from, k);
+        load8<CACHE>(static_cast<const char*>(a.v) + from, v);
+    }
+    if constexpr (row_scaled(CACHE)) {
         const float sk = a.k_scale[row], sv = a.v_scale[row];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -176,6 +191,7 @@ int kv_call(bool write, const pk_gpu_kv_cache* c, int dtype, const void* dk, int
     hipStream_t s = static_cast<hipStream_t>(stream);
     const hipError_t e = c->dtype == I8   ? launch_rows<I8>(write, dtype, c->head_dim, a, s)
                        : c->dtype == E4M3 ? launch_rows<E4M3>(write, dtype, c->head_dim, a, s)
+                       : c->dtype == E2M1 ? launch_rows<E2M1>(write, dtype, c->head_dim, a, s)
                        : c->dtype == F16  ? launch_rows<F16>(write, dtype, c->head_dim, a, s)
                                           : launch_rows<BF16>(write, dtype, c->head_dim, a, s);
     return e == hipSuccess ? PK_GPU_OK : rt::hip_error(e, who);
@@ -186,8 +202,8 @@ int kv_call(bool write, const pk_gpu_kv_cache* c, int dtype, const void* dk, int
 int check_cache(const pk_gpu_kv_cache* c, const char* who)
 {
     if (!c) return rt::error(PK_GPU_EINVAL, "%s: NULL cache", who);
-    if (c->dtype != F16 && c->dtype != BF16 && c->dtype != I8 && c->dtype != E4M3)
-        return rt::error(PK_GPU_EINVAL, "%s: a cache of type %d (F16, BF16, I8 or E4M3)", who, c->dtype);
+    if (c->dtype != F16 && c->dtype != BF16 && !row_scaled(c->dtype) && c->dtype != E2M1)
+        return rt::error(PK_GPU_EINVAL, "%s: a cache of type %d (F16, BF16, I8, E4M3 or E2M1)", who, c->dtype);
     if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
         return rt::error(PK_GPU_ENOTSUP, "%s: head_dim = %d (64, 128 or 256)", who, c->head_dim);
     if (c->page_size < 16 || (c->page_size & (c->page_size - 1)))
@@ -198,7 +214,7 @@ int check_cache(const pk_gpu_kv_cache* c, const char* who)
         return rt::error(PK_GPU_EINVAL, "%s: %d pages of %d exceed 2^31 slots", who, c->n_pages, c->page_size);
     if ((long long)c->heads * c->head_dim > 0x7fffffff)
         return rt::error(PK_GPU_EINVAL, "%s: %d heads of %d exceed 2^31 elements", who, c->heads, c->head_dim);
-    const bool coded = c->dtype == I8 || c->dtype == E4M3;
+    const bool coded = row_scaled(c->dtype) || c->dtype == E2M1;
     if (!c->k || !c->v || (coded && (!c->k_scale || !c->v_scale)))
         return rt::error(PK_GPU_EINVAL, "%s: the cache's k, v or their scales are NULL", who);
     if (!aligned16(c->k) || !aligned16(c->v) || (coded && (!aligned16(c->k_scale) || !aligned16(c->v_scale))))

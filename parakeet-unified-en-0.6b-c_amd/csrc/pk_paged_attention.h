@@ -25,8 +25,10 @@
 // head_dim / 16 elements of its 8 tokens and transposes them 4 x 4.
 //
 // Arithmetic: int8 and e4m3 codes are exact in bf16 and f16, and so are the
-// caches' 16-bit elements in their own type.  Queries enter with all their bits:
-// f16 and bf16 ones in their own type, f32 ones as a sum of 3 bf16 terms (8 bits
+// caches' 16-bit elements in their own type, and 4-bit ones in bf16 with their unit
+// multiplied in (one conversion for two of them; so they need no scale on scores or
+// weights).  Queries enter with all their bits: f16 and bf16 ones in their own type (f16
+// ones over 4 bits as 2 bf16 terms), f32 ones as a sum of 3 bf16 terms (8 bits
 // each, cut off: rounded, a query near the largest float would become infinite).  So
 // scores have fp32 accuracy.
 // p v_scale enters the second product in 2 bf16 terms for 16-bit outputs (16
@@ -143,8 +145,8 @@ __device__ inline int nth_longest(const PagedArgs& a, int nth, int* lens, int wa
 // Terms of the query and of p: see above.
 // Whether the scores are formed in f16: its own caches, and f16 queries over
 // codes, which f16 holds exactly too.
-constexpr bool keys_f16(int cache, int t) { return cache == F16 || t == F16; }
-constexpr int q_terms(int cache, int t) { return t == F32 ? 3 : 1; }
+constexpr bool keys_f16(int cache, int t) { return cache != E2M1 && (cache == F16 || t == F16); }
+constexpr int q_terms(int cache, int t) { return t == F32 ? 3 : cache == E2M1 && t == F16 ? 2 : 1; }
 constexpr int p_terms(int t) { return t == F32 ? 3 : 2; }
 
 template <bool IN_F16>
@@ -181,6 +183,20 @@ __device__ inline u32x2 codes_16(uint32_t w)
         const bf16x2 h = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true);
         return (u32x2){__builtin_bit_cast(uint32_t, l), __builtin_bit_cast(uint32_t, h)};
     }
+}
+
+// 4-bit elements 2 i and 2 i + 1 of a word, and all 8 of it, times their unit, as bf16: exactly.
+__device__ __forceinline__ uint32_t pair_of_e2m1(uint32_t w, uint32_t byte, int i)
+{
+    const float unit = __uint_as_float(byte << 23);
+    return __builtin_bit_cast(uint32_t, i == 0   ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, unit, 0)
+                                        : i == 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, unit, 1)
+                                        : i == 2 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, unit, 2)
+                                                 : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, unit, 3));
+}
+__device__ inline u32x4 bf16_of_e2m1(uint32_t w, uint32_t byte)
+{
+    return (u32x4){pair_of_e2m1(w, byte, 0), pair_of_e2m1(w, byte, 1), pair_of_e2m1(w, byte, 2), pair_of_e2m1(w, byte, 3)};
 }
 
 // 8 elements with infinities and NaN as zeros.
@@ -222,11 +238,13 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
 {
     constexpr int NW = waves_of(CACHE, T, DIM);
     constexpr int S = size_of(CACHE);
-    constexpr bool CODED = CACHE == I8 || CACHE == E4M3;
-    constexpr int KL = DIM * S / 64;           // 16-byte pieces of a key a lane holds
+    constexpr int RB = bytes_of(CACHE, DIM);   // bytes of a row
+    constexpr bool CODED = row_scaled(CACHE), FOUR = CACHE == E2M1;
+    constexpr int KL = RB < 64 ? 1 : RB / 64;  // 16-byte pieces of a key a lane holds (8 bytes of 4-bit heads of 64)
+    constexpr int KP = RB < 64 ? RB / 4 : 16;  // bytes of a piece
     constexpr int STEPS = DIM / 32;            // matrix instructions along a head
-    constexpr int VB = DIM * S / 16;           // bytes of a value a lane holds
-    constexpr int VW = VB / 4;
+    constexpr int VB = RB / 16;                // bytes of a value a lane holds
+    constexpr int VW = VB < 4 ? 1 : VB / 4;
     constexpr int E = DIM / 16;                // elements of those, accumulators
     constexpr int QT = q_terms(CACHE, T), PT = p_terms(T);
     constexpr float BIAS = CACHE == F16 ? 7.0f : 0.0f;
@@ -274,14 +292,16 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
     const int head = kvh * a.group + in_group;
 
     // queries: step c takes elements el(c, i) = i + 8 g + 32 c of a 16-bit cache's
-    // rows, i + 16 g + 8 (c % 2) + 64 (c / 2) of an 8-bit one's; every wave reads
+    // rows, i + 16 g + 8 (c % 2) + 64 (c / 2) of an 8-bit one's, i + 32 g + 8 (c % 4)
+    // + 128 (c / 4) of a 4-bit one's (16 g + 8 c in heads of 64); every wave reads
     // the same ones, in the order they are multiplied, from LDS
     constexpr int QS = (STEPS + NW - 1) / NW;  // steps a wave stages
     float qv[QS][8] = {};
 #pragma unroll
     for (int i = 0; i < QS; ++i) {
         const int c = wave + i * NW;
-        const int el = S == 2 ? 32 * c + 8 * g : 64 * (c / 2) + 16 * g + 8 * (c % 2);
+        const int el = FOUR ? (DIM == 64 ? 16 * g + 8 * c : 128 * (c / 4) + 32 * g + 8 * (c % 4))
+                       : S == 2 ? 32 * c + 8 * g : 64 * (c / 2) + 16 * g + 8 * (c % 2);
         if (c < STEPS && head_ok)
             load8<T>(a.q + (size_t)b * a.ldq + ((size_t)head * DIM + el) * size_of(T), qv[i]);
     }
@@ -311,16 +331,30 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
     u32x4 kr[2][KL];
     uint32_t vr[2][4][VW];
     f32x4 ks[2], vs[2];
+    // 4 bits: the units of a lane's pieces of a key (as floats' bits), and of its
+    // elements of 4 values (the group of those is E n / 32)
+    constexpr int UB = DIM / kGroup;           // bytes a row
+    uint32_t ku[2][FOUR ? KL : 1], vu[2][4];
     // scalar base + this lane's offset + a constant
-    const uint32_t k_off = n * (DIM * S) + 16 * g;
-    const uint32_t v_off = 4 * g * (DIM * S) + n * (VB > 16 ? 16 : VB);
+    const uint32_t k_off = n * RB + KP * g;
+    const uint32_t v_off = 4 * g * RB + n * (VB > 16 ? 16 : VB);
     const uint32_t s_off = 16 * g;
+    const uint32_t ku_off = n * UB + (DIM == 64 ? g / 2 : g), vu_off = 4 * g * UB + n * E / kGroup;
     auto load_k = [&](const Halves& h) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const char* base = a.k + h.row[u] * (DIM * S);
+            const char* base = a.k + h.row[u] * RB;
 #pragma unroll
-            for (int j = 0; j < KL; ++j) kr[u][j] = *reinterpret_cast<const u32x4*>(base + k_off + 64 * j);
+            for (int j = 0; j < KL; ++j) {
+                if constexpr (KP == 8) {
+                    const u32x2 w = *reinterpret_cast<const u32x2*>(base + k_off);
+                    kr[u][j] = (u32x4){w[0], w[1], 0, 0};
+                } else {
+                    kr[u][j] = *reinterpret_cast<const u32x4*>(base + k_off + 64 * j);
+                }
+                if constexpr (FOUR)
+                    ku[u][j] = (uint32_t)(reinterpret_cast<const uint8_t*>(a.k_scale) + h.row[u] * UB)[ku_off + 4 * j];
+            }
             if constexpr (CODED)
                 ks[u] = *reinterpret_cast<const f32x4*>(reinterpret_cast<const char*>(a.k_scale + h.row[u]) + s_off);
         }
@@ -328,11 +362,15 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
     auto load_v = [&](const Halves& h) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const char* base = a.v + h.row[u] * (DIM * S);
+            const char* base = a.v + h.row[u] * RB;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const char* p = base + v_off + i * (DIM * S);
-                if constexpr (VB == 4) {
+                const char* p = base + v_off + i * RB;
+                if constexpr (FOUR)
+                    vu[u][i] = (uint32_t)(reinterpret_cast<const uint8_t*>(a.v_scale) + h.row[u] * UB)[vu_off + i * UB];
+                if constexpr (VB == 2) {
+                    vr[u][i][0] = *reinterpret_cast<const uint16_t*>(p);
+                } else if constexpr (VB == 4) {
                     vr[u][i][0] = *reinterpret_cast<const uint32_t*>(p);
                 } else if constexpr (VB == 8) {
                     const u32x2 w = *reinterpret_cast<const u32x2*>(p);
@@ -411,6 +449,8 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
                     const u32x2 lo = codes_16<CACHE, KF>(kr[u][c / 2][2 * (c % 2)]);
                     const u32x2 hi = codes_16<CACHE, KF>(kr[u][c / 2][2 * (c % 2) + 1]);
                     f = (u32x4){lo[0], lo[1], hi[0], hi[1]};
+                } else if constexpr (FOUR) {
+                    f = bf16_of_e2m1(kr[u][c / 4][c % 4], ku[u][c / 4]);
                 } else {
                     f = kr[u][c];
                 }
@@ -438,6 +478,7 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
                     if (!in) {
                         s[u][r] = -__builtin_inff();
                         if constexpr (CODED) vs[u][r] = 0.0f;
+                        if constexpr (FOUR) vu[u][r] = 0;
 #pragma unroll
                         for (int d = 0; d < VW; ++d) vr[u][r][d] = 0;
                     }
@@ -506,15 +547,23 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
             }
         } else {
 #pragma unroll
-            for (int w = 0; w < VW; ++w) {
+            for (int w = 0; w < E / 2; ++w) {
+                uint32_t pair[2][4];           // elements 2 w and 2 w + 1 of the lane's tokens
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if constexpr (FOUR) pair[u][i] = pair_of_e2m1(vr[u][i][w / 4], vu[u][i], w % 4);
+                        else pair[u][i] = vr[u][i][w];
+                    }
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const uint32_t sel = i ? 0x07060302u : 0x05040100u;
                     u32x4 f;
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        f[2 * u] = __builtin_amdgcn_perm(vr[u][1][w], vr[u][0][w], sel);
-                        f[2 * u + 1] = __builtin_amdgcn_perm(vr[u][3][w], vr[u][2][w], sel);
+                        f[2 * u] = __builtin_amdgcn_perm(pair[u][1], pair[u][0], sel);
+                        f[2 * u + 1] = __builtin_amdgcn_perm(pair[u][3], pair[u][2], sel);
                     }
 #pragma unroll
                     for (int j = PT - 1; j >= 0; --j)
@@ -634,6 +683,7 @@ hipError_t launch_paged_f16(int t, int dim, const PagedArgs& a, dim3 grid, hipSt
 hipError_t launch_paged_bf16(int t, int dim, const PagedArgs& a, dim3 grid, hipStream_t s);
 hipError_t launch_paged_i8(int t, int dim, const PagedArgs& a, dim3 grid, hipStream_t s);
 hipError_t launch_paged_e4m3(int t, int dim, const PagedArgs& a, dim3 grid, hipStream_t s);
+hipError_t launch_paged_e2m1(int t, int dim, const PagedArgs& a, dim3 grid, hipStream_t s);
 
 template <int CACHE, int T>
 hipError_t launch_paged(int dim, const PagedArgs& a, dim3 grid, hipStream_t s)

@@ -130,7 +130,7 @@ long long cuts(const pk_gpu_kv_cache* c, long long pairs, long long span)
 {
     const long long rounds = (span + kRound - 1) / kRound;
     if (rounds <= 3) return 1;
-    const long long fill = 256 / pairs, two = 512 / pairs, large = span * 2 * c->head_dim * size_of(c->dtype) / (384 << 10);
+    const long long fill = 256 / pairs, two = 512 / pairs, large = span * 2 * bytes_of(c->dtype, c->head_dim) / (384 << 10);
     long long n = two < large ? two : large;
     if (n < fill) n = fill;
     if (n > rounds) n = rounds;
@@ -276,6 +276,7 @@ int pk_gpu_paged_attention_dev(const pk_gpu_kv_cache* cache, int dtype, const vo
     hipError_t e = cache->dtype == F16    ? launch_paged_f16(dtype, dim, a, grid, s)
                    : cache->dtype == BF16 ? launch_paged_bf16(dtype, dim, a, grid, s)
                    : cache->dtype == I8   ? launch_paged_i8(dtype, dim, a, grid, s)
+                   : cache->dtype == E2M1 ? launch_paged_e2m1(dtype, dim, a, grid, s)
                                           : launch_paged_e4m3(dtype, dim, a, grid, s);
     if (e == hipSuccess && p.splits > 1) {
         JoinArgs j{};

@@ -104,7 +104,7 @@ NUMERICS_DEFAULT, NUMERICS_EXACT, NUMERICS_FAST = 0, 1, 2
 # PK_GPU_STAGE_*: pk_gpu_encoder_profile_read's stages
 STAGE_GEMM_I4, STAGE_GEMM_I8, STAGE_GEMM_F32, STAGE_ATTENTION, STAGE_LAYER_NORM, STAGE_CONV, STAGE_COPY = range(7)
 # PK_GPU_F32 ...: element types
-F32, F16, BF16, I8, E4M3 = range(5)
+F32, F16, BF16, I8, E4M3, E2M1 = range(6)
 NOALLOC_BYTES = 64 << 20          # PK_GPU_NOALLOC_BYTES
 SPLIT_WORKSPACE_BYTES = 32 << 20  # PK_GPU_SPLIT_WORKSPACE_BYTES
 

@@ -1,0 +1,71 @@
+"""Plain 64-bit (numpy) forms of the 4-bit cache, and the cache itself on the
+device, beside decode_oracle's.  Nothing here calls the library's kernels."""
+import numpy as np
+
+import decode_oracle as do
+from pkgpu import pk
+
+GROUP = 32
+LEVELS = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6])
+KINDS = dict(do.KINDS, e2m1=pk.E2M1)
+
+
+def codes4(x):
+    """The documented rule: codes 0..15 of the last axis and a byte for each 32 of it."""
+    x = np.asarray(x, np.float32)
+    g = x.reshape(x.shape[:-1] + (-1, GROUP)).astype(np.float64)
+    bad = ~np.isfinite(g).all(-1)
+    a = np.where(bad, 0.0, np.abs(np.where(np.isfinite(g), g, 0)).max(-1))
+    none = (a < do.TINY) | bad
+    e = np.floor(np.log2(np.where(none, 1.0, a))) - 2          # a / 2^e in [4, 8)
+    e = np.minimum(np.where(a > 7 * 2.0 ** e, e + 1, e), 125)
+    y = np.abs(np.where(none[..., None], 0.0, np.where(np.isfinite(g), g, 0) / 2.0 ** e[..., None]))
+    border = (LEVELS[1:] + LEVELS[:-1]) / 2                    # ties go to the even code
+    up = np.where(np.arange(7) % 2 == 1, y[..., None] >= border, y[..., None] > border)
+    code = up.sum(-1) + 8 * (np.signbit(g) & ~none[..., None])
+    byte = np.where(bad, 255, np.where(none, 0, e + 127)).astype(np.uint8)
+    return code.reshape(x.shape).astype(np.uint8), byte
+
+
+def stand_for(code, byte):
+    """float64 values of codes and bytes."""
+    v = LEVELS[code & 7] * np.where(code & 8, -1.0, 1.0)
+    unit = np.where(byte == 255, np.nan, 2.0 ** (byte.astype(np.float64) - 127))
+    return v * np.repeat(unit, GROUP, -1)
+
+
+class Cache4(do.Cache):
+    """A 4-bit cache on the device, with guards."""
+
+    def __init__(self, pages, heads, page, dim, seed=0, filled=True, spread=3):
+        import torch
+        self.kind, self.pages, self.heads, self.page, self.dim = "e2m1", pages, heads, page, dim
+        rng = np.random.default_rng(seed)
+        self.arrays = {}
+        for name in ("k", "v"):
+            x = rng.integers(0, 256, (pages, heads, page, dim // 2)) if filled else np.zeros((pages, heads, page, dim // 2))
+            u = (rng.integers(127 - spread, 127, (pages, heads, page, dim // GROUP)) if filled
+                 else np.zeros((pages, heads, page, dim // GROUP)))
+            self._put(name, torch.from_numpy(x.astype(np.uint8)))
+            self._put(name + "_scale", torch.from_numpy(u.astype(np.uint8)))
+
+    def struct(self):
+        p = {n: self.part(n).data_ptr() for n in self.arrays}
+        return pk.KvCache(p["k"], p["v"], p["k_scale"], p["v_scale"], pk.E2M1, self.pages, self.page, self.heads, self.dim)
+
+    def codes(self, name):
+        """[slots][heads][dim] codes and [slots][heads][dim / 32] bytes."""
+        b = self.part(name).cpu().numpy()
+        c = np.stack([b & 15, b >> 4], -1).reshape(b.shape[:3] + (self.dim,))
+        u = self.part(name + "_scale").cpu().numpy()
+        return (c.transpose(0, 2, 1, 3).reshape(-1, self.heads, self.dim),
+                u.transpose(0, 2, 1, 3).reshape(-1, self.heads, self.dim // GROUP))
+
+    def rows(self, name):
+        return stand_for(*self.codes(name))
+
+
+def cache_of(kind, pages, heads, page, dim, seed=0, filled=True):
+    if kind == "e2m1":
+        return Cache4(pages, heads, page, dim, seed, filled)
+    return do.Cache(kind, pages, heads, page, dim, seed, filled)
