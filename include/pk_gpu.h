@@ -514,6 +514,54 @@ int pk_gpu_paged_attention_dev(const pk_gpu_kv_cache *cache, int dtype, const vo
                                int max_len, float scale, int window, void *dout, int ldo,
                                float *dlse, float *dws, size_t ws_floats, void *stream);
 
+/* Rotary positions.  The first rot_dim elements of a head (even, 2 at least) turn in pairs,
+ * pair i of a row at position p by p * freqs[i] radians:
+ *   a' = (a cos - b sin) * scale,   b' = (b cos + a sin) * scale
+ * where (a, b) are elements i and i + rot_dim / 2, or with `interleaved` 2 i and 2 i + 1.
+ * Elements from rot_dim on stay as they are.
+ *   freqs  [rot_dim / 2] floats on the device (pk_gpu_rope_freqs, or the caller's own)
+ *   scale  1, or what cos and sin are multiplied with in a scaled long context
+ * The angle is formed and reduced in fp64 (p * freqs[i] rounded once, good to 2^-22 where
+ * it reaches 2^31), cos and sin, the products and sums are fp32, rounded once to the
+ * rows' type.  Positions may be negative: turned by -p, a row comes back. */
+typedef struct {
+    const float *freqs;
+    float        scale;
+    int          rot_dim, interleaved;
+} pk_gpu_rope;
+
+/* The frequencies base^(-2 i / rot_dim), i < rot_dim / 2, into host memory, as scaled:
+ *   PLAIN   as they are
+ *   LINEAR  divided by factor: positions of a context factor times longer
+ *   BASE    with base * factor^(rot_dim / (rot_dim - 2)): the highest stays, the lowest is
+ *           divided by factor (rot_dim 4 at least)
+ *   PARTS   each by the turns it makes over `trained` positions: from `fast` turns on it
+ *           stays, up to `slow` it is divided by factor, in between the two are mixed
+ *           linearly (0 <= slow < fast)
+ * Formed in fp64, rounded once.  base > 0; factor > 0 (PLAIN ignores it, and all but PARTS
+ * the other three).  Needs no device. */
+#define PK_GPU_ROPE_PLAIN  0
+#define PK_GPU_ROPE_LINEAR 1
+#define PK_GPU_ROPE_BASE   2
+#define PK_GPU_ROPE_PARTS  3
+int pk_gpu_rope_freqs(int rot_dim, double base, int scaling, double factor, double trained,
+                      double slow, double fast, float *freqs);
+
+/* Turn n rows of heads * head_dim elements of `dtype` (F32, F16 or BF16) to the positions
+ * dpos[0..n): y of x, ldx and ldy elements apart, head_dim 2 to 1024.  y may be x in place
+ * (with ldy = ldx); other overlaps are the caller's error.  Any alignment of whole elements. */
+int pk_gpu_rope_dev(const pk_gpu_rope *rope, int dtype, const void *dx, int ldx, int heads,
+                    int head_dim, const int *dpos, int n, void *dy, int ldy, void *stream);
+/* The same for a step's or a prompt's rows, one launch: the n queries of `heads` heads (0: none)
+ * are turned into dqo, which may be dq in place; the keys are turned and, with the
+ * values, written into the cache's slots as pk_gpu_kv_write_dev does (padding, codes and
+ * limits as there; codes are of the turned keys in fp32).  head_dim and the key-value
+ * heads are the cache's; rows 16-byte aligned. */
+int pk_gpu_rope_kv_write_dev(const pk_gpu_rope *rope, const pk_gpu_kv_cache *cache, int dtype,
+                             const void *dq, int ldq, int heads, void *dqo, int ldqo,
+                             const void *dk, int ldk, const void *dv, int ldv, const int *dpos,
+                             const int *dslots, int n, void *stream);
+
 /* Root-mean-square norm of `rows` rows of D elements, any D >= 1, with the
  * residual's addition:
  *   h   = x + res in fp32, rounded to `dtype`  (res NULL: h = x)

@@ -10,7 +10,7 @@
 // Both kernels move 8 elements of K and of V a thread, head_dim / 8 lanes a
 // row, so that a wave's loads and stores are whole rows; the maximum is
 // reduced inside that lane group and nothing goes through LDS.
-#include "pk_decode.h"
+#include "pk_kv_rows.h"
 
 namespace pkgpu {
 namespace decode {
@@ -24,55 +24,13 @@ struct RowsArgs {
     const int* slots;
     uint32_t rows;                  // n * heads
     uint32_t heads;
-    int page_shift, page_size, n_slots;
+    int page_shift, n_slots;
 };
 
 // Threads of a workgroup: a launch of many rows takes 1024 (20011 tokens of 8
 // heads of 128 from int8 to bf16: 25.6 us against 27.5 of 256), one of few 256, on
 // more CUs.
 constexpr int kMostThreads = 1024;
-
-// Index of the cache row that row r = token * heads + head names, or -1.
-__device__ inline long long cache_row(const RowsArgs& a, uint32_t token, uint32_t head)
-{
-    const int slot = a.slots[token];
-    if (slot < 0 || slot >= a.n_slots) return -1;
-    const uint32_t page = (uint32_t)slot >> a.page_shift, off = (uint32_t)slot & (a.page_size - 1);
-    return ((long long)page * a.heads + head) * a.page_size + off;
-}
-
-__device__ inline uint32_t max_bits(const float* x)
-{
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint32_t b = __float_as_uint(x[i]) & 0x7fffffffu;
-        m = b > m ? b : m;
-    }
-    return m;
-}
-
-// One row's 8 elements of this lane into the cache at element `at`.
-template <int CACHE, int DIM>
-__device__ inline void write_part(void* cache, float* scales, long long row, int part, float* x)
-{
-    if constexpr (CACHE == E2M1) {
-        const uint32_t byte = group_byte(max_over<kGroup / 8>(max_bits(x)));
-        const uint32_t w = codes_e2m1(x, byte);
-        if (row < 0) return;
-        if (part % (kGroup / 8) == 0)
-            reinterpret_cast<uint8_t*>(scales)[(size_t)row * (DIM / kGroup) + part / (kGroup / 8)] = (uint8_t)byte;
-        reinterpret_cast<uint32_t*>(cache)[(size_t)row * (DIM / 8) + part] = w;
-        return;
-    } else if constexpr (row_scaled(CACHE)) {
-        const RowCode c = row_code(max_over<DIM / 8>(max_bits(x)), top_of(CACHE));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = coded(x[i], c);
-        if (row >= 0 && part == 0) scales[row] = c.scale;
-    }
-    if constexpr (CACHE != E2M1)
-        if (row >= 0) store8<CACHE>(static_cast<char*>(cache) + ((size_t)row * DIM + 8 * part) * size_of(CACHE), x);
-}
 
 template <int CACHE, int ROWS, int DIM>
 __global__ void __launch_bounds__(kMostThreads) kv_write(RowsArgs a)
@@ -82,7 +40,7 @@ __global__ void __launch_bounds__(kMostThreads) kv_write(RowsArgs a)
     const int part = threadIdx.x % LANES;
     if (r >= a.rows) return;                       // whole lane groups leave together
     const uint32_t token = r / a.heads, head = r - token * a.heads;
-    const long long row = cache_row(a, token, head);
+    const long long row = cache_row(a.slots[token], head, a.heads, a.page_shift, a.n_slots);
     const size_t at = (size_t)head * DIM + 8 * part;
     float k[8], v[8];
     // the rows' loads do not wait for the slot: padding rows are read too
@@ -100,7 +58,7 @@ __global__ void __launch_bounds__(kMostThreads) kv_read(RowsArgs a)
     const int part = threadIdx.x % LANES;
     if (r >= a.rows) return;
     const uint32_t token = r / a.heads, head = r - token * a.heads;
-    const long long row = cache_row(a, token, head);
+    const long long row = cache_row(a.slots[token], head, a.heads, a.page_shift, a.n_slots);
     if (row < 0) return;
     float k[8], v[8];
     if constexpr (CACHE == E2M1) {
@@ -185,7 +143,6 @@ int kv_call(bool write, const pk_gpu_kv_cache* c, int dtype, const void* dk, int
     a.slots = dslots;
     a.rows = (uint32_t)n * c->heads;
     a.heads = c->heads;
-    a.page_size = c->page_size;
     a.page_shift = __builtin_ctz(c->page_size);
     a.n_slots = c->n_pages * c->page_size;
     hipStream_t s = static_cast<hipStream_t>(stream);

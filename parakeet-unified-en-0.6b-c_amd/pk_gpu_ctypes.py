@@ -19,7 +19,7 @@ HEADER = os.path.join(os.path.dirname(HERE), "include", "pk_gpu.h")
 NOTRANS = 111
 
 _i, _f, _p = ctypes.c_int, ctypes.c_float, ctypes.c_void_p
-_ll, _sz = ctypes.c_longlong, ctypes.c_size_t
+_ll, _sz, _d = ctypes.c_longlong, ctypes.c_size_t, ctypes.c_double
 
 _PROTOS = {
     "pk_gpu_init": (_i, [_i]),
@@ -91,6 +91,9 @@ _PROTOS = {
     "pk_gpu_encoder_profile_read": (_i, [_p, _i, _p, _p, _p, _p]),
     "pk_gpu_kv_write_dev": (_i, [_p, _i, _p, _i, _p, _i, _p, _i, _p]),
     "pk_gpu_kv_read_dev": (_i, [_p, _i, _p, _i, _p, _i, _p, _i, _p]),
+    "pk_gpu_rope_freqs": (_i, [_i, _d, _i, _d, _d, _d, _d, _p]),
+    "pk_gpu_rope_dev": (_i, [_p, _i, _p, _i, _i, _i, _p, _i, _p, _i, _p]),
+    "pk_gpu_rope_kv_write_dev": (_i, [_p, _p, _i, _p, _i, _i, _p, _i, _p, _i, _p, _i, _p, _p, _i, _p]),
     "pk_gpu_rms_norm_dev": (_i, [_i, _p, _i, _p, _i, _p, _i, _p, _f, _i, _p, _i, _p, _i, _i, _p]),
     "pk_gpu_w8_panel_bytes": (_sz, [_i, _i]),
     "pk_gpu_w8_panel_dev": (_i, [_i, _i, _p, _i, _p, _p]),
@@ -105,6 +108,8 @@ NUMERICS_DEFAULT, NUMERICS_EXACT, NUMERICS_FAST = 0, 1, 2
 STAGE_GEMM_I4, STAGE_GEMM_I8, STAGE_GEMM_F32, STAGE_ATTENTION, STAGE_LAYER_NORM, STAGE_CONV, STAGE_COPY = range(7)
 # PK_GPU_F32 ...: element types
 F32, F16, BF16, I8, E4M3, E2M1 = range(6)
+# PK_GPU_ROPE_*: how frequencies are scaled
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_PARTS = range(4)
 NOALLOC_BYTES = 64 << 20          # PK_GPU_NOALLOC_BYTES
 SPLIT_WORKSPACE_BYTES = 32 << 20  # PK_GPU_SPLIT_WORKSPACE_BYTES
 
@@ -150,6 +155,11 @@ class KvCache(ctypes.Structure):
     """pk_gpu_kv_cache (include/pk_gpu.h): a paged key-value cache, device pointers."""
     _fields_ = [("k", _p), ("v", _p), ("k_scale", _p), ("v_scale", _p), ("dtype", _i),
                 ("n_pages", _i), ("page_size", _i), ("heads", _i), ("head_dim", _i)]
+
+
+class Rope(ctypes.Structure):
+    """pk_gpu_rope (include/pk_gpu.h): rotary positions, frequencies on the device."""
+    _fields_ = [("freqs", _p), ("scale", _f), ("rot_dim", _i), ("interleaved", _i)]
 
 
 STATUS = {0: "OK", -1: "EINVAL", -2: "ENOTSUP", -3: "ENOMEM", -4: "EHIP", -5: "ENODEV", -6: "EBUSY"}

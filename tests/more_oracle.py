@@ -69,3 +69,27 @@ def cache_of(kind, pages, heads, page, dim, seed=0, filled=True):
     if kind == "e2m1":
         return Cache4(pages, heads, page, dim, seed, filled)
     return do.Cache(kind, pages, heads, page, dim, seed, filled)
+
+
+# ---- rotary positions ---------------------------------------------------------
+
+def turned(x, pos, freqs, scale, rot, interleaved):
+    """x [n][heads][dim] turned, in 64 bits, and per element what its tolerance is made of: |a| + |b| of its
+    pair, times the scale (0 where it stays)."""
+    x = np.asarray(x, np.float64)
+    t = np.asarray(pos, np.float64)[:, None, None] * np.asarray(freqs, np.float64)
+    c, s = np.cos(t) * np.float32(scale), np.sin(t) * np.float32(scale)
+    i = np.arange(rot // 2)
+    ia, ib = (2 * i, 2 * i + 1) if interleaved else (i, i + rot // 2)
+    a, b = x[..., ia], x[..., ib]
+    y, size = x.copy(), np.zeros(x.shape)
+    y[..., ia], y[..., ib] = a * c - b * s, b * c + a * s
+    size[..., ia] = size[..., ib] = (np.abs(a) + np.abs(b)) * abs(np.float64(np.float32(scale)))
+    return y, size
+
+
+def turned_bound(want, size, rows, far=1.0):
+    """What the roundings add up to at most: cos and sin within 3 units in the last place of 1 or below (2^-24 each:
+    the function's 2 and the first-order step's), the scale's product, an element's product and the sum: 6 of
+    2^-24 of |a| + |b| times the scale; an angle of up to `far` radians is off by 2^-53 of it; the output's rounding."""
+    return size * (6 * 2.0 ** -24 + far * 2.0 ** -53) + do.HALF[rows] * np.abs(want) * 1.01 + 2.0 ** -24 * (rows == "f16")
