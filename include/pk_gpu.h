@@ -514,6 +514,52 @@ int pk_gpu_paged_attention_dev(const pk_gpu_kv_cache *cache, int dtype, const vo
                                int max_len, float scale, int window, void *dout, int ldo,
                                float *dlse, float *dws, size_t ws_floats, void *stream);
 
+/* What pk_gpu_prompt_attention_dev does to scores, and what a new token sees.  All zero
+ * but the scale: softmax of scale * q . k_t over the tokens up to the new one itself.
+ *   scale   any finite number
+ *   cap     > 0: a score s becomes cap * tanh(s / cap); 0: stays
+ *   slopes  NULL, or [query heads]: slopes[h] * |p - t| is taken off the score of the query
+ *           at position p and the key at position t, behind the cap
+ *   window  > 0: tokens up to p - window are not seen; 0: no such limit
+ *   first   NULL, or [rows]: tokens before first[i] are not seen by row i: where the
+ *           documents packed into a sequence begin
+ *   until   NULL, or [rows]: row i sees tokens up to until[i] - 1 also where they follow
+ *           it: a prefix whose tokens see each other.  window and first limit those too
+ * A row that sees nothing gives zeros. */
+typedef struct {
+    float        scale, cap;
+    const float *slopes;
+    int          window;
+    const int   *first, *until;
+} pk_gpu_attention_rules;
+
+/* Attention of several new tokens per sequence over the cache: prompts, chunks of
+ * prompts, drafts to be checked, or single tokens that need the rules.  Sequence b's new
+ * tokens are its last ones (write them first): rows dstarts[b] .. dstarts[b + 1] - 1 of q
+ * and out, in order, at positions dlens[b] - n + i for the n of them.
+ *   dstarts  [B + 1], rising; or NULL: one each, row b is sequence b's.  Rows of no sequence
+ *            are left as they were
+ *   rows     of q and out; what dstarts names outside of [0, rows) is not there
+ *   max_new  no sequence has more new tokens (of more, only the first max_new are taken for its
+ *            last tokens, and the other rows left as they were); at most 2^30.  Work is laid
+ *            out by it, so a close bound is the fast one
+ * The cache, dlens, max_len, the page table, dtype and lse ([rows][heads]) as in
+ * pk_gpu_paged_attention_dev, whose notes on absent pages, on what tokens that take no part may
+ * hold (of a token that some rows see and others do not: for those others too) and on
+ * |q| hold here too.
+ * Scores, sums and the softmax are fp32; its weights enter the second product with 16 or
+ * 24 bits or more as there, where up to 16 (new token, query head) pairs share a key-value
+ * head.  Results do not depend on timing.
+ * dws as there, of at least pk_gpu_prompt_attention_ws_floats floats: what is enough for
+ * B, rows, max_new, max_len and window is enough for less of each. */
+size_t pk_gpu_prompt_attention_ws_floats(const pk_gpu_kv_cache *cache, int B, int rows, int heads,
+                                         int max_new, int max_len, int window);
+int pk_gpu_prompt_attention_dev(const pk_gpu_kv_cache *cache, int dtype, const void *dq, int ldq,
+                                int heads, const int *dpages, int ld_pages, const int *dlens,
+                                const int *dstarts, int B, int rows, int max_new, int max_len,
+                                const pk_gpu_attention_rules *rules, void *dout, int ldo,
+                                float *dlse, float *dws, size_t ws_floats, void *stream);
+
 /* Rotary positions.  The first rot_dim elements of a head (even, 2 at least) turn in pairs,
  * pair i of a row at position p by p * freqs[i] radians:
  *   a' = (a cos - b sin) * scale,   b' = (b cos + a sin) * scale

@@ -64,9 +64,16 @@
 // A tile's keys and values stay in registers and are loaded one tile ahead: the
 // next keys once this tile's scores are formed, the next values once they
 // are added.  Bound by the cache's bytes.
+//
+// With RULES (pk_prompt_attention.hip's calls of few rows) a workgroup's 16 columns are
+// pairs of a new token and a head of the group, token by token, each with a range of
+// tokens [lo, hi) of its own, and scores are capped and biased before the softmax.  A
+// token that some columns see and others do not can carry an infinity into all of
+// them (0 times it), so here a workgroup whose sums have passed 2^100 or become NaN
+// takes its columns again one by one (pk_careful_attention.h).
 #pragma once
 
-#include "pk_decode.h"
+#include "pk_careful_attention.h"
 
 #include <cfloat>
 #include <type_traits>
@@ -85,14 +92,15 @@ struct PagedArgs {
     char* out;
     size_t ldo;                  // bytes
     float* lse;
-    float* part;                 // [B][heads][splits][dim], then
-    float* ml;                   // [B][heads][splits][2]
+    float* part;                 // [B][max_new][heads][splits][dim], then
+    float* ml;                   // [B][max_new][heads][splits][2]  (one new token: max_new = 1)
     float scale2;                // scale * log2(e)
     int B, max_len, window;
     int kv_heads, group, head_tiles;
     int n_pages, page_shift;
     int chunk, splits;
     int longest_first;
+    RuleArgs rules;              // of the calls that have them
 };
 
 // Tokens a sequence's new token sees, from `first` on; chunks start at `base`.
@@ -233,7 +241,7 @@ __device__ inline void split_pair(float x, float y, uint32_t* t)
     }
 }
 
-template <int CACHE, int T, int DIM>
+template <int CACHE, int T, int DIM, bool RULES>
 __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, T, DIM) / 4) paged_attention(PagedArgs a)
 {
     constexpr int NW = waves_of(CACHE, T, DIM);
@@ -283,13 +291,29 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const long long tt = (long long)split * a.chunk + 32 * (wave + i * NW) + 16 * u;
-            early[i][u] = a.window == 0 && tt < a.max_len ? pages[tt >> a.page_shift] : -1;
+            early[i][u] = !RULES && a.window == 0 && tt < a.max_len ? pages[tt >> a.page_shift] : -1;
         }
 
-    const int in_group = htile * 16 + n;
-    const bool head_ok = in_group < a.group;
     const int heads = a.kv_heads * a.group;
+    int in_group = htile * 16 + n, token = b;
+    bool head_ok = in_group < a.group;
+    RowRange see{};
+    size_t row = 0;                            // of the workspace and lse
+    if constexpr (RULES) {
+        const NewTokens news = new_tokens(a.rules, b);
+        if (htile * 16 >= news.count * a.group) return;
+        const int i = (uint32_t)in_group / (uint32_t)a.group;
+        in_group -= i * a.group;
+        head_ok = i < news.count;
+        token = news.row + (head_ok ? i : 0);
+        see = range_of(a.rules, len < 0 ? 0 : min(len, a.max_len), news.count, head_ok ? i : 0, token, a.window);
+        row = (size_t)b * a.rules.max_new + i;
+    } else {
+        row = b;
+    }
     const int head = kvh * a.group + in_group;
+    row = row * heads + head;
+    const float slope2 = RULES && a.rules.slopes && head_ok ? a.rules.slopes[head] * 1.4426950408889634f : 0.0f;
 
     // queries: step c takes elements el(c, i) = i + 8 g + 32 c of a 16-bit cache's
     // rows, i + 16 g + 8 (c % 2) + 64 (c / 2) of an 8-bit one's, i + 32 g + 8 (c % 4)
@@ -303,11 +327,32 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
         const int el = FOUR ? (DIM == 64 ? 16 * g + 8 * c : 128 * (c / 4) + 32 * g + 8 * (c % 4))
                        : S == 2 ? 32 * c + 8 * g : 64 * (c / 2) + 16 * g + 8 * (c % 2);
         if (c < STEPS && head_ok)
-            load8<T>(a.q + (size_t)b * a.ldq + ((size_t)head * DIM + el) * size_of(T), qv[i]);
+            load8<T>(a.q + (size_t)token * a.ldq + ((size_t)head * DIM + el) * size_of(T), qv[i]);
     }
 
-    const Span sp = span_of(len, a.max_len, a.window, a.chunk);
-    if (split > 0 && split >= sp.chunks) return;
+    Span sp;
+    int max_lo = 0, min_hi = 0;                // of the columns: between them all see a token
+    if constexpr (RULES) {
+        const bool any = head_ok && see.lo < see.hi;
+        sp.first = (int)(0x7fffffffu - max_over<16>(any ? 0x7fffffffu - (uint32_t)see.lo : 0u));
+        sp.len = (int)max_over<16>(any ? (uint32_t)see.hi : 0u);
+        max_lo = __builtin_amdgcn_readfirstlane((int)max_over<16>(head_ok ? (uint32_t)see.lo : 0u));
+        min_hi = __builtin_amdgcn_readfirstlane((int)(0x7fffffffu - max_over<16>(head_ok ? 0x7fffffffu - (uint32_t)see.hi : 0u)));
+        sp.first = __builtin_amdgcn_readfirstlane(sp.first);
+        sp.len = __builtin_amdgcn_readfirstlane(sp.len);
+        if (!sp.len) sp.first = 0;
+        sp.base = sp.first & ~31;
+        sp.chunks = sp.len ? (sp.len - sp.base + a.chunk - 1) / a.chunk : 0;
+    } else {
+        sp = span_of(len, a.max_len, a.window, a.chunk);
+    }
+    if (split > 0 && split >= sp.chunks) {
+        if (RULES && wave == 0 && g == 0 && head_ok) {          // the join looks at every chunk
+            a.ml[(row * a.splits + split) * 2] = -FLT_MAX;
+            a.ml[(row * a.splits + split) * 2 + 1] = 0.0f;
+        }
+        return;
+    }
     const int begin = sp.base + split * a.chunk;
     const int end = sp.chunks ? min(sp.len, begin + a.chunk) : begin;
 
@@ -397,7 +442,7 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
     int t = begin + 32 * wave;
     Halves cur{}, next{};
     if (t < end) {
-        if (a.window == 0) {
+        if (!RULES && a.window == 0) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 half(cur, u, t + 16 * u, early[0][u]);
@@ -462,11 +507,17 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                s[u][r] = __fmul_rn(s[u][r], CODED ? __fmul_rn(ks[u][r], a.scale2) : a.scale2);
+            for (int r = 0; r < 4; ++r) {
+                if constexpr (RULES)
+                    s[u][r] = ruled_score<T>(a.rules, CODED ? __fmul_rn(s[u][r], ks[u][r]) : s[u][r], a.scale2, slope2,
+                                             see.p - (t + 16 * u + 4 * g + r));
+                else
+                    s[u][r] = __fmul_rn(s[u][r], CODED ? __fmul_rn(ks[u][r], a.scale2) : a.scale2);
+            }
         if constexpr (MORE) load_k(next);
 
-        const bool whole = t >= sp.first && t + 32 <= end && cur.ok[0] && cur.ok[1];
+        const bool whole = t >= sp.first && t + 32 <= end && cur.ok[0] && cur.ok[1] &&
+                           (!RULES || (t >= max_lo && t + 32 <= min_hi));
         if (!whole) {
             // masked tokens: no score, and no value either (0 * NaN is NaN)
 #pragma unroll
@@ -475,8 +526,8 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
                 for (int r = 0; r < 4; ++r) {
                     const int tok = t + 16 * u + 4 * g + r;
                     const bool in = cur.ok[u] && tok >= sp.first && tok < end;
+                    if (!in || (RULES && (tok < see.lo || tok >= see.hi))) s[u][r] = -__builtin_inff();
                     if (!in) {
-                        s[u][r] = -__builtin_inff();
                         if constexpr (CODED) vs[u][r] = 0.0f;
                         if constexpr (FOUR) vu[u][r] = 0;
 #pragma unroll
@@ -576,6 +627,7 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
         next = after;
         t += 32 * NW;
     };
+    bool careful = false;
     if (t < end) {
         while (t + 32 * NW < end) tile(std::false_type{}, std::false_type{});
         tile(std::true_type{}, std::false_type{});
@@ -585,7 +637,9 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
 #pragma unroll
             for (int r = 0; r < 4; ++r) size[r] = __fadd_rn(size[r], fabsf(acc[e][r]));
         const float sum = __fadd_rn(__fadd_rn(size[0], size[1]), __fadd_rn(size[2], size[3]));
-        if (__any(!(sum < 0x1p100f))) {
+        if constexpr (RULES) {
+            careful = __any(!(sum < 0x1p100f));
+        } else if (__any(!(sum < 0x1p100f))) {
             m = -FLT_MAX;
             l = 0.0f;
 #pragma unroll
@@ -604,8 +658,32 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
     l = __fadd_rn(l, __shfl_xor(l, 16));
     l = __fadd_rn(l, __shfl_xor(l, 32));
     __shared__ float ml[NW][2][16];
+    __shared__ bool again[RULES ? NW : 1];
     if (g == 0) { ml[wave][0][n] = m; ml[wave][1][n] = l; }
+    if (RULES && lane == 0) again[wave] = careful;
     __syncthreads();                           // and nobody reads queries any more
+    if constexpr (RULES) {
+        bool any = false;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) any |= again[w];
+        if (any) {
+            const CacheView view{a.k, a.v, a.k_scale, a.v_scale, pages, a.n_pages, a.page_shift, a.kv_heads, kvh};
+#pragma unroll 1
+            for (int c = wave; c < 16; c += NW) {
+                if (!__builtin_amdgcn_readlane((int)head_ok, c)) break;      // columns behind the last
+                const int h = __builtin_amdgcn_readlane(head, c), q = __builtin_amdgcn_readlane(token, c);
+                const RowRange s{max(__builtin_amdgcn_readlane(see.lo, c), begin), min(__builtin_amdgcn_readlane(see.hi, c), end),
+                                 __builtin_amdgcn_readlane(see.p, c)};
+                const float slope = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(slope2), c));
+                const size_t at = ((size_t)b * a.rules.max_new + (q - new_tokens(a.rules, b).row)) * heads + h;
+                careful_row<CACHE, T, DIM>(view, a.rules, a.q + (size_t)q * a.ldq + (size_t)h * DIM * size_of(T), s, a.scale2,
+                                           slope, a.splits == 1 ? a.out + (size_t)q * a.ldo + (size_t)h * DIM * size_of(T) : nullptr,
+                                           a.lse ? a.lse + (size_t)q * heads + h : nullptr,
+                                           a.part + (at * a.splits + split) * DIM, a.ml + (at * a.splits + split) * 2);
+            }
+            return;
+        }
+    }
     float mx = ml[0][0][n];
 #pragma unroll
     for (int w = 1; w < NW; ++w) mx = fmaxf(mx, ml[w][0][n]);
@@ -634,10 +712,9 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
 
     // element e of row 4 g + r stands for el = (4 g + r) E + e of the head (or,
     // where a lane holds 32 bytes, 128 (e / 8) + 8 (4 g + r) + e % 8)
-    const bool direct = sp.chunks <= 1;
+    const bool direct = RULES ? a.splits == 1 : sp.chunks <= 1;
     const float inv = lt == 0.0f ? 0.0f : __fdiv_rn(1.0f, lt);
     constexpr int RUN = VB > 16 ? 8 : E;       // consecutive elements
-    const size_t row = (size_t)b * heads + head;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
 #pragma unroll
@@ -649,7 +726,7 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
             if (direct) {
 #pragma unroll
                 for (int i = 0; i < RUN; ++i) o[i] = lt == 0.0f ? 0.0f : __fmul_rn(o[i], inv);
-                char* p = a.out + (size_t)b * a.ldo + ((size_t)head * DIM + el) * size_of(T);
+                char* p = a.out + (size_t)token * a.ldo + ((size_t)head * DIM + el) * size_of(T);
                 if constexpr (RUN >= 8) {
 #pragma unroll
                     for (int i = 0; i < RUN; i += 8) store8<T>(p + i * size_of(T), o + i);
@@ -669,7 +746,7 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
     }
     if (g == 0) {
         if (direct) {
-            if (a.lse) a.lse[row] = lt == 0.0f ? -__builtin_inff()
+            if (a.lse) a.lse[(size_t)token * heads + head] = lt == 0.0f ? -__builtin_inff()
                                                : __fmul_rn(__fadd_rn(mx - BIAS, __builtin_amdgcn_logf(lt)),
                                                            0.69314718055994531f);
         } else {
@@ -679,19 +756,37 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
     }
 }
 
-hipError_t launch_paged_f16(int t, int dim, const PagedArgs& a, dim3 grid, hipStream_t s);
-hipError_t launch_paged_bf16(int t, int dim, const PagedArgs& a, dim3 grid, hipStream_t s);
-hipError_t launch_paged_i8(int t, int dim, const PagedArgs& a, dim3 grid, hipStream_t s);
-hipError_t launch_paged_e4m3(int t, int dim, const PagedArgs& a, dim3 grid, hipStream_t s);
-hipError_t launch_paged_e2m1(int t, int dim, const PagedArgs& a, dim3 grid, hipStream_t s);
+// `rules`: the kernels that take a.rules
+hipError_t launch_paged_f16(int t, int dim, bool rules, const PagedArgs& a, dim3 grid, hipStream_t s);
+hipError_t launch_paged_bf16(int t, int dim, bool rules, const PagedArgs& a, dim3 grid, hipStream_t s);
+hipError_t launch_paged_i8(int t, int dim, bool rules, const PagedArgs& a, dim3 grid, hipStream_t s);
+hipError_t launch_paged_e4m3(int t, int dim, bool rules, const PagedArgs& a, dim3 grid, hipStream_t s);
+hipError_t launch_paged_e2m1(int t, int dim, bool rules, const PagedArgs& a, dim3 grid, hipStream_t s);
 
-template <int CACHE, int T>
-hipError_t launch_paged(int dim, const PagedArgs& a, dim3 grid, hipStream_t s)
+// Both launches of a call: the attention over `grid` workgroups, and the join of `rows`
+// (token, head) rows where sequences are split.
+hipError_t launch_attention(int cache, int t, int dim, bool rules, const PagedArgs& a, uint32_t grid, uint32_t rows, hipStream_t s);
+hipError_t launch_joins(int t, int dim, bool rules, const PagedArgs& a, uint32_t rows, hipStream_t s);
+
+constexpr int kMaxSplits = 256;     // the join's threads: one a chunk
+// Chunks that a span of tokens is cut into for so many workgroups of one chunk each, and
+// the tokens of a chunk.
+long long cuts(int cache, int dim, long long pairs, long long span);
+struct Plan { int chunk, splits; };
+Plan plan_of(int cache, int dim, long long pairs, long long span);
+
+template <int CACHE, int T, bool RULES>
+hipError_t launch_paged_as(int dim, const PagedArgs& a, dim3 grid, hipStream_t s)
 {
     const dim3 block(64 * waves_of(CACHE, T, dim));
-    return dim == 64    ? launch(paged_attention<CACHE, T, 64>, grid, block, 0, s, a)
-           : dim == 128 ? launch(paged_attention<CACHE, T, 128>, grid, block, 0, s, a)
-                        : launch(paged_attention<CACHE, T, 256>, grid, block, 0, s, a);
+    return dim == 64    ? launch(paged_attention<CACHE, T, 64, RULES>, grid, block, 0, s, a)
+           : dim == 128 ? launch(paged_attention<CACHE, T, 128, RULES>, grid, block, 0, s, a)
+                        : launch(paged_attention<CACHE, T, 256, RULES>, grid, block, 0, s, a);
+}
+template <int CACHE, int T>
+hipError_t launch_paged(int dim, bool rules, const PagedArgs& a, dim3 grid, hipStream_t s)
+{
+    return rules ? launch_paged_as<CACHE, T, true>(dim, a, grid, s) : launch_paged_as<CACHE, T, false>(dim, a, grid, s);
 }
 
 }  // namespace decode

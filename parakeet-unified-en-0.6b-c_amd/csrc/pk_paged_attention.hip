@@ -6,8 +6,6 @@ namespace pkgpu {
 namespace decode {
 namespace {
 
-constexpr int kMaxSplits = 256;     // the join's threads: one a chunk
-
 struct JoinArgs {
     const float *part, *ml;
     const int* lens;
@@ -15,25 +13,35 @@ struct JoinArgs {
     size_t ldo;
     float* lse;
     int heads, splits, chunk, max_len, window;
+    RuleArgs rules;
 };
 
 // One workgroup joins the chunks of one head: out = sum_c 2^(m_c - m) o_c /
 // sum_c 2^(m_c - m) l_c.  DIM / 4 lanes cover the head, the other lanes take
 // every PARTS-th chunk; sums run in a fixed order.  All that it reads first,
 // the length, the chunks' (m, l) and EARLY chunks' outputs of a thread, is asked
-// for at once: the workspace holds them whether the sequence has them or not.
-template <int T, int DIM>
+// for at once: the workspace holds them whether the sequence has them or not.  With
+// RULES a row is a (sequence, new token, head), and a chunk that it sees nothing of has
+// said so by l = 0; what the workspace holds of that one's outputs is anything.
+template <int T, int DIM, bool RULES>
 __global__ void __launch_bounds__(256) paged_join(JoinArgs a)
 {
     constexpr int LANES = DIM / 4, PARTS = 256 / LANES, EARLY = 4;
     __shared__ float red[2][4];
     __shared__ float wgt[kMaxSplits];
     __shared__ f32x4 sum[PARTS][LANES];
-    const int b = blockIdx.x / (uint32_t)a.heads, head = blockIdx.x % (uint32_t)a.heads;
+    int b = blockIdx.x / (uint32_t)a.heads;
+    const int head = blockIdx.x % (uint32_t)a.heads;
     const size_t row = (size_t)b * a.heads + head;
+    if constexpr (RULES) {
+        const uint32_t seq = (uint32_t)b / (uint32_t)a.rules.max_new, i = b - seq * a.rules.max_new;
+        const NewTokens news = new_tokens(a.rules, seq);
+        if ((int)i >= news.count) return;
+        b = news.row + i;
+    }
     const int i = threadIdx.x, lane = i & 63, wave = i >> 6;
     const int part = i / LANES, d4 = i % LANES;
-    const int len = a.lens[b];
+    const int len = RULES ? 0 : a.lens[b];
     const float* ml = a.ml + row * a.splits * 2;
     float m = -FLT_MAX, l = 0.0f;
     if (i < a.splits) { m = ml[2 * i]; l = ml[2 * i + 1]; }
@@ -42,7 +50,7 @@ __global__ void __launch_bounds__(256) paged_join(JoinArgs a)
 #pragma unroll
     for (int e = 0; e < EARLY; ++e)
         if (part + e * PARTS < a.splits) v[e] = *reinterpret_cast<const f32x4*>(src + (size_t)(part + e * PARTS) * DIM);
-    const int chunks = span_of(len, a.max_len, a.window, a.chunk).chunks;
+    const int chunks = RULES ? a.splits : span_of(len, a.max_len, a.window, a.chunk).chunks;
     if (chunks <= 1) return;                        // written by the first launch
     if (i >= chunks) { m = -FLT_MAX; l = 0.0f; }
     float mx = m;
@@ -51,7 +59,7 @@ __global__ void __launch_bounds__(256) paged_join(JoinArgs a)
     if (lane == 0) red[0][wave] = mx;
     __syncthreads();
     mx = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    const float w = i < chunks ? __builtin_amdgcn_exp2f(m - mx) : 0.0f;
+    const float w = i < chunks && (!RULES || l != 0.0f) ? __builtin_amdgcn_exp2f(m - mx) : 0.0f;
     wgt[i] = w;
     float lt = __fmul_rn(l, w);
 #pragma unroll
@@ -63,12 +71,13 @@ __global__ void __launch_bounds__(256) paged_join(JoinArgs a)
 #pragma unroll
     for (int e = 0; e < EARLY; ++e) {
         const int c = part + e * PARTS;
-        if (c < chunks)
+        if (c < chunks && (!RULES || wgt[c] != 0.0f))
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[r] = __fmaf_rn(v[e][r], wgt[c], o[r]);
     }
 #pragma unroll 4
     for (int c = part + EARLY * PARTS; c < chunks; c += PARTS) {
+        if (RULES && wgt[c] == 0.0f) continue;
         const f32x4 x = *reinterpret_cast<const f32x4*>(src + (size_t)c * DIM);
 #pragma unroll
         for (int r = 0; r < 4; ++r) o[r] = __fmaf_rn(x[r], wgt[c], o[r]);
@@ -89,22 +98,27 @@ __global__ void __launch_bounds__(256) paged_join(JoinArgs a)
         *reinterpret_cast<u32x2*>(p) = T == F16 ? (u32x2){pack_f16(o[0], o[1]), pack_f16(o[2], o[3])}
                                                 : (u32x2){pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3])};
     if (d4 == 0 && a.lse)
-        a.lse[row] = lt == 0.0f ? -__builtin_inff()
+        a.lse[(size_t)b * a.heads + head] = lt == 0.0f ? -__builtin_inff()
                                 : __fmul_rn(__fadd_rn(mx, __builtin_amdgcn_logf(lt)), 0.69314718055994531f);
 }
 
-template <int T>
+template <int T, bool RULES>
 hipError_t launch_join(int dim, const JoinArgs& a, uint32_t rows, hipStream_t s)
 {
-    return dim == 64    ? launch(paged_join<T, 64>, dim3(rows), dim3(256), 0, s, a)
-           : dim == 128 ? launch(paged_join<T, 128>, dim3(rows), dim3(256), 0, s, a)
-                        : launch(paged_join<T, 256>, dim3(rows), dim3(256), 0, s, a);
+    return dim == 64    ? launch(paged_join<T, 64, RULES>, dim3(rows), dim3(256), 0, s, a)
+           : dim == 128 ? launch(paged_join<T, 128, RULES>, dim3(rows), dim3(256), 0, s, a)
+                        : launch(paged_join<T, 256, RULES>, dim3(rows), dim3(256), 0, s, a);
+}
+template <bool RULES>
+hipError_t launch_join_of(int t, int dim, const JoinArgs& a, uint32_t rows, hipStream_t s)
+{
+    return t == F32   ? launch_join<F32, RULES>(dim, a, rows, s)
+           : t == F16 ? launch_join<F16, RULES>(dim, a, rows, s)
+                      : launch_join<BF16, RULES>(dim, a, rows, s);
 }
 
 // 16 query heads of a key-value head a workgroup.
 int head_tiles(int group) { return (group + 15) / 16; }
-
-struct Plan { int chunk, splits; };
 
 // Tokens that the longest sequence's chunks cover: a window's begin up to 31 before it.
 long long span_at_most(int max_len, int window)
@@ -114,30 +128,6 @@ long long span_at_most(int max_len, int window)
     return span < 1 ? 1 : span;
 }
 
-constexpr int kRound = 256;         // 8 waves' tiles
-
-// Chunks that a sequence is cut into, before they are made whole rounds.  Up to 3
-// rounds one workgroup takes the whole: a round costs about 2 us, the second
-// launch that joins chunks 4 to 5 us.  Longer ones are cut until there is a
-// workgroup for each of the 256 CUs, and up to two where chunks keep 384 KB of
-// cache.  Measured (us; one chunk, 256, 512 workgroups):
-//   1 sequence of 100003 tokens, 8 heads of 128 in bf16     1059, 76, 78
-//   4 ragged ones up to 30000, 2 heads of 256 in bf16        615, 36, 29
-//   8 ragged ones up to 4000, 8 heads of 128 in int8           34, 16, 19.5
-//   32 ragged ones up to 2000, the same (256 unsplit)           22, 22, 27
-//   160 windows of 1024 over a head of 256 (160 unsplit)       21, 21, 30
-long long cuts(const pk_gpu_kv_cache* c, long long pairs, long long span)
-{
-    const long long rounds = (span + kRound - 1) / kRound;
-    if (rounds <= 3) return 1;
-    const long long fill = 256 / pairs, two = 512 / pairs, large = span * 2 * bytes_of(c->dtype, c->head_dim) / (384 << 10);
-    long long n = two < large ? two : large;
-    if (n < fill) n = fill;
-    if (n > rounds) n = rounds;
-    if (n > kMaxSplits) n = kMaxSplits;
-    return n < 1 ? 1 : n;
-}
-
 long long pairs_of(const pk_gpu_kv_cache* c, int B, int heads)
 {
     return (long long)B * c->heads * head_tiles(heads / c->heads);
@@ -145,10 +135,7 @@ long long pairs_of(const pk_gpu_kv_cache* c, int B, int heads)
 
 Plan plan(const pk_gpu_kv_cache* c, int B, int heads, int max_len, int window)
 {
-    const long long span = span_at_most(max_len, window), rounds = (span + kRound - 1) / kRound;
-    const long long n = cuts(c, pairs_of(c, B > 0 ? B : 1, heads), span);
-    const long long chunk = (rounds + n - 1) / n * kRound;
-    return {(int)chunk, (int)((span + chunk - 1) / chunk)};
+    return plan_of(c->dtype, c->head_dim, pairs_of(c, B > 0 ? B : 1, heads), span_at_most(max_len, window));
 }
 
 int check_attention(const pk_gpu_kv_cache* c, int B, int heads, int max_len, int window)
@@ -182,13 +169,75 @@ size_t ws_floats_up_to(const pk_gpu_kv_cache* c, int B, int heads, int max_len, 
     const long long span = span_at_most(max_len, window);
     size_t most = 0;
     for (int b = 1; b <= B && pairs_of(c, b, heads) <= 256; ++b) {
-        const size_t n = cuts(c, pairs_of(c, b, heads), span);
+        const size_t n = cuts(c->dtype, c->head_dim, pairs_of(c, b, heads), span);
         if (n > 1 && b * n > most) most = b * n;
     }
     return most * heads * (c->head_dim + 2);
 }
 
 }  // namespace
+
+constexpr int kRound = 256;         // 8 waves' tiles
+
+// Chunks that a sequence is cut into, before they are made whole rounds.  Up to 3
+// rounds one workgroup takes the whole: a round costs about 2 us, the second
+// launch that joins chunks 4 to 5 us.  Longer ones are cut until there is a
+// workgroup for each of the 256 CUs, and up to two where chunks keep 384 KB of
+// cache.  Measured (us; one chunk, 256, 512 workgroups):
+//   1 sequence of 100003 tokens, 8 heads of 128 in bf16     1059, 76, 78
+//   4 ragged ones up to 30000, 2 heads of 256 in bf16        615, 36, 29
+//   8 ragged ones up to 4000, 8 heads of 128 in int8           34, 16, 19.5
+//   32 ragged ones up to 2000, the same (256 unsplit)           22, 22, 27
+//   160 windows of 1024 over a head of 256 (160 unsplit)       21, 21, 30
+long long cuts(int cache, int dim, long long pairs, long long span)
+{
+    const long long rounds = (span + kRound - 1) / kRound;
+    if (rounds <= 3) return 1;
+    const long long fill = 256 / pairs, two = 512 / pairs, large = span * 2 * bytes_of(cache, dim) / (384 << 10);
+    long long n = two < large ? two : large;
+    if (n < fill) n = fill;
+    if (n > rounds) n = rounds;
+    if (n > kMaxSplits) n = kMaxSplits;
+    return n < 1 ? 1 : n;
+}
+
+Plan plan_of(int cache, int dim, long long pairs, long long span)
+{
+    const long long rounds = (span + kRound - 1) / kRound, n = cuts(cache, dim, pairs, span);
+    const long long chunk = (rounds + n - 1) / n * kRound;
+    return {(int)chunk, (int)((span + chunk - 1) / chunk)};
+}
+
+hipError_t launch_joins(int t, int dim, bool rules, const PagedArgs& a, uint32_t rows, hipStream_t s)
+{
+    JoinArgs j{};
+    j.part = a.part;
+    j.ml = a.ml;
+    j.lens = a.lens;
+    j.out = a.out;
+    j.ldo = a.ldo;
+    j.lse = a.lse;
+    j.heads = a.kv_heads * a.group;
+    j.splits = a.splits;
+    j.chunk = a.chunk;
+    j.max_len = a.max_len;
+    j.window = a.window;
+    j.rules = a.rules;
+    return rules ? launch_join_of<true>(t, dim, j, rows, s) : launch_join_of<false>(t, dim, j, rows, s);
+}
+
+hipError_t launch_attention(int cache, int t, int dim, bool rules, const PagedArgs& a, uint32_t workgroups, uint32_t rows,
+                            hipStream_t s)
+{
+    const dim3 grid(workgroups);
+    const hipError_t e = cache == F16    ? launch_paged_f16(t, dim, rules, a, grid, s)
+                         : cache == BF16 ? launch_paged_bf16(t, dim, rules, a, grid, s)
+                         : cache == I8   ? launch_paged_i8(t, dim, rules, a, grid, s)
+                         : cache == E2M1 ? launch_paged_e2m1(t, dim, rules, a, grid, s)
+                                         : launch_paged_e4m3(t, dim, rules, a, grid, s);
+    return e == hipSuccess && a.splits > 1 ? launch_joins(t, dim, rules, a, rows, s) : e;
+}
+
 }  // namespace decode
 }  // namespace pkgpu
 
@@ -270,32 +319,8 @@ int pk_gpu_paged_attention_dev(const pk_gpu_kv_cache* cache, int dtype, const vo
     // short sequences the counting costs more (256 of up to 1000: 87 against 67).
     a.longest_first = B > 1 && B <= kSortedMax && pairs * p.splits > 512 && max_len / 16 >= B &&
                       (window == 0 || window / 16 >= B);
-    const dim3 grid((uint32_t)(pairs * p.splits));
-    hipStream_t s = static_cast<hipStream_t>(stream);
-    const int dim = cache->head_dim;
-    hipError_t e = cache->dtype == F16    ? launch_paged_f16(dtype, dim, a, grid, s)
-                   : cache->dtype == BF16 ? launch_paged_bf16(dtype, dim, a, grid, s)
-                   : cache->dtype == I8   ? launch_paged_i8(dtype, dim, a, grid, s)
-                   : cache->dtype == E2M1 ? launch_paged_e2m1(dtype, dim, a, grid, s)
-                                          : launch_paged_e4m3(dtype, dim, a, grid, s);
-    if (e == hipSuccess && p.splits > 1) {
-        JoinArgs j{};
-        j.part = a.part;
-        j.ml = a.ml;
-        j.lens = dlens;
-        j.out = a.out;
-        j.ldo = a.ldo;
-        j.lse = dlse;
-        j.heads = heads;
-        j.splits = p.splits;
-        j.chunk = p.chunk;
-        j.max_len = max_len;
-        j.window = window;
-        const uint32_t rows = (uint32_t)((long long)B * heads);
-        e = dtype == F32   ? launch_join<F32>(dim, j, rows, s)
-            : dtype == F16 ? launch_join<F16>(dim, j, rows, s)
-                           : launch_join<BF16>(dim, j, rows, s);
-    }
+    const hipError_t e = launch_attention(cache->dtype, dtype, cache->head_dim, false, a, (uint32_t)(pairs * p.splits),
+                                          (uint32_t)((long long)B * heads), static_cast<hipStream_t>(stream));
     return e == hipSuccess ? PK_GPU_OK : rt::hip_error(e, who);
 }
 

@@ -4,10 +4,10 @@
 namespace pkgpu {
 namespace decode {
 
-hipError_t launch_paged_bf16(int t, int dim, const PagedArgs& a, dim3 grid, hipStream_t s)
+hipError_t launch_paged_bf16(int t, int dim, bool rules, const PagedArgs& a, dim3 grid, hipStream_t s)
 {
-    return t == BF16 ? launch_paged<BF16, BF16>(dim, a, grid, s)
-         : t == F32 ? launch_paged<BF16, F32>(dim, a, grid, s) : hipErrorInvalidValue;
+    return t == BF16 ? launch_paged<BF16, BF16>(dim, rules, a, grid, s)
+         : t == F32 ? launch_paged<BF16, F32>(dim, rules, a, grid, s) : hipErrorInvalidValue;
 }
 
 }  // namespace decode

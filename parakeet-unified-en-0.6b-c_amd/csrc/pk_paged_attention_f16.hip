@@ -4,9 +4,9 @@
 namespace pkgpu {
 namespace decode {
 
-hipError_t launch_paged_f16(int t, int dim, const PagedArgs& a, dim3 grid, hipStream_t s)
+hipError_t launch_paged_f16(int t, int dim, bool rules, const PagedArgs& a, dim3 grid, hipStream_t s)
 {
-    return t == F16 ? launch_paged<F16, F16>(dim, a, grid, s) : hipErrorInvalidValue;
+    return t == F16 ? launch_paged<F16, F16>(dim, rules, a, grid, s) : hipErrorInvalidValue;
 }
 
 }  // namespace decode

@@ -1,0 +1,167 @@
+// pk_prompt_attention.hip - host side of the attention of several new tokens per sequence
+// over a paged cache, with rules for scores and for what a token sees.
+#include "pk_paged_attention.h"
+
+#include <cmath>
+
+namespace pkgpu {
+namespace decode {
+namespace {
+
+constexpr const char* kWho = "prompt attention";
+
+// A call's sizes, as its workspace is made for.
+struct Sizes { int B, heads, max_new, max_len, window; };
+
+// 16 (new token, head) pairs of a key-value head a workgroup.
+long long tiles_of(long long rows) { return (rows + 15) / 16; }
+long long pairs_of(const pk_gpu_kv_cache* c, const Sizes& z, int B, long long tiles) { return (long long)B * c->heads * tiles; }
+
+// Tokens that a workgroup's columns see at most, from a multiple of 32 on.
+long long span_of_rows(const Sizes& z)
+{
+    const long long seen = z.window > 0 ? (long long)z.window + z.max_new + 30 : z.max_len;
+    const long long span = seen < z.max_len ? seen : z.max_len;
+    return span < 1 ? 1 : span;
+}
+
+int check_sizes(const pk_gpu_kv_cache* c, const Sizes& z)
+{
+    const int rc = check_cache(c, kWho);
+    if (rc) return rc;
+    if (z.B < 0 || z.max_new < 0 || z.max_len < 0 || z.window < 0)
+        return rt::error(PK_GPU_EINVAL, "%s: B = %d, max_new = %d, max_len = %d, window = %d", kWho, z.B, z.max_new,
+                         z.max_len, z.window);
+    if (z.max_len > 1 << 30 || z.max_new > 1 << 30)
+        return rt::error(PK_GPU_EINVAL, "%s: max_new = %d or max_len = %d is above 2^30", kWho, z.max_new, z.max_len);
+    if (z.heads < 1 || z.heads % c->heads)
+        return rt::error(PK_GPU_EINVAL, "%s: %d query heads over %d key-value heads", kWho, z.heads, c->heads);
+    return PK_GPU_OK;
+}
+
+// Floats that any call with these sizes at most takes; see ws_floats_up_to of the
+// one-token attention.  Above 256 pairs no sequence is split.
+size_t most_floats(const pk_gpu_kv_cache* c, const Sizes& z)
+{
+    const int group = z.heads / c->heads;
+    const long long span = span_of_rows(z);
+    size_t most = 0;
+    for (int b = 1; b <= z.B && pairs_of(c, z, b, 1) <= 256; ++b)
+        for (long long t = 1; pairs_of(c, z, b, t) <= 256; ++t) {
+            // the most new tokens of so many tiles
+            const long long n = 16 * t / group < z.max_new ? 16 * t / group : z.max_new;
+            if (n < 1) continue;
+            const size_t cut = cuts(c->dtype, c->head_dim, pairs_of(c, z, b, t), span);
+            if (cut > 1 && b * n * cut > most) most = b * n * cut;
+            if (n == z.max_new) break;
+        }
+    return most * z.heads * (c->head_dim + 2);
+}
+
+}  // namespace
+}  // namespace decode
+}  // namespace pkgpu
+
+extern "C" {
+
+using namespace pkgpu::decode;
+namespace rt = pkgpu::rt;
+
+size_t pk_gpu_prompt_attention_ws_floats(const pk_gpu_kv_cache* cache, int B, int rows, int heads, int max_new, int max_len,
+                                         int window)
+{
+    const Sizes z{B, heads, max_new < rows ? max_new : rows, max_len, window < max_len ? window : 0};
+    if (check_sizes(cache, z) != PK_GPU_OK) return 0;
+    return most_floats(cache, z);
+}
+
+int pk_gpu_prompt_attention_dev(const pk_gpu_kv_cache* cache, int dtype, const void* dq, int ldq, int heads,
+                                const int* dpages, int ld_pages, const int* dlens, const int* dstarts, int B, int rows,
+                                int max_new, int max_len, const pk_gpu_attention_rules* rules, void* dout, int ldo,
+                                float* dlse, float* dws, size_t ws_floats, void* stream)
+{
+    if (!rules) return rt::error(PK_GPU_EINVAL, "%s: NULL rules", kWho);
+    Sizes z{B, heads, max_new, max_len, rules->window};
+    int rc = check_sizes(cache, z);
+    if (rc) return rc;
+    if (rows < 0) return rt::error(PK_GPU_EINVAL, "%s: rows = %d", kWho, rows);
+    if (!is_float(dtype)) return rt::error(PK_GPU_EINVAL, "%s: queries of type %d (F32, F16 or BF16)", kWho, dtype);
+    if ((cache->dtype == F16 && dtype != F16) || (cache->dtype == BF16 && dtype == F16))
+        return rt::error(PK_GPU_ENOTSUP, "%s: queries of type %d over a cache of type %d (F16 caches take F16, "
+                         "BF16 caches BF16 or F32)", kWho, dtype, cache->dtype);
+    if (!std::isfinite(rules->scale) || !(rules->cap >= 0.0f) || !std::isfinite(rules->cap))
+        return rt::error(PK_GPU_EINVAL, "%s: scale = %g, cap = %g", kWho, rules->scale, rules->cap);
+    const long long wide = (long long)heads * cache->head_dim;
+    if (ldq < wide || ldo < wide)
+        return rt::error(PK_GPU_EINVAL, "%s: rows of %lld elements, ldq = %d, ldo = %d", kWho, wide, ldq, ldo);
+    if (ld_pages < 0 || ((long long)ld_pages << __builtin_ctz(cache->page_size)) < max_len)
+        return rt::error(PK_GPU_EINVAL, "%s: %d pages a sequence do not hold max_len = %d tokens", kWho, ld_pages, max_len);
+    const bool some = B && rows && max_new;
+    if (some && (!dq || !dout || !dlens || (max_len && !dpages)))
+        return rt::error(PK_GPU_EINVAL, "%s: NULL operand", kWho);
+    const size_t es = size_of(dtype);
+    if (!aligned16(dq) || !aligned16(dout) || (size_t)ldq * es % 16 || (size_t)ldo * es % 16)
+        return rt::error(PK_GPU_EINVAL, "%s: query and output rows must be 16-byte aligned", kWho);
+    if (!aligned(dpages, 4) || !aligned(dlens, 4) || !aligned(dlse, 4) || !aligned(dstarts, 4) || !aligned(rules->slopes, 4) ||
+        !aligned(rules->first, 4) || !aligned(rules->until, 4))
+        return rt::error(PK_GPU_EINVAL, "%s: pages, lengths, starts, lse or a rule's array are not aligned to their elements",
+                         kWho);
+    // no row has more, and a window that wide hides nothing
+    if (z.max_new > rows) z.max_new = rows;
+    if (!dstarts && z.max_new > 1) z.max_new = 1;
+    if (z.window >= max_len) z.window = 0;
+    const int group = heads / cache->heads;
+    const long long tiles = tiles_of((long long)z.max_new * group);
+    const long long pairs = pairs_of(cache, z, B, tiles);
+    const Plan p = plan_of(cache->dtype, cache->head_dim, pairs > 0 ? pairs : 1, span_of_rows(z));
+    const long long outs = (long long)B * z.max_new * heads;
+    if (!launchable(pairs * p.splits, 512) || outs > 0x7fffffff || (p.splits > 1 && !launchable(outs, 256)))
+        return rt::error(PK_GPU_EINVAL, "%s: %d sequences of %d new tokens and %d heads exceed the grid", kWho, B, z.max_new,
+                         heads);
+    const size_t need = p.splits <= 1 ? 0 : (size_t)outs * p.splits * (cache->head_dim + 2);
+    if (need && (!dws || ws_floats < need || !aligned16(dws)))
+        return rt::error(PK_GPU_EINVAL, "%s: needs a 16-byte aligned workspace of %zu floats "
+                         "(pk_gpu_prompt_attention_ws_floats)", kWho, need);
+    OnDevice on;
+    if (on.rc) return on.rc;
+    if (!some) return PK_GPU_OK;
+    PagedArgs a{};
+    a.k = static_cast<const char*>(cache->k);
+    a.v = static_cast<const char*>(cache->v);
+    a.k_scale = cache->k_scale;
+    a.v_scale = cache->v_scale;
+    a.q = static_cast<const char*>(dq);
+    a.ldq = (size_t)ldq * es;
+    a.pages = dpages;
+    a.ld_pages = ld_pages;
+    a.lens = dlens;
+    a.out = static_cast<char*>(dout);
+    a.ldo = (size_t)ldo * es;
+    a.lse = dlse;
+    a.part = dws;
+    a.ml = need ? dws + (size_t)outs * p.splits * cache->head_dim : nullptr;
+    a.scale2 = rules->scale * 1.4426950408889634f;
+    a.B = B;
+    a.max_len = max_len;
+    a.window = z.window;
+    a.kv_heads = cache->heads;
+    a.group = group;
+    a.head_tiles = (int)tiles;
+    a.n_pages = cache->n_pages;
+    a.page_shift = __builtin_ctz(cache->page_size);
+    a.chunk = p.chunk;
+    a.splits = p.splits;
+    a.rules.cap2 = rules->cap * 1.4426950408889634f;
+    a.rules.cap_in = rules->cap > 0.0f ? rules->scale / rules->cap : 0.0f;
+    a.rules.slopes = rules->slopes;
+    a.rules.first = rules->first;
+    a.rules.until = rules->until;
+    a.rules.starts = dstarts;
+    a.rules.rows = rows;
+    a.rules.max_new = z.max_new;
+    const hipError_t e = launch_attention(cache->dtype, dtype, cache->head_dim, true, a, (uint32_t)(pairs * p.splits),
+                                          (uint32_t)outs, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? PK_GPU_OK : rt::hip_error(e, kWho);
+}
+
+}  // extern "C"

@@ -91,6 +91,8 @@ _PROTOS = {
     "pk_gpu_encoder_profile_read": (_i, [_p, _i, _p, _p, _p, _p]),
     "pk_gpu_kv_write_dev": (_i, [_p, _i, _p, _i, _p, _i, _p, _i, _p]),
     "pk_gpu_kv_read_dev": (_i, [_p, _i, _p, _i, _p, _i, _p, _i, _p]),
+    "pk_gpu_prompt_attention_ws_floats": (_sz, [_p, _i, _i, _i, _i, _i, _i]),
+    "pk_gpu_prompt_attention_dev": (_i, [_p, _i, _p, _i, _i, _p, _i, _p, _p, _i, _i, _i, _i, _p, _p, _i, _p, _p, _sz, _p]),
     "pk_gpu_rope_freqs": (_i, [_i, _d, _i, _d, _d, _d, _d, _p]),
     "pk_gpu_rope_dev": (_i, [_p, _i, _p, _i, _i, _i, _p, _i, _p, _i, _p]),
     "pk_gpu_rope_kv_write_dev": (_i, [_p, _p, _i, _p, _i, _i, _p, _i, _p, _i, _p, _i, _p, _p, _i, _p]),
@@ -155,6 +157,11 @@ class KvCache(ctypes.Structure):
     """pk_gpu_kv_cache (include/pk_gpu.h): a paged key-value cache, device pointers."""
     _fields_ = [("k", _p), ("v", _p), ("k_scale", _p), ("v_scale", _p), ("dtype", _i),
                 ("n_pages", _i), ("page_size", _i), ("heads", _i), ("head_dim", _i)]
+
+
+class AttentionRules(ctypes.Structure):
+    """pk_gpu_attention_rules (include/pk_gpu.h): device pointers, or None."""
+    _fields_ = [("scale", _f), ("cap", _f), ("slopes", _p), ("window", _i), ("first", _p), ("until", _p)]
 
 
 class Rope(ctypes.Structure):

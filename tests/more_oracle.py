@@ -93,3 +93,90 @@ def turned_bound(want, size, rows, far=1.0):
     the function's 2 and the first-order step's), the scale's product, an element's product and the sum: 6 of
     2^-24 of |a| + |b| times the scale; an angle of up to `far` radians is off by 2^-53 of it; the output's rounding."""
     return size * (6 * 2.0 ** -24 + far * 2.0 ** -53) + do.HALF[rows] * np.abs(want) * 1.01 + 2.0 ** -24 * (rows == "f16")
+
+
+# ---- attention with rules -------------------------------------------------------
+
+def ranges(lens, starts, rows, max_new, max_len, window=0, first=None, until=None):
+    """Per row: sequence (-1: none), position, and the tokens [lo, hi) that it sees."""
+    b_of, p_of, lo, hi = (np.full(rows, -1), np.zeros(rows, int), np.zeros(rows, int), np.zeros(rows, int))
+    for b in range(len(lens)):
+        s = min(max(int(starts[b]), 0), rows)
+        n = min(min(max(int(starts[b + 1]), s), rows) - s, max_new)
+        length = min(max(int(lens[b]), 0), max_len)
+        for i in range(n):
+            r, p = s + i, length - n + i
+            b_of[r], p_of[r] = b, p
+            lo[r] = max(0, int(first[r]) if first is not None else 0, p - window + 1 if window else 0)
+            hi[r] = max(0, min(length, max(p + 1, int(until[r]) if until is not None else 0)))
+    return b_of, p_of, lo, hi
+
+
+class Ruled:
+    """Outputs of the plain 64-bit form, and what their tolerances are made of."""
+
+    def __init__(self, cache, q, table, lens, starts, max_new, max_len, scale, cap=0.0, slopes=None, window=0, first=None,
+                 until=None, exact_tanh=False):
+        rows, heads, dim = q.shape
+        k, v = cache.rows("k"), cache.rows("v")
+        group = heads // cache.heads
+        self.live, pos, lo, hi = ranges(lens, starts, rows, max_new, max_len, window, first, until)
+        self.out, self.a = np.zeros(q.shape), np.zeros(q.shape)
+        self.lse, self.d = np.full((rows, heads), -np.inf), np.zeros((rows, heads))
+        self.seen = np.zeros(rows, int)
+        for b in sorted(set(self.live) - {-1}):
+            mine = np.flatnonzero(self.live == b)
+            n = hi[mine].max(initial=0)
+            t = np.arange(n)
+            page = table[b][t // cache.page] if n else t
+            t = t[(page >= 0) & (page < cache.pages)]
+            at = table[b][t // cache.page].astype(np.int64) * cache.page + t % cache.page if n else t
+            p = pos[mine][:, None]
+            see = (t >= lo[mine][:, None]) & (t < hi[mine][:, None])
+            self.seen[mine] = see.sum(1)
+            use = mine[see.any(1)]
+            see, p = see[see.any(1)], p[see.any(1)]
+            if not len(use):
+                continue
+            for h in range(heads):
+                kk, vv = k[at, h // group], v[at, h // group]
+                with np.errstate(all="ignore"):
+                    s = scale * (q[use, h] @ kk.T)
+                    x = abs(scale) * (np.abs(q[use, h]) @ np.abs(kk).T)
+                    err = (dim + 8) * 2.0 ** -23 * x + 6 * 2.0 ** -24 * np.abs(s)
+                    if cap:
+                        s = cap * np.tanh(s / cap)
+                        # tanh: 8 units of 1, or with exact_tanh 18 of its value (tanh_of)
+                        err = err + 2.0 ** -24 * (18 * np.abs(s) if exact_tanh else 8 * cap) + 6 * 2.0 ** -24 * np.abs(s)
+                    if slopes is not None:
+                        bias = np.float64(slopes[h]) * np.abs(p - t)
+                        s = s - bias
+                        err = err + 4 * 2.0 ** -24 * (bias + np.abs(s))
+                    s = np.where(see, s, -np.inf)
+                    m = s.max(1, keepdims=True)
+                    w = np.exp(s - m)
+                    w = np.where(see, w, 0)
+                    l = w.sum(1, keepdims=True)
+                    # tokens that weigh less than 2^-40 of the heaviest move nothing, whatever their error
+                    self.d[use, h] = np.where(w > 2.0 ** -40, err, 0).max(1)
+                    vf = np.where(see.any(0)[:, None], vv, 0)
+                    self.out[use, h], self.lse[use, h] = (w @ vf) / l, (m + np.log(l))[:, 0]
+                    self.a[use, h] = (w @ np.abs(vf)) / l
+
+    def bound(self, kind, rows, half_p):
+        """As decode_oracle.attention_bound: scores' errors twice, exp2, a weight's rounding, sums, the output's."""
+        n = np.maximum(self.seen, 1)[:, None]
+        rel = 2 * self.d + 4 * 2.0 ** -23 + half_p + (n / 16 + 64 + n / 4 + 64) * 2.0 ** -23
+        small = n[..., None] * 2.0 ** -32 * 8.0 if kind == "f16" else 0.0
+        return (rel[..., None] * self.a * 1.01 + small + do.HALF[rows] * np.abs(self.out) * 1.01
+                + 2.0 ** -24 * (rows == "f16"))
+
+    def lse_bound(self):
+        n = np.maximum(self.seen, 1)[:, None]
+        return self.d + (n / 16 + 72) * 2.0 ** -23 + 4 * 2.0 ** -24 * np.where(np.isfinite(self.lse), np.abs(self.lse), 0)
+
+
+def half_of_weights(kind, rows):
+    """Half a step of what a softmax weight keeps in the second product where rows are few: 16 bits, 24 for f32 outputs, over f16
+    caches 22."""
+    return 2.0 ** -22 if kind == "f16" else {"bf16": 2.0 ** -16, "f16": 2.0 ** -16, "f32": 2.0 ** -24}[rows]
