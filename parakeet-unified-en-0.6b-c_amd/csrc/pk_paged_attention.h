@@ -294,11 +294,10 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
             early[i][u] = !RULES && a.window == 0 && tt < a.max_len ? pages[tt >> a.page_shift] : -1;
         }
 
-    const int heads = a.kv_heads * a.group;
     int in_group = htile * 16 + n, token = b;
     bool head_ok = in_group < a.group;
     RowRange see{};
-    size_t row = 0;                            // of the workspace and lse
+    int new_token = 0;
     if constexpr (RULES) {
         const NewTokens news = new_tokens(a.rules, b);
         if (htile * 16 >= news.count * a.group) return;
@@ -307,12 +306,12 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
         head_ok = i < news.count;
         token = news.row + (head_ok ? i : 0);
         see = range_of(a.rules, len < 0 ? 0 : min(len, a.max_len), news.count, head_ok ? i : 0, token, a.window);
-        row = (size_t)b * a.rules.max_new + i;
-    } else {
-        row = b;
+        new_token = i;
     }
+    const int heads = a.kv_heads * a.group;
     const int head = kvh * a.group + in_group;
-    row = row * heads + head;
+    // of the workspace
+    auto row_of = [&] { return (RULES ? (size_t)b * a.rules.max_new + new_token : (size_t)b) * heads + head; };
     const float slope2 = RULES && a.rules.slopes && head_ok ? a.rules.slopes[head] * 1.4426950408889634f : 0.0f;
 
     // queries: step c takes elements el(c, i) = i + 8 g + 32 c of a 16-bit cache's
@@ -348,8 +347,8 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
     }
     if (split > 0 && split >= sp.chunks) {
         if (RULES && wave == 0 && g == 0 && head_ok) {          // the join looks at every chunk
-            a.ml[(row * a.splits + split) * 2] = -FLT_MAX;
-            a.ml[(row * a.splits + split) * 2 + 1] = 0.0f;
+            a.ml[(row_of() * a.splits + split) * 2] = -FLT_MAX;
+            a.ml[(row_of() * a.splits + split) * 2 + 1] = 0.0f;
         }
         return;
     }
@@ -715,6 +714,7 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
     const bool direct = RULES ? a.splits == 1 : sp.chunks <= 1;
     const float inv = lt == 0.0f ? 0.0f : __fdiv_rn(1.0f, lt);
     constexpr int RUN = VB > 16 ? 8 : E;       // consecutive elements
+    const size_t row = row_of();
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
 #pragma unroll
@@ -746,7 +746,7 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
     }
     if (g == 0) {
         if (direct) {
-            if (a.lse) a.lse[(size_t)token * heads + head] = lt == 0.0f ? -__builtin_inff()
+            if (a.lse) a.lse[RULES ? (size_t)token * heads + head : row] = lt == 0.0f ? -__builtin_inff()
                                                : __fmul_rn(__fadd_rn(mx - BIAS, __builtin_amdgcn_logf(lt)),
                                                            0.69314718055994531f);
         } else {
