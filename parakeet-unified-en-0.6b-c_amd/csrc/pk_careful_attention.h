@@ -16,6 +16,7 @@ struct RuleArgs {
     const int *first, *until;    // of each query row
     const int* starts;           // [B + 1], or NULL: row b is sequence b's
     int rows, max_new;
+    int by_row;                  // the workspace's rows are q's, not (sequence, new token)s
 };
 
 // Sequence b's new tokens: rows row .. row + count - 1, whatever `starts` holds.
@@ -25,6 +26,21 @@ __device__ inline NewTokens new_tokens(const RuleArgs& r, int b)
     if (!r.starts) return {b, b < r.rows ? 1 : 0};
     const int s = min(max(r.starts[b], 0), r.rows), e = min(max(r.starts[b + 1], s), r.rows);
     return {s, min(e - s, r.max_new)};
+}
+
+// Whether row `row` is one of some sequence's new tokens.
+__device__ inline bool is_new_token(const RuleArgs& r, int B, int row)
+{
+    for (int b0 = 0; b0 < B; b0 += 64) {
+        const int b = b0 + (threadIdx.x & 63);
+        bool mine = false;
+        if (b < B) {
+            const NewTokens n = new_tokens(r, b);
+            mine = row >= n.row && row - n.row < n.count;
+        }
+        if (__any(mine)) return true;
+    }
+    return false;
 }
 
 // The tokens [lo, hi) that new token i of a sequence of `len` tokens sees, and its

@@ -12,7 +12,7 @@ struct JoinArgs {
     char* out;
     size_t ldo;
     float* lse;
-    int heads, splits, chunk, max_len, window;
+    int B, heads, splits, chunk, max_len, window;
     RuleArgs rules;
 };
 
@@ -21,7 +21,7 @@ struct JoinArgs {
 // every PARTS-th chunk; sums run in a fixed order.  All that it reads first,
 // the length, the chunks' (m, l) and EARLY chunks' outputs of a thread, is asked
 // for at once: the workspace holds them whether the sequence has them or not.  With
-// RULES a row is a (sequence, new token, head), and a chunk that it sees nothing of has
+// RULES a row is a (sequence, new token, head) or a (row of q, head), and a chunk that it sees nothing of has
 // said so by l = 0; what the workspace holds of that one's outputs is anything.
 template <int T, int DIM, bool RULES>
 __global__ void __launch_bounds__(256) paged_join(JoinArgs a)
@@ -33,7 +33,9 @@ __global__ void __launch_bounds__(256) paged_join(JoinArgs a)
     int b = blockIdx.x / (uint32_t)a.heads;
     const int head = blockIdx.x % (uint32_t)a.heads;
     const size_t row = (size_t)b * a.heads + head;
-    if constexpr (RULES) {
+    if (RULES && a.rules.by_row) {
+        if (!is_new_token(a.rules, a.B, b)) return;
+    } else if constexpr (RULES) {
         const uint32_t seq = (uint32_t)b / (uint32_t)a.rules.max_new, i = b - seq * a.rules.max_new;
         const NewTokens news = new_tokens(a.rules, seq);
         if ((int)i >= news.count) return;
@@ -217,6 +219,7 @@ hipError_t launch_joins(int t, int dim, bool rules, const PagedArgs& a, uint32_t
     j.out = a.out;
     j.ldo = a.ldo;
     j.lse = a.lse;
+    j.B = a.B;
     j.heads = a.kv_heads * a.group;
     j.splits = a.splits;
     j.chunk = a.chunk;

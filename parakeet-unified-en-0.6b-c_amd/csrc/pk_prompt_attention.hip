@@ -1,6 +1,6 @@
 // pk_prompt_attention.hip - host side of the attention of several new tokens per sequence
 // over a paged cache, with rules for scores and for what a token sees.
-#include "pk_paged_attention.h"
+#include "pk_prompt_attention.h"
 
 #include <cmath>
 
@@ -13,9 +13,10 @@ constexpr const char* kWho = "prompt attention";
 // A call's sizes, as its workspace is made for.
 struct Sizes { int B, heads, max_new, max_len, window; };
 
-// 16 (new token, head) pairs of a key-value head a workgroup.
-long long tiles_of(long long rows) { return (rows + 15) / 16; }
-long long pairs_of(const pk_gpu_kv_cache* c, const Sizes& z, int B, long long tiles) { return (long long)B * c->heads * tiles; }
+// Calls of few rows, (new token, head) pairs of a key-value head, go 16 a workgroup over
+// the tiles of the one-token attention, the others prompt_rows a workgroup.
+constexpr int kFewRows = 64;
+bool few_rows(const pk_gpu_kv_cache* c, const Sizes& z) { return (long long)z.max_new * (z.heads / c->heads) <= kFewRows; }
 
 // Tokens that a workgroup's columns see at most, from a multiple of 32 on.
 long long span_of_rows(const Sizes& z)
@@ -39,23 +40,88 @@ int check_sizes(const pk_gpu_kv_cache* c, const Sizes& z)
     return PK_GPU_OK;
 }
 
-// Floats that any call with these sizes at most takes; see ws_floats_up_to of the
-// one-token attention.  Above 256 pairs no sequence is split.
-size_t most_floats(const pk_gpu_kv_cache* c, const Sizes& z)
+// Chunks of a call of many rows, where its tiles are fewer than the CUs: 512 workgroups,
+// two a CU, of 512 tokens at least.
+constexpr int kSplitRows = 128;
+long long prompt_cuts(long long pairs, long long span)
+{
+    if (pairs >= 256) return 1;
+    const long long n = 512 / pairs, most = span / 512;
+    const long long cut = n < most ? n : most;
+    return cut < 1 ? 1 : cut > 64 ? 64 : cut;
+}
+// Tiles of a call's rows, whatever the sequences they are of.
+long long split_pairs(const pk_gpu_kv_cache* c, long long rows, int group)
+{
+    return ((rows * group + kSplitRows - 1) / kSplitRows) * c->heads;
+}
+
+// How a call is laid out: workgroups of one chunk, chunks, rows of the workspace.
+struct Layout {
+    bool few;
+    long long pairs, outs;
+    Plan plan;
+};
+Layout layout_of(const pk_gpu_kv_cache* c, const Sizes& z, int rows, int dtype)
+{
+    const int group = z.heads / c->heads;
+    const long long each = (long long)z.max_new * group, span = span_of_rows(z);
+    Layout l;
+    l.few = few_rows(c, z);
+    if (l.few) {
+        l.pairs = (each + 15) / 16 * z.B * c->heads;
+        l.outs = (long long)z.B * z.max_new * z.heads;
+        l.plan = plan_of(c->dtype, c->head_dim, l.pairs > 0 ? l.pairs : 1, span);
+    } else {
+        const int bm = prompt_rows(c->dtype, dtype, c->head_dim);
+        // tiles of every sequence, or of all rows with one that is not whole for each sequence
+        const long long a = (each + bm - 1) / bm * z.B, b = (long long)rows * group / bm + z.B;
+        l.pairs = (a < b ? a : b) * c->heads;
+        l.outs = (long long)rows * z.heads;
+        const long long n = prompt_cuts(split_pairs(c, rows, group), span);
+        const long long chunk = ((span + n - 1) / n + kKeys - 1) / kKeys * kKeys;
+        // a tile of rows begins anywhere in its chunk's first 64 tokens
+        l.plan = {(int)chunk, (int)(n == 1 ? 1 : (span + kKeys - 1 + chunk - 1) / chunk)};
+        if (n == 1) l.plan.chunk = 1 << 30;
+    }
+    return l;
+}
+
+// Floats that any call with these sizes at most takes.  Few rows: see ws_floats_up_to of
+// the one-token attention; above 256 pairs no sequence is split.  Many: chunks fall as
+// the rows' tiles grow, and there is one more than prompt_cuts at most.
+size_t most_floats(const pk_gpu_kv_cache* c, const Sizes& z, int rows)
 {
     const int group = z.heads / c->heads;
     const long long span = span_of_rows(z);
     size_t most = 0;
-    for (int b = 1; b <= z.B && pairs_of(c, z, b, 1) <= 256; ++b)
-        for (long long t = 1; pairs_of(c, z, b, t) <= 256; ++t) {
+    for (long long b = 1; b <= z.B && b * c->heads <= 256; ++b)
+        for (long long t = 1; 16 * t <= kFewRows + 15 && t * b * c->heads <= 256; ++t) {
             // the most new tokens of so many tiles
-            const long long n = 16 * t / group < z.max_new ? 16 * t / group : z.max_new;
+            long long n = 16 * t / group < kFewRows / group ? 16 * t / group : kFewRows / group;
+            n = n < z.max_new ? n : z.max_new;
             if (n < 1) continue;
-            const size_t cut = cuts(c->dtype, c->head_dim, pairs_of(c, z, b, t), span);
+            const size_t cut = cuts(c->dtype, c->head_dim, t * b * c->heads, span);
             if (cut > 1 && b * n * cut > most) most = b * n * cut;
-            if (n == z.max_new) break;
+        }
+    if (!few_rows(c, z))
+        for (long long t = 1; t * c->heads < 256; ++t) {
+            const long long n = kSplitRows * t / group < rows ? kSplitRows * t / group : rows;
+            const size_t cut = prompt_cuts(t * c->heads, span);
+            if (n >= 1 && cut > 1 && n * (cut + 1) > most) most = n * (cut + 1);
         }
     return most * z.heads * (c->head_dim + 2);
+}
+
+hipError_t launch_prompts(int cache, int t, int dim, const PagedArgs& a, uint32_t workgroups, uint32_t rows, hipStream_t s)
+{
+    const dim3 grid(workgroups);
+    const hipError_t e = cache == F16    ? launch_prompt_f16(t, dim, a, grid, s)
+                         : cache == BF16 ? launch_prompt_bf16(t, dim, a, grid, s)
+                         : cache == I8   ? launch_prompt_i8(t, dim, a, grid, s)
+                         : cache == E2M1 ? launch_prompt_e2m1(t, dim, a, grid, s)
+                                         : launch_prompt_e4m3(t, dim, a, grid, s);
+    return e == hipSuccess && a.splits > 1 ? launch_joins(t, dim, true, a, rows, s) : e;
 }
 
 }  // namespace
@@ -72,7 +138,7 @@ size_t pk_gpu_prompt_attention_ws_floats(const pk_gpu_kv_cache* cache, int B, in
 {
     const Sizes z{B, heads, max_new < rows ? max_new : rows, max_len, window < max_len ? window : 0};
     if (check_sizes(cache, z) != PK_GPU_OK) return 0;
-    return most_floats(cache, z);
+    return most_floats(cache, z, rows);
 }
 
 int pk_gpu_prompt_attention_dev(const pk_gpu_kv_cache* cache, int dtype, const void* dq, int ldq, int heads,
@@ -110,15 +176,12 @@ int pk_gpu_prompt_attention_dev(const pk_gpu_kv_cache* cache, int dtype, const v
     if (z.max_new > rows) z.max_new = rows;
     if (!dstarts && z.max_new > 1) z.max_new = 1;
     if (z.window >= max_len) z.window = 0;
-    const int group = heads / cache->heads;
-    const long long tiles = tiles_of((long long)z.max_new * group);
-    const long long pairs = pairs_of(cache, z, B, tiles);
-    const Plan p = plan_of(cache->dtype, cache->head_dim, pairs > 0 ? pairs : 1, span_of_rows(z));
-    const long long outs = (long long)B * z.max_new * heads;
-    if (!launchable(pairs * p.splits, 512) || outs > 0x7fffffff || (p.splits > 1 && !launchable(outs, 256)))
+    const Layout l = layout_of(cache, z, rows, dtype);
+    const Plan& p = l.plan;
+    if (!launchable(l.pairs * p.splits, 512) || l.outs > 0x7fffffff || (p.splits > 1 && !launchable(l.outs, 256)))
         return rt::error(PK_GPU_EINVAL, "%s: %d sequences of %d new tokens and %d heads exceed the grid", kWho, B, z.max_new,
                          heads);
-    const size_t need = p.splits <= 1 ? 0 : (size_t)outs * p.splits * (cache->head_dim + 2);
+    const size_t need = p.splits <= 1 ? 0 : (size_t)l.outs * p.splits * (cache->head_dim + 2);
     if (need && (!dws || ws_floats < need || !aligned16(dws)))
         return rt::error(PK_GPU_EINVAL, "%s: needs a 16-byte aligned workspace of %zu floats "
                          "(pk_gpu_prompt_attention_ws_floats)", kWho, need);
@@ -139,14 +202,14 @@ int pk_gpu_prompt_attention_dev(const pk_gpu_kv_cache* cache, int dtype, const v
     a.ldo = (size_t)ldo * es;
     a.lse = dlse;
     a.part = dws;
-    a.ml = need ? dws + (size_t)outs * p.splits * cache->head_dim : nullptr;
+    a.ml = need ? dws + (size_t)l.outs * p.splits * cache->head_dim : nullptr;
     a.scale2 = rules->scale * 1.4426950408889634f;
     a.B = B;
     a.max_len = max_len;
     a.window = z.window;
     a.kv_heads = cache->heads;
-    a.group = group;
-    a.head_tiles = (int)tiles;
+    a.group = heads / cache->heads;
+    a.head_tiles = (int)(l.pairs / (l.few ? (long long)B * cache->heads : cache->heads));
     a.n_pages = cache->n_pages;
     a.page_shift = __builtin_ctz(cache->page_size);
     a.chunk = p.chunk;
@@ -159,8 +222,11 @@ int pk_gpu_prompt_attention_dev(const pk_gpu_kv_cache* cache, int dtype, const v
     a.rules.starts = dstarts;
     a.rules.rows = rows;
     a.rules.max_new = z.max_new;
-    const hipError_t e = launch_attention(cache->dtype, dtype, cache->head_dim, true, a, (uint32_t)(pairs * p.splits),
-                                          (uint32_t)outs, static_cast<hipStream_t>(stream));
+    a.rules.by_row = !l.few;
+    const hipError_t e = l.few ? launch_attention(cache->dtype, dtype, cache->head_dim, true, a, (uint32_t)(l.pairs * p.splits),
+                                                  (uint32_t)l.outs, static_cast<hipStream_t>(stream))
+                               : launch_prompts(cache->dtype, dtype, cache->head_dim, a, (uint32_t)(l.pairs * p.splits),
+                                                (uint32_t)l.outs, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? PK_GPU_OK : rt::hip_error(e, kWho);
 }
 

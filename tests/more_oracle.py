@@ -176,7 +176,12 @@ class Ruled:
         return self.d + (n / 16 + 72) * 2.0 ** -23 + 4 * 2.0 ** -24 * np.where(np.isfinite(self.lse), np.abs(self.lse), 0)
 
 
-def half_of_weights(kind, rows):
-    """Half a step of what a softmax weight keeps in the second product where rows are few: 16 bits, 24 for f32 outputs, over f16
-    caches 22."""
+def half_of_weights(kind, rows, many=False):
+    """Half a step of what a softmax weight keeps in the second product: 16 bits, 24 for f32 outputs, over f16
+    caches 22.  Where rows are many, 16-bit outputs over caches of their own type and bf16 ones over codes take
+    one term: 8 bits in bf16 (half a step 2^-8 of the weight), 11 in f16 (2^-11)."""
+    if many and rows == "bf16":
+        return 2.0 ** -8
+    if many and kind == "f16":
+        return 2.0 ** -11
     return 2.0 ** -22 if kind == "f16" else {"bf16": 2.0 ** -16, "f16": 2.0 ** -16, "f32": 2.0 ** -24}[rows]

@@ -75,7 +75,8 @@ class Prompt:
         return got
 
     def half_p(self):
-        return mo.half_of_weights(self.cache.kind, self.rows)
+        many = min(self.max_new, self.n) * (self.heads // self.cache.heads) > 64
+        return mo.half_of_weights(self.cache.kind, self.rows, many and (self.starts is not None))
 
 
 def prompt(rng, kind, rows, kv, group, dim, page, new, lens, max_new=None, max_len=None, tail=0, pad=0, scale=None, seed=1,
