@@ -11,7 +11,7 @@ namespace pkgpu {
 namespace decode {
 
 struct RuleArgs {
-    float cap_in, cap2;          // scale / cap and cap * log2(e); cap2 = 0: no cap
+    float cap_in, cap_exp, cap2; // x = raw cap_in, e^2x = 2^(raw cap_exp), cap * log2(e); cap2 = 0: no cap
     const float* slopes;
     const int *first, *until;    // of each query row
     const int* starts;           // [B + 1], or NULL: row b is sequence b's
@@ -58,19 +58,20 @@ __device__ inline RowRange range_of(const RuleArgs& r, int len, int count, int i
     return s;
 }
 
-// tanh: 1 - 2 / (e^2x + 1), off by some units of 2^-24 of 1.  Where f32 outputs want
-// units of the value, small arguments take the quotient that the continued fraction
-// x / (1 + x^2 / (3 + x^2 / (5 + ...))) gives, cut off behind 13: within 2^-40 below 1/2.
+// cap tanh(raw scale / cap) in powers of two, with tanh x = 1 - 2 / (e^2x + 1): off by some
+// units of 2^-24 of the cap.  Where f32 outputs want units of the value, small arguments
+// take the quotient that the continued fraction x / (1 + x^2 / (3 + x^2 / (5 + ...)))
+// gives, cut off behind 13: within 2^-40 below 1/2.
 template <int T>
-__device__ inline float tanh_of(float x)
+__device__ inline float capped(const RuleArgs& r, float raw)
 {
-    const float e = __builtin_amdgcn_exp2f(__fmul_rn(x, 2.8853900817779268f));
-    float y = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(__fadd_rn(e, 1.0f)), 1.0f);
+    const float e = __builtin_amdgcn_exp2f(__fmul_rn(raw, r.cap_exp));
+    float y = __builtin_fmaf(__fmul_rn(-2.0f, r.cap2), __builtin_amdgcn_rcpf(__fadd_rn(e, 1.0f)), r.cap2);
     if constexpr (T == F32) {
-        const float z = __fmul_rn(x, x);
+        const float x = __fmul_rn(raw, r.cap_in), z = __fmul_rn(x, x);
         const float a = __builtin_fmaf(__builtin_fmaf(z + 378.0f, z, 17325.0f), z, 135135.0f);
         const float b = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(28.0f, z, 3150.0f), z, 62370.0f), z, 135135.0f);
-        const float small = __fmul_rn(x, __fmul_rn(a, __builtin_amdgcn_rcpf(b)));
+        const float small = __fmul_rn(__fmul_rn(x, r.cap2), __fmul_rn(a, __builtin_amdgcn_rcpf(b)));
         y = fabsf(x) < 0.5f ? small : y;
     }
     return y;
@@ -80,8 +81,8 @@ __device__ inline float tanh_of(float x)
 template <int T>
 __device__ inline float ruled_score(const RuleArgs& r, float raw, float scale2, float slope2, int ahead)
 {
-    float s = r.cap2 != 0.0f ? __fmul_rn(r.cap2, tanh_of<T>(__fmul_rn(raw, r.cap_in))) : __fmul_rn(raw, scale2);
-    if (r.slopes) s = __builtin_fmaf(-slope2, (float)abs(ahead), s);
+    float s = r.cap2 != 0.0f ? capped<T>(r, raw) : __fmul_rn(raw, scale2);
+    if (r.slopes) s = __builtin_fmaf(-slope2, fabsf((float)ahead), s);
     return s;
 }
 

@@ -274,8 +274,11 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, 
     const uint32_t pairs = (uint32_t)a.B * a.kv_heads * a.head_tiles;
     const int split = blockIdx.x / pairs;
     uint32_t x = (blockIdx.x + split) % pairs;
-    const int htile = x % (uint32_t)a.head_tiles;
-    x /= (uint32_t)a.head_tiles;
+    // With RULES the tiles of one key-value head that read the same chunk go to the same
+    // L2 where the other pairs are a multiple of 8.
+    const uint32_t others = (uint32_t)a.B * a.kv_heads;
+    const int htile = RULES ? x / others : x % (uint32_t)a.head_tiles;
+    x = RULES ? x - htile * others : x / (uint32_t)a.head_tiles;
     const int kvh = x % (uint32_t)a.kv_heads;
     int b = x / (uint32_t)a.kv_heads;
     if (a.longest_first) b = nth_longest(a, b, sh.lens, wave);

@@ -10,7 +10,12 @@ namespace decode {
 using f32x16 = __attribute__((ext_vector_type(16))) float;
 using s16x4 = __attribute__((ext_vector_type(4))) short;
 
-constexpr int kKeys = 64;                  // tokens of a tile
+// Tokens of a tile: as many as leave the registers of two workgroups a CU whole (one
+// at heads of 256, and there half as many where codes wait in registers too).
+constexpr int prompt_keys(int cache, int t, int dim)
+{
+    return dim == 64 ? 128 : dim == 128 ? 64 : cache == F16 || cache == BF16 || (cache == E2M1 && t == BF16) ? 64 : 32;
+}
 
 constexpr int prompt_p_terms(int cache, int t) { return t == F32 ? 3 : t == F16 && cache != F16 ? 2 : 1; }
 // column blocks of 32 rows a wave takes, and workgroups a CU
@@ -78,9 +83,10 @@ __global__ void __launch_bounds__(256, prompt_occupancy(CACHE, T, DIM)) prompt_a
     constexpr float BIAS = VF ? 7.0f : 0.0f;
     constexpr int PR = DIM / 8;                // 16-byte pieces of a row in LDS
     constexpr int STEPS = DIM / 16, DB = DIM / 32;
+    constexpr int KT = prompt_keys(CACHE, T, DIM), NU = KT / 32, NB = KT / 16;   // a tile's tokens, blocks of 32 and of 16
 
-    __shared__ u32x4 tiles[2][2][kKeys * PR];  // [stage][keys, values][row][piece]
-    __shared__ float scales[CODED ? 2 : 1][2][kKeys];
+    __shared__ u32x4 tiles[2][2][KT * PR];  // [stage][keys, values][row][piece]
+    __shared__ float scales[CODED ? 2 : 1][2][KT];
     __shared__ int spans[2][4];
 
     const int lane = threadIdx.x & 63;
@@ -135,7 +141,7 @@ __global__ void __launch_bounds__(256, prompt_occupancy(CACHE, T, DIM)) prompt_a
     int last = max(max(spans[1][0], spans[1][1]), max(spans[1][2], spans[1][3]));
     first = __builtin_amdgcn_readfirstlane(last ? first : 0);
     last = __builtin_amdgcn_readfirstlane(last);
-    const int base = first & ~(kKeys - 1);
+    const int base = first & ~(KT - 1);
     const long long from = base + (long long)split * a.chunk;
     const int begin = from < last ? (int)from : last;
     const int end = min((long long)last, from + a.chunk);
@@ -173,25 +179,29 @@ __global__ void __launch_bounds__(256, prompt_occupancy(CACHE, T, DIM)) prompt_a
         }
 
     // ---- staging ----
-    // The tile's 4 blocks of 16 tokens lie in one page each.  Rows outside of [begin or first, end) are
+    // The tile's blocks of 16 tokens lie in one page each.  Rows outside of [begin or first, end) are
     // copies of the nearest row inside, so that what lies there enters nothing, and an
     // absent page's are slot 0's: both are masked.
     const int lo_row = max(first, begin), page_mask = (1 << a.page_shift) - 1;
-    struct Blocks { size_t row[4]; int at[4]; uint32_t present; };
-    auto blocks = [&](int t0) {
+    // All are worked out at once, one a lane, from pages that were asked for a tile before.
+    struct Blocks { size_t mine, off[NB]; uint32_t present; };      // bytes into the cache's arrays
+    const size_t page_bytes = ((size_t)a.kv_heads << a.page_shift) * RB, head_bytes = ((size_t)kvh << a.page_shift) * RB;
+    auto block_at = [&](int t0, int j) { return 16 * min(max((t0 >> 4) + j, lo_row >> 4), (end - 1) >> 4); };
+    auto pages_of = [&](int t0) { return pages[block_at(t0, lane % NB) >> a.page_shift]; };
+    auto blocks = [&](int t0, int ids) {
+        const bool there = (uint32_t)ids < (uint32_t)a.n_pages;
+        const size_t off = (there ? (uint32_t)ids * page_bytes + head_bytes : 0) +
+                           (uint32_t)(block_at(t0, lane % NB) & page_mask) * (uint32_t)RB;
         Blocks s;
-        s.present = 0;
+        s.mine = off;
+        s.present = (uint32_t)__ballot(there) & ((1u << NB) - 1);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int blk = min(max((t0 >> 4) + j, lo_row >> 4), (end - 1) >> 4);
-            s.at[j] = 16 * blk;
-            const int id = __builtin_amdgcn_readfirstlane(pages[(16 * blk) >> a.page_shift]);
-            const bool there = (uint32_t)id < (uint32_t)a.n_pages;
-            s.present |= (uint32_t)there << j;
-            s.row[j] = there ? (((size_t)id * a.kv_heads + kvh) << a.page_shift) + ((16 * blk) & page_mask) : 0;
-        }
+        for (int j = 0; j < NB; ++j)
+            s.off[j] = (size_t)(uint32_t)__builtin_amdgcn_readlane((int)(off >> 32), j) << 32 |
+                       (uint32_t)__builtin_amdgcn_readlane((int)off, j);
         return s;
     };
+    auto inside = [&](int t0) { return t0 >= lo_row && t0 + KT <= end; };
     const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) char*)(char*)&tiles[0][0][0];
     // slot of a row's piece
     auto slot_k = [](int row, int piece) { return PR == 8 ? piece ^ ((row >> 1) & 7) : piece ^ (row & 15); };
@@ -199,52 +209,71 @@ __global__ void __launch_bounds__(256, prompt_occupancy(CACHE, T, DIM)) prompt_a
 
     // loads in registers on their way to LDS, of the caches that hold codes
     constexpr int CP = RB / 16;                // 16-byte pieces of a row in the cache
-    constexpr int LOADS = SIXTEEN ? 1 : (kKeys * CP + 255) / 256;
+    constexpr int LOADS = SIXTEEN ? 1 : (KT * CP + 255) / 256;
     u32x4 raw[2][LOADS];
     uint32_t unit[2][LOADS];
+    // a thread's row scale: keys' of waves 0 (and 1), values' of the others; rows of short tiles are taken twice
     float row_scale = 0.0f;
-    auto fetch = [&](const Blocks& s, int stage) {
+    const int scale_side = KT > 64 ? wave >> 1 : wave & 1;
+    constexpr int RPC = SIXTEEN ? 64 / PR : 1;     // rows of a wave's 1 KB
+    // a tile at t0, all of it within the rows that count (WHOLE) or not, on its way to a stage
+    auto pick = [](const Blocks& s, int blk) {
+        return (size_t)(uint32_t)__shfl((int)(s.mine >> 32), blk) << 32 | (uint32_t)__shfl((int)s.mine, blk);
+    };
+    auto fetch_as = [&](auto whole, const Blocks& s, int t0, int stage) {
+        constexpr bool WHOLE = decltype(whole)::value;
         if constexpr (SIXTEEN) {
-            constexpr int RPC = 64 / PR;       // rows of a wave's 1 KB
 #pragma unroll
-            for (int i = 0; i < kKeys / RPC / 4; ++i) {
-                const int c = 4 * i + wave;    // its block: i, i / 2, or 2 i and 2 i + 1 for two waves each
-                const int blk = PR == 16 ? i : PR == 32 ? i / 2 : 2 * i;
-                const size_t r0 = PR == 8 && wave >= 2 ? s.row[PR == 8 ? blk + 1 : 0] : s.row[blk];
-                const int at = PR == 8 && wave >= 2 ? s.at[PR == 8 ? blk + 1 : 0] : s.at[blk];
-                const int row = c * RPC + lane / PR;
-                const int t = min(max(at + row % 16, lo_row), end - 1) - at;
-                const uint32_t lds = lds0 + (stage * 2 * kKeys * PR + c * 64) * 16;
-                const char* const k = a.k + r0 * RB;
-                const char* const v = a.v + r0 * RB;
-                cache_to_lds(lds, k, t * RB + 16 * slot_k(row, lane % PR));
-                cache_to_lds(lds + kKeys * PR * 16, v, t * RB + 16 * slot_v(row, lane % PR));
+            for (int i = 0; i < KT / RPC / 4; ++i) {
+                // its block: i, i / 2, or 2 i and 2 i + 1 for two waves each
+                const int blk = PR == 16 ? i : PR == 32 ? i / 2 : 2 * i + (wave >> 1);
+                const size_t off = PR == 8 ? (wave >= 2 ? s.off[(2 * i + 1) % NB] : s.off[2 * i % NB]) : s.off[blk % NB];
+                const int row = (4 * i + wave) * RPC + lane / PR;
+                int t = row % 16;
+                if constexpr (!WHOLE) {
+                    const int at = block_at(t0, blk);
+                    t = min(max(at + t, lo_row), end - 1) - at;
+                }
+                const uint32_t lds = lds0 + (stage * 2 * KT * PR + (4 * i + wave) * 64) * 16;
+                cache_to_lds(lds, a.k + off, t * RB + 16 * slot_k(row, lane % PR));
+                cache_to_lds(lds + KT * PR * 16, a.v + off, t * RB + 16 * slot_v(row, lane % PR));
             }
         } else {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
-                const int p = threadIdx.x + 256 * i, row = p / CP % kKeys;
+                const int p = threadIdx.x + 256 * i, row = p / CP % KT;
                 // a wave's rows are of one block, or of several whose rows are picked by lane
                 const int blk = row / 16;
-                const size_t r0 = blk == 0 ? s.row[0] : blk == 1 ? s.row[1] : blk == 2 ? s.row[2] : s.row[3];
-                const int at = blk == 0 ? s.at[0] : blk == 1 ? s.at[1] : blk == 2 ? s.at[2] : s.at[3];
-                const int t = min(max(at + row % 16, lo_row), end - 1) - at;
-                const size_t r = r0 + t;
-                raw[0][i] = *reinterpret_cast<const u32x4*>(a.k + r * RB + 16 * (p % CP));
-                raw[1][i] = *reinterpret_cast<const u32x4*>(a.v + r * RB + 16 * (p % CP));
-                if constexpr (CACHE == E2M1) {
-                    unit[0][i] = reinterpret_cast<const uint8_t*>(a.k_scale)[r * (DIM / kGroup) + p % CP];
-                    unit[1][i] = reinterpret_cast<const uint8_t*>(a.v_scale)[r * (DIM / kGroup) + p % CP];
+                const size_t off = pick(s, blk);
+                int t = row % 16;
+                if constexpr (!WHOLE) {
+                    const int at = block_at(t0, blk);
+                    t = min(max(at + t, lo_row), end - 1) - at;
+                }
+                const size_t b = off + t * RB + 16 * (p % CP);
+                raw[0][i] = *reinterpret_cast<const u32x4*>(a.k + b);
+                raw[1][i] = *reinterpret_cast<const u32x4*>(a.v + b);
+                if constexpr (CACHE == E2M1) {     // a byte for each 16
+                    unit[0][i] = reinterpret_cast<const uint8_t*>(a.k_scale)[b / 16];
+                    unit[1][i] = reinterpret_cast<const uint8_t*>(a.v_scale)[b / 16];
                 }
             }
             if constexpr (CODED) {
-                const int row = threadIdx.x % kKeys, blk = row / 16;
-                const size_t r0 = blk == 0 ? s.row[0] : blk == 1 ? s.row[1] : blk == 2 ? s.row[2] : s.row[3];
-                const int at = blk == 0 ? s.at[0] : blk == 1 ? s.at[1] : blk == 2 ? s.at[2] : s.at[3];
-                const size_t r = r0 + min(max(at + row % 16, lo_row), end - 1) - at;
-                if (wave < 2) row_scale = (wave ? a.v_scale : a.k_scale)[r];
+                const int row = lane % KT + (KT > 64 ? 64 * (wave & 1) : 0), blk = row / 16;
+                const size_t off = pick(s, blk);
+                int t = row % 16;
+                if constexpr (!WHOLE) {
+                    const int at = block_at(t0, blk);
+                    t = min(max(at + t, lo_row), end - 1) - at;
+                }
+                const size_t r = off / RB + t;
+                row_scale = (scale_side ? a.v_scale : a.k_scale)[r];
             }
         }
+    };
+    auto fetch = [&](const Blocks& s, int t0, int stage) {
+        if (inside(t0)) fetch_as(std::true_type{}, s, t0, stage);
+        else fetch_as(std::false_type{}, s, t0, stage);
     };
     auto put = [&](int stage) {
         if constexpr (!SIXTEEN) {
@@ -253,7 +282,7 @@ __global__ void __launch_bounds__(256, prompt_occupancy(CACHE, T, DIM)) prompt_a
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
                 const int p = threadIdx.x + 256 * i, row = p / CP;
-                if (LOADS * 256 > kKeys * CP && row >= kKeys) break;
+                if (LOADS * 256 > KT * CP && row >= KT) break;
                 if constexpr (CACHE == E2M1) {
 #pragma unroll
                     for (int d = 0; d < 4; ++d) {
@@ -271,7 +300,7 @@ __global__ void __launch_bounds__(256, prompt_occupancy(CACHE, T, DIM)) prompt_a
                 }
             }
             if constexpr (CODED)
-                if (wave < 2) scales[stage][wave][threadIdx.x % kKeys] = row_scale;
+                scales[stage][scale_side][lane % KT + (KT > 64 ? 64 * (wave & 1) : 0)] = row_scale;
         }
     };
 
@@ -296,11 +325,21 @@ __global__ void __launch_bounds__(256, prompt_occupancy(CACHE, T, DIM)) prompt_a
         v_off[d] = (4 * g + vrow) * (PR * 16) + 16 * slot_v(vrow, piece) + 8 * (lane & 1);
     }
 
-    auto compute = [&](int t0, int stage, uint32_t present) {
-        const u32x4* const k = tiles[stage][0];
-        f32x16 s[2][NQ];
+    // Accumulators of more than half the registers stay in the matrix cores' half.
+    auto pin = [&] {
+        if constexpr (DIM == 256)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+            for (int j = 0; j < NQ; ++j)
+#pragma unroll
+                for (int d = 0; d < DB; ++d) __asm__ volatile("" : "+a"(acc[j][d]));
+    };
+    auto compute = [&](int t0, auto at, uint32_t present) {
+        pin();
+        constexpr int stage = decltype(at)::value;
+        const u32x4* const k = tiles[stage][0];
+        f32x16 s[NU][NQ];
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
 #pragma unroll
             for (int j = 0; j < NQ; ++j)
 #pragma unroll
@@ -319,7 +358,7 @@ __global__ void __launch_bounds__(256, prompt_occupancy(CACHE, T, DIM)) prompt_a
         float scale = a.scale2;
         if constexpr (CODED) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < NU; ++u)
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
                     const f32x4 ks = *reinterpret_cast<const f32x4*>(&scales[stage][0][32 * u + 2 * i + 4 * g]);
@@ -331,22 +370,41 @@ __global__ void __launch_bounds__(256, prompt_occupancy(CACHE, T, DIM)) prompt_a
         }
         if (!plain) {
             scale = 1.0f;
+            if (a.rules.cap2 != 0.0f) {
 #pragma unroll
-            for (int j = 0; j < NQ; ++j)
+                for (int j = 0; j < NQ; ++j)
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                    for (int u = 0; u < NU; ++u)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        s[u][j][i] = ruled_score<T>(a.rules, s[u][j][i], a.scale2, slope2[j],
-                                                    see[j].p - (t0 + 32 * u + 8 * (i / 4) + 4 * g + i % 4));
+                        for (int i = 0; i < 16; ++i) s[u][j][i] = capped<T>(a.rules, s[u][j][i]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < NQ; ++j)
+#pragma unroll
+                    for (int u = 0; u < NU; ++u)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) s[u][j][i] = __fmul_rn(s[u][j][i], a.scale2);
+            }
+            if (a.rules.slopes) {
+#pragma unroll
+                for (int j = 0; j < NQ; ++j) {
+                    const float ahead = (float)(see[j].p - t0 - 4 * g);
+#pragma unroll
+                    for (int u = 0; u < NU; ++u)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            s[u][j][i] = __builtin_fmaf(-slope2[j], fabsf(__fsub_rn(ahead, (float)(32 * u + 8 * (i / 4) + i % 4))),
+                                                        s[u][j][i]);
+                }
+            }
         }
-        const bool whole = present == 15 && t0 >= max(all_lo, begin) && t0 + kKeys <= min(all_hi, end);
+        const bool whole = present == (1u << NB) - 1 && t0 >= max(all_lo, begin) && t0 + KT <= min(all_hi, end);
         if (!whole) {
 #pragma unroll
             for (int j = 0; j < NQ; ++j) {
                 const int from = max(see[j].lo, begin) - t0 - 4 * g, to = min(see[j].hi, end) - t0 - 4 * g;
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int u = 0; u < NU; ++u)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const int t = 32 * u + 8 * (i / 4) + i % 4;
@@ -355,12 +413,12 @@ __global__ void __launch_bounds__(256, prompt_occupancy(CACHE, T, DIM)) prompt_a
                     }
             }
         }
-        u32x4 pf[NQ][PT][4];
+        u32x4 pf[NQ][PT][NB];
 #pragma unroll
         for (int j = 0; j < NQ; ++j) {
             float top = s[0][j][0];
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < NU; ++u)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][j][i]);
             top = __fmul_rn(top, scale);
@@ -374,9 +432,11 @@ __global__ void __launch_bounds__(256, prompt_occupancy(CACHE, T, DIM)) prompt_a
 #pragma unroll
                     for (int i = 0; i < 16; ++i) acc[j][d][i] = __fmul_rn(acc[j][d][i], f);
             }
+            __builtin_amdgcn_s_setprio(1);
+            pin();
             const float off = BIAS - m[j];
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < NU; ++u)
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) {
                     float w[2];
@@ -397,9 +457,9 @@ __global__ void __launch_bounds__(256, prompt_occupancy(CACHE, T, DIM)) prompt_a
                 }
         }
         // k index 8 g + i of step c is token 16 c + 8 (i / 4) + 4 g + i % 4
-        const uint32_t vbase = lds0 + (stage * 2 + 1) * kKeys * PR * 16;
+        const uint32_t vbase = lds0 + (stage * 2 + 1) * KT * PR * 16;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < NB; ++c) {
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
                 u32x4 f;
@@ -420,33 +480,40 @@ __global__ void __launch_bounds__(256, prompt_occupancy(CACHE, T, DIM)) prompt_a
     };
 
     auto arrived = [] {
-        __asm__ volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_setprio(0);
+        __asm__ volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0070);        // vmcnt and lgkmcnt 0, and the compiler knows it
         __builtin_amdgcn_s_barrier();
         __asm__ volatile("" ::: "memory");         // nothing of the new stage is read before
     };
-    int t = begin & ~(kKeys - 1), stage = 0;
+    // Two tiles a turn, so that their stages are constants.
     if (begin < end) {
-        Blocks s = blocks(t);
-        fetch(s, 0);
+        int t = begin & ~(KT - 1), ids = pages_of(t + KT);
+        const Blocks s = blocks(t, pages_of(t));
+        fetch(s, t, 0);
         put(0);
         uint32_t present = s.present;
         arrived();
-        while (true) {
-            const bool more = t + kKeys < end;
+        auto step = [&](auto at) {
+            constexpr int stage = decltype(at)::value;
+            const bool more = t + KT < end;
             uint32_t next = 0;
             if (more) {
-                const Blocks s1 = blocks(t + kKeys);
+                const Blocks s1 = blocks(t + KT, ids);
+                ids = pages_of(t + 2 * KT);
                 next = s1.present;
-                fetch(s1, stage ^ 1);
+                fetch(s1, t + KT, stage ^ 1);
             }
-            if (t < wave_hi && t + kKeys > wave_lo) compute(t, stage, present);
-            if (!more) break;
+            if (t < wave_hi && t + KT > wave_lo) compute(t, at, present);
+            if (!more) return false;
             put(stage ^ 1);
             arrived();
             present = next;
-            stage ^= 1;
-            t += kKeys;
-        }
+            t += KT;
+            return true;
+        };
+#pragma unroll 1
+        while (step(std::integral_constant<int, 0>{}) && step(std::integral_constant<int, 1>{})) {}
     }
 
     // sums that have left the range, or a NaN: the workgroup's rows again, one by one

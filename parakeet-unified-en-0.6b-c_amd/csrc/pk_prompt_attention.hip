@@ -13,11 +13,6 @@ constexpr const char* kWho = "prompt attention";
 // A call's sizes, as its workspace is made for.
 struct Sizes { int B, heads, max_new, max_len, window; };
 
-// Calls of few rows, (new token, head) pairs of a key-value head, go 16 a workgroup over
-// the tiles of the one-token attention, the others prompt_rows a workgroup.
-constexpr int kFewRows = 64;
-bool few_rows(const pk_gpu_kv_cache* c, const Sizes& z) { return (long long)z.max_new * (z.heads / c->heads) <= kFewRows; }
-
 // Tokens that a workgroup's columns see at most, from a multiple of 32 on.
 long long span_of_rows(const Sizes& z)
 {
@@ -40,13 +35,38 @@ int check_sizes(const pk_gpu_kv_cache* c, const Sizes& z)
     return PK_GPU_OK;
 }
 
-// Chunks of a call of many rows, where its tiles are fewer than the CUs: 512 workgroups,
-// two a CU, of 512 tokens at least.
-constexpr int kSplitRows = 128;
-long long prompt_cuts(long long pairs, long long span)
+// Calls of few rows, (new token, head) pairs of a key-value head, go 16 a workgroup over
+// the tiles of the one-token attention, the others prompt_rows a workgroup.
+//
+// Up to 64 rows the cache's bytes are what counts, and those tiles fetch them faster.  Beyond,
+// they do while there are as many CUs as workgroups and these are short: 16 rows start
+// sooner than 128, and keys that need no way through LDS sooner still where that way is
+// a conversion.  Measured (us, few and many; 8 heads of 128 on as many key-value heads,
+// queries and cache in bf16; f32 queries; bf16 over int8):
+//   1 x 256 of 256 tokens           8.3 11.2    8.7 17.2    8.4 13.3
+//   1 x 417 of 417                  9.9 13.7   10.5 22.8   10.5 17.8
+//   1 x 128 of 4000                26.8 23.3   27.2 35.2   20.9 28.5
+//   1 x 1024 of 1024               27.2 28.8   29.6 38.9   26.0 33.1
+//   8 x 256 of 256                 27.3 11.8   31.9 18.6   27.5 13.8
+bool few_rows(const pk_gpu_kv_cache* c, const Sizes& z, int dtype)
+{
+    const long long each = (long long)z.max_new * (z.heads / c->heads), pairs = (each + 15) / 16 * z.B * c->heads;
+    const bool narrow = dtype != F32 && (c->dtype == F16 || c->dtype == BF16);
+    return each <= 64 || (pairs <= (narrow ? 256 : 512) && pairs * span_of_rows(z) <= (narrow ? 160 << 10 : 512 << 10));
+}
+
+// Chunks of a call of many rows, where its tiles are fewer than the CUs: up to `slots`
+// workgroups, as many as run at a time (the CUs, or two on each), of 512 tokens at least, or
+// 256 where tiles are few.  Measured (us; 32 heads over 8 of 128 in bf16; chunks of 512
+// and of 256 tokens at least):
+//   64 new of 4000 tokens, 16 tiles     24.9 21.5
+//   128 of 1500, 32                     30.1 23.8
+//   512 of 1000, 128                    25.9 38.7
+constexpr int kSplitRows = 128, kSplitKeys = 128;    // the most of a tile
+long long prompt_cuts(long long pairs, long long span, int slots)
 {
     if (pairs >= 256) return 1;
-    const long long n = 512 / pairs, most = span / 512;
+    const long long n = slots / pairs, most = span / (pairs <= 64 ? 256 : 512);
     const long long cut = n < most ? n : most;
     return cut < 1 ? 1 : cut > 64 ? 64 : cut;
 }
@@ -67,7 +87,7 @@ Layout layout_of(const pk_gpu_kv_cache* c, const Sizes& z, int rows, int dtype)
     const int group = z.heads / c->heads;
     const long long each = (long long)z.max_new * group, span = span_of_rows(z);
     Layout l;
-    l.few = few_rows(c, z);
+    l.few = few_rows(c, z, dtype);
     if (l.few) {
         l.pairs = (each + 15) / 16 * z.B * c->heads;
         l.outs = (long long)z.B * z.max_new * z.heads;
@@ -78,38 +98,36 @@ Layout layout_of(const pk_gpu_kv_cache* c, const Sizes& z, int rows, int dtype)
         const long long a = (each + bm - 1) / bm * z.B, b = (long long)rows * group / bm + z.B;
         l.pairs = (a < b ? a : b) * c->heads;
         l.outs = (long long)rows * z.heads;
-        const long long n = prompt_cuts(split_pairs(c, rows, group), span);
-        const long long chunk = ((span + n - 1) / n + kKeys - 1) / kKeys * kKeys;
-        // a tile of rows begins anywhere in its chunk's first 64 tokens
-        l.plan = {(int)chunk, (int)(n == 1 ? 1 : (span + kKeys - 1 + chunk - 1) / chunk)};
+        const long long n = prompt_cuts(split_pairs(c, rows, group), span, 256 * prompt_occupancy(c->dtype, dtype, c->head_dim));
+        const long long chunk = ((span + n - 1) / n + kSplitKeys - 1) / kSplitKeys * kSplitKeys;
+        // a tile of rows begins anywhere in its chunk's first tile of tokens
+        l.plan = {(int)chunk, (int)(n == 1 ? 1 : (span + kSplitKeys - 1 + chunk - 1) / chunk)};
         if (n == 1) l.plan.chunk = 1 << 30;
     }
     return l;
 }
 
-// Floats that any call with these sizes at most takes.  Few rows: see ws_floats_up_to of
-// the one-token attention; above 256 pairs no sequence is split.  Many: chunks fall as
-// the rows' tiles grow, and there is one more than prompt_cuts at most.
+// Floats that any call with these sizes at most takes, few rows or many.  Few: see
+// ws_floats_up_to of the one-token attention; above 256 pairs no sequence is split.
+// Many: chunks fall as the rows' tiles grow, and there is one more than prompt_cuts at most.
 size_t most_floats(const pk_gpu_kv_cache* c, const Sizes& z, int rows)
 {
     const int group = z.heads / c->heads;
     const long long span = span_of_rows(z);
     size_t most = 0;
     for (long long b = 1; b <= z.B && b * c->heads <= 256; ++b)
-        for (long long t = 1; 16 * t <= kFewRows + 15 && t * b * c->heads <= 256; ++t) {
+        for (long long t = 1; t * b * c->heads <= 256; ++t) {
             // the most new tokens of so many tiles
-            long long n = 16 * t / group < kFewRows / group ? 16 * t / group : kFewRows / group;
-            n = n < z.max_new ? n : z.max_new;
+            const long long n = 16 * t / group < z.max_new ? 16 * t / group : z.max_new;
             if (n < 1) continue;
             const size_t cut = cuts(c->dtype, c->head_dim, t * b * c->heads, span);
             if (cut > 1 && b * n * cut > most) most = b * n * cut;
         }
-    if (!few_rows(c, z))
-        for (long long t = 1; t * c->heads < 256; ++t) {
-            const long long n = kSplitRows * t / group < rows ? kSplitRows * t / group : rows;
-            const size_t cut = prompt_cuts(t * c->heads, span);
-            if (n >= 1 && cut > 1 && n * (cut + 1) > most) most = n * (cut + 1);
-        }
+    for (long long t = 1; t * c->heads < 256; ++t) {
+        const long long n = kSplitRows * t / group < rows ? kSplitRows * t / group : rows;
+        const size_t cut = prompt_cuts(t * c->heads, span, 512);
+        if (n >= 1 && cut > 1 && n * (cut + 1) > most) most = n * (cut + 1);
+    }
     return most * z.heads * (c->head_dim + 2);
 }
 
@@ -216,6 +234,7 @@ int pk_gpu_prompt_attention_dev(const pk_gpu_kv_cache* cache, int dtype, const v
     a.splits = p.splits;
     a.rules.cap2 = rules->cap * 1.4426950408889634f;
     a.rules.cap_in = rules->cap > 0.0f ? rules->scale / rules->cap : 0.0f;
+    a.rules.cap_exp = rules->cap > 0.0f ? rules->scale / rules->cap * 2.8853900817779268f : 0.0f;     // 2 log2(e)
     a.rules.slopes = rules->slopes;
     a.rules.first = rules->first;
     a.rules.until = rules->until;
