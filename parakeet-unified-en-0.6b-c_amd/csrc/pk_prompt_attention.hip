@@ -62,7 +62,7 @@ bool few_rows(const pk_gpu_kv_cache* c, const Sizes& z, int dtype)
 //   64 new of 4000 tokens, 16 tiles     24.9 21.5
 //   128 of 1500, 32                     30.1 23.8
 //   512 of 1000, 128                    25.9 38.7
-constexpr int kSplitRows = 128, kSplitKeys = 128;    // the most of a tile
+constexpr int kSplitRows = 128;
 long long prompt_cuts(long long pairs, long long span, int slots)
 {
     if (pairs >= 256) return 1;
@@ -99,9 +99,10 @@ Layout layout_of(const pk_gpu_kv_cache* c, const Sizes& z, int rows, int dtype)
         l.pairs = (a < b ? a : b) * c->heads;
         l.outs = (long long)rows * z.heads;
         const long long n = prompt_cuts(split_pairs(c, rows, group), span, 256 * prompt_occupancy(c->dtype, dtype, c->head_dim));
-        const long long chunk = ((span + n - 1) / n + kSplitKeys - 1) / kSplitKeys * kSplitKeys;
+        const int keys = prompt_keys(c->dtype, dtype, c->head_dim);
+        const long long chunk = ((span + n - 1) / n + keys - 1) / keys * keys;
         // a tile of rows begins anywhere in its chunk's first tile of tokens
-        l.plan = {(int)chunk, (int)(n == 1 ? 1 : (span + kSplitKeys - 1 + chunk - 1) / chunk)};
+        l.plan = {(int)chunk, (int)(n == 1 ? 1 : (span + keys - 1 + chunk - 1) / chunk)};
         if (n == 1) l.plan.chunk = 1 << 30;
     }
     return l;

@@ -75,8 +75,18 @@ class Prompt:
         return got
 
     def half_p(self):
-        many = min(self.max_new, self.n) * (self.heads // self.cache.heads) > 64
-        return mo.half_of_weights(self.cache.kind, self.rows, many and (self.starts is not None))
+        return mo.half_of_weights(self.cache.kind, self.rows, self.many())
+
+    def many(self):
+        """Whether the call takes the kernel of many rows: by the rows of a sequence and key-value head, the
+        16-row tiles of all and the tokens that a tile may see."""
+        new = min(self.max_new, self.n) if self.starts is not None else 1
+        each = new * (self.heads // self.cache.heads)
+        tiles = -(-each // 16) * self.B * self.cache.heads
+        window = self.how["window"] if self.how["window"] < self.max_len else 0
+        span = min(window + new + 30, self.max_len) if window else self.max_len
+        narrow = self.rows != "f32" and self.cache.kind in ("f16", "bf16")
+        return each > 64 and (tiles > (256 if narrow else 512) or tiles * span > (160 << 10 if narrow else 512 << 10))
 
 
 def prompt(rng, kind, rows, kv, group, dim, page, new, lens, max_new=None, max_len=None, tail=0, pad=0, scale=None, seed=1,

@@ -73,12 +73,13 @@ def test_against_plain_form(kind, rows, kv, group, dim, page, new, lens, how):
 
 
 @pytest.mark.parametrize("rows,kind", [("bf16", "bf16"), ("f32", "int8"), ("f16", "f16"), ("bf16", "e2m1")])
-@pytest.mark.parametrize("new,length", [(1, 50), (4, 50), (90, 140)])
-def test_rows_that_see_nothing(rows, kind, new, length):
+@pytest.mark.parametrize("new,length,kv", [(1, 50, 2), (4, 50, 2), (90, 140, 2), (90, 140, 16)])
+def test_rows_that_see_nothing(rows, kind, new, length, kv):
     """Empty ranges in the middle, first past the query, absent pages: zeros, and lse -inf."""
     rng = np.random.default_rng(new)
     first = lambda b, p: np.where(p % 3 == 0, 1 << 30, np.where(p % 3 == 1, -7, p))
-    c = prompt(rng, kind, rows, 2, 2, 128, 16, [new, new, 0, new], [length, length, 9, length], first=first)
+    c = prompt(rng, kind, rows, kv, 2, 128, 16, [new, new, 0, new], [length, length, 9, length], first=first)
+    assert c.many() == (kv == 16)
     c.table_h[1] = -1                                     # nothing of sequence 1
     c.table_h[3, 1:3] = c.cache.pages + 5
     c.table.copy_(do_int(c.table_h))
@@ -119,14 +120,15 @@ def test_starts_lengths_and_counts_out_of_range():
 
 @pytest.mark.parametrize("kind,rows", [("int8", "bf16"), ("e4m3", "f32"), ("bf16", "bf16"), ("f16", "f16"), ("e2m1", "bf16"),
                                        ("e2m1", "f16")])
-@pytest.mark.parametrize("new", [3, 150])
-def test_masked_places_may_hold_anything(kind, rows, new):
+@pytest.mark.parametrize("new,kv", [(3, 2), (150, 2), (150, 16)])
+def test_masked_places_may_hold_anything(kind, rows, new, kv):
     """NaN and infinities wherever no row looks: behind the lengths, before the window, in absent pages' and other
     documents' places."""
     import torch
     rng = np.random.default_rng(new)
     lens = [250, 200]
-    c = prompt(rng, kind, rows, 2, 2, 64, 16, [new, new], lens, window=40, first=lambda b, p: p // 32 * 32, spare=4)
+    c = prompt(rng, kind, rows, kv, 2, 64, 16, [new, new], lens, window=40, first=lambda b, p: p // 32 * 32, spare=4)
+    assert c.many() == (kv == 16)
     c.table_h[0, 10] = -1
     c.table.copy_(do_int(c.table_h))
     want = c.plain()
@@ -166,11 +168,12 @@ def fill(cache, hide):
 
 @pytest.mark.parametrize("kind,rows", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "f32"), ("e2m1", "bf16"), ("e4m3", "bf16"),
                                        ("int8", "f16")])
-@pytest.mark.parametrize("new,length", [(4, 60), (140, 140)])
-def test_a_token_that_only_later_rows_see_may_hold_anything(kind, rows, new, length):
+@pytest.mark.parametrize("new,length,kv", [(4, 60, 2), (140, 140, 2), (140, 140, 32)])
+def test_a_token_that_only_later_rows_see_may_hold_anything(kind, rows, new, length, kv):
     """A NaN or an infinity in a new token's value does not reach the rows before it; it does reach the later ones."""
     rng = np.random.default_rng(5)
-    c = prompt(rng, kind, rows, 2, 2, 64, 16, [new], [length])
+    c = prompt(rng, kind, rows, kv, 2, 64, 16, [new], [length])
+    assert c.many() == (kv == 32)
     at = length - new // 2                                    # the token
     want = c.plain()
     page, off = c.table_h[0, at // 16], at % 16
@@ -181,31 +184,32 @@ def test_a_token_that_only_later_rows_see_may_hold_anything(kind, rows, new, len
     else:
         v[page, 0, off, 3], v[page, 1, off, 5] = float("nan"), -float("inf")
     got = c.run(want)
-    before = np.arange(c.n) < c.n - new // 2
     before = np.arange(c.n) + length - new < at
     tol = want.bound(kind, rows, c.half_p())
     assert np.all(np.abs(got - want.out)[before] <= tol[before])
     if kind in ("e2m1", "int8", "e4m3"):
         assert np.isnan(got[~before]).all()
     else:
-        assert np.isnan(got[~before][:, :2, 3]).all() and np.all(got[~before][:, 2:, 5] == -np.inf)
+        assert np.isnan(got[~before][:, :2, 3]).all() and np.all(got[~before][:, 2:4, 5] == -np.inf)
         rest = np.abs(got - want.out) <= tol
-        rest[:, :2, 3] = rest[:, 2:, 5] = True
+        rest[:, :2, 3] = rest[:, 2:4, 5] = True
         assert rest.all()
 
 
 LARGE = 3.3e38
 
 
-@pytest.mark.parametrize("kind,rows,dim,new,lens", [
-    ("bf16", "bf16", 128, [5], [700]), ("bf16", "f32", 64, [3, 2], [5000, 31]), ("bf16", "bf16", 64, [100], [300]),
-    ("int8", "bf16", 128, [70], [200]), ("e4m3", "f32", 64, [66], [66]), ("bf16", "f32", 256, [40], [90]),
+@pytest.mark.parametrize("kind,rows,dim,kv,new,lens", [
+    ("bf16", "bf16", 128, 1, [5], [700]), ("bf16", "f32", 64, 1, [3, 2], [5000, 31]), ("bf16", "bf16", 64, 1, [100], [300]),
+    ("int8", "bf16", 128, 1, [70], [200]), ("e4m3", "f32", 64, 1, [66], [66]), ("bf16", "f32", 256, 1, [40], [90]),
+    ("bf16", "bf16", 128, 16, [150], [150]), ("int8", "bf16", 64, 32, [140], [200]), ("bf16", "f32", 64, 32, [140], [150]),
 ])
-def test_values_near_the_largest_float(kind, rows, dim, new, lens):
+def test_values_near_the_largest_float(kind, rows, dim, kv, new, lens):
     """Outputs are means of them, so they stay finite (weights 2^-18 off, as in the one-token attention)."""
     import torch
     rng = np.random.default_rng(dim)
-    c = prompt(rng, kind, rows, 1, 2, dim, 16, new, lens)
+    c = prompt(rng, kind, rows, kv, 2, dim, 16, new, lens)
+    assert c.many() == (kv > 1)
     v = c.cache.part("v")
     size = rng.uniform(0.2, 1.0, tuple(v.shape)) * rng.choice([-1.0, 1.0], tuple(v.shape))
     top = do.TOP.get(kind, LARGE)
@@ -220,8 +224,9 @@ def test_values_near_the_largest_float(kind, rows, dim, new, lens):
 def test_large_flat_and_negative_scores():
     rng = np.random.default_rng(8)
     for scale in (20.0, -3.0, 0.0):
-        for new in (3, 200):
-            c = prompt(rng, "bf16", "f32", 1, 2, 64, 16, [new], [300], scale=scale or None)
+        for new, kv, rows in ((3, 1, "f32"), (200, 1, "f32"), (200, 16, "bf16"), (200, 32, "f32")):
+            c = prompt(rng, "bf16", rows, kv, 2, 64, 16, [new], [300], scale=scale or None)
+            assert c.many() == (kv > 1)
             c.rules.scale = c.how["scale"] = scale
             c.check()
 
@@ -229,8 +234,10 @@ def test_large_flat_and_negative_scores():
 def test_caps_small_and_large():
     rng = np.random.default_rng(9)
     for cap in (1e-3, 0.5, 1e4):
-        for rows, new in (("f32", 2), ("f32", 90), ("bf16", 90)):
-            prompt(rng, "bf16", rows, 1, 2, 64, 16, [new], [200], cap=cap, scale=1.0).check()
+        for rows, new, kv in (("f32", 2, 1), ("f32", 90, 1), ("bf16", 90, 1), ("bf16", 90, 32), ("f32", 90, 64)):
+            c = prompt(rng, "bf16", rows, kv, 2, 64, 16, [new], [200], cap=cap, scale=1.0)
+            assert c.many() == (kv > 1)
+            c.check()
 
 
 def test_no_rows_is_no_work():
@@ -248,8 +255,9 @@ def test_two_graphs_and_a_second_stream():
     import torch
     rng = np.random.default_rng(12)
     calls, graphs, streams = [], [], []
-    for i, (new, kind) in enumerate(((4, "int8"), (70, "bf16"), (1, "e2m1"))):
-        c = prompt(rng, kind, "bf16", 2, 2, 64, 16, [new, new], [1500, 800], max_new=new, tail=2, cap=9.0, seed=20 + i)
+    for i, (new, kind, kv) in enumerate(((4, "int8", 2), (70, "bf16", 2), (70, "bf16", 16), (1, "e2m1", 2), (1100, "int8", 2))):
+        c = prompt(rng, kind, "bf16", kv, 2, 64, 16, [new, new], [1500, 1200], max_new=new, tail=2, cap=9.0, seed=20 + i)
+        assert c.many() == (kv == 16 or new == 1100)
         c.table_h[:] = rng.permutation(c.cache.pages)[:c.table_h.size].reshape(c.table_h.shape)
         c.table.copy_(do_int(c.table_h))
         calls.append(c)
@@ -259,7 +267,7 @@ def test_two_graphs_and_a_second_stream():
             c.enqueue(s.cuda_stream)
         graphs.append(g)
         streams.append(s)
-    for lens, part in (([1500, 800], 1.0), ([1500, 1499], 0.5), ([70, 700], 1.0)):
+    for lens, part in (([1500, 1200], 1.0), ([1500, 1499], 0.5), ([70, 700], 1.0)):
         want = []
         for c in calls:
             n = max(1, int(c.max_new * part))
@@ -282,8 +290,9 @@ def test_two_graphs_and_a_second_stream():
 def test_the_same_call_gives_the_same_bits():
     import torch
     rng = np.random.default_rng(3)
-    for new, kind in ((3, "bf16"), (200, "int8")):
+    for new, kind in ((3, "bf16"), (200, "int8"), (200, "bf16")):
         c = prompt(rng, kind, "bf16", 1, 4, 128, 16, [new, new], [5000, 2222], window=4000)
+        assert c.floats > 0
         want = c.plain()
         first = c.run(want)
         for i in range(5):
