@@ -98,8 +98,8 @@ Layout layout_of(const pk_gpu_kv_cache* c, const Sizes& z, int rows, int dtype)
         const long long a = (each + bm - 1) / bm * z.B, b = (long long)rows * group / bm + z.B;
         l.pairs = (a < b ? a : b) * c->heads;
         l.outs = (long long)rows * z.heads;
-        const long long n = prompt_cuts(split_pairs(c, rows, group), span, 256 * prompt_occupancy(c->dtype, dtype, c->head_dim));
-        const int keys = prompt_keys(c->dtype, dtype, c->head_dim);
+        const long long n = prompt_cuts(split_pairs(c, rows, group), span, prompt_slots(c->dtype, dtype, c->head_dim));
+        const int keys = prompt_keys(c->head_dim);
         const long long chunk = ((span + n - 1) / n + keys - 1) / keys * keys;
         // a tile of rows begins anywhere in its chunk's first tile of tokens
         l.plan = {(int)chunk, (int)(n == 1 ? 1 : (span + keys - 1 + chunk - 1) / chunk)};
