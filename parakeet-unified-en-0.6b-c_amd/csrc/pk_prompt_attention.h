@@ -17,8 +17,13 @@ constexpr int prompt_waves(int cache, int t, int dim) { return dim == 256 ? 8 : 
 constexpr int prompt_rows(int cache, int t, int dim) { return prompt_block(dim) * prompt_waves(cache, t, dim); }
 // Tokens of a tile, two stages of which are 64 KB, 128 KB at heads of 256.
 constexpr int prompt_keys(int dim) { return dim == 64 ? 128 : 64; }
-// Waves of a SIMD, and so workgroups that run at a time.
-constexpr int prompt_occupancy(int cache, int t, int dim) { return t == F32 && dim < 256 ? 1 : 2; }
+// Waves of a SIMD, and so workgroups that run at a time.  f32 queries in 3 terms over 16-bit
+// heads of 128 spill at two (4096 tokens of 32 heads 354 us, 366), elsewhere they gain
+// (over int8 404 against 462, heads of 64 357 against 434).
+constexpr int prompt_occupancy(int cache, int t, int dim)
+{
+    return t == F32 && dim == 128 && (cache == F16 || cache == BF16) ? 1 : 2;
+}
 constexpr int prompt_slots(int cache, int t, int dim) { return 256 * 4 * prompt_occupancy(cache, t, dim) / prompt_waves(cache, t, dim); }
 
 template <bool IN_F16>
