@@ -35,6 +35,13 @@ __device__ inline f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c)
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+// Words d ^ turn of x.
+__device__ inline u32x4 turned_words(u32x4 x, int turn)
+{
+    x = turn & 1 ? (u32x4){x[1], x[0], x[3], x[2]} : x;
+    return turn & 2 ? (u32x4){x[2], x[3], x[0], x[1]} : x;
+}
+
 // 16 bytes a lane from base + off to LDS at lds + 16 * lane, past the registers.  The
 // compiler does not see it: whoever reads waits for vmcnt(0) first.
 __device__ inline void cache_to_lds(uint32_t lds, const char* base, uint32_t off)
@@ -270,10 +277,15 @@ __global__ void __launch_bounds__(64 * prompt_waves(CACHE, T, DIM), prompt_occup
                 const int p = threadIdx.x + THREADS * i, row = p / CP;
                 if (LOADS * THREADS > KT * CP && row >= KT) break;
                 if constexpr (CACHE == E2M1) {
+                    // A lane's 4 pieces lie next to each other, so lanes write theirs in orders of
+                    // their own, d ^ turn, that put 16 lanes' into different banks.
+                    const int far = PR == 32 ? p % CP >> 2 : 0;
+                    const int turn_k = 2 * far, turn_v = PR == 32 ? far : row & 3;
+                    const u32x4 xk = turned_words(raw[0][i], turn_k), xv = turned_words(raw[1][i], turn_v);
 #pragma unroll
                     for (int d = 0; d < 4; ++d) {
-                        k[row * PR + slot_k(row, 4 * (p % CP) + d)] = bf16_of_e2m1(raw[0][i][d], unit[0][i]);
-                        v[row * PR + slot_v(row, 4 * (p % CP) + d)] = bf16_of_e2m1(raw[1][i][d], unit[1][i]);
+                        k[row * PR + slot_k(row, 4 * (p % CP) + (d ^ turn_k))] = bf16_of_e2m1(xk[d], unit[0][i]);
+                        v[row * PR + slot_v(row, 4 * (p % CP) + (d ^ turn_v))] = bf16_of_e2m1(xv[d], unit[1][i]);
                     }
                 } else if constexpr (CODED) {
 #pragma unroll
@@ -329,6 +341,15 @@ __global__ void __launch_bounds__(64 * prompt_waves(CACHE, T, DIM), prompt_occup
                 for (int i = QT - 1; i >= 0; --i) s[u] = multiply(keys_type, f, qf[i][c], s[u]);
             }
         }
+        // in this order: reads of keys AHEAD steps before their product (0x100: LDS reads, 8: products)
+        constexpr int AHEAD = QT == 1 ? 8 : 4;
+        __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+        for (int i = 0; i < NU * STEPS - AHEAD; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, QT, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, AHEAD * QT, 0);
         // register i of block u is token R u + 8 (i / 4) + 4 g + i % 4
         float scale = a.scale2;
         if constexpr (CODED) {
@@ -437,6 +458,14 @@ __global__ void __launch_bounds__(64 * prompt_waves(CACHE, T, DIM), prompt_occup
                 for (int x = PT - 1; x >= 0; --x) acc[d] = multiply(values_type, f, pf[x][c], acc[d]);
             }
         }
+        // values, two reads each, 4 products ahead
+        __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+#pragma unroll
+        for (int i = 0; i < NS * DB - 4; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, PT, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 4 * PT, 0);
     };
 
     auto arrived = [] {
