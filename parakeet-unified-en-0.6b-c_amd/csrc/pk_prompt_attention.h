@@ -15,14 +15,16 @@ constexpr int prompt_p_terms(int cache, int t) { return t == F32 ? 3 : t == F16 
 constexpr int prompt_block(int dim) { return dim == 256 ? 16 : 32; }
 constexpr int prompt_waves(int cache, int t, int dim) { return dim == 256 ? 8 : 4; }
 constexpr int prompt_rows(int cache, int t, int dim) { return prompt_block(dim) * prompt_waves(cache, t, dim); }
-// Tokens of a tile, two stages of which are 64 KB, 128 KB at heads of 256.
-constexpr int prompt_keys(int dim) { return dim == 64 ? 128 : 64; }
-// Waves of a SIMD, and so workgroups that run at a time.  f32 queries in 3 terms over 16-bit
-// heads of 128 spill at two (4096 tokens of 32 heads 354 us, 366), elsewhere they gain
-// (over int8 404 against 462, heads of 64 357 against 434).
+// Tokens of a tile: 64, whose two stages take 32 to 128 KB.  4-bit heads of 64 would leave half
+// the threads without a piece to convert (4096 tokens of 64 heads 184 us, of 128 tokens 167).
+constexpr int prompt_keys(int cache, int dim) { return dim == 64 && cache == E2M1 ? 128 : 64; }
+// Waves of a SIMD, and so workgroups that run at a time: as many as the registers take.  f32
+// queries in 3 terms over 16-bit heads of 128 spill at two (4096 tokens of 32 heads 354 us,
+// 366), elsewhere two gain (over int8 404 against 462, heads of 64 357 against 434); heads
+// of 64 leave room for three (bf16 over int8 214 against 236).
 constexpr int prompt_occupancy(int cache, int t, int dim)
 {
-    return t == F32 && dim == 128 && (cache == F16 || cache == BF16) ? 1 : 2;
+    return t == F32 && dim == 128 && (cache == F16 || cache == BF16) ? 1 : dim == 64 && t != F32 && cache != E2M1 ? 3 : 2;
 }
 constexpr int prompt_slots(int cache, int t, int dim) { return 256 * 4 * prompt_occupancy(cache, t, dim) / prompt_waves(cache, t, dim); }
 
@@ -97,7 +99,7 @@ __global__ void __launch_bounds__(64 * prompt_waves(CACHE, T, DIM), prompt_occup
     constexpr int PR = DIM / 8;                // 16-byte pieces of a row in LDS
     constexpr int KS = 512 / R;                // of a matrix instruction's sum
     constexpr int STEPS = DIM / KS, DB = DIM / R;
-    constexpr int KT = prompt_keys(DIM), NU = KT / R, NS = KT / KS, NB = KT / 16;
+    constexpr int KT = prompt_keys(CACHE, DIM), NU = KT / R, NS = KT / KS, NB = KT / 16;
 
     __shared__ u32x4 tiles[2][2][KT * PR];     // [stage][keys, values][row][piece]
     __shared__ float scales[CODED ? 2 : 1][2][KT];

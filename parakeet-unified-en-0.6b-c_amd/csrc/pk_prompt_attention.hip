@@ -62,7 +62,7 @@ bool few_rows(const pk_gpu_kv_cache* c, const Sizes& z, int dtype)
 //   64 new of 4000 tokens, 16 tiles     24.9 21.5
 //   128 of 1500, 32                     30.1 23.8
 //   512 of 1000, 128                    25.9 38.7
-constexpr int kSplitRows = 128;
+constexpr int kSplitRows = 128, kMostSlots = 768;    // of prompt_rows and prompt_slots, whatever the types
 long long prompt_cuts(long long pairs, long long span, int slots)
 {
     if (pairs >= 256) return 1;
@@ -99,7 +99,7 @@ Layout layout_of(const pk_gpu_kv_cache* c, const Sizes& z, int rows, int dtype)
         l.pairs = (a < b ? a : b) * c->heads;
         l.outs = (long long)rows * z.heads;
         const long long n = prompt_cuts(split_pairs(c, rows, group), span, prompt_slots(c->dtype, dtype, c->head_dim));
-        const int keys = prompt_keys(c->head_dim);
+        const int keys = prompt_keys(c->dtype, c->head_dim);
         const long long chunk = ((span + n - 1) / n + keys - 1) / keys * keys;
         // a tile of rows begins anywhere in its chunk's first tile of tokens
         l.plan = {(int)chunk, (int)(n == 1 ? 1 : (span + keys - 1 + chunk - 1) / chunk)};
@@ -126,7 +126,7 @@ size_t most_floats(const pk_gpu_kv_cache* c, const Sizes& z, int rows)
         }
     for (long long t = 1; t * c->heads < 256; ++t) {
         const long long n = kSplitRows * t / group < rows ? kSplitRows * t / group : rows;
-        const size_t cut = prompt_cuts(t * c->heads, span, 512);
+        const size_t cut = prompt_cuts(t * c->heads, span, kMostSlots);
         if (n >= 1 && cut > 1 && n * (cut + 1) > most) most = n * (cut + 1);
     }
     return most * z.heads * (c->head_dim + 2);

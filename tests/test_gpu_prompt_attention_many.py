@@ -89,11 +89,11 @@ def splits(c):
 
 SPLIT = [
     # kind, rows, kv, group, dim, new, lens, rules, chunks
-    ("bf16", "bf16", 2, 4, 128, [200], [2600], {}, 9), ("int8", "bf16", 4, 4, 64, [300, 20], [3000, 1800], {}, 9),
+    ("bf16", "bf16", 2, 4, 128, [200], [2600], {}, 9), ("int8", "bf16", 4, 4, 64, [300, 20], [3000, 1800], {}, 10),
     ("e2m1", "f32", 2, 3, 64, [400], [8000], dict(window=4000), 12),
     ("bf16", "bf16", 1, 2, 256, [500, 100, 0], [3100, 2000, 5], {}, 10),
     ("f16", "f16", 3, 3, 128, [230], [1500], dict(docs=700, prefix=300), 5),
-    ("bf16", "f32", 1, 8, 64, [260], [5000], dict(cap=4.0), 14),
+    ("bf16", "f32", 1, 8, 64, [260], [5000], dict(cap=4.0), 16),
 ]
 
 
