@@ -3,11 +3,12 @@
 //
 //   a' = (a cos t - b sin t) scale,   b' = (b cos t + a sin t) scale,   t = p freq_i
 //
-// A workgroup takes up to 4 tokens and a slice of their heads.  It forms cos and sin of
-// its tokens' angles once, one angle a thread, into LDS (fp64 for the product and the
-// reduction, so that far positions keep their bits); a thread then keeps those of its
-// elements in registers over all heads.  Bound by the rows' bytes, each read and
-// written once.
+// A workgroup takes up to 4 tokens.  It forms cos and sin of their angles once, one angle a
+// thread, into LDS (fp64 for the product and the reduction, so that far positions keep
+// their bits); a thread then keeps those of its elements in registers over all heads.
+// Bound by the rows' bytes, each read and written once: 8191 tokens of 32 + 8 + 8 heads
+// of 128 in bf16, keys and values into int8 codes, 33 us, 4.8 TB/s; 4001 rows of 16 heads
+// of 64 in f32 8.6, 3.8.
 #include "pk_kv_rows.h"
 
 #include <cmath>
@@ -26,7 +27,6 @@ struct RopeArgs {
     int rot, interleaved;
     const int* pos;
     int n, tokens;                  // all, and of a workgroup
-    int slices;                     // of the heads
     const char* x;                  // rows that are turned
     char* y;
     size_t ldx, ldy;                // elements
@@ -71,12 +71,12 @@ __device__ inline void make_turns(const RopeArgs& a, int token0, int tokens, Tur
     __syncthreads();
 }
 
-// Heads [h0, h1) of the workgroup's rows.  A thread has one place of a head (8 pairs of
+// The heads of the workgroup's rows.  A thread has one place of a head (8 pairs of
 // the half layout, 4 of the interleaved one, 8 elements that stay; one pair or element
 // where rows are not wide) and goes over tokens and heads; it reads both elements of its
 // pairs before it writes them, so rows may be turned in place.
 template <int T>
-__device__ inline void turn_rows(const RopeArgs& a, int token0, int tokens, int h0, int h1, const Turn* turns)
+__device__ inline void turn_rows(const RopeArgs& a, int token0, int tokens, const Turn* turns)
 {
     constexpr int S = size_of(T);
     const int half = a.rot / 2, per = a.wide ? 8 : 1;
@@ -97,7 +97,7 @@ __device__ inline void turn_rows(const RopeArgs& a, int token0, int tokens, int 
             const Turn* const of = turns + t * half;
             if (!a.wide) {
                 const Turn w = turns_here ? of[u] : Turn{1.0f, 0.0f};
-                for (int h = h0 + head0; h < h1; h += step) {
+                for (int h = head0; h < a.heads; h += step) {
                     const size_t at = (size_t)h * a.dim;
                     const float p = load1<T>(x, at + e);
                     if (!turns_here) {
@@ -116,7 +116,7 @@ __device__ inline void turn_rows(const RopeArgs& a, int token0, int tokens, int 
                 for (int i = 0; i < 8; ++i)
                     w[i] = a.interleaved ? of[e / 2 + i / 2] : of[e + i];
             }
-            for (int h = h0 + head0; h < h1; h += step) {
+            for (int h = head0; h < a.heads; h += step) {
                 const size_t at = (size_t)h * a.dim;
                 float p[8];
                 load8<T>(x + (at + e) * S, p);
@@ -144,18 +144,12 @@ __device__ inline void turn_rows(const RopeArgs& a, int token0, int tokens, int 
     }
 }
 
-// What a workgroup does: token0.. and the heads of its slice.
-struct Part { int token0, tokens, slice; };
+struct Part { int token0, tokens; };
 __device__ inline Part part_of(const RopeArgs& a)
 {
-    Part p;
-    const uint32_t tile = blockIdx.x / (uint32_t)a.slices;
-    p.slice = blockIdx.x - tile * a.slices;
-    p.token0 = tile * a.tokens;
-    p.tokens = min(a.tokens, a.n - p.token0);
-    return p;
+    const int token0 = blockIdx.x * a.tokens;
+    return {token0, min(a.tokens, a.n - token0)};
 }
-__device__ inline int share(int heads, int slice, int slices) { return (int)((long long)heads * slice / slices); }
 
 template <int T>
 __global__ void __launch_bounds__(kThreads) rope_rows(RopeArgs a)
@@ -163,7 +157,7 @@ __global__ void __launch_bounds__(kThreads) rope_rows(RopeArgs a)
     extern __shared__ Turn turns[];
     const Part p = part_of(a);
     make_turns(a, p.token0, p.tokens, turns);
-    turn_rows<T>(a, p.token0, p.tokens, share(a.heads, p.slice, a.slices), share(a.heads, p.slice + 1, a.slices), turns);
+    turn_rows<T>(a, p.token0, p.tokens, turns);
 }
 
 // Keys and values as pk_kv_cache.hip writes them, 8 elements of a row a lane; a lane
@@ -175,10 +169,9 @@ __global__ void __launch_bounds__(kThreads) rope_kv_write(RopeArgs a)
     extern __shared__ Turn turns[];
     const Part w = part_of(a);
     make_turns(a, w.token0, w.tokens, turns);
-    const int h0 = share(a.kv_heads, w.slice, a.slices), heads = share(a.kv_heads, w.slice + 1, a.slices) - h0;
     const int part = threadIdx.x % LANES, half = a.rot / 2, e0 = 8 * part;
-    for (int r = threadIdx.x / LANES; r < heads * w.tokens; r += ROWS) {      // whole lane groups leave together
-        const int t = r / heads, head = h0 + r - t * heads, token = w.token0 + t;
+    for (int r = threadIdx.x / LANES; r < a.kv_heads * w.tokens; r += ROWS) {      // whole lane groups leave together
+        const int t = r / a.kv_heads, head = r - t * a.kv_heads, token = w.token0 + t;
         const long long row = cache_row(a.slots[token], head, a.kv_heads, a.page_shift, a.n_slots);
         const size_t at = (size_t)head * DIM;
         const char* const xk = a.rk + (size_t)token * a.ldk * S;
@@ -216,23 +209,18 @@ __global__ void __launch_bounds__(kThreads) rope_kv_write(RopeArgs a)
         write_part<CACHE, DIM>(a.k, a.k_scale, row, part, k);
         write_part<CACHE, DIM>(a.v, a.v_scale, row, part, v);
     }
-    if (a.heads)
-        turn_rows<T>(a, w.token0, w.tokens, share(a.heads, w.slice, a.slices), share(a.heads, w.slice + 1, a.slices), turns);
+    if (a.heads) turn_rows<T>(a, w.token0, w.tokens, turns);
 }
 
 struct Launch { long long workgroups; size_t lds; };
-// 4 tokens a workgroup where that leaves 512 workgroups or more (an angle a thread at
-// 128 turning elements), else one, and the heads over up to 8 workgroups until there
-// are as many.
-Launch launch_of(RopeArgs* a, int heads)
+// 4 tokens a workgroup from 416 such workgroups on, else one: an angle a thread at 128
+// turning elements, and less of it to wait for before rows move.  Measured (us, 4 and
+// one; 32 + 8 + 8 heads of 128 in bf16 and into bf16):
+//   1500 tokens  12.6 11.6      1800  13.1 13.6      8191  43.6 62.4
+Launch launch_of(RopeArgs* a)
 {
-    a->tokens = a->n >= 512 * kTokens ? kTokens : 1;
-    const long long tiles = ((long long)a->n + a->tokens - 1) / a->tokens;
-    long long s = tiles ? 512 / tiles : 1;
-    s = s > 8 ? 8 : s;
-    s = s > heads ? heads : s;
-    a->slices = s < 1 ? 1 : (int)s;
-    return {tiles * a->slices, (size_t)a->tokens * (a->rot / 2) * sizeof(Turn)};
+    a->tokens = a->n >= 416 * kTokens ? kTokens : 1;
+    return {((long long)a->n + a->tokens - 1) / a->tokens, (size_t)a->tokens * (a->rot / 2) * sizeof(Turn)};
 }
 
 int check_rope(const pk_gpu_rope* r, const char* who, int dtype, int heads, int dim, int n)
@@ -348,7 +336,7 @@ int pk_gpu_rope_dev(const pk_gpu_rope* rope, int dtype, const void* dx, int ldx,
         return rt::error(PK_GPU_EINVAL, "%s: in place with ldx = %d, ldy = %d", who, ldx, ldy);
     RopeArgs a = rope_args(rope, dpos, n, dx, ldx, heads, head_dim, dy, ldy);
     a.wide = wide_rows(a, es);
-    const Launch l = launch_of(&a, heads);
+    const Launch l = launch_of(&a);
     if (!launchable(l.workgroups, kThreads)) return rt::error(PK_GPU_EINVAL, "%s: %d rows exceed the grid", who, n);
     OnDevice on;
     if (on.rc) return on.rc;
@@ -401,7 +389,7 @@ int pk_gpu_rope_kv_write_dev(const pk_gpu_rope* rope, const pk_gpu_kv_cache* cac
     a.kv_heads = cache->heads;
     a.page_shift = __builtin_ctz(cache->page_size);
     a.n_slots = cache->n_pages * cache->page_size;
-    const Launch l = launch_of(&a, heads > cache->heads ? heads : cache->heads);
+    const Launch l = launch_of(&a);
     if (!launchable(l.workgroups, kThreads)) return rt::error(PK_GPU_EINVAL, "%s: %d tokens exceed the grid", who, n);
     OnDevice on;
     if (on.rc) return on.rc;
