@@ -119,8 +119,13 @@ __device__ __host__ inline Span span_of(int len, int max_len, int window, int ch
 // busy by themselves; which sequences are split all the same, cuts() says.  The
 // kernels with most registers (heads of 256, queries in 3 terms) run one wave a
 // SIMD: 64 sequences of 2000 tokens, 2 heads of 256 in int8, f32 queries 34.8 us;
-// 8 waves, which spill, 44.
-constexpr int waves_of(int cache, int t, int dim) { return t == F32 && dim == 256 ? 4 : 8; }
+// 8 waves, which spill, 44.  With rules so do 16-bit heads of 256: 16 sequences of 4000
+// tokens, 16 heads over 4, 57.3 us; 8 waves 74.2 (codes do not: in int8 31.7 and 30.1 over
+// 50000 tokens of one).
+constexpr int waves_of(int cache, int t, int dim, bool rules)
+{
+    return dim == 256 && (t == F32 || (rules && (cache == F16 || cache == BF16))) ? 4 : 8;
+}
 
 // The sequence with nth sequences before it in order of falling length (ties
 // by index), counted by every workgroup for itself: lens of the launch's up to
@@ -242,9 +247,9 @@ __device__ inline void split_pair(float x, float y, uint32_t* t)
 }
 
 template <int CACHE, int T, int DIM, bool RULES>
-__global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM), waves_of(CACHE, T, DIM) / 4) paged_attention(PagedArgs a)
+__global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM, RULES), waves_of(CACHE, T, DIM, RULES) / 4) paged_attention(PagedArgs a)
 {
-    constexpr int NW = waves_of(CACHE, T, DIM);
+    constexpr int NW = waves_of(CACHE, T, DIM, RULES);
     constexpr int S = size_of(CACHE);
     constexpr int RB = bytes_of(CACHE, DIM);   // bytes of a row
     constexpr bool CODED = row_scaled(CACHE), FOUR = CACHE == E2M1;
@@ -781,7 +786,7 @@ Plan plan_of(int cache, int dim, long long pairs, long long span);
 template <int CACHE, int T, bool RULES>
 hipError_t launch_paged_as(int dim, const PagedArgs& a, dim3 grid, hipStream_t s)
 {
-    const dim3 block(64 * waves_of(CACHE, T, dim));
+    const dim3 block(64 * waves_of(CACHE, T, dim, RULES));
     return dim == 64    ? launch(paged_attention<CACHE, T, 64, RULES>, grid, block, 0, s, a)
            : dim == 128 ? launch(paged_attention<CACHE, T, 128, RULES>, grid, block, 0, s, a)
                         : launch(paged_attention<CACHE, T, 256, RULES>, grid, block, 0, s, a);
