@@ -38,11 +38,21 @@ int check_sizes(const pk_gpu_kv_cache* c, const Sizes& z)
 // Calls of few rows, (new token, head) pairs of a key-value head, go 16 a workgroup over
 // the tiles of the one-token attention, the others prompt_rows a workgroup.
 //
-// Up to 64 rows the cache's bytes are what counts, and those tiles fetch them faster.  Beyond,
-// they do while there are as many CUs as workgroups and these are short: 16 rows start
-// sooner than 128, and keys that need no way through LDS sooner still where that way is
-// a conversion.  Measured (us, few and many; 8 heads of 128 on as many key-value heads,
-// queries and cache in bf16; f32 queries; bf16 over int8):
+// 16 rows, or fewer, read the cache once that way, and faster.  Where sequences have more, each
+// 16 of them read it again, if from L2: up to 32 that still is less than what 128 rows
+// lose while there are not two workgroups of these for a CU, up to 48 where keys need a
+// conversion or 3 terms.  Measured (us, few and many; 32 heads over 8 of 128, queries and
+// cache in bf16; f32 queries; bf16 over 4 bits):
+//   16 x 4 of 4000                 56.2 -       58.1 -       23.0 -
+//   16 x 8 of 4000                 65.3 77.0    68.0 106     28.4 52.3
+//   16 x 12 of 4000                94.0 78.8    98.3 116     42.3 58.5
+//   64 x 8 of 1000                 90.4 52.2    95.4 88.7    30.8 28.4
+//   64 x 12 of 1000                126  53.8    134  91.0    42.9 33.7
+//
+// Of more rows still go that way the calls of at most as many such workgroups as CUs, if
+// short: 16 rows start sooner than 128, and keys that need no way through LDS sooner still
+// where that way is a conversion.  Measured (the same; 8 heads of 128 on as many key-value
+// heads; the third column bf16 over int8):
 //   1 x 256 of 256 tokens           8.3 11.2    8.7 17.2    8.4 13.3
 //   1 x 417 of 417                  9.9 13.7   10.5 22.8   10.5 17.8
 //   1 x 128 of 4000                26.8 23.3   27.2 35.2   20.9 28.5
@@ -52,7 +62,8 @@ bool few_rows(const pk_gpu_kv_cache* c, const Sizes& z, int dtype)
 {
     const long long each = (long long)z.max_new * (z.heads / c->heads), pairs = (each + 15) / 16 * z.B * c->heads;
     const bool narrow = dtype != F32 && (c->dtype == F16 || c->dtype == BF16);
-    return each <= 64 || (pairs <= (narrow ? 256 : 512) && pairs * span_of_rows(z) <= (narrow ? 160 << 10 : 512 << 10));
+    return each <= 16 || (each <= (dtype == F32 || c->dtype == E2M1 ? 48 : 32) && (long long)z.B * c->heads < 512) ||
+           (pairs <= (narrow ? 256 : 512) && pairs * span_of_rows(z) <= (narrow ? 160 << 10 : 512 << 10));
 }
 
 // Chunks of a call of many rows, where its tiles are fewer than the CUs: up to `slots`

@@ -86,7 +86,10 @@ class Prompt:
         window = self.how["window"] if self.how["window"] < self.max_len else 0
         span = min(window + new + 30, self.max_len) if window else self.max_len
         narrow = self.rows != "f32" and self.cache.kind in ("f16", "bf16")
-        return each > 64 and (tiles > (256 if narrow else 512) or tiles * span > (160 << 10 if narrow else 512 << 10))
+        two_tiles = 48 if self.rows == "f32" or self.cache.kind == "e2m1" else 32
+        few = (each <= 16 or (each <= two_tiles and self.B * self.cache.heads < 512) or
+               (tiles <= (256 if narrow else 512) and tiles * span <= (160 << 10 if narrow else 512 << 10)))
+        return not few
 
 
 def prompt(rng, kind, rows, kv, group, dim, page, new, lens, max_new=None, max_len=None, tail=0, pad=0, scale=None, seed=1,
