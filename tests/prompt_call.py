@@ -78,18 +78,24 @@ class Prompt:
         return mo.half_of_weights(self.cache.kind, self.rows, self.many())
 
     def many(self):
-        """Whether the call takes the kernel of many rows: by the rows of a sequence and key-value head, the
-        16-row tiles of all and the tokens that a tile may see."""
+        """Whether the call takes the kernel of many rows."""
         new = min(self.max_new, self.n) if self.starts is not None else 1
-        each = new * (self.heads // self.cache.heads)
-        tiles = -(-each // 16) * self.B * self.cache.heads
-        window = self.how["window"] if self.how["window"] < self.max_len else 0
-        span = min(window + new + 30, self.max_len) if window else self.max_len
-        narrow = self.rows != "f32" and self.cache.kind in ("f16", "bf16")
-        two_tiles = 48 if self.rows == "f32" or self.cache.kind == "e2m1" else 32
-        few = (each <= 16 or (each <= two_tiles and self.B * self.cache.heads < 512) or
-               (tiles <= (256 if narrow else 512) and tiles * span <= (160 << 10 if narrow else 512 << 10)))
-        return not few
+        return many_rows(self.cache.kind, self.rows, self.cache.heads, self.heads // self.cache.heads, self.B, new, self.max_len,
+                         self.how["window"])
+
+
+def many_rows(kind, rows, kv, group, B, new, max_len, window):
+    """The rule: by the rows of a sequence and key-value head, the 16-row tiles of all and the tokens that a
+    tile may see."""
+    each = new * group
+    tiles = -(-each // 16) * B * kv
+    window = window if window < max_len else 0
+    span = min(window + new + 30, max_len) if window else max_len
+    narrow = rows != "f32" and kind in ("f16", "bf16")
+    two_tiles = 48 if rows == "f32" or kind == "e2m1" else 32
+    few = (each <= 16 or (each <= two_tiles and B * kv < 512) or
+           (tiles <= (256 if narrow else 512) and tiles * span <= (160 << 10 if narrow else 512 << 10)))
+    return not few
 
 
 def prompt(rng, kind, rows, kv, group, dim, page, new, lens, max_new=None, max_len=None, tail=0, pad=0, scale=None, seed=1,
