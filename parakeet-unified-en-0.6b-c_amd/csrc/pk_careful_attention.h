@@ -17,6 +17,7 @@ struct RuleArgs {
     const int* starts;           // [B + 1], or NULL: row b is sequence b's
     int rows, max_new;
     int by_row;                  // the workspace's rows are q's, not (sequence, new token)s
+    int per_seq;                 // row tiles of every sequence, 0: by its rows
 };
 
 // Sequence b's new tokens: rows row .. row + count - 1, whatever `starts` holds.

@@ -1,5 +1,41 @@
 // pk_prompt_attention.h - attention of many new tokens per sequence over a paged
 // key-value cache: the kernel, instantiated per cache type by pk_prompt_attention_*.hip.
+//
+// For each row, a (new token, query head) pair, over the tokens [lo, hi) that it sees,
+//   s_t = cap tanh(scale q.k_t / cap) - slope |p - t|,  o = sum_t e^(s_t) v_t / sum_t e^(s_t)
+// in one pass: a running maximum m, l = sum 2^(s - m) and acc = sum 2^(s - m) v, with s in
+// powers of two.  m moves, and acc and l are scaled, only once a score is 8 above it, which
+// most tiles of tokens spare; weights stay below 2^8 (times 2^BIAS over f16 values).
+//
+// A workgroup holds prompt_rows rows of one key-value head, the rows of its query heads
+// next to each other, so a group's heads share what it stages: tiles of prompt_keys
+// tokens, keys and values, in 16 bits, two stages in LDS.  16-bit caches go there past the
+// registers, codes through a conversion; a tile's loads are out while the one before is
+// multiplied.  Row scales of 8-bit codes are taken on scores and weights.
+//   S^T = K Q^T: a lane gets scores of one row, so the row's statistics are its registers'
+//     but for one or three exchanges, and its scores are, in order, the second operand of
+//   O^T = V^T P^T: weights go from register to register, never through LDS.  V^T comes from
+//     LDS by transposing reads.
+// Pieces of 16 bytes are XORed with their row, such that the 16 lanes that read at a time
+// meet all banks.
+//
+// Roundings.  The first product is exact but for fp32 sums: codes and 16-bit elements are
+// held as they are, f32 queries in 3 bf16 terms (24 bits), f16 queries over codes in 2 (they
+// have 11 bits).  Weights are rounded for the second product: into one term for bf16 queries
+// (8 bits) and for f16 over f16 (11, scaled by 2^7 so that weights above 2^-21 are normal
+// numbers), as the output is itself: each weight is off by half a step relative to it, the
+// output by no more than sqrt(2) of its own rounding where errors are independent, two
+// at the worst; l sums the unrounded.  f16 queries over codes take 2 terms (16 bits), f32 3.
+// One term where 2 or 3 are taken elsewhere is what the product's time is: 4096 tokens of
+// 32 heads of 128 take 135 us in one, 352 with f32's 3 by 3.
+//
+// What bounds it: 8192 tokens of 32 heads over 8 of 128 in bf16 take 504 us, 1090 of the
+// 1267 TFLOP/s that a product of two 8192 x 8192 matrices reaches here; both are held by the
+// clock, which matrix instructions bring down to some 1.8 GHz.  Blocks of 32x32 halve the
+// reads of LDS for a row against 16x16; heads of 256 do not leave the registers for them.
+// Heads of 64 do half the products per score, so the exponentials and their like count as much
+// as they: 842 TFLOP/s.  4 bits under a cap (2 more transcendental instructions a score) is the
+// vector unit's: 16000 tokens of 16 heads of 256 behind 24000 others, window 1024, 209 us.
 #pragma once
 
 #include "pk_paged_attention.h"
@@ -53,36 +89,60 @@ __device__ inline void cache_to_lds(uint32_t lds, const char* base, uint32_t off
                      "global_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
 
-// The sequence and row tile of the launch's tau-th row tile: tiles of BM rows, sequence by
-// sequence, the last tiles (whose rows see most) first.  False behind the last.
+// The sequence and row tile of the launch's tau-th row tile, false where there is none: tiles of BM
+// rows, sequence by sequence, so that workgroups that run together read the same tokens, a
+// sequence's last ones (whose rows see most) first.  Either every sequence has per_seq of them, or
+// as many as its rows take: for up to 64 sequences a sum over the lanes; beyond, sequence b has
+// those from floor(S_b / BM) + b on, with S_b the rows before it, which is never fewer than they
+// take and can be searched 64 sequences at a time.  Measured (us): 4000 sequences of up to 100
+// rows 233 searched, 577 summed; 8 of up to 2000, where a workgroup without rows may
+// cost another round, 209 summed and 207 to 223 searched.
 struct RowTile { int b, tile; };
 template <int BM>
-__device__ inline bool row_tile(const PagedArgs& a, int tau, RowTile* out)
+__device__ inline bool row_tile(const PagedArgs& a, uint32_t tau, RowTile* out)
 {
     const int lane = threadIdx.x & 63;
-    for (int b0 = 0; b0 < a.B; b0 += 64) {
-        const int b = b0 + lane;
-        int n = b < a.B ? (int)(((long long)new_tokens(a.rules, b).count * a.group + BM - 1) / BM) : 0;
-        int upto = n;
-        if (a.B > 1) {
+    auto tiles_of = [&](int b) { return (int)(((long long)new_tokens(a.rules, b).count * a.group + BM - 1) / BM); };
+    uint32_t nth;
+    if (a.rules.per_seq) {
+        out->b = tau / (uint32_t)a.rules.per_seq;
+        nth = tau - (uint32_t)out->b * a.rules.per_seq;
+    } else if (a.B <= 64) {
+        const int mine = lane < a.B ? tiles_of(lane) : 0;
+        uint32_t upto = mine;
 #pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const int o = __shfl_up(upto, d);
-                upto += lane >= d ? o : 0;
-            }
-        } else {
-            upto = __builtin_amdgcn_readfirstlane(n);
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t o = __shfl_up(upto, d);
+            upto += lane >= d ? o : 0;
         }
-        const unsigned long long mine = __ballot(upto > tau);
-        if (mine) {
-            const int l = __builtin_ctzll(mine);
-            out->b = b0 + l;
-            out->tile = __builtin_amdgcn_readlane(upto, l) - 1 - tau;
-            return true;
-        }
-        tau -= __builtin_amdgcn_readlane(upto, 63);
+        const unsigned long long behind = __ballot(upto > tau);
+        if (!behind) return false;
+        out->b = __builtin_ctzll(behind);
+        out->tile = __builtin_amdgcn_readlane((int)upto, out->b) - 1 - (int)tau;
+        return true;
+    } else {
+        auto tiles_before = [&](int b) {
+            const int s = a.rules.starts ? min(max(a.rules.starts[b], 0), a.rules.rows) : min(b, a.rules.rows);
+            return (uint32_t)((unsigned long long)s * (uint32_t)a.group / BM) + (uint32_t)b;
+        };
+        int lo = 0, n = a.B;
+        uint32_t before;
+        do {
+            const int step = (n + 63) / 64, at = lane * step;
+            const uint32_t t = at < n ? tiles_before(lo + at) : 0xffffffffu;
+            const unsigned long long upto = __ballot(t <= tau);
+            if (!upto) return false;
+            const int l = 63 - __builtin_clzll(upto);
+            before = __builtin_amdgcn_readlane((int)t, l);
+            lo += l * step;
+            n = min(step, n - l * step);
+        } while (n > 1);
+        out->b = lo;
+        nth = tau - before;
     }
-    return false;
+    const int n = tiles_of(out->b);
+    out->tile = n - 1 - (int)nth;
+    return nth < (uint32_t)n;
 }
 
 template <int CACHE, int T, int DIM>
@@ -115,14 +175,14 @@ __global__ void __launch_bounds__(64 * prompt_waves(CACHE, T, DIM), prompt_occup
     const int kvh = in_split % (uint32_t)a.kv_heads;
     RowTile rt;
     if (!row_tile<BM>(a, in_split / (uint32_t)a.kv_heads, &rt)) return;
-    const int b = __builtin_amdgcn_readfirstlane(rt.b);
+    const int b = rt.b;
     const NewTokens news = new_tokens(a.rules, b);
     const int* const pages = a.pages + (size_t)b * a.ld_pages;
     const int len = min(max(a.lens[b], 0), a.max_len);
     const int heads = a.kv_heads * a.group;
 
     // this lane's row
-    const uint32_t r = (uint32_t)__builtin_amdgcn_readfirstlane(rt.tile) * BM + wave * R + n;
+    const uint32_t r = (uint32_t)rt.tile * BM + wave * R + n;
     const int nth = r / (uint32_t)a.group;
     const bool ok = nth < news.count;
     const int head = kvh * a.group + (int)(r - (uint32_t)nth * a.group);

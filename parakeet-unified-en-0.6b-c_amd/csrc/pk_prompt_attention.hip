@@ -90,6 +90,7 @@ long long split_pairs(const pk_gpu_kv_cache* c, long long rows, int group)
 // How a call is laid out: workgroups of one chunk, chunks, rows of the workspace.
 struct Layout {
     bool few;
+    int per_seq;
     long long pairs, outs;
     Plan plan;
 };
@@ -97,7 +98,7 @@ Layout layout_of(const pk_gpu_kv_cache* c, const Sizes& z, int rows, int dtype)
 {
     const int group = z.heads / c->heads;
     const long long each = (long long)z.max_new * group, span = span_of_rows(z);
-    Layout l;
+    Layout l{};
     l.few = few_rows(c, z, dtype);
     if (l.few) {
         l.pairs = (each + 15) / 16 * z.B * c->heads;
@@ -106,8 +107,9 @@ Layout layout_of(const pk_gpu_kv_cache* c, const Sizes& z, int rows, int dtype)
     } else {
         const int bm = prompt_rows(c->dtype, dtype, c->head_dim);
         // tiles of every sequence, or of all rows with one that is not whole for each sequence
-        const long long a = (each + bm - 1) / bm * z.B, b = (long long)rows * group / bm + z.B;
-        l.pairs = (a < b ? a : b) * c->heads;
+        const long long per = (each + bm - 1) / bm, all = (long long)rows * group / bm + z.B;
+        l.per_seq = per * z.B <= all ? (int)per : 0;
+        l.pairs = (l.per_seq ? per * z.B : all) * c->heads;
         l.outs = (long long)rows * z.heads;
         const long long n = prompt_cuts(split_pairs(c, rows, group), span, prompt_slots(c->dtype, dtype, c->head_dim));
         const int keys = prompt_keys(c->dtype, c->head_dim);
@@ -254,6 +256,7 @@ int pk_gpu_prompt_attention_dev(const pk_gpu_kv_cache* cache, int dtype, const v
     a.rules.rows = rows;
     a.rules.max_new = z.max_new;
     a.rules.by_row = !l.few;
+    a.rules.per_seq = l.per_seq;
     const hipError_t e = l.few ? launch_attention(cache->dtype, dtype, cache->head_dim, true, a, (uint32_t)(l.pairs * p.splits),
                                                   (uint32_t)l.outs, static_cast<hipStream_t>(stream))
                                : launch_prompts(cache->dtype, dtype, cache->head_dim, a, (uint32_t)(l.pairs * p.splits),

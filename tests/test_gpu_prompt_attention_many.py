@@ -145,3 +145,30 @@ def test_a_cache_past_4_gib():
     want = mo.Ruled(held, do.values(q).reshape(n, heads, dim), np.arange(n)[None], [n], [0, n], n, n, 0.0625)
     err = np.abs(do.values(out).reshape(n, heads, dim) - want.out)
     assert np.all(err <= want.bound("bf16", "bf16", 2.0 ** -8))
+
+
+@pytest.mark.parametrize("B,most,kv,group,max_new,shift", [(64, 25, 3, 3, 60, 3), (65, 25, 3, 3, 60, 0), (150, 40, 2, 4, 60, 3),
+                                                          (300, 9, 2, 2, 250, 0), (4200, 3, 1, 1, 130, 2), (4099, 2, 1, 1, 400, 0)])
+def test_many_sequences(B, most, kv, group, max_new, shift):
+    """As many row tiles as a sequence has rows, found among up to 64 sequences and among more; a bound on them
+    that is not close, sequences without new tokens, and rows before the first sequence's."""
+    import torch
+    rng = np.random.default_rng(B)
+    new = rng.integers(0, most + 1, B)
+    new[::7], new[B // 2] = 0, most
+    lens = new + rng.integers(0, 20, B)
+    c = prompt(rng, "bf16", "bf16", kv, group, 64, 16, new.tolist(), lens.tolist(), max_new=max_new, tail=shift + 2,
+               max_len=max_new + 20)
+    c.starts_h = (c.starts_h + shift).astype(np.int32)
+    c.starts.copy_(torch.from_numpy(c.starts_h))
+    assert c.many()
+    c.check()
+
+
+def test_single_tokens_of_many_heads():
+    """No starts: row b is sequence b's, 17 query heads to a key-value head."""
+    rng = np.random.default_rng(17)
+    c = prompt(rng, "int8", "bf16", 1, 17, 64, 16, [1] * 520, rng.integers(1, 60, 520).tolist())
+    c.starts = c.starts_h = None
+    assert c.many()
+    c.check()
