@@ -516,8 +516,9 @@ int pk_gpu_paged_attention_dev(const pk_gpu_kv_cache *cache, int dtype, const vo
 
 /* What pk_gpu_prompt_attention_dev does to scores, and what a new token sees.  All zero
  * but the scale: softmax of scale * q . k_t over the tokens up to the new one itself.
- *   scale   any finite number
- *   cap     > 0: a score s becomes cap * tanh(s / cap); 0: stays
+ *   scale   of a magnitude up to 2^120
+ *   cap     > 0: a score s becomes cap * tanh(s / cap), to 2^-21 of the cap (f32 queries: of its
+ *           value); 0: stays.  cap and |scale| / cap up to 2^120
  *   slopes  NULL, or [query heads]: slopes[h] * |p - t| is taken off the score of the query
  *           at position p and the key at position t, behind the cap
  *   window  > 0: tokens up to p - window are not seen; 0: no such limit
@@ -547,9 +548,11 @@ typedef struct {
  * pk_gpu_paged_attention_dev, whose notes on absent pages, on what tokens that take no part may
  * hold (of a token that some rows see and others do not: for those others too) and on
  * |q| hold here too.
- * Scores, sums and the softmax are fp32; its weights enter the second product with 16 or
- * 24 bits or more as there, where up to 16 (new token, query head) pairs share a key-value
- * head.  Results do not depend on timing.
+ * Scores, sums and the softmax are fp32.  Where a sequence has few (new token, query head)
+ * pairs for a key-value head (16, or somewhat more in short or small calls), weights enter the
+ * second product as there.  Where it has many they keep what the output keeps: 8 bits for BF16,
+ * 11 for F16 over F16 caches (16 over codes), 24 for F32.  Results do not depend on timing, and
+ * of the call's sizes, not of its lengths, is which of the two is taken.
  * dws as there, of at least pk_gpu_prompt_attention_ws_floats floats: what is enough for
  * B, rows, max_new, max_len and window is enough for less of each. */
 size_t pk_gpu_prompt_attention_ws_floats(const pk_gpu_kv_cache *cache, int B, int rows, int heads,

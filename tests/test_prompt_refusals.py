@@ -30,6 +30,8 @@ def attention(code=-1, text=None, **kw):
     (dict(rules=rules(window=-1)), -1, "window"), (dict(rules=rules(scale=float("nan"))), -1, "scale"),
     (dict(rules=rules(scale=float("inf"))), -1, "scale"), (dict(rules=rules(cap=-1.0)), -1, "cap"),
     (dict(rules=rules(cap=float("nan"))), -1, "cap"), (dict(rules=rules(cap=float("inf"))), -1, "cap"),
+    (dict(rules=rules(scale=1.5e36)), -1, "scale"), (dict(rules=rules(cap=1.5e36)), -1, "cap"),
+    (dict(rules=rules(scale=-1.5e36)), -1, "scale"), (dict(rules=rules(scale=1.0, cap=1e-37)), -1, "cap"),
     (dict(ldq=511), -1, "ldq"), (dict(ldo=511), -1, "ldo"), (dict(ld_pages=7), -1, "pages"), (dict(ld_pages=-1), -1, "pages"),
     (dict(q=None), -1, "NULL"), (dict(out=None), -1, "NULL"), (dict(lens=None), -1, "NULL"), (dict(pages=None), -1, "NULL"),
     (dict(q=P + 8), -1, "aligned"), (dict(out=P + 4), -1, "aligned"), (dict(ldq=514), -1, "aligned"),
