@@ -26,16 +26,18 @@
 // numbers), as the output is itself: each weight is off by half a step relative to it, the
 // output by no more than sqrt(2) of its own rounding where errors are independent, two
 // at the worst; l sums the unrounded.  f16 queries over codes take 2 terms (16 bits), f32 3.
-// One term where 2 or 3 are taken elsewhere is what the product's time is: 4096 tokens of
-// 32 heads of 128 take 135 us in one, 352 with f32's 3 by 3.
+// More terms are more products: 4096 tokens of 32 heads of 128 take 141 us with one for
+// each, 352 with f32's 3 by 3.
 //
-// What bounds it: 8192 tokens of 32 heads over 8 of 128 in bf16 take 504 us, 1090 of the
+// What bounds it: 8192 tokens of 32 heads over 8 of 128 in bf16 take 504 to 511 us, 1080 of the
 // 1267 TFLOP/s that a product of two 8192 x 8192 matrices reaches here; both are held by the
 // clock, which matrix instructions bring down to some 1.8 GHz.  Blocks of 32x32 halve the
-// reads of LDS for a row against 16x16; heads of 256 do not leave the registers for them.
-// Heads of 64 do half the products per score, so the exponentials and their like count as much
-// as they: 842 TFLOP/s.  4 bits under a cap (2 more transcendental instructions a score) is the
-// vector unit's: 16000 tokens of 16 heads of 256 behind 24000 others, window 1024, 209 us.
+// reads of LDS for a row against 16x16.  Heads of 256 do not leave the registers for them:
+// LDS gives 128 bytes a clock, so their tiles take twice as long to read as to multiply
+// (4096 tokens of 16 heads in bf16 149 us, 920 TFLOP/s; 4 bits, through a conversion, 161).
+// Heads of 64 do half the products per score, so the exponentials and their like count as
+// much as they (168 us, 820 TFLOP/s), and a cap adds 2 transcendental instructions to one (128:
+// 141 us, 174 capped).
 #pragma once
 
 #include "pk_paged_attention.h"
