@@ -33,8 +33,8 @@
 // 1267 TFLOP/s that a product of two 8192 x 8192 matrices reaches here; both are held by the
 // clock, which matrix instructions bring down to some 1.8 GHz.  Blocks of 32x32 halve the
 // reads of LDS for a row against 16x16.  Heads of 256 do not leave the registers for them:
-// LDS gives 128 bytes a clock, so their tiles take twice as long to read as to multiply
-// (4096 tokens of 16 heads in bf16 149 us, 920 TFLOP/s; 4 bits, through a conversion, 161).
+// each wave reads a tile for 16 rows, which keeps LDS busier than the matrix cores (4096
+// tokens of 16 heads in bf16 149 us, 920 TFLOP/s; 4 bits, through a conversion, 161).
 // Heads of 64 do half the products per score, so the exponentials and their like count as
 // much as they (168 us, 820 TFLOP/s), and a cap adds 2 transcendental instructions to one (128:
 // 141 us, 174 capped).
