@@ -74,9 +74,8 @@
 // them (0 times it), so here a workgroup whose sums have passed 2^100 or become NaN
 // takes its columns again one by one (pk_careful_attention.h).  64 single tokens behind up to
 // 6000 others with a cap, slopes and a window of 2048, 32 heads over 8 of 128 over int8, take
-// 53.5 us (5.1 TB/s).  The 16-row tiles of a sequence that has more than one are
-// launched far apart, on the same L2: 16 sequences of 4000 tokens in bf16, 4 new tokens
-// 56 us, 8 new ones 65.
+// 53.5 us (5.1 TB/s); 16 sequences of 4000 tokens in bf16, 4 new ones 56, 8, which are
+// two tiles that read the same chunks, 65.
 #pragma once
 
 #include "pk_careful_attention.h"
@@ -285,11 +284,29 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM, RULES), waves_of(
     const uint32_t pairs = (uint32_t)a.B * a.kv_heads * a.head_tiles;
     const int split = blockIdx.x / pairs;
     uint32_t x = (blockIdx.x + split) % pairs;
-    // With RULES the tiles of one key-value head that read the same chunk go to the same
-    // L2 where the other pairs are a multiple of 8.
-    const uint32_t others = (uint32_t)a.B * a.kv_heads;
-    const int htile = RULES ? x / others : x % (uint32_t)a.head_tiles;
-    x = RULES ? x - htile * others : x / (uint32_t)a.head_tiles;
+    // With RULES the tiles of one key-value head that read the same chunk go to the same L2:
+    // all first tiles, all second ones (where the other pairs are a multiple of 8).  Where
+    // sequences are whole a launch may be longer than the card, and the second tiles would
+    // come when the L2 has other keys, so 32 pairs' first ones and second ones take turns: 50
+    // sequences of 2000 tokens, 8 new ones, 32 heads over 8 of 128 in bf16, 109 us, 147 in
+    // the other order.  (8 at a time alternate on an XCD and so meet every other of its
+    // shader engines: ragged batches, whose second tiles may be empty, took a third longer.)
+    int htile = 0;
+    if constexpr (RULES) {
+        const uint32_t others = (uint32_t)a.B * a.kv_heads;
+        if (a.head_tiles > 1 && a.splits > 1) {
+            htile = x / others;
+            x -= htile * others;
+        } else if (a.head_tiles > 1) {
+            const uint32_t first = 32 * (x / (32u * a.head_tiles)), wide = min(others - first, 32u);
+            x -= first * a.head_tiles;
+            htile = x / wide;
+            x += first - htile * wide;
+        }
+    } else {
+        htile = x % (uint32_t)a.head_tiles;
+        x /= (uint32_t)a.head_tiles;
+    }
     const int kvh = x % (uint32_t)a.kv_heads;
     int b = x / (uint32_t)a.kv_heads;
     if (a.longest_first) b = nth_longest(a, b, sh.lens, wave);

@@ -38,16 +38,18 @@ int check_sizes(const pk_gpu_kv_cache* c, const Sizes& z)
 // Calls of few rows, (new token, head) pairs of a key-value head, go 16 a workgroup over
 // the tiles of the one-token attention, the others prompt_rows a workgroup.
 //
-// 16 rows, or fewer, read the cache once that way, and faster.  Where sequences have more, each
-// 16 of them read it again, if from L2: up to 32 that still is less than what 128 rows
-// lose while there are not two workgroups of these for a CU, up to 48 where keys need a
-// conversion or 3 terms.  Measured (us, few and many; 32 heads over 8 of 128, queries and
-// cache in bf16; f32 queries; bf16 over 4 bits):
-//   16 x 4 of 4000                 56.2 -       58.1 -       23.0 -
-//   16 x 8 of 4000                 65.3 77.0    68.0 106     28.4 52.3
-//   16 x 12 of 4000                94.0 78.8    98.3 116     42.3 58.5
-//   64 x 8 of 1000                 90.4 52.2    95.4 88.7    30.8 28.4
-//   64 x 12 of 1000                126  53.8    134  91.0    42.9 33.7
+// 16 rows, or fewer, read the cache once that way, and faster.  Where sequences have up to 32,
+// the second 16 of them read it again, from L2; that still is less than what 128 rows lose, but
+// where sequences are short and there is more than one workgroup of these for a CU. f32
+// queries (3 terms) and 4 bits (a conversion, for few rows) lose more by them, and hold out up to 48
+// rows while there are not two for a CU.  Measured (us, few and many; 32 heads over 8 of
+// 128, queries and cache in bf16; f32 queries; bf16 over int8; over 4 bits):
+//   60 x 8 of 300                  29.6 17.3    36.2 36.8    30.4 17.7    18.2 14.5
+//   60 x 6 of 1000                 66.6 48.1    73.8 86.9    50.7 38.3    29.5 28.3
+//   60 x 6 of up to 1000           35.2 40.2    39.1 84.1    32.3 43.8    20.5 37.9
+//   100 x 8 of 2000                191  211     204  311     148  177     82.6 138
+//   16 x 8 of 4000                 65.3 77.0    68.0 106     49.5 64.3    28.4 52.3
+//   16 x 12 of 4000                94.0 78.8    98.3 116     69.6 72.5    42.3 58.5
 //
 // Of more rows still go that way the calls of at most as many such workgroups as CUs, if
 // short: 16 rows start sooner than 128, and keys that need no way through LDS sooner still
@@ -61,9 +63,11 @@ int check_sizes(const pk_gpu_kv_cache* c, const Sizes& z)
 bool few_rows(const pk_gpu_kv_cache* c, const Sizes& z, int dtype)
 {
     const long long each = (long long)z.max_new * (z.heads / c->heads), pairs = (each + 15) / 16 * z.B * c->heads;
-    const bool narrow = dtype != F32 && (c->dtype == F16 || c->dtype == BF16);
-    return each <= 16 || (each <= (dtype == F32 || c->dtype == E2M1 ? 48 : 32) && (long long)z.B * c->heads < 512) ||
-           (pairs <= (narrow ? 256 : 512) && pairs * span_of_rows(z) <= (narrow ? 160 << 10 : 512 << 10));
+    const long long heads = (long long)z.B * c->heads, span = span_of_rows(z);
+    const bool narrow = dtype != F32 && (c->dtype == F16 || c->dtype == BF16), wide = dtype == F32 || c->dtype == E2M1;
+    return each <= 16 || (each <= 32 && (heads < 256 || span >= (wide ? 512 : 1536))) ||
+           (each > 32 && each <= 48 && wide && heads < 512) ||
+           (pairs <= (narrow ? 256 : 512) && pairs * span <= (narrow ? 160 << 10 : 512 << 10));
 }
 
 // Chunks of a call of many rows, where its tiles are fewer than the CUs: up to `slots`
@@ -260,6 +264,11 @@ int pk_gpu_prompt_attention_dev(const pk_gpu_kv_cache* cache, int dtype, const v
     a.rules.max_new = z.max_new;
     a.rules.by_row = !l.few;
     a.rules.per_seq = l.per_seq;
+    // Where there are more workgroups of whole sequences than CUs, the longest sequences go
+    // first (see the one-token call) if they are long for what counting them costs: 33 of 3000
+    // tokens, 8 new ones, 32 heads over 8 of 128 in bf16, ragged 50 us, 63 in order, all
+    // equal 119 against 115; 60 of 1000, 5 new ones, 37 against 34 and 74 against 67.
+    a.longest_first = l.few && p.splits == 1 && l.pairs > 256 && B > 1 && B <= kSortedMax && max_len / 32 >= B && z.window == 0;
     const hipError_t e = l.few ? launch_attention(cache->dtype, dtype, cache->head_dim, true, a, (uint32_t)(l.pairs * p.splits),
                                                   (uint32_t)l.outs, static_cast<hipStream_t>(stream))
                                : launch_prompts(cache->dtype, dtype, cache->head_dim, a, (uint32_t)(l.pairs * p.splits),

@@ -92,8 +92,9 @@ def many_rows(kind, rows, kv, group, B, new, max_len, window):
     window = window if window < max_len else 0
     span = min(window + new + 30, max_len) if window else max_len
     narrow = rows != "f32" and kind in ("f16", "bf16")
-    two_tiles = 48 if rows == "f32" or kind == "e2m1" else 32
-    few = (each <= 16 or (each <= two_tiles and B * kv < 512) or
+    wide = rows == "f32" or kind == "e2m1"
+    few = (each <= 16 or (each <= 32 and (B * kv < 256 or span >= (512 if wide else 1536))) or
+           (32 < each <= 48 and wide and B * kv < 512) or
            (tiles <= (256 if narrow else 512) and tiles * span <= (160 << 10 if narrow else 512 << 10)))
     return not few
 

@@ -298,3 +298,20 @@ def test_the_same_call_gives_the_same_bits():
         for i in range(5):
             c.ws[:c.floats] = torch.randn((c.floats,), device="cuda:0") * 10.0 ** (i - 3)
             assert np.array_equal(c.run(want), first)
+
+
+@pytest.mark.parametrize("B,kv,group,new,lens,kind,rows", [
+    # more workgroups of whole sequences than CUs, one tile of rows each and two; 37 pairs beyond whole groups of 32
+    (37, 5, 4, 8, 700, "bf16", "f32"), (41, 7, 3, 1, 1400, "int8", "bf16"), (90, 3, 16, 2, 690, "e2m1", "bf16"),
+    (43, 6, 4, 7, 1600, "bf16", "bf16"), (300, 1, 20, 1, 600, "e2m1", "f32")])
+def test_batches_longer_than_the_card(B, kv, group, new, lens, kind, rows):
+    """Ragged batches: longest sequences first where they are long for their number, and the tiles of a key-value
+    head in turn; some sequences without new tokens, some without any."""
+    rng = np.random.default_rng(B)
+    n = rng.integers(0, new + 1, B)
+    n[0] = new
+    ln = np.maximum(n, rng.integers(0, lens + 1, B))
+    ln[1], n[2], ln[2] = lens, 0, 0
+    c = prompt(rng, kind, rows, kv, group, 64, 16, n.tolist(), ln.tolist(), tail=1, max_len=lens, max_new=new)
+    assert not c.many()
+    c.check()
