@@ -7,7 +7,7 @@
 // powers of two.  m moves, and acc and l are scaled, only once a score is 8 above it, which
 // most tiles of tokens spare; weights stay below 2^8 (times 2^BIAS over f16 values).
 //
-// A workgroup holds prompt_rows rows of one key-value head, the rows of its query heads
+// A workgroup holds kPromptRows rows of one key-value head, the rows of its query heads
 // next to each other, so a group's heads share what it stages: tiles of prompt_keys
 // tokens, keys and values, in 16 bits, two stages in LDS.  16-bit caches go there past the
 // registers, codes through a conversion; a tile's loads are out while the one before is
@@ -16,6 +16,9 @@
 //     but for one or three exchanges, and its scores are, in order, the second operand of
 //   O^T = V^T P^T: weights go from register to register, never through LDS.  V^T comes from
 //     LDS by transposing reads.
+// With two sides two waves have the same 32 rows and half of each tile's tokens each, so a
+// workgroup is through its tokens sooner: launches that do not fill the card many times over are
+// as long as their longest workgroup.  Their sums are joined in LDS at the end.
 // Pieces of 16 bytes are XORed with their row, such that the 16 lanes that read at a time
 // meet all banks.
 //
@@ -49,22 +52,33 @@ using f32x16 = __attribute__((ext_vector_type(16))) float;
 using s16x4 = __attribute__((ext_vector_type(4))) short;
 
 constexpr int prompt_p_terms(int cache, int t) { return t == F32 ? 3 : t == F16 && cache != F16 ? 2 : 1; }
-// Rows of a wave, its matrix instructions' (32x32x16 or 16x16x32), and waves of a workgroup.
+// Rows of a wave, its matrix instructions' (32x32x16 or 16x16x32), waves of a workgroup, and
+// its rows.  With two sides (heads of 64 and 128) two waves have the same rows and half of each
+// tile's tokens each, and join their sums at the end.
 constexpr int prompt_block(int dim) { return dim == 256 ? 16 : 32; }
-constexpr int prompt_waves(int cache, int t, int dim) { return dim == 256 ? 8 : 4; }
-constexpr int prompt_rows(int cache, int t, int dim) { return prompt_block(dim) * prompt_waves(cache, t, dim); }
+constexpr int prompt_waves(int dim, int sides) { return dim == 256 ? 8 : 4 * sides; }
+constexpr int kPromptRows = 128;
 // Tokens of a tile: 64, whose two stages take 32 to 128 KB.  4-bit heads of 64 would leave half
 // the threads without a piece to convert (4096 tokens of 64 heads 184 us, of 128 tokens 167).
 constexpr int prompt_keys(int cache, int dim) { return dim == 64 && cache == E2M1 ? 128 : 64; }
-// Waves of a SIMD, and so workgroups that run at a time: as many as the registers take.  f32
-// queries in 3 terms over 16-bit heads of 128 spill at two (4096 tokens of 32 heads 354 us,
-// 366), elsewhere two gain (over int8 404 against 462, heads of 64 357 against 434); heads
-// of 64 leave room for three (bf16 over int8 214 against 236).
-constexpr int prompt_occupancy(int cache, int t, int dim)
+// Which of them there are (prompt_sides in pk_prompt_attention.hip says which a call takes): heads
+// of 256 have no registers for two, 4-bit heads of 64 spill with two at the occupancy that
+// pays, and f32 queries in 3 terms over heads of 128 are better by two always (one spills).
+constexpr bool has_sides(int cache, int t, int dim, int sides)
 {
-    return t == F32 && dim == 128 && (cache == F16 || cache == BF16) ? 1 : dim == 64 && t != F32 && cache != E2M1 ? 3 : 2;
+    return dim == 256 || (dim == 64 && cache == E2M1)      ? sides == 1
+           : dim == 128 && t == F32 && cache != E2M1 ? sides == 2 : true;
 }
-constexpr int prompt_slots(int cache, int t, int dim) { return 256 * 4 * prompt_occupancy(cache, t, dim) / prompt_waves(cache, t, dim); }
+// Waves of a SIMD, and so workgroups that run at a time: as many as the registers take.
+// Heads of 64 leave room for three (bf16 over int8 214 against 236) or four by two sides.
+constexpr int prompt_occupancy(int cache, int t, int dim, int sides)
+{
+    return dim != 64 || t == F32 || cache == E2M1 ? 2 : sides == 2 ? 4 : 3;
+}
+constexpr int prompt_slots(int cache, int t, int dim, int sides)
+{
+    return 256 * 4 * prompt_occupancy(cache, t, dim, sides) / prompt_waves(dim, sides);
+}
 
 template <bool IN_F16>
 __device__ inline f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c)
@@ -147,10 +161,12 @@ __device__ inline bool row_tile(const PagedArgs& a, uint32_t tau, RowTile* out)
     return nth < (uint32_t)n;
 }
 
-template <int CACHE, int T, int DIM>
-__global__ void __launch_bounds__(64 * prompt_waves(CACHE, T, DIM), prompt_occupancy(CACHE, T, DIM)) prompt_attention(PagedArgs a)
+template <int CACHE, int T, int DIM, int SIDES>
+__global__ void __launch_bounds__(64 * prompt_waves(DIM, SIDES), prompt_occupancy(CACHE, T, DIM, SIDES)) prompt_attention(PagedArgs a)
 {
-    constexpr int R = prompt_block(DIM), W = prompt_waves(CACHE, T, DIM), BM = R * W, THREADS = 64 * W;
+    constexpr int R = prompt_block(DIM), W = prompt_waves(DIM, SIDES), THREADS = 64 * W;
+    constexpr int WR = W / SIDES, BM = kPromptRows;
+    static_assert(BM == R * WR, "rows of a workgroup");
     constexpr int NR = R * R / 64;             // registers of a block of sums
     using Sums = __attribute__((ext_vector_type(NR))) float;
     constexpr int RB = bytes_of(CACHE, DIM);
@@ -161,7 +177,8 @@ __global__ void __launch_bounds__(64 * prompt_waves(CACHE, T, DIM), prompt_occup
     constexpr int PR = DIM / 8;                // 16-byte pieces of a row in LDS
     constexpr int KS = 512 / R;                // of a matrix instruction's sum
     constexpr int STEPS = DIM / KS, DB = DIM / R;
-    constexpr int KT = prompt_keys(CACHE, DIM), NU = KT / R, NS = KT / KS, NB = KT / 16;
+    constexpr int KT = prompt_keys(CACHE, DIM), NB = KT / 16;
+    constexpr int KW = KT / SIDES, NU = KW / R, NS = KW / KS;      // tokens of a wave's part of a tile
 
     __shared__ u32x4 tiles[2][2][KT * PR];     // [stage][keys, values][row][piece]
     __shared__ float scales[CODED ? 2 : 1][2][KT];
@@ -170,6 +187,7 @@ __global__ void __launch_bounds__(64 * prompt_waves(CACHE, T, DIM), prompt_occup
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane % R, g = lane / R;
+    const int side = SIDES == 1 ? 0 : wave / WR, in_side = SIDES == 1 ? wave : wave % WR;
 
     const uint32_t per_split = (uint32_t)a.head_tiles * a.kv_heads;
     const int split = blockIdx.x / per_split;
@@ -184,7 +202,7 @@ __global__ void __launch_bounds__(64 * prompt_waves(CACHE, T, DIM), prompt_occup
     const int heads = a.kv_heads * a.group;
 
     // this lane's row
-    const uint32_t r = (uint32_t)rt.tile * BM + wave * R + n;
+    const uint32_t r = (uint32_t)rt.tile * BM + in_side * R + n;
     const int nth = r / (uint32_t)a.group;
     const bool ok = nth < news.count;
     const int head = kvh * a.group + (int)(r - (uint32_t)nth * a.group);
@@ -283,9 +301,9 @@ __global__ void __launch_bounds__(64 * prompt_waves(CACHE, T, DIM), prompt_occup
                 // its block: one for all waves, or W / PER for PER waves each
                 constexpr int MANY = W > PER ? W / PER : 1;
                 const int blk = W > PER ? MANY * i + wave / PER : W * i / PER;
-                size_t off = s.off[W > PER ? MANY * i : W * i / PER];
-#pragma unroll
-                for (int j = 1; j < MANY; ++j) off = wave / PER == j ? s.off[(MANY * i + j) % NB] : off;
+                const size_t off = W > PER ? (size_t)(uint32_t)__builtin_amdgcn_readlane((int)(s.mine >> 32), blk) << 32 |
+                                             (uint32_t)__builtin_amdgcn_readlane((int)s.mine, blk)
+                                           : s.off[W * i / PER];
                 const int row = (W * i + wave) * RPC + lane / PR;
                 int t = row % 16;
                 if constexpr (!WHOLE) {
@@ -390,6 +408,8 @@ __global__ void __launch_bounds__(64 * prompt_waves(CACHE, T, DIM), prompt_occup
     }
 
     auto compute = [&](int t0, auto at, uint32_t present) {
+        t0 += KW * side;
+        if constexpr (SIDES > 1) present = present >> (KW / 16 * side) & ((1u << KW / 16) - 1);
         constexpr int stage = decltype(at)::value;
         const u32x4* const k = tiles[stage][0];
         Sums s[NU];
@@ -399,14 +419,14 @@ __global__ void __launch_bounds__(64 * prompt_waves(CACHE, T, DIM), prompt_occup
             for (int i = 0; i < NR; ++i) s[u][i] = 0.0f;
 #pragma unroll
             for (int c = 0; c < STEPS; ++c) {
-                const int row = R * u + n;
+                const int row = KW * side + R * u + n;
                 const u32x4 f = k[row * PR + slot_k(row, KS / 8 * c + g)];
 #pragma unroll
                 for (int i = QT - 1; i >= 0; --i) s[u] = multiply(keys_type, f, qf[i][c], s[u]);
             }
         }
         // in this order: reads of keys AHEAD steps before their product (0x100: LDS reads, 8: products)
-        constexpr int AHEAD = QT == 1 ? 8 : 4;
+        constexpr int AHEAD = QT == 1 && NU * STEPS >= 8 ? 8 : 4;
         __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
 #pragma unroll
         for (int i = 0; i < NU * STEPS - AHEAD; ++i) {
@@ -421,7 +441,7 @@ __global__ void __launch_bounds__(64 * prompt_waves(CACHE, T, DIM), prompt_occup
             for (int u = 0; u < NU; ++u)
 #pragma unroll
                 for (int i = 0; i < NR; i += 4) {
-                    const f32x4 ks = *reinterpret_cast<const f32x4*>(&scales[stage][0][R * u + 2 * i + 4 * g]);
+                    const f32x4 ks = *reinterpret_cast<const f32x4*>(&scales[stage][0][KW * side + R * u + 2 * i + 4 * g]);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) s[u][i + r] = __fmul_rn(s[u][i + r], ks[r]);
                 }
@@ -448,7 +468,7 @@ __global__ void __launch_bounds__(64 * prompt_waves(CACHE, T, DIM), prompt_occup
                         s[u][i] = __builtin_fmaf(-slope2, fabsf(__fsub_rn(ahead, (float)(R * u + 8 * (i / 4) + i % 4))), s[u][i]);
             }
         }
-        const bool whole = present == (1u << NB) - 1 && t0 >= max(all_lo, begin) && t0 + KT <= min(all_hi, end);
+        const bool whole = present == (1u << KW / 16) - 1 && t0 >= max(all_lo, begin) && t0 + KW <= min(all_hi, end);
         if (!whole) {
             const int from = max(see.lo, begin) - t0 - 4 * g, to = min(see.hi, end) - t0 - 4 * g;
 #pragma unroll
@@ -491,7 +511,7 @@ __global__ void __launch_bounds__(64 * prompt_waves(CACHE, T, DIM), prompt_occup
                     l = __fadd_rn(l, w[r]);
                 }
                 if constexpr (CODED) {
-                    const float* const vs = &scales[stage][1][R * u + 8 * (i / 4) + 4 * g + i % 4];
+                    const float* const vs = &scales[stage][1][KW * side + R * u + 8 * (i / 4) + 4 * g + i % 4];
                     w[0] = __fmul_rn(w[0], vs[0]);
                     w[1] = __fmul_rn(w[1], vs[1]);
                 }
@@ -504,7 +524,7 @@ __global__ void __launch_bounds__(64 * prompt_waves(CACHE, T, DIM), prompt_occup
                 }
             }
         // k index 8 g + i of step c is token KS c + KS / 2 (i / 4) + 4 g + i % 4
-        const uint32_t vbase = lds0 + (stage * 2 + 1) * KT * PR * 16;
+        const uint32_t vbase = lds0 + ((stage * 2 + 1) * KT + KW * side) * PR * 16;
 #pragma unroll
         for (int c = 0; c < NS; ++c) {
 #pragma unroll
@@ -557,7 +577,7 @@ __global__ void __launch_bounds__(64 * prompt_waves(CACHE, T, DIM), prompt_occup
                 next = s1.present;
                 fetch(s1, t + KT, stage ^ 1);
             }
-            if (t < mine_hi && t + KT > mine_lo) compute(t, at, present);
+            if (t + KW * side < mine_hi && t + KW * side + KW > mine_lo) compute(t, at, present);
             if (!more) return false;
             put(stage ^ 1);
             arrived();
@@ -577,6 +597,33 @@ __global__ void __launch_bounds__(64 * prompt_waves(CACHE, T, DIM), prompt_occup
     for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int i = 0; i < NR; ++i) size = __fadd_rn(size, fabsf(acc[d][i]));
+    if constexpr (SIDES > 1) {
+        // the two sides of a block of rows: one leaves its sums in LDS, the other adds them
+        static_assert(SIDES == 2 && WR * 64 * DB * NR * 4 <= sizeof(tiles), "sums of half the waves fit");
+        __shared__ float others[WR][3][64];
+        __syncthreads();                           // the tiles are read
+        float* const sums = reinterpret_cast<float*>(&tiles[0][0][0]) + in_side * (64 * DB * NR) + lane;
+        if (side) {
+            others[in_side][0][lane] = m;
+            others[in_side][1][lane] = l;
+            others[in_side][2][lane] = size;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < NR; ++i) sums[64 * (NR * d + i)] = acc[d][i];
+        }
+        __syncthreads();
+        if (side) return;
+        const float m1 = others[in_side][0][lane], mn = fmaxf(m, m1);
+        const float f0 = __builtin_amdgcn_exp2f(m - mn), f1 = __builtin_amdgcn_exp2f(m1 - mn);
+        size = __fadd_rn(size, others[in_side][2][lane]);
+        l = __fadd_rn(__fmul_rn(l, f0), __fmul_rn(others[in_side][1][lane], f1));
+        m = mn;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < NR; ++i) acc[d][i] = __fadd_rn(__fmul_rn(acc[d][i], f0), __fmul_rn(sums[64 * (NR * d + i)], f1));
+    }
     if (__any(!(size < 0x1p100f))) {
         const CacheView view{a.k, a.v, a.k_scale, a.v_scale, pages, a.n_pages, a.page_shift, a.kv_heads, kvh};
 #pragma unroll 1
@@ -628,23 +675,27 @@ __global__ void __launch_bounds__(64 * prompt_waves(CACHE, T, DIM), prompt_occup
     }
 }
 
-hipError_t launch_prompt_f16(int t, int dim, const PagedArgs& a, dim3 grid, hipStream_t s);
-hipError_t launch_prompt_bf16(int t, int dim, const PagedArgs& a, dim3 grid, hipStream_t s);
-hipError_t launch_prompt_i8(int t, int dim, const PagedArgs& a, dim3 grid, hipStream_t s);
-hipError_t launch_prompt_e4m3(int t, int dim, const PagedArgs& a, dim3 grid, hipStream_t s);
-hipError_t launch_prompt_e2m1(int t, int dim, const PagedArgs& a, dim3 grid, hipStream_t s);
+hipError_t launch_prompt_f16(int t, int dim, int sides, const PagedArgs& a, dim3 grid, hipStream_t s);
+hipError_t launch_prompt_bf16(int t, int dim, int sides, const PagedArgs& a, dim3 grid, hipStream_t s);
+hipError_t launch_prompt_i8(int t, int dim, int sides, const PagedArgs& a, dim3 grid, hipStream_t s);
+hipError_t launch_prompt_e4m3(int t, int dim, int sides, const PagedArgs& a, dim3 grid, hipStream_t s);
+hipError_t launch_prompt_e2m1(int t, int dim, int sides, const PagedArgs& a, dim3 grid, hipStream_t s);
 
 template <int CACHE, int T, int DIM>
-hipError_t launch_prompt_as(const PagedArgs& a, dim3 grid, hipStream_t s)
+hipError_t launch_prompt_as(int sides, const PagedArgs& a, dim3 grid, hipStream_t s)
 {
-    return launch(prompt_attention<CACHE, T, DIM>, grid, dim3(64 * prompt_waves(CACHE, T, DIM)), 0, s, a);
+    const dim3 block(64 * prompt_waves(DIM, sides));
+    if constexpr (has_sides(CACHE, T, DIM, 2))
+        if (sides == 2) return launch(prompt_attention<CACHE, T, DIM, 2>, grid, block, 0, s, a);
+    if constexpr (has_sides(CACHE, T, DIM, 1)) return launch(prompt_attention<CACHE, T, DIM, 1>, grid, block, 0, s, a);
+    else return hipErrorInvalidValue;
 }
 template <int CACHE, int T>
-hipError_t launch_prompt(int dim, const PagedArgs& a, dim3 grid, hipStream_t s)
+hipError_t launch_prompt(int dim, int sides, const PagedArgs& a, dim3 grid, hipStream_t s)
 {
-    return dim == 64    ? launch_prompt_as<CACHE, T, 64>(a, grid, s)
-           : dim == 128 ? launch_prompt_as<CACHE, T, 128>(a, grid, s)
-                        : launch_prompt_as<CACHE, T, 256>(a, grid, s);
+    return dim == 64    ? launch_prompt_as<CACHE, T, 64>(sides, a, grid, s)
+           : dim == 128 ? launch_prompt_as<CACHE, T, 128>(sides, a, grid, s)
+                        : launch_prompt_as<CACHE, T, 256>(sides, a, grid, s);
 }
 
 }  // namespace decode

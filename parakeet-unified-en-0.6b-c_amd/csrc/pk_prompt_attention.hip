@@ -77,7 +77,7 @@ bool few_rows(const pk_gpu_kv_cache* c, const Sizes& z, int dtype)
 //   64 new of 4000 tokens, 16 tiles     24.9 21.5
 //   128 of 1500, 32                     30.1 23.8
 //   512 of 1000, 128                    25.9 38.7
-constexpr int kSplitRows = 128, kMostSlots = 768;    // of prompt_rows and prompt_slots, whatever the types
+constexpr int kMostSlots = 768;     // of prompt_slots, whatever the types
 long long prompt_cuts(long long pairs, long long span, int slots)
 {
     if (pairs >= 256) return 1;
@@ -88,17 +88,43 @@ long long prompt_cuts(long long pairs, long long span, int slots)
 // Tiles of a call's rows, whatever the sequences they are of.
 long long split_pairs(const pk_gpu_kv_cache* c, long long rows, int group)
 {
-    return ((rows * group + kSplitRows - 1) / kSplitRows) * c->heads;
+    return ((rows * group + kPromptRows - 1) / kPromptRows) * c->heads;
+}
+
+// Sides of a workgroup's rows.  Two make it faster by itself, one gets more work out of a full
+// card: so two for launches that are one round of workgroups, or two of long ones; and for packed
+// documents, whose longest one a launch waits for.  Where tiles are few and tokens many, more
+// chunks do as much, and few tokens are not worth the join.  Measured (us, one side and two; 32 heads over 8;
+// heads of 128 in bf16, of 128 over int8, of 64 in bf16):
+//   16 x 16 of 200 tokens, 128 tiles  11.4 12.1
+//   300 of 6000, 80                   51.2 54.5    60.7 67.5    40.5 40.3
+//   700 of 9000, 176                  139  148     188  205     (2 chunks and 1)
+//   500 of 500, 128                   15.9 15.9    21.1 19.2    12.6 11.8
+//   800 of 3000, 200                  74.6 55.5    90.0 74.1    60.0 62.8
+//   1000 of 8000, 256                 153  139     243  184     120  98.3
+//   2000 of 2000, 504                 51.1 50.3    72.1 64.0    36.5 33.3
+//   4 x 400 of 400, 416               19.4 25.2    23.9 29.4    13.5 14.2
+//   4096 of 4096, 1024                136  168     178  214     88.2 97.2
+//   8191 in documents of 900, 16 heads over 4, 1024                  57 to 96, 53 to 81
+// f32 queries over heads of 128 354 and 342 in bf16, 88.2 and 51.8 for 1000 over int8.
+int prompt_sides(const pk_gpu_kv_cache* c, int dtype, long long pairs, long long split, long long span, bool packed)
+{
+    const int dim = c->head_dim;
+    if (!has_sides(c->dtype, dtype, dim, 2)) return 1;
+    if (!has_sides(c->dtype, dtype, dim, 1)) return 2;
+    const long long most = dim == 64 ? (packed && dtype != F32 ? 1024 : 512) : span >= 1024 ? 512 : 256;
+    if (pairs > most || span < 384) return 1;
+    return pairs >= 192 || prompt_cuts(split, span, prompt_slots(c->dtype, dtype, dim, 1)) == 1 ? 2 : 1;
 }
 
 // How a call is laid out: workgroups of one chunk, chunks, rows of the workspace.
 struct Layout {
     bool few;
-    int per_seq;
+    int per_seq, sides;
     long long pairs, outs;
     Plan plan;
 };
-Layout layout_of(const pk_gpu_kv_cache* c, const Sizes& z, int rows, int dtype)
+Layout layout_of(const pk_gpu_kv_cache* c, const Sizes& z, int rows, int dtype, bool packed)
 {
     const int group = z.heads / c->heads;
     const long long each = (long long)z.max_new * group, span = span_of_rows(z);
@@ -109,13 +135,15 @@ Layout layout_of(const pk_gpu_kv_cache* c, const Sizes& z, int rows, int dtype)
         l.outs = (long long)z.B * z.max_new * z.heads;
         l.plan = plan_of(c->dtype, c->head_dim, l.pairs > 0 ? l.pairs : 1, span);
     } else {
-        const int bm = prompt_rows(c->dtype, dtype, c->head_dim);
+        const int bm = kPromptRows;
         // tiles of every sequence, or of all rows with one that is not whole for each sequence
         const long long per = (each + bm - 1) / bm, all = (long long)rows * group / bm + z.B;
         l.per_seq = per * z.B <= all ? (int)per : 0;
         l.pairs = (l.per_seq ? per * z.B : all) * c->heads;
         l.outs = (long long)rows * z.heads;
-        const long long n = prompt_cuts(split_pairs(c, rows, group), span, prompt_slots(c->dtype, dtype, c->head_dim));
+        const long long split = split_pairs(c, rows, group);
+        l.sides = prompt_sides(c, dtype, l.pairs, split, span, packed);
+        const long long n = prompt_cuts(split, span, prompt_slots(c->dtype, dtype, c->head_dim, l.sides));
         const int keys = prompt_keys(c->dtype, c->head_dim);
         const long long chunk = ((span + n - 1) / n + keys - 1) / keys * keys;
         // a tile of rows begins anywhere in its chunk's first tile of tokens
@@ -142,21 +170,21 @@ size_t most_floats(const pk_gpu_kv_cache* c, const Sizes& z, int rows)
             if (cut > 1 && b * n * cut > most) most = b * n * cut;
         }
     for (long long t = 1; t * c->heads < 256; ++t) {
-        const long long n = kSplitRows * t / group < rows ? kSplitRows * t / group : rows;
+        const long long n = kPromptRows * t / group < rows ? kPromptRows * t / group : rows;
         const size_t cut = prompt_cuts(t * c->heads, span, kMostSlots);
         if (n >= 1 && cut > 1 && n * (cut + 1) > most) most = n * (cut + 1);
     }
     return most * z.heads * (c->head_dim + 2);
 }
 
-hipError_t launch_prompts(int cache, int t, int dim, const PagedArgs& a, uint32_t workgroups, uint32_t rows, hipStream_t s)
+hipError_t launch_prompts(int cache, int t, int dim, int sides, const PagedArgs& a, uint32_t workgroups, uint32_t rows, hipStream_t s)
 {
     const dim3 grid(workgroups);
-    const hipError_t e = cache == F16    ? launch_prompt_f16(t, dim, a, grid, s)
-                         : cache == BF16 ? launch_prompt_bf16(t, dim, a, grid, s)
-                         : cache == I8   ? launch_prompt_i8(t, dim, a, grid, s)
-                         : cache == E2M1 ? launch_prompt_e2m1(t, dim, a, grid, s)
-                                         : launch_prompt_e4m3(t, dim, a, grid, s);
+    const hipError_t e = cache == F16    ? launch_prompt_f16(t, dim, sides, a, grid, s)
+                         : cache == BF16 ? launch_prompt_bf16(t, dim, sides, a, grid, s)
+                         : cache == I8   ? launch_prompt_i8(t, dim, sides, a, grid, s)
+                         : cache == E2M1 ? launch_prompt_e2m1(t, dim, sides, a, grid, s)
+                                         : launch_prompt_e4m3(t, dim, sides, a, grid, s);
     return e == hipSuccess && a.splits > 1 ? launch_joins(t, dim, true, a, rows, s) : e;
 }
 
@@ -215,7 +243,7 @@ int pk_gpu_prompt_attention_dev(const pk_gpu_kv_cache* cache, int dtype, const v
     if (z.max_new > rows) z.max_new = rows;
     if (!dstarts && z.max_new > 1) z.max_new = 1;
     if (z.window >= max_len) z.window = 0;
-    const Layout l = layout_of(cache, z, rows, dtype);
+    const Layout l = layout_of(cache, z, rows, dtype, rules->first != nullptr);
     const Plan& p = l.plan;
     if (!launchable(l.pairs * p.splits, 512) || l.outs > 0x7fffffff || (p.splits > 1 && !launchable(l.outs, 256)))
         return rt::error(PK_GPU_EINVAL, "%s: %d sequences of %d new tokens and %d heads exceed the grid", kWho, B, z.max_new,
@@ -271,7 +299,7 @@ int pk_gpu_prompt_attention_dev(const pk_gpu_kv_cache* cache, int dtype, const v
     a.longest_first = l.few && p.splits == 1 && l.pairs > 256 && B > 1 && B <= kSortedMax && max_len / 32 >= B && z.window == 0;
     const hipError_t e = l.few ? launch_attention(cache->dtype, dtype, cache->head_dim, true, a, (uint32_t)(l.pairs * p.splits),
                                                   (uint32_t)l.outs, static_cast<hipStream_t>(stream))
-                               : launch_prompts(cache->dtype, dtype, cache->head_dim, a, (uint32_t)(l.pairs * p.splits),
+                               : launch_prompts(cache->dtype, dtype, cache->head_dim, l.sides, a, (uint32_t)(l.pairs * p.splits),
                                                 (uint32_t)l.outs, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? PK_GPU_OK : rt::hip_error(e, kWho);
 }

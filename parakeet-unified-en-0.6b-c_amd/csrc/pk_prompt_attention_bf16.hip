@@ -4,10 +4,10 @@
 namespace pkgpu {
 namespace decode {
 
-hipError_t launch_prompt_bf16(int t, int dim, const PagedArgs& a, dim3 grid, hipStream_t s)
+hipError_t launch_prompt_bf16(int t, int dim, int sides, const PagedArgs& a, dim3 grid, hipStream_t s)
 {
-    return t == BF16 ? launch_prompt<BF16, BF16>(dim, a, grid, s)
-         : t == F32 ? launch_prompt<BF16, F32>(dim, a, grid, s) : hipErrorInvalidValue;
+    return t == BF16 ? launch_prompt<BF16, BF16>(dim, sides, a, grid, s)
+         : t == F32 ? launch_prompt<BF16, F32>(dim, sides, a, grid, s) : hipErrorInvalidValue;
 }
 
 }  // namespace decode

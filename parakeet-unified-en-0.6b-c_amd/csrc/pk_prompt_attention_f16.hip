@@ -4,9 +4,9 @@
 namespace pkgpu {
 namespace decode {
 
-hipError_t launch_prompt_f16(int t, int dim, const PagedArgs& a, dim3 grid, hipStream_t s)
+hipError_t launch_prompt_f16(int t, int dim, int sides, const PagedArgs& a, dim3 grid, hipStream_t s)
 {
-    return t == F16 ? launch_prompt<F16, F16>(dim, a, grid, s) : hipErrorInvalidValue;
+    return t == F16 ? launch_prompt<F16, F16>(dim, sides, a, grid, s) : hipErrorInvalidValue;
 }
 
 }  // namespace decode

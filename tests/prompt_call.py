@@ -84,6 +84,24 @@ class Prompt:
                          self.how["window"])
 
 
+def sides(c):
+    """Whether two waves share rows in the kernel of many rows: its rule for what a call's tiles are."""
+    kind, rows, dim, heads = c.cache.kind, c.rows, c.cache.dim, c.cache.heads
+    if dim == 256 or (dim == 64 and kind == "e2m1"):
+        return 1
+    if dim == 128 and rows == "f32" and kind != "e2m1":
+        return 2
+    group, new = c.heads // heads, min(c.max_new, c.n)
+    window = c.how["window"] if c.how["window"] < c.max_len else 0
+    span = min(window + new + 30, c.max_len) if window else c.max_len
+    pairs = min(-(-new * group // 128) * c.B, c.n * group // 128 + c.B) * heads
+    split = -(-c.n * group // 128) * heads
+    most = (1024 if c.how["first"] is not None and rows != "f32" else 512) if dim == 64 else 512 if span >= 1024 else 256
+    slots = 768 if dim == 64 and rows != "f32" else 512
+    cuts = 1 if split >= 256 else max(1, min(slots // split, span // (256 if split <= 64 else 512), 64))
+    return 2 if pairs <= most and span >= 384 and (pairs >= 192 or cuts == 1) else 1
+
+
 def many_rows(kind, rows, kv, group, B, new, max_len, window):
     """The rule: by the rows of a sequence and key-value head, the 16-row tiles of all and the tokens that a
     tile may see."""

@@ -8,7 +8,7 @@ import pytest
 
 import decode_oracle as do
 from pkgpu import pk
-from prompt_call import prompt
+from prompt_call import prompt, sides
 from test_gpu_prompt_attention import rules_of
 
 pytestmark = pytest.mark.gpu
@@ -172,3 +172,52 @@ def test_single_tokens_of_many_heads():
     c.starts = c.starts_h = None
     assert c.many()
     c.check()
+
+
+TWO = [(kind, rows, dim) for kind, rows in PAIRINGS for dim in (64, 128) if (kind, dim) != ("e2m1", 64)]
+
+
+@pytest.mark.parametrize("kind,rows,dim", TWO)
+def test_two_sides(kind, rows, dim):
+    """Two waves with the same rows: a ragged batch in which some waves' halves see nothing, and values that leave a
+    side's range, an absent page, a NaN in one side's tokens."""
+    import torch
+    rng = np.random.default_rng(dim + len(kind))
+    c = prompt(rng, kind, rows, 11, 3, dim, 16, [70, 0, 33, 129], [470, 40, 450, 431], tail=5, pad=64)
+    assert c.many() and sides(c) == 2
+    c.check()
+    c.table_h[0, [3, 4, 9]] = -1
+    c.table.copy_(torch.from_numpy(c.table_h))
+    c.check()
+    if kind == "bf16":
+        c.cache.part("v")[c.table_h[2, 6]] = 3e38
+        c.check(more=2.0 ** -18)
+        c.cache.part("v")[c.table_h[2, 6]] = 0.5
+    assert c.cache.guards_whole()
+
+
+@pytest.mark.parametrize("kind,rows,dim", [("bf16", "bf16", 128), ("f16", "f16", 64), ("e2m1", "f16", 128), ("int8", "f32", 128),
+                                           ("bf16", "f32", 64), ("e4m3", "bf16", 64)])
+@pytest.mark.parametrize("how", [dict(window=1, limit=600), dict(window=420), dict(docs=50), dict(docs=33, prefix=7),
+                                 dict(prefix=100), dict(cap=3.0), dict(cap=20.0, slopes=True, docs=64, window=400)])
+def test_rules_of_two_sides(kind, rows, dim, how):
+    how = dict(how)
+    how.pop("limit", None)
+    rng = np.random.default_rng(dim + len(how))
+    c = prompt(rng, kind, rows, 16, 2, dim, 16, [130, 61], [460, 61], **rules_of(how, 32))
+    assert c.many() and (sides(c) == 2 or how.get("window") == 1)
+    c.check()
+
+
+@pytest.mark.parametrize("kind,rows,dim,chunks", [("bf16", "bf16", 64, 3), ("int8", "f16", 64, 3), ("bf16", "f32", 128, 3)])
+def test_two_sides_and_chunks(kind, rows, dim, chunks):
+    """Two chunks of 576 tokens, and one for rows that begin inside their first tile."""
+    rng = np.random.default_rng(dim)
+    kv = 32 if dim == 64 else 12
+    c = prompt(rng, kind, rows, kv, 2, dim, 16, [400], [1100], tail=3)
+    assert c.many() and sides(c) == 2
+    assert splits(c) == chunks, splits(c)
+    c.check()
+    if kind == "bf16":
+        c.cache.part("v")[5:9] = 3e38
+        c.check(more=2.0 ** -18)
