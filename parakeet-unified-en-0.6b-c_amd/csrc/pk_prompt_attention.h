@@ -30,7 +30,7 @@
 // output by no more than sqrt(2) of its own rounding where errors are independent, two
 // at the worst; l sums the unrounded.  f16 queries over codes take 2 terms (16 bits), f32 3.
 // More terms are more products: 4096 tokens of 32 heads of 128 take 141 us with one for
-// each, 352 with f32's 3 by 3.
+// each, 341 with f32's 3 by 3.
 //
 // What bounds it: 8192 tokens of 32 heads over 8 of 128 in bf16 take 504 to 511 us, 1080 of the
 // 1267 TFLOP/s that a product of two 8192 x 8192 matrices reaches here; both are held by the

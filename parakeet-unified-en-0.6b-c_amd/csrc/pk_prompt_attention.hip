@@ -53,21 +53,24 @@ int check_sizes(const pk_gpu_kv_cache* c, const Sizes& z)
 //
 // Of more rows still go that way the calls of at most as many such workgroups as CUs, if
 // short: 16 rows start sooner than 128, and keys that need no way through LDS sooner still
-// where that way is a conversion.  Measured (the same; 8 heads of 128 on as many key-value
-// heads; the third column bf16 over int8):
-//   1 x 256 of 256 tokens           8.3 11.2    8.7 17.2    8.4 13.3
-//   1 x 417 of 417                  9.9 13.7   10.5 22.8   10.5 17.8
-//   1 x 128 of 4000                26.8 23.3   27.2 35.2   20.9 28.5
-//   1 x 1024 of 1024               27.2 28.8   29.6 38.9   26.0 33.1
-//   8 x 256 of 256                 27.3 11.8   31.9 18.6   27.5 13.8
+// where that way is a conversion, of which 4 bits need most.  Measured (the same; 8 heads of 128
+// on as many key-value heads):
+//   1 x 256 of 256 tokens           8.7 10.8     9.0 18.3     9.0 13.4     8.1 11.2
+//   1 x 417 of 417                 10.1 14.2    10.6 21.8    10.8 16.7     8.8 15.3
+//   1 x 128 of 4000                19.4 17.9    20.3 25.2    19.3 20.8    16.2 17.9
+//   1 x 1024 of 1024               23.1 24.9    24.7 32.0    22.0 27.5    14.4 25.2
+//   1 x 1400 of 1400               34.6 35.1    38.8 47.4    32.3 42.7    20.9 36.8
+//   1 x 500 of 3000                42.1 26.3    44.5 32.9    28.1 29.9    21.9 27.4
+//   8 x 256 of 256                 27.3 11.8    31.9 18.6    27.5 13.8
 bool few_rows(const pk_gpu_kv_cache* c, const Sizes& z, int dtype)
 {
     const long long each = (long long)z.max_new * (z.heads / c->heads), pairs = (each + 15) / 16 * z.B * c->heads;
     const long long heads = (long long)z.B * c->heads, span = span_of_rows(z);
-    const bool narrow = dtype != F32 && (c->dtype == F16 || c->dtype == BF16), wide = dtype == F32 || c->dtype == E2M1;
+    const bool narrow = dtype != F32 && (c->dtype == F16 || c->dtype == BF16), four = c->dtype == E2M1;
+    const bool wide = dtype == F32 || four;
     return each <= 16 || (each <= 32 && (heads < 256 || span >= (wide ? 512 : 1536))) ||
            (each > 32 && each <= 48 && wide && heads < 512) ||
-           (pairs <= (narrow ? 256 : 512) && pairs * span <= (narrow ? 160 << 10 : 512 << 10));
+           (pairs <= (narrow ? 256 : 512) && pairs * span <= (narrow ? 160 << 10 : four && dtype != F32 ? 1 << 20 : 512 << 10));
 }
 
 // Chunks of a call of many rows, where its tiles are fewer than the CUs: up to `slots`

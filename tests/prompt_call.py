@@ -113,7 +113,8 @@ def many_rows(kind, rows, kv, group, B, new, max_len, window):
     wide = rows == "f32" or kind == "e2m1"
     few = (each <= 16 or (each <= 32 and (B * kv < 256 or span >= (512 if wide else 1536))) or
            (32 < each <= 48 and wide and B * kv < 512) or
-           (tiles <= (256 if narrow else 512) and tiles * span <= (160 << 10 if narrow else 512 << 10)))
+           (tiles <= (256 if narrow else 512) and
+            tiles * span <= (160 << 10 if narrow else 1 << 20 if kind == "e2m1" and rows != "f32" else 512 << 10)))
     return not few
 
 
