@@ -549,7 +549,7 @@ typedef struct {
  * hold (of a token that some rows see and others do not: for those others too) and on
  * |q| hold here too.
  * Scores, sums and the softmax are fp32.  Where a sequence has few (new token, query head)
- * pairs for a key-value head (16, or somewhat more in short or small calls), weights enter the
+ * pairs for a key-value head (16, up to 48 in many calls, more in short ones), weights enter the
  * second product as there.  Where it has many they keep what the output keeps: 8 bits for BF16,
  * 11 for F16 over F16 caches (16 over codes), 24 for F32.  Results do not depend on timing, and
  * of the call's sizes, not of its lengths, is which of the two is taken.

@@ -36,7 +36,7 @@ int check_sizes(const pk_gpu_kv_cache* c, const Sizes& z)
 }
 
 // Calls of few rows, (new token, head) pairs of a key-value head, go 16 a workgroup over
-// the tiles of the one-token attention, the others prompt_rows a workgroup.
+// the tiles of the one-token attention, the others kPromptRows a workgroup.
 //
 // 16 rows, or fewer, read the cache once that way, and faster.  Where sequences have up to 32,
 // the second 16 of them read it again, from L2; that still is less than what 128 rows lose, but
