@@ -221,3 +221,37 @@ def test_two_sides_and_chunks(kind, rows, dim, chunks):
     if kind == "bf16":
         c.cache.part("v")[5:9] = 3e38
         c.check(more=2.0 ** -18)
+
+
+@pytest.mark.parametrize("new,kv", [(3, 2), (150, 16), (500, 16)])
+def test_no_tokens_at_all(new, kv):
+    """max_len 0 takes no page table; rows see nothing: zeros, lse -inf, and rows of no sequence stay."""
+    import ctypes
+    import torch
+    cache = do.Cache("bf16", 2, kv, 16, 64)
+    st = cache.struct()
+    n = 2 * new + 1
+    q = torch.randn((n, kv * 64), device="cuda:0").bfloat16()
+    out, lse = torch.full_like(q, 3.0), torch.full((n, kv), 3.0, device="cuda:0")
+    ints = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda:0")
+    lens, starts = ints(5, 0), ints(0, new, 2 * new)
+    r = pk.AttentionRules(1.0, 0.0, None, 0, None, None)
+    pk.call("pk_gpu_prompt_attention_dev", do.ref(st), pk.BF16, q.data_ptr(), kv * 64, kv, None, 0, lens.data_ptr(),
+            starts.data_ptr(), 2, n, new, 0, ctypes.byref(r), out.data_ptr(), kv * 64, lse.data_ptr(), None, 0, do.stream())
+    torch.cuda.synchronize()
+    assert bool((out[:-1] == 0).all()) and bool((out[-1] == 3).all())
+    assert bool(torch.isneginf(lse[:-1]).all()) and bool((lse[-1] == 3).all())
+
+
+@pytest.mark.parametrize("new,kv,kind,rows", [(5, 2, "int8", "bf16"), (130, 16, "bf16", "bf16"), (130, 16, "int8", "f32")])
+def test_the_largest_and_smallest_of_a_rule(new, kv, kind, rows):
+    """Ranges that begin behind everything or before it, and end so: as the documented maximum and minimum say."""
+    rng = np.random.default_rng(new)
+    big = 2 ** 31 - 1
+    pick = lambda *v: (lambda b, p: np.where(b >= 0, np.array(v)[np.arange(len(p)) % len(v)], 0))
+    c = prompt(rng, kind, rows, kv, 2, 64, 16, [new, new], [new + 300, new], first=pick(0, -big - 1, 7, big, 100, -1),
+               until=pick(big, 0, -big - 1, big, 5))
+    assert c.many() == (new > 5)
+    c.check()
+    c = prompt(rng, kind, rows, kv, 2, 64, 16, [new, new], [new + 300, new], window=new + 299, until=pick(big, 0, 90))
+    c.check()
