@@ -98,7 +98,8 @@ struct PagedArgs {
     size_t ldo;                  // bytes
     float* lse;
     float* part;                 // [B][max_new][heads][splits][dim], then
-    float* ml;                   // [B][max_new][heads][splits][2]  (one new token: max_new = 1)
+    float* ml;                   // [B][max_new][heads][splits][2]  (one new token: max_new = 1): m, l; with
+                                 // rules m = -inf: `part` holds nothing of it
     float scale2;                // scale * log2(e)
     int B, max_len, window;
     int kv_heads, group, head_tiles;
@@ -377,8 +378,8 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM, RULES), waves_of(
         sp = span_of(len, a.max_len, a.window, a.chunk);
     }
     if (split > 0 && split >= sp.chunks) {
-        if (RULES && wave == 0 && g == 0 && head_ok) {          // the join looks at every chunk
-            a.ml[(row_of() * a.splits + split) * 2] = -FLT_MAX;
+        if (RULES && wave == 0 && g == 0 && head_ok) {          // the join looks at every chunk; no outputs here
+            a.ml[(row_of() * a.splits + split) * 2] = -__builtin_inff();
             a.ml[(row_of() * a.splits + split) * 2 + 1] = 0.0f;
         }
         return;

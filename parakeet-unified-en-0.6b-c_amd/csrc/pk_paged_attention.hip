@@ -21,8 +21,9 @@ struct JoinArgs {
 // every PARTS-th chunk; sums run in a fixed order.  All that it reads first,
 // the length, the chunks' (m, l) and EARLY chunks' outputs of a thread, is asked
 // for at once: the workspace holds them whether the sequence has them or not.  With
-// RULES a row is a (sequence, new token, head) or a (row of q, head), and a chunk that it sees nothing of has
-// said so by l = 0; what the workspace holds of that one's outputs is anything.
+// RULES a row is a (sequence, new token, head) or a (row of q, head), and a chunk whose outputs
+// are not in the workspace, since the row sees nothing of it, has said so by m = -inf.  Of every
+// other one an infinity or a NaN is passed on, also where the chunk's weight is 0 beside the others'.
 template <int T, int DIM, bool RULES>
 __global__ void __launch_bounds__(256) paged_join(JoinArgs a)
 {
@@ -61,28 +62,31 @@ __global__ void __launch_bounds__(256) paged_join(JoinArgs a)
     if (lane == 0) red[0][wave] = mx;
     __syncthreads();
     mx = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    const float w = i < chunks && (!RULES || l != 0.0f) ? __builtin_amdgcn_exp2f(m - mx) : 0.0f;
-    wgt[i] = w;
+    const float w = i < chunks && (!RULES || m >= -FLT_MAX) ? __builtin_amdgcn_exp2f(m - mx) : 0.0f;
+    wgt[i] = RULES && !(m >= -FLT_MAX) ? -1.0f : w;        // -1: nothing there
     float lt = __fmul_rn(l, w);
 #pragma unroll
     for (int d = 32; d; d >>= 1) lt = __fadd_rn(lt, __shfl_xor(lt, d));
     if (lane == 0) red[1][wave] = lt;
     __syncthreads();
     lt = __fadd_rn(__fadd_rn(red[1][0], red[1][1]), __fadd_rn(red[1][2], red[1][3]));
+    auto add = [](float x, float by, float to) {
+        return !RULES || fabsf(x) <= FLT_MAX ? __fmaf_rn(x, by, to) : __fadd_rn(to, x);
+    };
     f32x4 o = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int e = 0; e < EARLY; ++e) {
         const int c = part + e * PARTS;
-        if (c < chunks && (!RULES || wgt[c] != 0.0f))
+        if (c < chunks && !(RULES && wgt[c] < 0.0f))
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] = __fmaf_rn(v[e][r], wgt[c], o[r]);
+            for (int r = 0; r < 4; ++r) o[r] = add(v[e][r], wgt[c], o[r]);
     }
 #pragma unroll 4
     for (int c = part + EARLY * PARTS; c < chunks; c += PARTS) {
-        if (RULES && wgt[c] == 0.0f) continue;
+        if (RULES && wgt[c] < 0.0f) continue;
         const f32x4 x = *reinterpret_cast<const f32x4*>(src + (size_t)c * DIM);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[r] = __fmaf_rn(x[r], wgt[c], o[r]);
+        for (int r = 0; r < 4; ++r) o[r] = add(x[r], wgt[c], o[r]);
     }
     sum[part][d4] = o;
     __syncthreads();

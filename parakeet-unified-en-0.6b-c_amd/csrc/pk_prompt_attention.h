@@ -666,7 +666,7 @@ __global__ void __launch_bounds__(64 * prompt_waves(DIM, SIDES), prompt_occupanc
         }
     if (g == 0) {
         if (!direct) {
-            a.ml[(row * a.splits + split) * 2] = m - BIAS;
+            a.ml[(row * a.splits + split) * 2] = l == 0.0f ? -__builtin_inff() : m - BIAS;     // without outputs
             a.ml[(row * a.splits + split) * 2 + 1] = l;
         } else if (a.lse) {
             a.lse[row] = l == 0.0f ? -__builtin_inff()
