@@ -588,7 +588,8 @@ typedef struct {
  *           stays, up to `slow` it is divided by factor, in between the two are mixed
  *           linearly (0 <= slow < fast)
  * Formed in fp64, rounded once.  base > 0; factor > 0 (PLAIN ignores it, and all but PARTS
- * the other three).  Needs no device. */
+ * the other three); frequencies that a float does not hold are refused, ones too small for it
+ * are 0.  Needs no device. */
 #define PK_GPU_ROPE_PLAIN  0
 #define PK_GPU_ROPE_LINEAR 1
 #define PK_GPU_ROPE_BASE   2

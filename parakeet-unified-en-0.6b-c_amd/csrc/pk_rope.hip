@@ -304,7 +304,7 @@ int pk_gpu_rope_freqs(int rot_dim, double base, int scaling, double factor, doub
         return rt::error(PK_GPU_EINVAL, "%s: trained = %g, slow = %g, fast = %g", who, trained, slow, fast);
     if (!freqs) return rt::error(PK_GPU_EINVAL, "%s: NULL freqs", who);
     if (scaling == PK_GPU_ROPE_BASE) base *= std::pow(factor, (double)rot_dim / (rot_dim - 2));
-    for (int i = 0; i < rot_dim / 2; ++i) {
+    auto freq = [&](int i) {
         double f = std::pow(base, -2.0 * i / rot_dim);
         if (scaling == PK_GPU_ROPE_LINEAR) f /= factor;
         if (scaling == PK_GPU_ROPE_PARTS) {
@@ -312,8 +312,13 @@ int pk_gpu_rope_freqs(int rot_dim, double base, int scaling, double factor, doub
             keep = keep < 0.0 ? 0.0 : keep > 1.0 ? 1.0 : keep;
             f = f * keep + f / factor * (1.0 - keep);
         }
-        freqs[i] = (float)f;
-    }
+        return (float)f;
+    };
+    for (int i = 0; i < rot_dim / 2; ++i)
+        if (!std::isfinite(base) || !std::isfinite(freq(i)))
+            return rt::error(PK_GPU_EINVAL, "%s: base = %g, factor = %g give frequencies that floats do not hold", who, base,
+                             factor);
+    for (int i = 0; i < rot_dim / 2; ++i) freqs[i] = freq(i);
     return PK_GPU_OK;
 }
 
