@@ -78,6 +78,15 @@ __device__ inline float capped(const RuleArgs& r, float raw)
     return y;
 }
 
+// A head's slope in powers of two, 0 without slopes.  One that the factor would make infinite
+// stays at the largest float, so that its token at distance 0 is not 0 times infinity.
+__device__ inline float slope_of(const RuleArgs& r, int head)
+{
+    if (!r.slopes) return 0.0f;
+    const float s = r.slopes[head], t = s * 1.4426950408889634f;
+    return fabsf(s) <= FLT_MAX && fabsf(t) > FLT_MAX ? copysignf(FLT_MAX, s) : t;
+}
+
 // A score in powers of two: raw = q . k, `ahead` the query's position less the key's.
 template <int T>
 __device__ inline float ruled_score(const RuleArgs& r, float raw, float scale2, float slope2, int ahead)

@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(64 * waves_of(CACHE, T, DIM, RULES), waves_of(
     const int head = kvh * a.group + in_group;
     // of the workspace
     auto row_of = [&] { return (RULES ? (size_t)b * a.rules.max_new + new_token : (size_t)b) * heads + head; };
-    const float slope2 = RULES && a.rules.slopes && head_ok ? a.rules.slopes[head] * 1.4426950408889634f : 0.0f;
+    const float slope2 = RULES && head_ok ? slope_of(a.rules, head) : 0.0f;
 
     // queries: step c takes elements el(c, i) = i + 8 g + 32 c of a 16-bit cache's
     // rows, i + 16 g + 8 (c % 2) + 64 (c / 2) of an 8-bit one's, i + 32 g + 8 (c % 4)

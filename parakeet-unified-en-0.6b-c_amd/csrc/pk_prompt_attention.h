@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(64 * prompt_waves(DIM, SIDES), prompt_occupanc
     const int head = kvh * a.group + (int)(r - (uint32_t)nth * a.group);
     const int token = news.row + (ok ? nth : 0);
     const RowRange see = range_of(a.rules, len, news.count, ok ? nth : 0, token, a.window);
-    const float slope2 = a.rules.slopes ? a.rules.slopes[head] * 1.4426950408889634f : 0.0f;
+    const float slope2 = slope_of(a.rules, head);
     // tokens that any row of the wave sees, and that all do
     const bool sees = ok && see.lo < see.hi;
     const int wave_lo = (int)(0x7fffffffu - max_over<R>(sees ? 0x7fffffffu - (uint32_t)see.lo : 0u));
