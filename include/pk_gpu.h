@@ -518,7 +518,7 @@ int pk_gpu_paged_attention_dev(const pk_gpu_kv_cache *cache, int dtype, const vo
  * but the scale: softmax of scale * q . k_t over the tokens up to the new one itself.
  *   scale   of a magnitude up to 2^120
  *   cap     > 0: a score s becomes cap * tanh(s / cap), to 2^-21 of the cap (f32 queries: of its
- *           value); 0: stays.  cap and |scale| / cap up to 2^120
+ *           value); 0: stays.  cap up to 2^120, |scale| / cap 0 or from 2^-126 to 2^120
  *   slopes  NULL, or [query heads]: slopes[h] * |p - t| is taken off the score of the query
  *           at position p and the key at position t, behind the cap
  *   window  > 0: tokens up to p - window are not seen; 0: no such limit

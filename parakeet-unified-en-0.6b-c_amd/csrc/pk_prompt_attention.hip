@@ -222,10 +222,12 @@ int pk_gpu_prompt_attention_dev(const pk_gpu_kv_cache* cache, int dtype, const v
     if ((cache->dtype == F16 && dtype != F16) || (cache->dtype == BF16 && dtype == F16))
         return rt::error(PK_GPU_ENOTSUP, "%s: queries of type %d over a cache of type %d (F16 caches take F16, "
                          "BF16 caches BF16 or F32)", kWho, dtype, cache->dtype);
-    // times what turns them into powers of two they stay below the largest float
-    const float most = 0x1p120f;
-    if (!(std::fabs(rules->scale) <= most) || !(rules->cap >= 0.0f) || !(rules->cap <= most) ||
-        (rules->cap > 0.0f && !(std::fabs(rules->scale / rules->cap) <= most)))
+    // times what turns them into powers of two they stay below the largest float; a quotient below
+    // the normal ones has lost bits, which times the cap are bits of the score
+    const float most = 0x1p120f, least = 0x1p-126f;
+    const double of_cap = rules->cap > 0.0f ? std::fabs((double)rules->scale / rules->cap) : 0.0;
+    if (!(std::fabs(rules->scale) <= most) || !(rules->cap >= 0.0f) || !(rules->cap <= most) || of_cap > most ||
+        (rules->scale != 0.0f && rules->cap > 0.0f && of_cap < least))
         return rt::error(PK_GPU_EINVAL, "%s: scale = %g, cap = %g", kWho, rules->scale, rules->cap);
     const long long wide = (long long)heads * cache->head_dim;
     if (ldq < wide || ldo < wide)
