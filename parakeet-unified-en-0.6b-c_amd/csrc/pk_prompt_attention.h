@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(64 * prompt_waves(DIM, SIDES), prompt_occupanc
     auto blocks = [&](int t0, int ids) {
         const bool there = (uint32_t)ids < (uint32_t)a.n_pages;
         const size_t off = (there ? (uint32_t)ids * page_bytes + head_bytes : 0) +
-                           (uint32_t)(block_at(t0, lane % NB) & page_mask) * (uint32_t)RB;
+                           (size_t)(uint32_t)(block_at(t0, lane % NB) & page_mask) * RB;     // a page may pass 4 GiB
         Blocks s;
         s.mine = off;
         s.present = (uint32_t)__ballot(there) & ((1u << NB) - 1);
