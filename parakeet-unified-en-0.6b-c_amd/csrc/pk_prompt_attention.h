@@ -23,12 +23,13 @@
 // meet all banks.
 //
 // Roundings.  The first product is exact but for fp32 sums: codes and 16-bit elements are
-// held as they are, f32 queries in 3 bf16 terms (24 bits), f16 queries over codes in 2 (they
-// have 11 bits).  Weights are rounded for the second product: into one term for bf16 queries
-// (8 bits) and for f16 over f16 (11, scaled by 2^7 so that weights above 2^-21 are normal
-// numbers), as the output is itself: each weight is off by half a step relative to it, the
-// output by no more than sqrt(2) of its own rounding where errors are independent, two
-// at the worst; l sums the unrounded.  f16 queries over codes take 2 terms (16 bits), f32 3.
+// held as they are, and so are bf16 and f16 queries, in their own type (f16 ones over 4 bits as
+// 2 bf16 terms); f32 ones are 3 bf16 terms (24 bits).  Weights are rounded for the second
+// product: into one term for bf16 queries (8 bits) and for f16 over f16 (11, scaled by 2^7 so that
+// weights above 2^-21 are normal numbers), as the output is itself.  Each weight w is off by half a
+// step relative to it, so the output by half a step of sum w |v| / l at the worst: as much as its
+// own rounding where values have one sign, more where they cancel, less where many tokens' errors
+// are independent; l sums the unrounded.  f16 queries over codes take 2 terms (16 bits), f32 3.
 // More terms are more products: 4096 tokens of 32 heads of 128 take 141 us with one for
 // each, 341 with f32's 3 by 3.
 //

@@ -62,6 +62,16 @@ int check_sizes(const pk_gpu_kv_cache* c, const Sizes& z)
 //   1 x 1400 of 1400               34.6 35.1    38.8 47.4    32.3 42.7    20.9 36.8
 //   1 x 500 of 3000                42.1 26.3    44.5 32.9    28.1 29.9    21.9 27.4
 //   8 x 256 of 256                 27.3 11.8    31.9 18.6    27.5 13.8
+// Above 512 such workgroups (16-bit caches: 256) batches and groups gain by 128 rows, and so calls of
+// all kinds go that way.  Single long prompts with a head for each key-value head lose by it up to
+// 1400 tokens, over 4 bits beyond, and the rule does not tell them from the others (f32 queries; bf16
+// over int8; over 4 bits; few and many, the same heads, in brackets workgroups of 16 rows):
+//   1 x 1100 of 1100 (552)                      31.7 41.2    26.9 36.2    17.2 31.4
+//   1 x 1400 of 1400 (704)                      38.8 47.8    32.6 42.7    20.9 36.9
+//   1 x 2000 of 2000 (1000)                     64.2 62.8    54.6 52.0    31.7 46.7
+//   4 x 300 of 600 (608)                        30.4 28.4    26.7 21.6    17.4 19.6
+//   8 x 160 of 160 (640)                        21.0 15.1    17.6 11.0    12.3  9.2
+//   1 x 500 of 500, 32 heads over 8 (1000)      33.4 25.9    27.9 19.5    17.7 18.1
 bool few_rows(const pk_gpu_kv_cache* c, const Sizes& z, int dtype)
 {
     const long long each = (long long)z.max_new * (z.heads / c->heads), pairs = (each + 15) / 16 * z.B * c->heads;
@@ -95,8 +105,8 @@ long long split_pairs(const pk_gpu_kv_cache* c, long long rows, int group)
 }
 
 // Sides of a workgroup's rows.  Two make it faster by itself, one gets more work out of a full
-// card: so two for launches that are one round of workgroups, or two of long ones; and for packed
-// documents, whose longest one a launch waits for.  Where tiles are few and tokens many, more
+// card: so two for launches that are one round of workgroups, or two of long ones; and for more of packed
+// documents (`first`), whose longest one a launch waits for.  Where tiles are few and tokens many, more
 // chunks do as much, and few tokens are not worth the join.  Measured (us, one side and two; 32 heads over 8;
 // heads of 128 in bf16, of 128 over int8, of 64 in bf16):
 //   16 x 16 of 200 tokens, 128 tiles  11.4 12.1
@@ -108,14 +118,24 @@ long long split_pairs(const pk_gpu_kv_cache* c, long long rows, int group)
 //   2000 of 2000, 504                 51.1 50.3    72.1 64.0    36.5 33.3
 //   4 x 400 of 400, 416               19.4 25.2    23.9 29.4    13.5 14.2
 //   4096 of 4096, 1024                136  168     178  214     88.2 97.2
-//   8191 in documents of 900, 16 heads over 4, 1024                  57 to 96, 53 to 81
 // f32 queries over heads of 128 354 and 342 in bf16, 88.2 and 51.8 for 1000 over int8.
+// With documents the limit for heads of 64 is two rounds of what runs at a time.  Documents of 300, 900
+// and 3000 tokens on average, 16 heads over 4, three draws each (heads of 64 in f16, of 128 in bf16):
+//   3000 tokens, 379 tiles       23.1 20.4   36.6 30.7   50.2 45.1     32.4 29.4   41.2 36.6   53.6 46.2
+//   5000, 629                    28.1 25.6   41.9 36.4   69.3 60.0     34.2 42.2   53.5 58.1   83.3 82.8
+//   9000, 1129                   39.4 38.4   59.3 55.1   97.3 92.0     58.1 71.4   102  117    190  204
+//   16000, 2004                  56.7 60.9   112  110    180  172      86.6 116    179  205    350  384
+//   32000, 4004                  94.9 107    206  204    468  470      162  231    290  359    943  1076
+// and with documents of 300 and 3000, heads of 64, bf16 over int8 and f32 over bf16:
+//   5000, 629                    34.4 33.0   127  112                  40.9 42.8   117  111
+//   9000, 1129                   47.4 51.1   204  200                  59.5 69.4   175  173
 int prompt_sides(const pk_gpu_kv_cache* c, int dtype, long long pairs, long long split, long long span, bool packed)
 {
     const int dim = c->head_dim;
     if (!has_sides(c->dtype, dtype, dim, 2)) return 1;
     if (!has_sides(c->dtype, dtype, dim, 1)) return 2;
-    const long long most = dim == 64 ? (packed && dtype != F32 ? 1024 : 512) : span >= 1024 ? 512 : 256;
+    const long long rounds = 2ll * prompt_slots(c->dtype, dtype, dim, 2);
+    const long long most = dim == 64 ? (packed && rounds > 512 ? rounds : 512) : span >= 1024 ? 512 : 256;
     if (pairs > most || span < 384) return 1;
     return pairs >= 192 || prompt_cuts(split, span, prompt_slots(c->dtype, dtype, dim, 1)) == 1 ? 2 : 1;
 }

@@ -7,8 +7,9 @@
 // thread, into LDS (fp64 for the product and the reduction, so that far positions keep
 // their bits); a thread then keeps those of its elements in registers over all heads.
 // Bound by the rows' bytes, each read and written once: 8191 tokens of 32 + 8 + 8 heads
-// of 128 in bf16, keys and values into int8 codes, 33 us, 4.8 TB/s; 4001 rows of 16 heads
-// of 64 in f32 8.6, 3.8.
+// of 128 in bf16, keys and values into int8 codes, 32 us, 5.8 TB/s (passes over the same rows, some
+// of which the card's large cache then holds: a copy of 1 GiB makes 5.15); 4001 rows of 16 heads of
+// 64 in f32 8.6, 3.8.
 #include "pk_kv_rows.h"
 
 #include <cmath>
