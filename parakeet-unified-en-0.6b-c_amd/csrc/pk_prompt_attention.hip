@@ -2,6 +2,7 @@
 // over a paged cache, with rules for scores and for what a token sees.
 #include "pk_prompt_attention.h"
 
+#include <climits>
 #include <cmath>
 
 namespace pkgpu {
@@ -12,6 +13,14 @@ constexpr const char* kWho = "prompt attention";
 
 // A call's sizes, as its workspace is made for.
 struct Sizes { int B, heads, max_new, max_len, window; };
+
+// a * b of sizes, at most the largest number: bounds of a call may be far from what it holds, and
+// products of four of them pass 64 bits.
+long long times(long long a, long long b)
+{
+    long long r;
+    return __builtin_mul_overflow(a, b, &r) ? LLONG_MAX : r;
+}
 
 // Tokens that a workgroup's columns see at most, from a multiple of 32 on.
 long long span_of_rows(const Sizes& z)
@@ -74,13 +83,13 @@ int check_sizes(const pk_gpu_kv_cache* c, const Sizes& z)
 //   1 x 500 of 500, 32 heads over 8 (1000)      33.4 25.9    27.9 19.5    17.7 18.1
 bool few_rows(const pk_gpu_kv_cache* c, const Sizes& z, int dtype)
 {
-    const long long each = (long long)z.max_new * (z.heads / c->heads), pairs = (each + 15) / 16 * z.B * c->heads;
+    const long long each = (long long)z.max_new * (z.heads / c->heads), pairs = times(times((each + 15) / 16, z.B), c->heads);
     const long long heads = (long long)z.B * c->heads, span = span_of_rows(z);
     const bool narrow = dtype != F32 && (c->dtype == F16 || c->dtype == BF16), four = c->dtype == E2M1;
     const bool wide = dtype == F32 || four;
     return each <= 16 || (each <= 32 && (heads < 256 || span >= (wide ? 512 : 1536))) ||
            (each > 32 && each <= 48 && wide && heads < 512) ||
-           (pairs <= (narrow ? 256 : 512) && pairs * span <= (narrow ? 160 << 10 : four && dtype != F32 ? 1 << 20 : 512 << 10));
+           (pairs <= (narrow ? 256 : 512) && times(pairs, span) <= (narrow ? 160 << 10 : four && dtype != F32 ? 1 << 20 : 512 << 10));
 }
 
 // Chunks of a call of many rows, where its tiles are fewer than the CUs: up to `slots`
@@ -154,15 +163,15 @@ Layout layout_of(const pk_gpu_kv_cache* c, const Sizes& z, int rows, int dtype, 
     Layout l{};
     l.few = few_rows(c, z, dtype);
     if (l.few) {
-        l.pairs = (each + 15) / 16 * z.B * c->heads;
-        l.outs = (long long)z.B * z.max_new * z.heads;
+        l.pairs = times(times((each + 15) / 16, z.B), c->heads);
+        l.outs = times(times(z.B, z.max_new), z.heads);
         l.plan = plan_of(c->dtype, c->head_dim, l.pairs > 0 ? l.pairs : 1, span);
     } else {
         const int bm = kPromptRows;
         // tiles of every sequence, or of all rows with one that is not whole for each sequence
         const long long per = (each + bm - 1) / bm, all = (long long)rows * group / bm + z.B;
-        l.per_seq = per * z.B <= all ? (int)per : 0;
-        l.pairs = (l.per_seq ? per * z.B : all) * c->heads;
+        l.per_seq = times(per, z.B) <= all ? (int)per : 0;
+        l.pairs = times(l.per_seq ? per * z.B : all, c->heads);
         l.outs = (long long)rows * z.heads;
         const long long split = split_pairs(c, rows, group);
         l.sides = prompt_sides(c, dtype, l.pairs, split, span, packed);
@@ -270,7 +279,7 @@ int pk_gpu_prompt_attention_dev(const pk_gpu_kv_cache* cache, int dtype, const v
     if (z.window >= max_len) z.window = 0;
     const Layout l = layout_of(cache, z, rows, dtype, rules->first != nullptr);
     const Plan& p = l.plan;
-    if (!launchable(l.pairs * p.splits, 512) || l.outs > 0x7fffffff || (p.splits > 1 && !launchable(l.outs, 256)))
+    if (!launchable(times(l.pairs, p.splits), 512) || l.outs > 0x7fffffff || (p.splits > 1 && !launchable(l.outs, 256)))
         return rt::error(PK_GPU_EINVAL, "%s: %d sequences of %d new tokens and %d heads exceed the grid", kWho, B, z.max_new,
                          heads);
     const size_t need = p.splits <= 1 ? 0 : (size_t)l.outs * p.splits * (cache->head_dim + 2);
